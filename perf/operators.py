@@ -325,15 +325,18 @@ def _plain_window(state):
 def _seen_count(case, first, n, length):
     """Visible (query, key) pairs of n queries at positions first .. first + n - 1 over `length` keys, and the keys
     that one of them sees at least."""
+    window = case["window"] or 1 << 60
+    sinks = min(case["sinks"], length) if case["window"] else 0
+
+    def near(p):
+        return max(0, p - window + 1), min(length - 1, p if case["causal"] else p + window - 1)
+
     pairs = 0
-    window, sinks = case["window"] or 1 << 60, case["sinks"] if case["window"] else 0
     for p in range(first, first + n):
-        hi = min(length - 1, p if case["causal"] else p + window - 1)
-        lo = max(0, p - window + 1)
-        pairs += max(0, hi - lo + 1) + max(0, min(sinks, lo, hi + 1))
-    hi = min(length, first + n if case["causal"] else first + n - 1 + window)
-    lo = max(0, first - window + 1)
-    return pairs, max(0, hi - lo) + max(0, min(sinks, lo, hi))
+        lo, hi = near(p)
+        pairs += hi - lo + 1 + min(sinks, lo) + (0 if case["causal"] else max(0, sinks - hi - 1))
+    lo, hi = near(first)[0], near(first + n - 1)[1]
+    return pairs, hi - lo + 1 + min(sinks, lo) + (0 if case["causal"] else max(0, sinks - hi - 1))
 
 
 def work(case):
