@@ -430,6 +430,81 @@ int sol_attention_noalloc(const void* q, const int64_t* q_strides,
                           int64_t local_blocks, int64_t kv_sink_tokens,
                           int64_t query_sink_tokens, void* out, int32_t* counts, void* stream);
 
+/* ---- Paged K/V cache and windowed attention ------------------------------
+ * For a model that generates its sequence piece by piece.  No counterpart in
+ * the reference.
+ *
+ * A cache is two stored tensors, K and V, of [pages, heads, page_size,
+ * head_dim] elements (page_size a power of two, 16 to 4096), contiguous and
+ * 16-byte aligned:
+ *   SOL_CACHE_BF16  BF16; scales unused (NULL)
+ *   SOL_CACHE_INT8  int8 codes, value = code * scale, scale = max|row| / 127
+ *   SOL_CACHE_FP8   e4m3 codes (OCP, finite), scale = max|row| / 448
+ * with scales fp32 [pages, heads, page_size], one per token, head and operand.
+ * Codes are the row times 127 / max (448 / max), INT8 rounded half to even,
+ * FP8 to the nearest e4m3 value.  A row of zeros has scale 0; a row with an
+ * infinity or a NaN has scale NaN and reads back as NaN.
+ *
+ * A batch of `sequences` is three int32 arrays in device memory, read by the
+ * kernels (so a captured launch follows what they hold at replay):
+ *   page_table [sequences, table_width]: position p of sequence s is row p %
+ *     page_size of page page_table[s][p / page_size];
+ *   context_lengths [sequences]: keys of each sequence, its new tokens included;
+ *   query_offsets [sequences + 1]: rows query_offsets[s] .. [s + 1] - 1 of the
+ *     call's K, V or Q are sequence s's new tokens, its last positions.
+ * They are not validated on the host.  Lengths are clamped into the table's
+ * range and offsets into [0, rows]; a page outside [0, pages) is no page: not
+ * written, read as zeros, not attended; a new token whose position is
+ * negative is not written.  So no content makes a kernel leave the given
+ * tensors.  Offsets have to ascend, and no two new tokens may name one row of
+ * one page: which of them stays, or a mix of both, is not defined then.  Rows
+ * at and past query_offsets[sequences] are not read, and their outputs are
+ * left as they were. */
+#define SOL_CACHE_BF16 0
+#define SOL_CACHE_INT8 1
+#define SOL_CACHE_FP8 2
+
+/* Stores the new tokens' K and V rows: k and v are BF16 [rows, heads,
+ * head_dim] by their {batch (ignored), token, head} strides. */
+int sol_cache_write(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, int64_t rows,
+                    const int32_t* page_table, const int32_t* context_lengths, const int32_t* query_offsets,
+                    int64_t sequences, int64_t table_width, int64_t pages, int64_t page_size, int64_t heads,
+                    int64_t head_dim, int format, void* cache_k, void* cache_v, float* k_scales, float* v_scales,
+                    void* stream);
+
+/* Reads positions start .. start + tokens - 1 of every sequence back: code *
+ * scale in FP32, rounded once to BF16, into contiguous BF16 [sequences, tokens,
+ * heads, head_dim] K and V; zeros at and past a sequence's context length. */
+int sol_cache_read(const void* cache_k, const void* cache_v, const float* k_scales, const float* v_scales,
+                   const int32_t* page_table, const int32_t* context_lengths, int64_t sequences, int64_t table_width,
+                   int64_t pages, int64_t page_size, int64_t heads, int64_t head_dim, int format, int64_t start,
+                   int64_t tokens, void* k_out, void* v_out, void* stream);
+
+/* Attention of the new tokens over the cache, FP32 scores, softmax and sums.
+ * q: BF16 [rows, query_heads, head_dim] by its {batch (ignored), token, head}
+ * strides; query head h attends key head h / (query_heads / heads).  The query
+ * at position p sees key j of its sequence iff (j <= p, or causal is 0) and
+ * (window is 0, or |p - j| < window, or j < sink_tokens); a query that sees no
+ * key gets zeros.  Values at positions a query does not see never reach its
+ * result, infinities and NaN included.  out: contiguous BF16 [rows,
+ * query_heads, head_dim]. */
+int sol_paged_attention(const void* q, const int64_t* q_strides, int64_t rows, const void* cache_k,
+                        const void* cache_v, const float* k_scales, const float* v_scales, const int32_t* page_table,
+                        const int32_t* context_lengths, const int32_t* query_offsets, int64_t sequences,
+                        int64_t table_width, int64_t pages, int64_t page_size, int64_t query_heads, int64_t heads,
+                        int64_t head_dim, int format, double scale, int causal, int64_t window, int64_t sink_tokens,
+                        void* out, void* stream);
+
+/* The same over plain BF16 K and V [batch, key_tokens, heads, head_dim] and Q
+ * [batch, query_tokens, query_heads, head_dim] by their {batch, token, head}
+ * strides: query t has position key_tokens - query_tokens + t (the queries
+ * are the last tokens of the key sequence; a negative position sees no key
+ * when causal).  out: contiguous BF16 shaped like Q. */
+int sol_window_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                         const void* v, const int64_t* v_strides, int64_t batch, int64_t query_tokens,
+                         int64_t key_tokens, int64_t query_heads, int64_t heads, int64_t head_dim, double scale,
+                         int causal, int64_t window, int64_t sink_tokens, void* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -65,6 +65,14 @@ _SIGNATURES = {
     "sol_attention_workspace_size": ([_i64, _i64, _i64, _i64, _i64, _dbl, _i64, _i64, _i64], ctypes.c_int64),
     "sol_attention_all_in": ([_p, _i64p, _p, _i64p, _p, _i64p, _i64, _i64, _i64, _i64, _i64,
                               _dbl, _dbl, _i64, _i64, _i64, _p, _i64, _p, _p, _p], ctypes.c_int),
+    "sol_cache_write": ([_p, _i64p, _p, _i64p, _i64, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _int,
+                         _p, _p, _p, _p, _p], ctypes.c_int),
+    "sol_cache_read": ([_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _int, _i64, _i64,
+                        _p, _p, _p], ctypes.c_int),
+    "sol_paged_attention": ([_p, _i64p, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                             _int, _dbl, _int, _i64, _i64, _p, _p], ctypes.c_int),
+    "sol_window_attention": ([_p, _i64p, _p, _i64p, _p, _i64p, _i64, _i64, _i64, _i64, _i64, _i64, _dbl, _int,
+                              _i64, _i64, _p, _p], ctypes.c_int),
 }
 
 
@@ -709,4 +717,75 @@ def launch_dense(q, k, v, scale, rows=None, out=None):
                              k.data_ptr(), _strides(k), v.data_ptr(), _strides(v),
                              b, tq, nk, h, d, float(scale), _ptr(tiles), out.data_ptr(),
                              _ptr(rows if scatter else None), _stream(q.device)))
+    return out
+
+
+CACHE_FORMATS = {torch.bfloat16: 0, torch.int8: 1, torch.float8_e4m3fn: 2}  # SOL_CACHE_*
+
+
+def _plan_args(plan):
+    return plan.page_table.data_ptr(), plan.context_lengths.data_ptr(), plan.query_offsets.data_ptr()
+
+
+def launch_cache_write(k, v, cache, plan):
+    """Stores K and V rows (NHD) in a paged cache (``sol_cache_write``)."""
+    n, h, d = k.shape
+    if n == 0 or plan.context_lengths.shape[0] == 0:
+        return
+    k, v = _rows(k), _rows(v)
+    table, lengths, offsets = _plan_args(plan)
+    s, width = plan.page_table.shape
+    pages, _, page_size, _ = cache.k.shape
+    _check(library().sol_cache_write(
+        k.data_ptr(), _strides(k, True), v.data_ptr(), _strides(v, True), n, table, lengths, offsets, s, width, pages,
+        page_size, h, d, CACHE_FORMATS[cache.k.dtype], cache.k.data_ptr(), cache.v.data_ptr(), _ptr(cache.k_scales),
+        _ptr(cache.v_scales), _stream(k.device)))
+
+
+def launch_cache_read(cache, plan, start, tokens):
+    """``(k, v)`` BTHD of positions ``start`` .. ``start + tokens - 1`` (``sol_cache_read``)."""
+    pages, h, page_size, d = cache.k.shape
+    s, width = plan.page_table.shape
+    dev = cache.k.device
+    out = torch.empty((2, s, tokens, h, d), device=dev, dtype=torch.bfloat16)
+    k, v = out[0], out[1]
+    if s == 0 or tokens == 0:
+        return k, v
+    table, lengths, _ = _plan_args(plan)
+    _check(library().sol_cache_read(
+        cache.k.data_ptr(), cache.v.data_ptr(), _ptr(cache.k_scales), _ptr(cache.v_scales), table, lengths, s, width,
+        pages, page_size, h, d, CACHE_FORMATS[cache.k.dtype], start, tokens, k.data_ptr(), v.data_ptr(),
+        _stream(dev)))
+    return k, v
+
+
+def launch_paged(q, cache, plan, scale, causal, window, sinks, out=None):
+    """Attention of new tokens (NHD) over a paged cache (``sol_paged_attention``); ``window`` 0: none."""
+    n, hq, d = q.shape
+    pages, h, page_size, _ = cache.k.shape
+    s, width = plan.page_table.shape
+    dev = q.device
+    if out is None:
+        out = torch.empty((n, hq, d), device=dev, dtype=torch.bfloat16)
+    if n == 0 or s == 0:
+        return out
+    q = _rows(q)
+    table, lengths, offsets = _plan_args(plan)
+    _check(library().sol_paged_attention(
+        q.data_ptr(), _strides(q, True), n, cache.k.data_ptr(), cache.v.data_ptr(), _ptr(cache.k_scales),
+        _ptr(cache.v_scales), table, lengths, offsets, s, width, pages, page_size, hq, h, d,
+        CACHE_FORMATS[cache.k.dtype], scale, causal, window, sinks, out.data_ptr(), _stream(dev)))
+    return out
+
+
+def launch_window(q, k, v, scale, causal, window, sinks):
+    """Windowed attention over plain BTHD tensors (``sol_window_attention``); ``window`` 0: none."""
+    q, q_ptr, q_strides = _bthd_rows(q)
+    k, k_ptr, k_strides = _bthd_rows(k)
+    v, v_ptr, v_strides = _bthd_rows(v)
+    b, tq, hq, d = q.shape
+    tk, h = k.shape[1:3]
+    out = torch.empty((b, tq, hq, d), device=q.device, dtype=torch.bfloat16)
+    _check(library().sol_window_attention(q_ptr, q_strides, k_ptr, k_strides, v_ptr, v_strides, b, tq, tk, hq, h, d,
+                                          scale, causal, window, sinks, out.data_ptr(), _stream(q.device)))
     return out

@@ -34,12 +34,14 @@ class SolStats:
         return self.exact_blocks.float().mean().item() / self.key_blocks
 
 
-def _validate(q, k, v, scale):
-    """Input contract of ``attention.py:19-39``; returns the effective scale."""
+def _validate(q, k, v, scale, grouped=False):
+    """Input contract of ``attention.py:19-39``; returns the effective scale.
+    ``grouped``: several query heads may share a K/V head."""
     qs, ks, device = q.shape, k.shape, q.device
     if len(qs) != 4 or len(ks) != 4 or v.ndim != 4:
         raise ValueError("Q/K/V must have BTHD rank-4 layout")
-    if ks != v.shape or qs[0] != ks[0] or qs[2:] != ks[2:] or min(qs + ks) <= 0:
+    if ks != v.shape or qs[0] != ks[0] or min(qs + ks) <= 0 or (
+            qs[2:] != ks[2:] and not (grouped and qs[3] == ks[3] and qs[2] % ks[2] == 0)):
         raise ValueError("Q/K/V batch, head and dimension shapes must agree and be nonempty")
     if q.dtype != torch.bfloat16 or k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
         raise ValueError("Only BF16 Q/K/V are implemented")
@@ -96,6 +98,38 @@ def dense_attention(q, k, v, *, scale=None):
     scale = _validate(q, k, v, scale)
     with _on(q.device):
         return _native.launch_dense(q, k, v, scale)
+
+
+def _visibility(causal, window, sink_tokens):
+    """Checks the arguments that say which keys a query sees; returns the window, 0 for none."""
+    if not isinstance(causal, bool):
+        raise ValueError("causal must be True or False")
+    _nonnegative_integer("sink_tokens", sink_tokens)
+    if window is None:
+        return 0
+    if not isinstance(window, int) or isinstance(window, bool) or window <= 0:
+        raise ValueError("window must be None or a positive integer")
+    return min(window, 1 << 30)  # no position is further away
+
+
+def window_attention(q, k, v, *, causal=True, window=None, sink_tokens=0, scale=None):
+    """BF16 attention in which a query sees the keys near it and the first ones.
+
+    ``q`` ``[B, Tq, Hq, D]``, ``k``/``v`` ``[B, Tk, H, D]``, Hq a multiple of
+    H: query head h attends K/V head ``h // (Hq // H)``.  The queries are the
+    last tokens of the key sequence: query t has position ``p = Tk - Tq + t``.
+    It sees key j if ``j <= p`` (unless ``causal=False``) and, with a
+    ``window``, if ``abs(p - j) < window`` or ``j < sink_tokens`` (first tokens
+    that stay visible).  ``window=None`` limits nothing.  A query that sees no
+    key gets zeros; what a query does not see never reaches its result,
+    infinities and NaN included.  FP32 scores, softmax and accumulation; keys
+    outside every window are not read.  Not in the reference, whose attention
+    is noncausal over all keys (:func:`dense_attention`).
+    """
+    scale = _validate(q, k, v, scale, grouped=True)
+    window = _visibility(causal, window, sink_tokens)
+    with _on(q.device):
+        return _native.launch_window(q, k, v, scale, causal, window, min(sink_tokens, k.shape[1]))
 
 
 THRESHOLD_ESTIMATORS = ("diagonal_covariance", "full_covariance")

@@ -1,10 +1,12 @@
 // extern "C" entry points: argument checks, parameter packing, launches.
+#include <algorithm>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <mutex>
 #include <string>
 
+#include "paged_internal.h"
 #include "sol_attn_amd.h"
 #include "sol_internal.h"
 
@@ -865,6 +867,214 @@ int sol_attention_noalloc(const void* q, const int64_t* q_strides, const void* k
   return all_in("sol_attention_noalloc", q, q_strides, k, k_strides, v, v_strides, batch, query_tokens, key_tokens,
                 heads, head_dim, scale, beta, local_blocks, kv_sink_tokens, query_sink_tokens, nullptr,
                 SOL_NOALLOC_SCRATCH_BYTES, true, out, counts, stream);
+}
+
+}  // extern "C"
+
+namespace {
+
+constexpr int64_t kMaxPositions = int64_t(1) << 30;  // positions of one sequence, and new rows of one call
+
+// Checks a sequence batch over a cache (its arrays' contents the kernels
+// check themselves) and its sizes, and fills `b`.
+int paged_batch_ok(const char* what, const int32_t* page_table, const int32_t* context_lengths,
+                   const int32_t* query_offsets, int64_t rows, int64_t sequences, int64_t table_width, int64_t pages,
+                   int64_t page_size, int64_t heads, int64_t head_dim, int format, sol::PagedBatch* b) {
+  auto bad = [&](const char* msg) {
+    g_last_error = std::string(what) + ": " + msg;
+    return SOL_ERR_INVALID;
+  };
+  if (head_dim != 64 && head_dim != 128) return bad("unsupported shape (head_dim must be 64 or 128)");
+  if (format != SOL_CACHE_BF16 && format != SOL_CACHE_INT8 && format != SOL_CACHE_FP8)
+    return bad("format must be SOL_CACHE_BF16, SOL_CACHE_INT8 or SOL_CACHE_FP8");
+  if (page_size < 16 || page_size > 4096 || (page_size & (page_size - 1)))
+    return bad("page_size must be a power of two from 16 to 4096");
+  if (rows < 0 || rows >= kMaxPositions || sequences <= 0 || sequences > (1 << 20) || table_width <= 0 || pages <= 0 ||
+      pages >= (int64_t(1) << 31) || heads <= 0 || heads >= (1 << 16) ||
+      table_width > kMaxPositions / page_size)
+    return bad("invalid shape");
+  if (!page_table || !context_lengths) return bad("page_table and context_lengths are required");
+  std::memset(b, 0, sizeof(*b));
+  b->table = page_table;
+  b->lengths = context_lengths;
+  b->offsets = query_offsets;
+  b->S = int(sequences);
+  b->width = int(table_width);
+  b->pages = int(pages);
+  while ((int64_t(1) << b->page_shift) < page_size) ++b->page_shift;
+  b->rows = int(rows);
+  return SOL_OK;
+}
+
+// The stored tensors of a cache and their scales.
+int store_ok(const char* what, const void* cache_k, const void* cache_v, const float* k_scales, const float* v_scales,
+             int format) {
+  if (!cache_k || !cache_v || !aligned16(cache_k) || !aligned16(cache_v)) {
+    g_last_error = std::string(what) + ": the cache needs 16-byte aligned K and V";
+    return SOL_ERR_INVALID;
+  }
+  if (format != SOL_CACHE_BF16 && (!k_scales || !v_scales)) {
+    g_last_error = std::string(what) + ": an INT8 or FP8 cache needs its scales";
+    return SOL_ERR_INVALID;
+  }
+  return SOL_OK;
+}
+
+// Arguments the two windowed attention entry points share.
+int window_args_ok(const char* what, int64_t query_heads, int64_t heads, double scale, int64_t window,
+                   int64_t sink_tokens, const void* out) {
+  auto bad = [&](const char* msg) {
+    g_last_error = std::string(what) + ": " + msg;
+    return SOL_ERR_INVALID;
+  };
+  if (query_heads <= 0 || query_heads >= (1 << 16) || query_heads % heads)
+    return bad("query heads must be a positive multiple of the key heads");
+  if (!std::isfinite(scale) || scale <= 0) return bad("scale must be finite and positive");
+  if (window < 0 || sink_tokens < 0) return bad("window and sink_tokens must not be negative");
+  if (!out || !aligned16(out)) return bad("out must be 16-byte aligned");
+  return SOL_OK;
+}
+
+void window_params(sol::PagedParams* p, int64_t query_heads, int64_t heads, double scale, int causal, int64_t window,
+                   int64_t sink_tokens, void* out) {
+  p->out = static_cast<uint16_t*>(out);
+  p->H = int(heads);
+  p->G = int(query_heads / heads);
+  p->scale_log2 = float(scale * 1.4426950408889634);
+  p->causal = causal != 0;
+  p->window = int(window == 0 ? kMaxPositions : std::min(window, kMaxPositions));
+  p->sinks = window == 0 ? 0 : int(std::min(sink_tokens, kMaxPositions));
+}
+
+}  // namespace
+
+extern "C" {
+
+int sol_cache_write(const void* k, const int64_t* k_strides, const void* v, const int64_t* v_strides, int64_t rows,
+                    const int32_t* page_table, const int32_t* context_lengths, const int32_t* query_offsets,
+                    int64_t sequences, int64_t table_width, int64_t pages, int64_t page_size, int64_t heads,
+                    int64_t head_dim, int format, void* cache_k, void* cache_v, float* k_scales, float* v_scales,
+                    void* stream) {
+  const char* what = "sol_cache_write";
+  sol::CacheParams p;
+  std::memset(&p, 0, sizeof(p));
+  int rc = paged_batch_ok(what, page_table, context_lengths, query_offsets, rows, sequences, table_width, pages,
+                          page_size, heads, head_dim, format, &p.batch);
+  if (rc != SOL_OK) return rc;
+  if (!query_offsets) return fail(SOL_ERR_INVALID, "sol_cache_write: query_offsets is required");
+  rc = store_ok(what, cache_k, cache_v, k_scales, v_scales, format);
+  if (rc != SOL_OK) return rc;
+  if (rows == 0) return SOL_OK;
+  if (!operand_ok(k, k_strides, true) || !operand_ok(v, v_strides, true))
+    return fail(SOL_ERR_INVALID, "sol_cache_write: K and V need 16-byte aligned rows and positive strides");
+  if (rows * heads >= (int64_t(1) << 33)) return fail(SOL_ERR_UNSUPPORTED, "sol_cache_write: grid too large");
+  p.rows[0] = static_cast<const uint16_t*>(k);
+  p.rows[1] = static_cast<const uint16_t*>(v);
+  p.st[0] = k_strides[1], p.sh[0] = k_strides[2];
+  p.st[1] = v_strides[1], p.sh[1] = v_strides[2];
+  p.store[0] = static_cast<uint8_t*>(cache_k);
+  p.store[1] = static_cast<uint8_t*>(cache_v);
+  p.scale[0] = k_scales;
+  p.scale[1] = v_scales;
+  p.H = int(heads);
+  return hip_status(sol::launch_cache_write(p, int(head_dim), format, static_cast<hipStream_t>(stream)));
+}
+
+int sol_cache_read(const void* cache_k, const void* cache_v, const float* k_scales, const float* v_scales,
+                   const int32_t* page_table, const int32_t* context_lengths, int64_t sequences, int64_t table_width,
+                   int64_t pages, int64_t page_size, int64_t heads, int64_t head_dim, int format, int64_t start,
+                   int64_t tokens, void* k_out, void* v_out, void* stream) {
+  const char* what = "sol_cache_read";
+  sol::CacheParams p;
+  std::memset(&p, 0, sizeof(p));
+  int rc = paged_batch_ok(what, page_table, context_lengths, nullptr, 0, sequences, table_width, pages, page_size, heads,
+                          head_dim, format, &p.batch);
+  if (rc != SOL_OK) return rc;
+  rc = store_ok(what, cache_k, cache_v, k_scales, v_scales, format);
+  if (rc != SOL_OK) return rc;
+  if (start < 0 || start >= kMaxPositions || tokens < 0 || tokens >= kMaxPositions)
+    return fail(SOL_ERR_INVALID, "sol_cache_read: invalid token range");
+  if (tokens == 0) return SOL_OK;
+  if (!k_out || !v_out || !aligned16(k_out) || !aligned16(v_out))
+    return fail(SOL_ERR_INVALID, "sol_cache_read: the outputs must be 16-byte aligned");
+  if (sequences * cdiv(tokens, 4) * heads >= (int64_t(1) << 33))
+    return fail(SOL_ERR_UNSUPPORTED, "sol_cache_read: grid too large");
+  p.store[0] = const_cast<uint8_t*>(static_cast<const uint8_t*>(cache_k));
+  p.store[1] = const_cast<uint8_t*>(static_cast<const uint8_t*>(cache_v));
+  p.scale[0] = const_cast<float*>(k_scales);
+  p.scale[1] = const_cast<float*>(v_scales);
+  p.out[0] = static_cast<uint16_t*>(k_out);
+  p.out[1] = static_cast<uint16_t*>(v_out);
+  p.H = int(heads);
+  p.start = int(start);
+  p.tokens = int(tokens);
+  return hip_status(sol::launch_cache_read(p, int(head_dim), format, static_cast<hipStream_t>(stream)));
+}
+
+int sol_paged_attention(const void* q, const int64_t* q_strides, int64_t rows, const void* cache_k,
+                        const void* cache_v, const float* k_scales, const float* v_scales, const int32_t* page_table,
+                        const int32_t* context_lengths, const int32_t* query_offsets, int64_t sequences,
+                        int64_t table_width, int64_t pages, int64_t page_size, int64_t query_heads, int64_t heads,
+                        int64_t head_dim, int format, double scale, int causal, int64_t window, int64_t sink_tokens,
+                        void* out, void* stream) {
+  const char* what = "sol_paged_attention";
+  sol::PagedParams p;
+  std::memset(&p, 0, sizeof(p));
+  int rc = paged_batch_ok(what, page_table, context_lengths, query_offsets, rows, sequences, table_width, pages,
+                          page_size, heads, head_dim, format, &p.batch);
+  if (rc != SOL_OK) return rc;
+  if (!query_offsets) return fail(SOL_ERR_INVALID, "sol_paged_attention: query_offsets is required");
+  rc = store_ok(what, cache_k, cache_v, k_scales, v_scales, format);
+  if (rc != SOL_OK) return rc;
+  if (rows == 0) return SOL_OK;
+  rc = window_args_ok(what, query_heads, heads, scale, window, sink_tokens, out);
+  if (rc != SOL_OK) return rc;
+  if (!operand_ok(q, q_strides, true))
+    return fail(SOL_ERR_INVALID, "sol_paged_attention: Q needs 16-byte aligned rows and positive strides");
+  if (rows * query_heads >= (int64_t(1) << 31))
+    return fail(SOL_ERR_UNSUPPORTED, "sol_paged_attention: grid too large");
+  p.q = static_cast<const uint16_t*>(q);
+  p.q_st = q_strides[1], p.q_sh = q_strides[2];
+  const int64_t row_bytes = head_dim * (format == SOL_CACHE_BF16 ? 2 : 1);
+  for (int i = 0; i < 2; ++i) {
+    p.store[i] = static_cast<const uint8_t*>(i ? cache_v : cache_k);
+    p.scale[i] = i ? v_scales : k_scales;
+    p.st[i] = row_bytes;
+    p.sh[i] = row_bytes * page_size;
+    p.sb[i] = p.sh[i] * heads;
+  }
+  window_params(&p, query_heads, heads, scale, causal, window, sink_tokens, out);
+  return hip_status(sol::launch_paged(p, int(head_dim), format, static_cast<hipStream_t>(stream)));
+}
+
+int sol_window_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                         const void* v, const int64_t* v_strides, int64_t batch, int64_t query_tokens,
+                         int64_t key_tokens, int64_t query_heads, int64_t heads, int64_t head_dim, double scale,
+                         int causal, int64_t window, int64_t sink_tokens, void* out, void* stream) {
+  const char* what = "sol_window_attention";
+  if (!shape_ok(batch, query_tokens, query_heads, head_dim) || key_tokens <= 0 || key_tokens >= kMaxPositions ||
+      heads <= 0)
+    return fail(SOL_ERR_INVALID, "sol_window_attention: unsupported shape (head_dim must be 64 or 128)");
+  const int rc = window_args_ok(what, query_heads, heads, scale, window, sink_tokens, out);
+  if (rc != SOL_OK) return rc;
+  if (!operand_ok(q, q_strides, false) || !operand_ok(k, k_strides, false) || !operand_ok(v, v_strides, false))
+    return fail(SOL_ERR_INVALID, "sol_window_attention: Q, K and V need 16-byte aligned rows and positive strides");
+  if (batch * query_tokens * query_heads >= (int64_t(1) << 31))
+    return fail(SOL_ERR_UNSUPPORTED, "sol_window_attention: grid too large");
+  sol::PagedParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.batch.S = int(batch);
+  p.q = static_cast<const uint16_t*>(q);
+  p.q_sb = q_strides[0], p.q_st = q_strides[1], p.q_sh = q_strides[2];
+  for (int i = 0; i < 2; ++i) {
+    const int64_t* strides = i ? v_strides : k_strides;
+    p.store[i] = static_cast<const uint8_t*>(i ? v : k);
+    p.sb[i] = 2 * strides[0], p.st[i] = 2 * strides[1], p.sh[i] = 2 * strides[2];
+  }
+  p.Tq = int(query_tokens);
+  p.Tk = int(key_tokens);
+  window_params(&p, query_heads, heads, scale, causal, window, sink_tokens, out);
+  return hip_status(sol::launch_paged(p, int(head_dim), SOL_CACHE_BF16, static_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"
