@@ -487,23 +487,34 @@ int sol_cache_read(const void* cache_k, const void* cache_v, const float* k_scal
  * (window is 0, or |p - j| < window, or j < sink_tokens); a query that sees no
  * key gets zeros.  Values at positions a query does not see never reach its
  * result, infinities and NaN included.  out: contiguous BF16 [rows,
- * query_heads, head_dim]. */
+ * query_heads, head_dim].  workspace: 16-byte aligned device memory of at least
+ * sol_paged_attention_workspace_size() bytes for the same sizes (NULL when that
+ * is 0): the partial states of calls that split their keys over workgroups. */
 int sol_paged_attention(const void* q, const int64_t* q_strides, int64_t rows, const void* cache_k,
                         const void* cache_v, const float* k_scales, const float* v_scales, const int32_t* page_table,
                         const int32_t* context_lengths, const int32_t* query_offsets, int64_t sequences,
                         int64_t table_width, int64_t pages, int64_t page_size, int64_t query_heads, int64_t heads,
                         int64_t head_dim, int format, double scale, int causal, int64_t window, int64_t sink_tokens,
-                        void* out, void* stream);
+                        void* workspace, int64_t workspace_bytes, void* out, void* stream);
+int64_t sol_paged_attention_workspace_size(int64_t rows, int64_t sequences, int64_t table_width, int64_t page_size,
+                                           int64_t query_heads, int64_t heads, int64_t head_dim, int causal,
+                                           int64_t window, int64_t sink_tokens);
 
 /* The same over plain BF16 K and V [batch, key_tokens, heads, head_dim] and Q
  * [batch, query_tokens, query_heads, head_dim] by their {batch, token, head}
  * strides: query t has position key_tokens - query_tokens + t (the queries
  * are the last tokens of the key sequence; a negative position sees no key
- * when causal).  out: contiguous BF16 shaped like Q. */
+ * when causal).  K and V token strides below 2^24 elements.  out: contiguous
+ * BF16 shaped like Q; workspace as above, of
+ * sol_window_attention_workspace_size() bytes. */
 int sol_window_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                          const void* v, const int64_t* v_strides, int64_t batch, int64_t query_tokens,
                          int64_t key_tokens, int64_t query_heads, int64_t heads, int64_t head_dim, double scale,
-                         int causal, int64_t window, int64_t sink_tokens, void* out, void* stream);
+                         int causal, int64_t window, int64_t sink_tokens, void* workspace, int64_t workspace_bytes,
+                         void* out, void* stream);
+int64_t sol_window_attention_workspace_size(int64_t batch, int64_t query_tokens, int64_t key_tokens,
+                                            int64_t query_heads, int64_t heads, int64_t head_dim, int causal,
+                                            int64_t window, int64_t sink_tokens);
 
 #ifdef __cplusplus
 }

@@ -70,9 +70,11 @@ _SIGNATURES = {
     "sol_cache_read": ([_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _int, _i64, _i64,
                         _p, _p, _p], ctypes.c_int),
     "sol_paged_attention": ([_p, _i64p, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
-                             _int, _dbl, _int, _i64, _i64, _p, _p], ctypes.c_int),
+                             _int, _dbl, _int, _i64, _i64, _p, _i64, _p, _p], ctypes.c_int),
+    "sol_paged_attention_workspace_size": ([_i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _i64, _i64], _i64),
     "sol_window_attention": ([_p, _i64p, _p, _i64p, _p, _i64p, _i64, _i64, _i64, _i64, _i64, _i64, _dbl, _int,
-                              _i64, _i64, _p, _p], ctypes.c_int),
+                              _i64, _i64, _p, _i64, _p, _p], ctypes.c_int),
+    "sol_window_attention_workspace_size": ([_i64, _i64, _i64, _i64, _i64, _i64, _int, _i64, _i64], _i64),
 }
 
 
@@ -759,6 +761,22 @@ def launch_cache_read(cache, plan, start, tokens):
     return k, v
 
 
+@functools.lru_cache(maxsize=1024)
+def _paged_size(n, s, width, page_size, hq, h, d, causal, window, sinks):
+    return library().sol_paged_attention_workspace_size(n, s, width, page_size, hq, h, d, causal, window, sinks)
+
+
+@functools.lru_cache(maxsize=1024)
+def _window_size(b, tq, tk, hq, h, d, causal, window, sinks):
+    return library().sol_window_attention_workspace_size(b, tq, tk, hq, h, d, causal, window, sinks)
+
+
+def _workspace(size, device):
+    if size < 0:
+        raise RuntimeError("the workspace size function rejected the sizes")
+    return torch.empty(size, device=device, dtype=torch.uint8) if size else None
+
+
 def launch_paged(q, cache, plan, scale, causal, window, sinks, out=None):
     """Attention of new tokens (NHD) over a paged cache (``sol_paged_attention``); ``window`` 0: none."""
     n, hq, d = q.shape
@@ -771,21 +789,29 @@ def launch_paged(q, cache, plan, scale, causal, window, sinks, out=None):
         return out
     q = _rows(q)
     table, lengths, offsets = _plan_args(plan)
+    size = _paged_size(n, s, width, page_size, hq, h, d, causal, window, sinks)
+    ws = _workspace(size, dev)
     _check(library().sol_paged_attention(
         q.data_ptr(), _strides(q, True), n, cache.k.data_ptr(), cache.v.data_ptr(), _ptr(cache.k_scales),
         _ptr(cache.v_scales), table, lengths, offsets, s, width, pages, page_size, hq, h, d,
-        CACHE_FORMATS[cache.k.dtype], scale, causal, window, sinks, out.data_ptr(), _stream(dev)))
+        CACHE_FORMATS[cache.k.dtype], scale, causal, window, sinks, _ptr(ws), size, out.data_ptr(), _stream(dev)))
     return out
 
 
 def launch_window(q, k, v, scale, causal, window, sinks):
-    """Windowed attention over plain BTHD tensors (``sol_window_attention``); ``window`` 0: none."""
+    """Windowed attention over plain BTHD tensors (``sol_window_attention``); ``window`` 0: none.
+    Keys 2^24 elements or more apart are copied first."""
+    if max(k.stride(1), v.stride(1)) >= 1 << 24:
+        k, v = (x.clone(memory_format=torch.contiguous_format) for x in (k, v))
     q, q_ptr, q_strides = _bthd_rows(q)
     k, k_ptr, k_strides = _bthd_rows(k)
     v, v_ptr, v_strides = _bthd_rows(v)
     b, tq, hq, d = q.shape
     tk, h = k.shape[1:3]
     out = torch.empty((b, tq, hq, d), device=q.device, dtype=torch.bfloat16)
+    size = _window_size(b, tq, tk, hq, h, d, causal, window, sinks)
+    ws = _workspace(size, q.device)
     _check(library().sol_window_attention(q_ptr, q_strides, k_ptr, k_strides, v_ptr, v_strides, b, tq, tk, hq, h, d,
-                                          scale, causal, window, sinks, out.data_ptr(), _stream(q.device)))
+                                          scale, causal, window, sinks, _ptr(ws), size, out.data_ptr(),
+                                          _stream(q.device)))
     return out

@@ -873,6 +873,7 @@ int sol_attention_noalloc(const void* q, const int64_t* q_strides, const void* k
 
 namespace {
 
+constexpr int64_t kRowsStrideMax = int64_t(1) << 24;  // elements between plain keys
 constexpr int64_t kMaxPositions = int64_t(1) << 30;  // positions of one sequence, and new rows of one call
 
 // Checks a sequence batch over a cache (its arrays' contents the kernels
@@ -932,6 +933,26 @@ int window_args_ok(const char* what, int64_t query_heads, int64_t heads, double 
   if (!std::isfinite(scale) || scale <= 0) return bad("scale must be finite and positive");
   if (window < 0 || sink_tokens < 0) return bad("window and sink_tokens must not be negative");
   if (!out || !aligned16(out)) return bad("out must be 16-byte aligned");
+  return SOL_OK;
+}
+
+// Keys that the new tokens of one sequence see at most.
+int64_t window_keys(int64_t rows, int64_t keys, int causal, int64_t window, int64_t sink_tokens) {
+  if (window == 0) return keys;
+  window = std::min(window, kMaxPositions);
+  sink_tokens = std::min(sink_tokens, kMaxPositions);
+  return std::min(keys, rows + (causal ? 1 : 2) * window + sink_tokens);
+}
+
+int paged_workspace_ok(const char* what, const sol::PagedSize& size, const void* workspace, int64_t workspace_bytes) {
+  if (size.grid >= (int64_t(1) << 31)) {
+    g_last_error = std::string(what) + ": grid too large";
+    return SOL_ERR_UNSUPPORTED;
+  }
+  if (size.bytes && (!workspace || !aligned16(workspace) || workspace_bytes < size.bytes)) {
+    g_last_error = std::string(what) + ": needs a 16-byte aligned workspace of the size its size function returns";
+    return SOL_ERR_INVALID;
+  }
   return SOL_OK;
 }
 
@@ -1016,7 +1037,7 @@ int sol_paged_attention(const void* q, const int64_t* q_strides, int64_t rows, c
                         const int32_t* context_lengths, const int32_t* query_offsets, int64_t sequences,
                         int64_t table_width, int64_t pages, int64_t page_size, int64_t query_heads, int64_t heads,
                         int64_t head_dim, int format, double scale, int causal, int64_t window, int64_t sink_tokens,
-                        void* out, void* stream) {
+                        void* workspace, int64_t workspace_bytes, void* out, void* stream) {
   const char* what = "sol_paged_attention";
   sol::PagedParams p;
   std::memset(&p, 0, sizeof(p));
@@ -1033,6 +1054,11 @@ int sol_paged_attention(const void* q, const int64_t* q_strides, int64_t rows, c
     return fail(SOL_ERR_INVALID, "sol_paged_attention: Q needs 16-byte aligned rows and positive strides");
   if (rows * query_heads >= (int64_t(1) << 31))
     return fail(SOL_ERR_UNSUPPORTED, "sol_paged_attention: grid too large");
+  const sol::PagedSize size =
+      sol::paged_size(rows, sequences, window_keys(rows, table_width * page_size, causal, window, sink_tokens), heads,
+                      query_heads / heads, head_dim);
+  rc = paged_workspace_ok(what, size, workspace, workspace_bytes);
+  if (rc != SOL_OK) return rc;
   p.q = static_cast<const uint16_t*>(q);
   p.q_st = q_strides[1], p.q_sh = q_strides[2];
   const int64_t row_bytes = head_dim * (format == SOL_CACHE_BF16 ? 2 : 1);
@@ -1044,23 +1070,45 @@ int sol_paged_attention(const void* q, const int64_t* q_strides, int64_t rows, c
     p.sb[i] = p.sh[i] * heads;
   }
   window_params(&p, query_heads, heads, scale, causal, window, sink_tokens, out);
-  return hip_status(sol::launch_paged(p, int(head_dim), format, static_cast<hipStream_t>(stream)));
+  p.workspace = workspace;
+  return hip_status(sol::launch_paged(p, size, int(head_dim), format, static_cast<hipStream_t>(stream)));
+}
+
+int64_t sol_paged_attention_workspace_size(int64_t rows, int64_t sequences, int64_t table_width, int64_t page_size,
+                                           int64_t query_heads, int64_t heads, int64_t head_dim, int causal,
+                                           int64_t window, int64_t sink_tokens) {
+  if (rows < 0 || rows >= kMaxPositions || sequences <= 0 || sequences > (1 << 20) || table_width <= 0 ||
+      page_size <= 0 || table_width > kMaxPositions / page_size || heads <= 0 || heads >= (1 << 16) || query_heads <= 0 ||
+      query_heads % heads || query_heads >= (1 << 16) || (head_dim != 64 && head_dim != 128) || window < 0 ||
+      sink_tokens < 0)
+    return -1;
+  if (rows == 0) return 0;
+  return sol::paged_size(rows, sequences, window_keys(rows, table_width * page_size, causal, window, sink_tokens), heads,
+                         query_heads / heads, head_dim).bytes;
 }
 
 int sol_window_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
                          const void* v, const int64_t* v_strides, int64_t batch, int64_t query_tokens,
                          int64_t key_tokens, int64_t query_heads, int64_t heads, int64_t head_dim, double scale,
-                         int causal, int64_t window, int64_t sink_tokens, void* out, void* stream) {
+                         int causal, int64_t window, int64_t sink_tokens, void* workspace, int64_t workspace_bytes,
+                         void* out, void* stream) {
   const char* what = "sol_window_attention";
   if (!shape_ok(batch, query_tokens, query_heads, head_dim) || key_tokens <= 0 || key_tokens >= kMaxPositions ||
       heads <= 0)
     return fail(SOL_ERR_INVALID, "sol_window_attention: unsupported shape (head_dim must be 64 or 128)");
-  const int rc = window_args_ok(what, query_heads, heads, scale, window, sink_tokens, out);
+  int rc = window_args_ok(what, query_heads, heads, scale, window, sink_tokens, out);
   if (rc != SOL_OK) return rc;
   if (!operand_ok(q, q_strides, false) || !operand_ok(k, k_strides, false) || !operand_ok(v, v_strides, false))
     return fail(SOL_ERR_INVALID, "sol_window_attention: Q, K and V need 16-byte aligned rows and positive strides");
   if (batch * query_tokens * query_heads >= (int64_t(1) << 31))
     return fail(SOL_ERR_UNSUPPORTED, "sol_window_attention: grid too large");
+  if (k_strides[1] >= kRowsStrideMax || v_strides[1] >= kRowsStrideMax)
+    return fail(SOL_ERR_UNSUPPORTED, "sol_window_attention: K and V token strides must be below 2^24 elements");
+  const sol::PagedSize size =
+      sol::paged_size(batch * query_tokens, batch, window_keys(query_tokens, key_tokens, causal, window, sink_tokens),
+                      heads, query_heads / heads, head_dim);
+  rc = paged_workspace_ok(what, size, workspace, workspace_bytes);
+  if (rc != SOL_OK) return rc;
   sol::PagedParams p;
   std::memset(&p, 0, sizeof(p));
   p.batch.S = int(batch);
@@ -1074,7 +1122,19 @@ int sol_window_attention(const void* q, const int64_t* q_strides, const void* k,
   p.Tq = int(query_tokens);
   p.Tk = int(key_tokens);
   window_params(&p, query_heads, heads, scale, causal, window, sink_tokens, out);
-  return hip_status(sol::launch_paged(p, int(head_dim), SOL_CACHE_BF16, static_cast<hipStream_t>(stream)));
+  p.workspace = workspace;
+  return hip_status(sol::launch_paged(p, size, int(head_dim), SOL_CACHE_BF16, static_cast<hipStream_t>(stream)));
+}
+
+int64_t sol_window_attention_workspace_size(int64_t batch, int64_t query_tokens, int64_t key_tokens,
+                                            int64_t query_heads, int64_t heads, int64_t head_dim, int causal,
+                                            int64_t window, int64_t sink_tokens) {
+  if (!shape_ok(batch, query_tokens, query_heads, head_dim) || key_tokens <= 0 || key_tokens >= kMaxPositions ||
+      heads <= 0 || heads >= (1 << 16) || query_heads % heads || window < 0 || sink_tokens < 0)
+    return -1;
+  return sol::paged_size(batch * query_tokens, batch,
+                         window_keys(query_tokens, key_tokens, causal, window, sink_tokens), heads,
+                         query_heads / heads, head_dim).bytes;
 }
 
 }  // extern "C"

@@ -4,13 +4,35 @@
 // Query i of an entry with n queries and L keys has position p = L - n + i; key
 // j < L is visible iff (j <= p or not causal) and (|p - j| < window or j <
 // sinks).  O = sum_j softmax_j(scale q . k_j) v_j over the visible keys, 0 for
-// a query that sees none.  Scores, softmax statistics and sums are FP32.
+// a query that sees none.  Scores, softmax statistics and sums are FP32; the
+// probabilities are rounded to BF16 for their product with V, as everywhere in
+// this library (the denominator sums the unrounded ones).
+//
+// The rows of a (sequence, K/V head) are its new tokens times the G query
+// heads that share the head, token by token: row r is token r / G, query head
+// r % G of the group.  They are cut into tiles of R rows; a tile's keys are the
+// union of what its rows see, in key tiles, and may be split over several
+// workgroups ("parts"), whose softmax states the merge kernel joins.
+//   step_kernel  R = 32, for few rows per sequence (single tokens): four waves,
+//                each with key tiles of its own; bound by reading the cache
+//   wide_kernel  R = 128, for chunks: four waves of 32 rows share every key tile;
+//                bound by the matrix cores and the softmax's vector work
+//
+// Cached INT8 and FP8 codes are converted to BF16 (exact) on their way into
+// LDS; a key's scale multiplies its score, a value's scale its probability.
+#include "attn_common.h"
 #include "paged_internal.h"
-#include "sol_device.h"
 
 namespace sol {
 
 namespace {
+
+constexpr int kNT = 256;  // threads per workgroup
+constexpr int kWaves = kNT / kWave;
+
+__device__ __forceinline__ int cdiv_i(int a, int b) { return (a + b - 1) / b; }
+
+// ---- what is visible --------------------------------------------------------
 
 // The keys a position sees: [lo, hi] and [0, sink).
 struct Visible {
@@ -25,110 +47,1063 @@ __device__ __forceinline__ Visible visible(const PagedParams& p, int pos, int le
   return v;
 }
 
-template <int F>
-__device__ __forceinline__ float element(const uint8_t* row, int i) {
-  if constexpr (F == kBf16) return bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(row)[i]);
-  else if constexpr (F == kInt8) return float(int8_t(row[i]));
-  else return __builtin_amdgcn_cvt_pk_f32_fp8(int(row[i]), false)[0];
+// The key tiles (of TK keys) that positions first .. last see: tiles [0, ns)
+// and n - ns tiles from w0.
+struct Span {
+  int ns, w0, n;
+  __device__ __forceinline__ int tile(int i) const { return i < ns ? i : w0 + (i - ns); }
+};
+
+template <int TK>
+__device__ __forceinline__ Span span_of(const PagedParams& p, int first, int last, int length) {
+  const int lo = visible(p, first, length).lo;
+  const Visible v = visible(p, last, length);
+  Span s;
+  s.ns = v.sink > 0 ? (v.sink - 1) / TK + 1 : 0;
+  s.w0 = max(s.ns, lo / TK);
+  s.n = s.ns + (v.hi >= lo ? max(0, v.hi / TK + 1 - s.w0) : 0);
+  return s;
 }
 
-// One wave per (query row, query head): a key per lane for the scores, a
-// feature (two at D = 128) per lane for the values.
-template <int D, int F>
-__global__ __launch_bounds__(64) void attend_rows_kernel(PagedParams p) {
-  const PagedBatch& bt = p.batch;
-  const int lane = threadIdx.x;
-  const int heads = p.H * p.G;
-  const int64_t row = blockIdx.x / heads;
-  const int hq = int(blockIdx.x % heads), h = hq / p.G;
-  int s, i, n, length;
-  if (bt.table) {
-    s = 0;
-    while (s + 1 < bt.S && bt.offset(s + 1) <= row) ++s;
-    if (row < bt.offset(s) || row >= bt.offset(s + 1)) return;
-    n = bt.offset(s + 1) - bt.offset(s);
-    i = int(row) - bt.offset(s);
-    length = bt.length(s);
-  } else {
-    s = int(row / p.Tq);
-    i = int(row % p.Tq);
-    n = p.Tq;
-    length = p.Tk;
-  }
-  const Visible v = visible(p, length - n + i, length);
-  const uint16_t* q = p.q + (bt.table ? row * p.q_st : s * p.q_sb + i * p.q_st) + hq * p.q_sh;
-  auto address = [&](int kv, int j) -> const uint8_t* {
-    int64_t unit = s;
-    if (bt.table) {
-      unit = bt.table[int64_t(s) * bt.width + (j >> bt.page_shift)];
-      if (unit < 0 || unit >= bt.pages) return nullptr;
-      return p.store[kv] + unit * p.sb[kv] + h * p.sh[kv] + (j & ((1 << bt.page_shift) - 1)) * p.st[kv];
-    }
-    return p.store[kv] + unit * p.sb[kv] + h * p.sh[kv] + j * p.st[kv];
+// ---- which rows and keys a workgroup takes ----------------------------------
+
+__device__ __forceinline__ int entry_offset(const PagedParams& p, int s) {
+  return p.batch.table ? p.batch.offset(s) : s * p.Tq;
+}
+
+__device__ __forceinline__ int entry_length(const PagedParams& p, int s) {
+  return p.batch.table ? p.batch.length(s) : p.Tk;
+}
+
+struct Item {
+  int s, off, n, length;  // the sequence: first row, new tokens, keys
+  int r0, rows;           // the tile's rows r0 .. r0 + rows - 1 of the sequence's n G
+  int part, parts;        // its share of the tile's keys
+};
+
+// Item `id` of the launch, in order of sequences, row tiles and parts; false
+// past the last one.  Every workgroup forms the whole plan from the lengths on
+// the device (two scans over the sequences, a few microseconds), so that a
+// captured launch follows them and no launch or copy comes before this one.
+// With p.target, parts are of at most z key tiles, z such that about p.target
+// workgroups per head share all key tiles evenly: sum ceil(n_s / z) tiles_s is
+// at most target + sum tiles_s, the grid.  Without, one part each.
+template <int R, int TK>
+__device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item& it) {
+  __shared__ int64_t s_total[kWaves];
+  __shared__ int s_found[4];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int S = p.batch.S;
+  // Row tiles and key tiles of sequence s.
+  auto sizes = [&](int s, int& row_tiles, int& key_tiles) {
+    const int n = entry_offset(p, s + 1) - entry_offset(p, s), length = entry_length(p, s);
+    row_tiles = n > 0 ? (n * p.G - 1) / R + 1 : 0;
+    key_tiles = n > 0 ? max(1, span_of<TK>(p, length - n, length - 1, length).n) : 0;
   };
-  auto scale_of = [&](int kv, int j) {
-    if (F == kBf16) return 1.f;
-    const int64_t page = bt.table[int64_t(s) * bt.width + (j >> bt.page_shift)];
-    return p.scale[kv][((page * p.H + h) << bt.page_shift) + (j & ((1 << bt.page_shift) - 1))];
-  };
-  float m = -__builtin_huge_valf(), den = 0.f, acc[2] = {0.f, 0.f};
-  bool any = false;
-  for (int j0 = 0; j0 <= max(v.hi, v.sink - 1); j0 += 64) {
-    if (j0 + 63 < v.lo && j0 >= v.sink) continue;
-    const int j = j0 + lane;
-    const bool in = (j <= v.hi && j >= v.lo) || j < v.sink;
-    const uint8_t* k = in ? address(0, j) : nullptr;
-    float x = -__builtin_huge_valf();
-    if (k) {
-      float dot = 0.f;
-      for (int d = 0; d < D; ++d) dot = fmaf(bf16_bits_to_f32(q[d]), element<F>(k, d), dot);
-      x = dot * scale_of(0, j) * p.scale_log2;
+  int z = 1 << 30;
+  if (p.target) {
+    int64_t sum = 0;
+    for (int s = tid; s < S; s += kNT) {
+      int rt, kt;
+      sizes(s, rt, kt);
+      sum += int64_t(rt) * kt;
     }
-    const uint64_t seen = __builtin_amdgcn_ballot_w64(k != nullptr);
-    if (!seen) continue;
-    any = true;
-    float top = x;
-    for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off));
-    const float mn = fmaxf(m, top), ms = mn == -__builtin_huge_valf() ? 0.f : mn;
-    const float alpha = fast_exp2(m - ms);
-    const float e = k ? fast_exp2(x - ms) : 0.f;
-    float sum = e;
+#pragma unroll
     for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
-    den = den * alpha + sum;
-    m = mn;
-    acc[0] *= alpha;
-    acc[1] *= alpha;
-    for (int r = 0; r < 64; ++r) {
-      if (!((seen >> r) & 1)) continue;
-      const float w = __shfl(e, r) * scale_of(1, j0 + r);
-      const uint8_t* vr = address(1, j0 + r);
+    if (lane == 0) s_total[wave] = sum;
+    __syncthreads();
+    sum = 0;
 #pragma unroll
-      for (int t = 0; t < D / 64; ++t) acc[t] = fmaf(w, element<F>(vr, lane + 64 * t), acc[t]);
-    }
+    for (int w = 0; w < kWaves; ++w) sum += s_total[w];
+    z = int(min(int64_t(1) << 30, max(int64_t(p.min_tiles), (sum + p.target - 1) / p.target)));
+    __syncthreads();
   }
+  int64_t base = 0;
+  for (int s0 = 0; s0 < S; s0 += kNT) {
+    const int s = s0 + tid;
+    int rt = 0, parts = 1;
+    if (s < S) {
+      int kt;
+      sizes(s, rt, kt);
+      if (rt) parts = (kt - 1) / z + 1;
+    }
+    const int64_t mine = int64_t(rt) * parts;
+    int64_t end = mine;  // inclusive sum over the wave
 #pragma unroll
-  for (int t = 0; t < D / 64; ++t)
-    p.out[(row * heads + hq) * D + lane + 64 * t] = f32_to_bf16_bits(any ? acc[t] / den : 0.f);
+    for (int off = 1; off < 64; off <<= 1) {
+      const int64_t x = __shfl_up(end, off);
+      if (lane >= off) end += x;
+    }
+    if (lane == 63) s_total[wave] = end;
+    __syncthreads();
+    int64_t all = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      if (w == wave) end += all + base;
+      all += s_total[w];
+    }
+    if (id >= end - mine && id < end) {
+      const int k = int(id - (end - mine));
+      s_found[0] = s;
+      s_found[1] = p.causal ? rt - 1 - k / parts : k / parts;  // the longest first
+      s_found[2] = k % parts;
+      s_found[3] = parts;
+    }
+    __syncthreads();
+    base += all;
+    if (id < base) break;
+  }
+  if (id >= base) return false;
+  it.s = __builtin_amdgcn_readfirstlane(s_found[0]);
+  it.off = __builtin_amdgcn_readfirstlane(entry_offset(p, it.s));
+  it.n = __builtin_amdgcn_readfirstlane(entry_offset(p, it.s + 1)) - it.off;
+  it.length = __builtin_amdgcn_readfirstlane(entry_length(p, it.s));
+  it.r0 = __builtin_amdgcn_readfirstlane(s_found[1]) * R;
+  it.rows = min(R, it.n * p.G - it.r0);
+  it.part = __builtin_amdgcn_readfirstlane(s_found[2]);
+  it.parts = __builtin_amdgcn_readfirstlane(s_found[3]);
+  return true;
 }
 
+// ---- where the keys lie -----------------------------------------------------
+
+// The pages of a key tile's groups of 16 rows (a page holds at least 16), and
+// a bit for each group that has one.
+template <int TK>
+struct TilePages {
+  int page[TK / 16];
+  uint32_t valid;
+};
+
+constexpr uint32_t kAllGroups = 0xFu;
+
+__device__ __forceinline__ int pick(bool second, int a, int b) { return second ? b : a; }
+
+// K and V rows of one (sequence, head): in a cache, rows of kRowBytes that
+// both operands (and their scales) have at the same index; or plain, at strides
+// of their own.
+template <int D, int F, bool PAGED>
+struct Keys {
+  static constexpr uint32_t kRowBytes = D * kElemBytes<F>;
+  const uint8_t* base[2];
+  const float* scale[2];
+  const int32_t* table;
+  uint32_t st[2];             // plain: bytes between rows
+  int shift, pages, H, h, last;  // last: the last key
+
+  __device__ __forceinline__ Keys(const PagedParams& p, const Item& it, int head) {
+    shift = p.batch.page_shift;
+    pages = p.batch.pages;
+    H = p.H;
+    h = head;
+    last = it.length - 1;
+    table = PAGED ? p.batch.table + int64_t(it.s) * p.batch.width : nullptr;
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      base[kv] = p.store[kv] + (PAGED ? 0 : int64_t(h) * p.sh[kv] + int64_t(it.s) * p.sb[kv]);
+      scale[kv] = p.scale[kv];
+      st[kv] = PAGED ? kRowBytes : uint32_t(p.st[kv]);
+    }
+  }
+
+  // Through the scalar cache.  `tile` is uniform; groups past the last key
+  // take its page.
+  template <int TK>
+  __device__ __forceinline__ TilePages<TK> pages_of(int tile) const {
+    TilePages<TK> t;
+    t.valid = kAllGroups;
+    if constexpr (PAGED) {
+      typedef const int32_t __attribute__((address_space(4)))* scalar_ptr;
+      const scalar_ptr tab = (scalar_ptr)(uintptr_t)table;
+      t.valid = 0;
+#pragma unroll
+      for (int g = 0; g < TK / 16; ++g) {
+        const int page = tab[min(tile * TK + 16 * g, last) >> shift];
+        const bool ok = uint32_t(page) < uint32_t(pages);
+        t.page[g] = ok ? page : 0;
+        t.valid |= ok ? 1u << g : 0u;
+      }
+      if constexpr (TK == 32) t.valid |= t.valid << 2;
+    }
+    return t;
+  }
+
+  // Index in the cache of position pos, which lies in `page` (uniform).  The
+  // rows of a group of 16 follow one another, those past the last key too.
+  __device__ __forceinline__ int64_t row(int page, int pos) const {
+    return ((int64_t(page) * H + h) << shift) + (pos & ((1 << shift) - 1));
+  }
+};
+
+// ---- codes ------------------------------------------------------------------
+
+typedef const u32x4 __attribute__((address_space(1)))* global_chunk_ptr;
+
+__device__ __forceinline__ u32x4 load_chunk(const uint8_t* p) { return *(global_chunk_ptr)(uintptr_t)p; }
+
+// Eight codes as BF16 (exact: at most 8 significant bits).
+template <int F>
+__device__ __forceinline__ u32x4 codes_to_bf16(uint32_t lo, uint32_t hi) {
+  u32x4 o;
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    const uint32_t c = w ? hi : lo;
+    if constexpr (F == kInt8) {
+      float v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = float(int32_t(c << (24 - 8 * i)) >> 24);
+      o[2 * w] = pack_bf16x2(v[0], v[1]);
+      o[2 * w + 1] = pack_bf16x2(v[2], v[3]);
+    } else {
+      o[2 * w] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.f, false));
+      o[2 * w + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.f, true));
+    }
+  }
+  return o;
+}
+
+// LDS image of a key tile of TK rows: K then V, BF16, in TileLayout's order.
+template <int D, int TK>
+struct TileImage {
+  static constexpr int kElems = TK * D;
+  static constexpr int CPR = D / 8;
+  __device__ static __forceinline__ void put(uint16_t* slot, int kv, int row, int chunk, const u32x4& x) {
+    const int at = kv ? kElems + TileLayout<D>::v_offset(row, chunk) : TileLayout<D>::k_offset(row, chunk);
+    *reinterpret_cast<u32x4*>(slot + at) = x;
+  }
+  // This lane's K operand of half t, k-step ks.
+  __device__ static __forceinline__ u32x4 k(const uint16_t* slot, int col, int hh, int t, int ks) {
+    return *reinterpret_cast<const u32x4*>(slot + (32 * t + col) * D + (TileLayout<D>::k_lane_xor(col, hh) ^ (16 * ks)));
+  }
+  // This lane's V^T operand (FragLane's addresses): feature 32 dt + col, keys
+  // 32 t + 16 c4 + 4 hh + {0..3, 8..11}.
+  __device__ static __forceinline__ u32x4 v(const uint16_t* slot, int col, int hh, int t, int c4, int dt) {
+    const int chunk = hh * 4 * CPR + 4 * ((col >> 2) & 3) + 2 * (col >> 4) + ((col & 3) >> 1);
+    const uint32_t lane = lds_address(slot) + uint32_t(2 * (kElems + 8 * chunk + 4 * (col & 1)));
+    const uint32_t a = lane + uint32_t(64 * CPR * (8 * t + 4 * c4) + 256 * dt);
+    const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SOL_LDS i16x4*)(uintptr_t)a);
+    const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SOL_LDS i16x4*)(uintptr_t)(a + 128u * CPR));
+    const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
+    const u32x4 r = {x[0], x[1], y[0], y[1]};
+    return r;
+  }
+};
+
+// ---- the softmax and P V of 32 keys -----------------------------------------
+
+// Bit 15 of every 16-bit half that is an infinity or a NaN.
+__device__ __forceinline__ uint32_t nonfinite(uint32_t x) { return ((x & 0x7F807F80u) + 0x00800080u) & 0x80008000u; }
+
+// Adds V's elements that are not finite, of half t of a tile, to the sums of the
+// queries that see their keys.  (A product with P = 0 must not spread them to
+// the others, so the matrix cores take zeros for them.)  Rare: a loop over the
+// keys, written for few registers; the sums are added to in place.
+template <int D, int TK>
+__device__ __forceinline__ void add_nonfinite(State<D>& st, const uint16_t* slot, int t, int hh, uint32_t seen) {
+  using Image = TileImage<D, TK>;
+  // The adds below are inline assembly, before which the compiler does not keep
+  // the distance that a vector instruction needs from the matrix instruction
+  // whose result it reads (19 wait states at most).
+#pragma unroll
+  for (int dt = 0; dt < Shape<D>::DT; ++dt) asm volatile("s_nop 15\n\ts_nop 7" : "+v"(st.acc[dt]));
+  // Key r is score element 4 (r / 8) + r % 4 of lane half (r / 4) % 2.
+  const auto both = __builtin_amdgcn_permlane32_swap(seen, seen, false, false);
+#pragma unroll 1
+  for (int r = 0; r < 32; ++r) {
+    const bool on = (((r & 4) ? both[1] : both[0]) >> (4 * (r >> 3) + (r & 3))) & 1u;
+#pragma unroll
+    for (int dt = 0; dt < Shape<D>::DT; ++dt)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int at = Image::kElems + TileLayout<D>::v_offset(32 * t + r, 4 * dt + q) + 4 * hh;
+        const u32x2 x = *reinterpret_cast<const u32x2*>(slot + at);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t b = (i & 1) ? x[i >> 1] >> 16 : x[i >> 1] & 0xFFFFu;
+          const float add = on && (b & 0x7F80u) == 0x7F80u ? bf16_bits_to_f32(b) : 0.f;
+          asm volatile("v_add_f32 %0, %0, %1" : "+v"(st.acc[dt][4 * q + i]) : "v"(add));
+        }
+      }
+  }
+}
+
+// The rows of lane (col, hh): what its query sees, and whether it saw a key.
+struct LaneRow {
+  Visible v;
+  bool any;
+};
+
+// Sixteen per-key factors of this lane's score elements of a half (key 8 (e /
+// 4) + 4 hh + e % 4), from LDS.
+__device__ __forceinline__ f32x16 key_factors(const float* half, int hh) {
+  f32x16 f;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const f32x4 x = *reinterpret_cast<const f32x4*>(half + 8 * q + 4 * hh);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[4 * q + i] = x[i];
+  }
+  return f;
+}
+
+// Online softmax of raw scores s (half t of the tile in `slot`, keys from j0 on)
+// and O^T += V^T P^T,
+// hidden keys taking no part, whatever their score, value and scale hold.
+// `valid`: bits of the half's two groups of 16 rows that have a page.  scales:
+// the half's K scales in LDS (V's TK floats on), or null.
+template <int D, int TK>
+__device__ __forceinline__ void attend_masked(State<D>& st, LaneRow& row, f32x16 s, const uint16_t* slot, int t, int j0,
+                                              uint32_t valid, int col, int hh, float c, const float* scales) {
+  if (scales) {
+    const f32x16 sk = key_factors(scales, hh);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[e] *= sk[e];
+  }
+  uint32_t seen = 0;
+  const int a = j0 + 4 * hh;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    const int j = a + 8 * (e >> 2) + (e & 3);
+    const bool in = (((j <= row.v.hi) & (j >= row.v.lo)) | (j < row.v.sink)) & (((valid >> (e >> 3)) & 1u) != 0);
+    s[e] = in ? s[e] : kNegInf;
+    seen |= in ? 1u << e : 0u;
+  }
+  row.any |= seen != 0;
+  float mx = s[0];
+#pragma unroll
+  for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
+  mx = pair_max(mx) * c;
+  if (__builtin_amdgcn_ballot_w64(mx > st.m)) {
+    const float mnew = fmaxf(st.m, mx);
+    const float alpha = mnew == kNegInf ? 1.f : fast_exp2(st.m - mnew);
+    st.m = mnew;
+    st.den *= alpha;
+    rescale_acc<D>(st, alpha);
+  }
+  const float neg_m = st.m == kNegInf ? 0.f : -st.m;
+  float sum = 0.f;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) {
+    s[e] = fast_exp2(fmaf(s[e], c, neg_m));
+    sum += s[e];
+  }
+  st.den += sum;
+  if (scales) {
+    const f32x16 sv = key_factors(scales + TK, hh);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[e] = (seen >> e) & 1u ? s[e] * sv[e] : 0.f;
+  }
+  const bf16x8 pb[2] = {pack8(s, 0), pack8(s, 8)};
+  // Scheduled apart from the scores: V's operands are not held meanwhile.
+  chunk_end();
+  u32x4 v[2][Shape<D>::DT];
+  uint32_t bad = 0;
+#pragma unroll
+  for (int c4 = 0; c4 < 2; ++c4)
+#pragma unroll
+    for (int dt = 0; dt < Shape<D>::DT; ++dt) {
+      v[c4][dt] = TileImage<D, TK>::v(slot, col, hh, t, c4, dt);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bad |= nonfinite(v[c4][dt][i]);
+    }
+  const bool some = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
+  if (some) {
+#pragma unroll
+    for (int c4 = 0; c4 < 2; ++c4)
+#pragma unroll
+      for (int dt = 0; dt < Shape<D>::DT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[c4][dt][i] &= ~((nonfinite(v[c4][dt][i]) >> 15) * 0xFFFFu);
+  }
+#pragma unroll
+  for (int c4 = 0; c4 < 2; ++c4)
+#pragma unroll
+    for (int dt = 0; dt < Shape<D>::DT; ++dt) st.acc[dt] = mfma32x32x16(as_bf16x8(v[c4][dt]), pb[c4], st.acc[dt]);
+  if (some) add_nonfinite<D, TK>(st, slot, t, hh, seen);
+}
+
+// ---- results ----------------------------------------------------------------
+
+// Partial states of split tiles: per workgroup (record) a header, and per row
+// D sums, the maximum, the denominator and whether a key was seen.
+struct Header {
+  int parts, off, r0, rows;  // parts 0: nothing to join at this record
+};
+
+template <int D>
+constexpr int kRecordRow = D + 4;
+
+__device__ __forceinline__ Header* headers(const PagedParams& p) { return static_cast<Header*>(p.workspace); }
+
+template <int D, int R>
+__device__ __forceinline__ float* record(const PagedParams& p, int64_t i) {
+  return reinterpret_cast<float*>(static_cast<Header*>(p.workspace) + p.records) + i * R * kRecordRow<D>;
+}
+
+// Element offset of row r (of a sequence's n G) of the output.
+template <int D>
+__device__ __forceinline__ int64_t output_row(const PagedParams& p, int off, int r, int h) {
+  return ((int64_t(off) + r / p.G) * (p.H * p.G) + h * p.G + r % p.G) * D;
+}
+
+// Four features of a finished row.
+__device__ __forceinline__ void store4(uint16_t* out, const f32x4& x, float den, bool any) {
+  const float inv = __fdiv_rn(1.f, den);
+  u32x2 o;
+  o[0] = pack_bf16x2(quotient(x[0], den, inv), quotient(x[1], den, inv));
+  o[1] = pack_bf16x2(quotient(x[2], den, inv), quotient(x[3], den, inv));
+  if (!any) o[0] = o[1] = 0u;
+  *reinterpret_cast<u32x2*>(out) = o;
+}
+
+// Joins the parts of split tiles: m = max_s m_s, O = sum_s 2^(m_s - m) acc_s /
+// sum_s 2^(m_s - m) den_s over the parts in ascending order.  One workgroup per
+// record; those that begin a split tile work, a thread per row and 4 features.
+template <int D, int R>
+__global__ __launch_bounds__(kNT) void merge_kernel(PagedParams p) {
+  Header hd = headers(p)[blockIdx.x];
+  if (hd.parts <= 1) return;
+  constexpr int kChunks = D / 4;
+  const int h = blockIdx.x % p.H;
+  // Offsets that do not ascend can name more parts than the launch has.
+  hd.parts = min(hd.parts, int((p.records - 1 - blockIdx.x) / p.H) + 1);
+  for (int i = threadIdx.x; i < hd.rows * kChunks; i += kNT) {
+    const int r = i / kChunks, c = i % kChunks;
+    auto row = [&](int s) { return record<D, R>(p, int64_t(blockIdx.x) + int64_t(s) * p.H) + r * kRecordRow<D>; };
+    float m = kNegInf;
+    for (int s = 0; s < hd.parts; ++s) m = fmaxf(m, row(s)[D]);
+    float den = 0.f;
+    bool any = false;
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < hd.parts; ++s) {
+      const f32x4 tail = *reinterpret_cast<const f32x4*>(row(s) + D);
+      const f32x4 x = *reinterpret_cast<const f32x4*>(row(s) + 4 * c);
+      any |= tail[2] != 0.f;
+      if (tail[0] == kNegInf && tail[1] == 0.f) continue;
+      const float w = tail[0] == kNegInf ? 1.f : fast_exp2(tail[0] - m);
+      den += w * tail[1];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[k] += w * x[k];
+    }
+    store4(p.out + output_row<D>(p, hd.off, hd.r0 + r, h) + 4 * c, o, den, any);
+  }
+}
+
+// ---- few rows ---------------------------------------------------------------
+
+// Keeps a wave's LDS writes and reads of its own slot in program order (the
+// hardware runs them in order; nothing is emitted).
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// A key tile on its way from memory to LDS, in registers.
+template <int D, int F, bool PAGED, int TK>
+struct RawTile {
+  static constexpr int kRowLanes = F == kBf16 ? D / 8 : D / 16;  // 16 bytes each
+  static constexpr int kRows = 64 / kRowLanes;                   // rows per load
+  static constexpr int kLoads = TK / kRows;
+  static_assert(kRows <= 16, "the rows of a load lie in one page");
+  u32x4 x[2][kLoads];
+  float scale[2];
+
+  __device__ __forceinline__ void load(const Keys<D, F, PAGED>& keys, int t, const TilePages<TK>& pages, int lane) {
+    if constexpr (PAGED) {
+      const uint32_t off = uint32_t(lane / kRowLanes) * keys.kRowBytes + 16u * (lane % kRowLanes);
+      int64_t row[TK / 16];
+#pragma unroll
+      for (int g = 0; g < TK / 16; ++g) row[g] = keys.row(pages.page[g], t * TK + 16 * g);
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+          x[kv][i] = load_chunk(keys.base[kv] + row[kRows * i / 16] * keys.kRowBytes + off + kRows * i % 16 * keys.kRowBytes);
+      if constexpr (F != kBf16) {
+        int64_t at = row[0] + (lane & 15);
+#pragma unroll
+        for (int g = 1; g < TK / 16; ++g) at = (lane % TK) >= 16 * g ? row[g] + (lane & 15) : at;
+        scale[0] = keys.scale[0][at];
+        scale[1] = keys.scale[1][at];
+      }
+    } else {
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+          x[kv][i] = load_chunk(keys.base[kv] + uint64_t(min(t * TK + kRows * i + lane / kRowLanes, keys.last)) * keys.st[kv] +
+                                16 * (lane % kRowLanes));
+    }
+  }
+
+  __device__ __forceinline__ void put(uint16_t* slot, float* scales, int lane) const {
+    using Image = TileImage<D, TK>;
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int row = kRows * i + lane / kRowLanes, c = lane % kRowLanes;
+        if constexpr (F == kBf16) {
+          Image::put(slot, kv, row, c, x[kv][i]);
+        } else {
+          Image::put(slot, kv, row, 2 * c, codes_to_bf16<F>(x[kv][i][0], x[kv][i][1]));
+          Image::put(slot, kv, row, 2 * c + 1, codes_to_bf16<F>(x[kv][i][2], x[kv][i][3]));
+        }
+      }
+      if constexpr (F != kBf16)
+        if (lane < TK) scales[kv * TK + lane] = scale[kv];
+    }
+  }
+};
+
+template <int D, int F, bool PAGED>
+__global__ __launch_bounds__(kNT, 2) void step_kernel(PagedParams p) {
+  using S = Shape<D>;
+  constexpr int R = 32;
+  constexpr int TK = D == 128 ? 32 : 64;      // 16 KB of LDS per wave
+  constexpr int kSets = F == kBf16 ? 1 : 2;   // tiles in flight per wave: 16 KB
+  using Image = TileImage<D, TK>;
+  __shared__ __align__(256) uint16_t s_tile[kWaves][2 * TK * D];
+  __shared__ __align__(16) float s_scale[kWaves][F == kBf16 ? 1 : 2 * TK];
+  __shared__ float s_md[kWaves][3][kWave];
+
+  const int h = blockIdx.x % p.H;
+  Item it;
+  if (!take_item<R, TK>(p, blockIdx.x / p.H, it)) {
+    if (p.records && threadIdx.x == 0) headers(p)[blockIdx.x] = Header{0, 0, 0, 0};
+    return;
+  }
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, hh = lane >> 5;
+
+  // This lane's query, straight into its operand registers.
+  const int pos0 = it.length - it.n;
+  const int r = it.r0 + min(col, it.rows - 1);
+  const int token = r / p.G;
+  const uint16_t* q = p.q + (PAGED ? (it.off + token) * p.q_st : it.s * p.q_sb + token * p.q_st) +
+                      (h * p.G + r % p.G) * p.q_sh;
+  bf16x8 qf[S::KT];
+#pragma unroll
+  for (int ks = 0; ks < S::KT; ++ks) qf[ks] = as_bf16x8(load16(q + 16 * ks + 8 * hh));
+  LaneRow row;
+  row.v = visible(p, pos0 + token, it.length);
+  row.any = false;
+
+  const int first = pos0 + it.r0 / p.G, last = pos0 + (it.r0 + it.rows - 1) / p.G;
+  const Span span = span_of<TK>(p, first, last, it.length);
+  const int t0 = int(int64_t(it.part) * span.n / it.parts), t1 = int(int64_t(it.part + 1) * span.n / it.parts);
+  State<D> st;
+  state_init(st);
+  const Keys<D, F, PAGED> keys(p, it, h);
+  uint16_t* slot = s_tile[wave];
+  float* scales = s_scale[wave];
+  auto at = [&](int i) { return span.tile(min(i, t1 - 1)); };
+
+  auto attend = [&](int tile, uint32_t valid) {
+#pragma unroll 1
+    for (int t = 0; t < TK / 32; ++t) {
+      f32x16 s = zero16();
+#pragma unroll
+      for (int ks = 0; ks < S::KT; ++ks) s = mfma32x32x16(as_bf16x8(Image::k(slot, col, hh, t, ks)), qf[ks], s);
+      chunk_end();
+      attend_masked<D, TK>(st, row, s, slot, t, tile * TK + 32 * t, valid >> (2 * t), col, hh, p.scale_log2,
+                           F == kBf16 ? nullptr : scales + 32 * t);
+    }
+  };
+
+  if (t0 + wave < t1) {
+    RawTile<D, F, PAGED, TK> raw[kSets];
+    uint32_t valid[kSets];
+    TilePages<TK> ahead[kSets];
+    int i = t0 + wave;
+#pragma unroll
+    for (int u = 0; u < kSets; ++u) {
+      const int n = at(i + u * kWaves);
+      const TilePages<TK> pages = keys.template pages_of<TK>(n);
+      valid[u] = pages.valid;
+      raw[u].load(keys, n, pages, lane);
+    }
+#pragma unroll
+    for (int u = 0; u < kSets; ++u) ahead[u] = keys.template pages_of<TK>(at(i + (kSets + u) * kWaves));
+    while (i < t1) {
+#pragma unroll
+      for (int u = 0; u < kSets; ++u) {
+        if (i < t1) {
+          wave_order();
+          raw[u].put(slot, scales, lane);
+          wave_order();
+          const uint32_t now = valid[u];
+          if (i + kSets * kWaves < t1) {
+            raw[u].load(keys, at(i + kSets * kWaves), ahead[u], lane);
+            valid[u] = ahead[u].valid;
+            ahead[u] = keys.template pages_of<TK>(at(i + 2 * kSets * kWaves));
+          }
+          attend(at(i), now);
+        }
+        i += kWaves;
+      }
+    }
+  }
+
+  // Join the four waves' states: each writes its sums over its own tiles.
+  wave_order();
+  f32x4* mine = reinterpret_cast<f32x4*>(slot);
+  constexpr int NC = D / 8;  // groups of 4 features per lane
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const f32x4 x = {st.acc[c / 4][4 * (c % 4)], st.acc[c / 4][4 * (c % 4) + 1], st.acc[c / 4][4 * (c % 4) + 2],
+                     st.acc[c / 4][4 * (c % 4) + 3]};
+    mine[c * kWave + lane] = x;
+  }
+  s_md[wave][0][lane] = st.m;
+  s_md[wave][1][lane] = st.den;
+  s_md[wave][2][lane] = row.any ? 1.f : 0.f;
+  __syncthreads();
+  float m = kNegInf, den = 0.f, w[kWaves], seen = 0.f;
+#pragma unroll
+  for (int g = 0; g < kWaves; ++g) m = fmaxf(m, s_md[g][0][lane]);
+#pragma unroll
+  for (int g = 0; g < kWaves; ++g) {
+    const float mg = s_md[g][0][lane];
+    w[g] = mg == kNegInf ? 1.f : fast_exp2(mg - m);
+    den += w[g] * s_md[g][1][lane];
+    seen += s_md[g][2][lane];
+  }
+  // Both lanes of a pair saw different keys of each tile.
+  den = pair_sum(den);
+  seen = pair_sum(seen);
+  const int64_t rec = blockIdx.x;
+  if (p.records && tid == 0)
+    headers(p)[rec] = Header{it.part == 0 && it.parts > 1 ? it.parts : 0, it.off, it.r0, it.rows};
+  if (col >= it.rows) return;
+#pragma unroll
+  for (int c = wave; c < NC; c += kWaves) {
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int g = 0; g < kWaves; ++g) {
+      const f32x4 x = reinterpret_cast<const f32x4*>(s_tile[g])[c * kWave + lane];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] += w[g] * x[i];
+    }
+    const int feature = 32 * (c / 4) + 8 * (c % 4) + 4 * hh;
+    if (it.parts > 1) {
+      float* row_out = record<D, R>(p, rec) + col * kRecordRow<D>;
+      *reinterpret_cast<f32x4*>(row_out + feature) = o;
+      if (c == 0 && hh == 0) {
+        const f32x4 tail = {m, den, seen, 0.f};
+        *reinterpret_cast<f32x4*>(row_out + D) = tail;
+      }
+    } else {
+      store4(p.out + output_row<D>(p, it.off, r, h) + feature, o, den, seen > 0.f);
+    }
+  }
+}
+
+// ---- many rows --------------------------------------------------------------
+
+// The DMA of a BF16 key tile into an LDS slot, in kRounds rounds per wave of 1
+// KB each: round r of K (then of V) moves rows R0 = r kRoundRows + wave
+// kPieceRows on, all in one group of 16, so its address is one uniform row
+// address and a per-lane offset that is the same in every round (the swizzles
+// repeat).  Plain keys' tail tile repeats the last key instead of reading past
+// it (its lanes' offsets are formed per round); a page's rows past the last key
+// exist.
+template <int D, bool PAGED>
+struct DmaTile {
+  using Source = Keys<D, kBf16, PAGED>;
+  static constexpr int kHalf = 64 * D * 2 / 16 / kNT;
+  static constexpr int kRounds = 2 * kHalf;
+  static constexpr int kRoundRows = kNT * 16 / (2 * D);
+  static constexpr int kPieceRows = kRoundRows / kWaves;
+  uint64_t base[2], off[PAGED ? kHalf : 1];
+  uint32_t lane[2];  // per-lane offsets in a whole tile
+  uint32_t lds, st[2];
+  int pos0, last, l, wave;
+  bool tail;
+
+  __device__ __forceinline__ static int lane_row(int kv, int l) {
+    return kv ? (D == 128 ? 0 : 4 * (l / 32)) + ((l >> 2) & 3) : l / (D / 8);
+  }
+  __device__ __forceinline__ static int lane_byte(int kv, int l, int wave) {
+    const int m = D == 128 ? l : l % 32;
+    return 16 * (kv ? 4 * (m >> 4) + (m & 3)
+                    : (l % (D / 8)) ^ TileLayout<D>::k_swizzle(wave * kPieceRows + l / (D / 8)));
+  }
+
+  __device__ __forceinline__ DmaTile(const Source& keys, const TilePages<64>& pages, int tile, uint32_t dst, int w,
+                                     int lane_id, const uint32_t (&lanes)[2])
+      : l(lane_id), wave(w) {
+    last = keys.last;
+    tail = !PAGED && tile * 64 + 63 > last;
+    pos0 = tile * 64 + w * kPieceRows;
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      base[kv] = reinterpret_cast<uint64_t>(keys.base[kv]);
+      st[kv] = keys.st[kv];
+      lane[kv] = lanes[kv];
+    }
+    if constexpr (PAGED) {
+#pragma unroll
+      for (int r = 0; r < kHalf; ++r) {
+        const int page = D == 128 ? pages.page[r] : pick(w >= 2, pages.page[2 * r], pages.page[2 * r + 1]);
+        off[r] = uint64_t(keys.row(page, pos0 + r * kRoundRows)) * Source::kRowBytes;
+      }
+    }
+    lds = dst + uint32_t(w) * 1024u;
+  }
+  // This lane's offsets in whole tiles.
+  __device__ __forceinline__ static void lane_offsets(const Source& keys, int w, int lane_id, uint32_t (&lanes)[2]) {
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) lanes[kv] = lane_row(kv, lane_id) * keys.st[kv] + lane_byte(kv, lane_id, w);
+  }
+  __device__ __forceinline__ void round(int i) const {
+    const int kv = i / kHalf, r = i % kHalf;
+    const uint32_t dst = lds + uint32_t(kv * 64 * D * 2 + r * kNT * 16);
+    if constexpr (PAGED) {
+      dma16(base[kv] + off[r] + round_offset(0u), lane[kv], dst);
+    } else {
+      const int pos = pos0 + r * kRoundRows, first = min(pos, last);
+      uint32_t at = lane[kv];
+      if (tail) at = uint32_t(min(pos + lane_row(kv, fresh(l)), last) - first) * st[kv] + lane_byte(kv, fresh(l), wave);
+      dma16(base[kv] + uint64_t(uint32_t(first)) * st[kv] + round_offset(0u), at, dst);
+    }
+  }
+  __device__ __forceinline__ void all() const {
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) round(r);
+  }
+  template <int N>
+  __device__ __forceinline__ void after_step(int k) const {
+#pragma unroll
+    for (int r = k * kRounds / N; r < (k + 1) * kRounds / N; ++r) round(r);
+  }
+};
+
+// Nothing to move beside a tile's products.
+struct NoStep {
+  __device__ __forceinline__ void all() const {}
+  template <int N>
+  __device__ __forceinline__ void after_step(int) const {}
+};
+
+// An 8-bit key tile on its way, in the workgroup's registers: loaded while
+// the tile before it is attended, converted into its slot afterwards.
 template <int D, int F>
-void launch_rows(const PagedParams& p, hipStream_t stream) {
-  const int64_t rows = p.batch.table ? p.batch.rows : int64_t(p.batch.S) * p.Tq;
-  hipLaunchKernelGGL((attend_rows_kernel<D, F>), dim3(unsigned(rows * p.H * p.G)), dim3(64), 0, stream, p);
+struct CodeTile {
+  static constexpr int kRowLanes = D / 16;
+  static constexpr int kLoads = 64 * kRowLanes / kNT;
+  u32x4 x[2][kLoads];
+  float scale;
+
+  __device__ __forceinline__ void load(const Keys<D, F, true>& keys, const TilePages<64>& pages, int tile, int wave, int l) {
+    const uint32_t off = uint32_t(l / kRowLanes) * keys.kRowBytes + 16u * (l % kRowLanes);
+    // A wave's 64 chunks are 8 (D = 128) or 16 rows of one group.
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int page = D == 128 ? pick(wave >= 2, pages.page[2 * i], pages.page[2 * i + 1])
+                                : pick(wave >= 2, pick(wave & 1, pages.page[0], pages.page[1]),
+                                       pick(wave & 1, pages.page[2], pages.page[3]));
+      const int64_t at = keys.row(page, tile * 64 + (i * kNT + wave * kWave) / kRowLanes) * keys.kRowBytes;
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) x[kv][i] = load_chunk(keys.base[kv] + at + off);
+    }
+    if (wave < 2) {  // wave 0 the keys' scales, wave 1 the values'
+      const int page = pick(l >= 32, pick(l & 16, pages.page[0], pages.page[1]), pick(l & 16, pages.page[2], pages.page[3]));
+      scale = (wave ? keys.scale[1] : keys.scale[0])[keys.row(page, tile * 64 + l)];
+    }
+  }
+  __device__ __forceinline__ void put(uint16_t* slot, float* scales, int tid) const {
+    using Image = TileImage<D, 64>;
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const int row = (i * kNT + tid) / kRowLanes, c = tid % kRowLanes;
+        Image::put(slot, kv, row, 2 * c, codes_to_bf16<F>(x[kv][i][0], x[kv][i][1]));
+        Image::put(slot, kv, row, 2 * c + 1, codes_to_bf16<F>(x[kv][i][2], x[kv][i][3]));
+      }
+    if (tid < 128) scales[tid] = scale;
+  }
+};
+
+// FastHalf with the values' scales (SCALED): the probabilities are multiplied
+// by them before they are packed.
+template <int D, bool SCALED>
+struct WideHalf : FastHalf<D> {
+  template <int N>
+  __device__ __forceinline__ void step(int k, State<D>& st, float c, const float* sv, int hh) {
+#pragma unroll
+    for (int i = k * 8 / N; i < (k + 1) * 8 / N; ++i) {
+      if (SCALED && i == 5) scale(this->s, sv, hh);
+      this->stage(i, st, c);
+    }
+  }
+  __device__ static __forceinline__ void scale(f32x16& x, const float* factors, int hh) {
+    const f32x16 f = key_factors(factors, hh);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) x[e] *= f[e];
+  }
+  template <typename Raw>
+  __device__ __forceinline__ void finish(State<D>& st, float c, const float* sv, int hh, Raw raw) {
+    if (this->redo) {
+      HalfSoftmax<D> full;
+      full.s = raw();
+#pragma unroll
+      for (int i = 0; i < 6; ++i) full.stage(i, st, c);
+      if (SCALED) scale(full.s, sv, hh);
+      full.stage(6, st, c);
+      full.stage(7, st, c);
+      if (full.rescale) rescale_acc<D>(st, full.alpha);
+      this->pw[0] = full.pw[0];
+      this->pw[1] = full.pw[1];
+    }
+  }
+};
+
+// A key tile that every row of the wave sees whole, pipelined over its two
+// halves inside the wave so that the softmax's vector work runs beside the
+// matrix products:
+//   chunks 0 .. KT - 1  half 0's scores; half 1's K reads
+//   next KT             half 1's scores; half 0's softmax; half 0's V^T reads
+//   next 2 DT           half 0's P V; half 1's softmax; half 1's V^T reads
+//   next 2 DT           half 1's P V
+// The next tile's DMA rounds are spread over the score chunks.
+template <int D, bool SCALED, typename Refill>
+__device__ __forceinline__ void wide_tile(State<D>& st, const uint16_t* buf, const float* scales,
+                                          const bf16x8 (&qf)[Shape<D>::KT], int col, int hh, float c,
+                                          const Refill& refill) {
+  constexpr int KT = Shape<D>::KT, DT = Shape<D>::DT;
+  const FragLane<D> fl(fresh(col), fresh(hh));
+  const uint32_t vbase = fl.v_base(buf);
+  u32x4 k0[KT], k1[KT];
+#pragma unroll
+  for (int ks = 0; ks < KT; ++ks) k0[ks] = fl.k(buf, 0, ks);
+  auto raw = [&](int t) {
+    const FragLane<D> fr(fresh(col), fresh(hh));
+    f32x16 s = zero16();
+#pragma unroll
+    for (int ks = 0; ks < KT; ++ks) s = mfma32x32x16(as_bf16x8(fr.k(buf, t, ks)), qf[ks], s);
+    if (SCALED) WideHalf<D, SCALED>::scale(s, scales + 32 * t, hh);
+    return s;
+  };
+  WideHalf<D, SCALED> h0, h1;
+  h0.s = zero16();
+  chunk_end();
+#pragma unroll
+  for (int ks = 0; ks < KT; ++ks) {
+    h0.s = mfma32x32x16(as_bf16x8(k0[ks]), qf[ks], h0.s);
+    k1[ks] = fl.k(buf, 1, ks);
+    refill.template after_step<2 * KT>(ks);
+    chunk_end();
+  }
+  if (SCALED) h0.scale(h0.s, scales, hh);
+  u32x4 va[2][DT], vb[2][DT];
+  h1.s = zero16();
+#pragma unroll
+  for (int ks = 0; ks < KT; ++ks) {
+    h1.s = mfma32x32x16(as_bf16x8(k1[ks]), qf[ks], h1.s);
+    h0.template step<KT>(ks, st, c, scales + 64, hh);
+    if (ks >= KT / 2) {
+#pragma unroll
+      for (int f = 2 * (ks - KT / 2); f < 2 * (ks - KT / 2) + 2; ++f) va[f / DT][f % DT] = fl.v(vbase, 0, f / DT, f % DT);
+    }
+    refill.template after_step<2 * KT>(KT + ks);
+    chunk_end();
+  }
+  h0.finish(st, c, scales + 64, hh, [&] { return raw(0); });
+  if (SCALED) h1.scale(h1.s, scales + 32, hh);
+#pragma unroll
+  for (int f = 0; f < 2 * DT; ++f) {
+    const int c4 = f / DT, dt = f % DT;
+    st.acc[dt] = mfma32x32x16(as_bf16x8(va[c4][dt]), h0.pb(c4), st.acc[dt]);
+    vb[c4][dt] = fl.v(vbase, 1, c4, dt);
+    h1.template step<2 * DT>(f, st, c, scales + 96, hh);
+    chunk_end();
+  }
+  h1.finish(st, c, scales + 96, hh, [&] { return raw(1); });
+#pragma unroll
+  for (int f = 0; f < 2 * DT; ++f) {
+    const int c4 = f / DT, dt = f % DT;
+    st.acc[dt] = mfma32x32x16(as_bf16x8(vb[c4][dt]), h1.pb(c4), st.acc[dt]);
+  }
+}
+
+template <int D, int F, bool PAGED>
+__global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
+  using S = Shape<D>;
+  constexpr int R = 128, TK = 64;
+  constexpr bool SCALED = F != kBf16;
+  __shared__ __align__(256) uint16_t ring[2][S::TILE];
+  __shared__ __align__(16) float s_scale[2][SCALED ? 2 * TK : 1];
+
+  const int h = blockIdx.x % p.H;
+  Item it;
+  if (!take_item<R, TK>(p, blockIdx.x / p.H, it)) {
+    if (p.records && threadIdx.x == 0) headers(p)[blockIdx.x] = Header{0, 0, 0, 0};
+    return;
+  }
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, hh = lane >> 5;
+  const int wrows = min(32, it.rows - 32 * wave);  // this wave's rows (none: it only moves tiles)
+
+  const int pos0 = it.length - it.n;
+  const int r = it.r0 + min(32 * wave + col, it.rows - 1);
+  const int token = r / p.G;
+  const uint16_t* q = p.q + (PAGED ? (it.off + token) * p.q_st : it.s * p.q_sb + token * p.q_st) +
+                      (h * p.G + r % p.G) * p.q_sh;
+  bf16x8 qf[S::KT];
+#pragma unroll
+  for (int ks = 0; ks < S::KT; ++ks) qf[ks] = as_bf16x8(load16(q + 16 * ks + 8 * hh));
+  LaneRow row;
+  row.v = visible(p, pos0 + token, it.length);
+  row.any = false;
+
+  const Span span = span_of<TK>(p, pos0 + it.r0 / p.G, pos0 + (it.r0 + it.rows - 1) / p.G, it.length);
+  const int t0 = int(int64_t(it.part) * span.n / it.parts), t1 = int(int64_t(it.part + 1) * span.n / it.parts);
+  const Visible va = visible(p, pos0 + (it.r0 + 32 * wave) / p.G, it.length);
+  const Visible vb = visible(p, pos0 + (it.r0 + 32 * wave + max(wrows, 1) - 1) / p.G, it.length);
+
+  State<D> st;
+  state_init(st);
+  const Keys<D, F, PAGED> keys(p, it, h);
+  auto at = [&](int i) { return span.tile(min(i, t1 - 1)); };
+  const uint32_t ring_lds = lds_address(ring[0]);
+
+  auto attend = [&](int tile, uint32_t valid, const uint16_t* buf, const float* scales, const auto& refill) {
+    const int a = tile * TK, b = a + TK - 1;
+    if (wrows <= 0 || ((a > vb.hi || b < va.lo) && a >= vb.sink)) {
+      refill.all();  // hidden from every row of the wave
+    } else if (valid == kAllGroups && b <= va.hi && (a >= vb.lo || b < va.sink)) {
+      row.any = true;
+      wide_tile<D, SCALED>(st, buf, scales, qf, col, hh, p.scale_log2, refill);
+    } else {
+      refill.all();
+#pragma unroll 1
+      for (int t = 0; t < 2; ++t) {
+        f32x16 s = zero16();
+#pragma unroll
+        for (int ks = 0; ks < S::KT; ++ks)
+          s = mfma32x32x16(as_bf16x8(TileImage<D, TK>::k(buf, col, hh, t, ks)), qf[ks], s);
+        chunk_end();
+        attend_masked<D, TK>(st, row, s, buf, t, a + 32 * t, valid >> (2 * t), col, hh, p.scale_log2,
+                             SCALED ? scales + 32 * t : nullptr);
+      }
+    }
+  };
+
+  if (t0 < t1) {
+    TilePages<TK> now = keys.template pages_of<TK>(at(t0)), next = keys.template pages_of<TK>(at(t0 + 1));
+    if constexpr (!SCALED) {
+      uint32_t lanes[2];
+      DmaTile<D, PAGED>::lane_offsets(keys, wave, lane, lanes);
+      DmaTile<D, PAGED>(keys, now, at(t0), ring_lds, wave, lane, lanes).all();
+      for (int i = t0; i < t1; ++i) {
+        wait_vmcnt<0>();
+        lds_barrier();
+        const int slot = (i - t0) & 1;
+        // Past the last tile that tile again, into the slot nobody reads.
+        const DmaTile<D, PAGED> refill(keys, next, at(i + 1), ring_lds + uint32_t((slot ^ 1) * S::TILE * 2), wave, lane,
+                                       lanes);
+        const uint32_t valid = now.valid;
+        now = next;
+        next = keys.template pages_of<TK>(at(i + 2));
+        attend(at(i), valid, ring[slot], nullptr, refill);
+      }
+      wait_vmcnt<0>();
+    } else {
+      CodeTile<D, F> code;
+      code.load(keys, now, at(t0), wave, lane);
+      code.put(ring[0], s_scale[0], tid);
+      for (int i = t0; i < t1; ++i) {
+        lds_barrier();
+        const int slot = (i - t0) & 1;
+        code.load(keys, next, at(i + 1), wave, lane);
+        const uint32_t valid = now.valid;
+        now = next;
+        next = keys.template pages_of<TK>(at(i + 2));
+        attend(at(i), valid, ring[slot], s_scale[slot], NoStep{});
+        code.put(ring[slot ^ 1], s_scale[slot ^ 1], tid);
+      }
+    }
+  }
+
+  const float den = pair_sum(st.den), seen = pair_sum(row.any ? 1.f : 0.f);
+  if (p.records && tid == 0)
+    headers(p)[blockIdx.x] = Header{it.part == 0 && it.parts > 1 ? it.parts : 0, it.off, it.r0, it.rows};
+  if (col >= wrows) return;
+  float* row_out = record<D, R>(p, blockIdx.x) + (32 * wave + col) * kRecordRow<D>;
+  uint16_t* out = p.out + output_row<D>(p, it.off, r, h);
+#pragma unroll
+  for (int c = 0; c < D / 8; ++c) {
+    const f32x4 o = {st.acc[c / 4][4 * (c % 4)], st.acc[c / 4][4 * (c % 4) + 1], st.acc[c / 4][4 * (c % 4) + 2],
+                     st.acc[c / 4][4 * (c % 4) + 3]};
+    const int feature = 32 * (c / 4) + 8 * (c % 4) + 4 * hh;
+    if (it.parts > 1)
+      *reinterpret_cast<f32x4*>(row_out + feature) = o;
+    else
+      store4(out + feature, o, den, seen > 0.f);
+  }
+  if (it.parts > 1 && hh == 0) {
+    const f32x4 tail = {st.m, den, seen, 0.f};
+    *reinterpret_cast<f32x4*>(row_out + D) = tail;
+  }
+}
+
+// ---- launches ---------------------------------------------------------------
+
+template <int D, int F, bool PAGED>
+void launch_variant(const PagedParams& p, const PagedSize& size, hipStream_t stream) {
+  const dim3 grid(unsigned(size.grid));
+  if (size.step)
+    hipLaunchKernelGGL((step_kernel<D, F, PAGED>), grid, dim3(kNT), 0, stream, p);
+  else
+    hipLaunchKernelGGL((wide_kernel<D, F, PAGED>), grid, dim3(kNT), 0, stream, p);
+  if (size.target) {
+    if (size.step)
+      hipLaunchKernelGGL((merge_kernel<D, 32>), grid, dim3(kNT), 0, stream, p);
+    else
+      hipLaunchKernelGGL((merge_kernel<D, 128>), grid, dim3(kNT), 0, stream, p);
+  }
+}
+
+template <int D>
+void launch_format(const PagedParams& p, const PagedSize& size, int format, hipStream_t stream) {
+  if (!p.batch.table) launch_variant<D, kBf16, false>(p, size, stream);
+  else if (format == kBf16) launch_variant<D, kBf16, true>(p, size, stream);
+  else if (format == kInt8) launch_variant<D, kInt8, true>(p, size, stream);
+  else launch_variant<D, kFp8, true>(p, size, stream);
 }
 
 }  // namespace
 
-hipError_t launch_paged(const PagedParams& p, int D, int format, hipStream_t stream) {
-  if (D == 128) {
-    if (format == kBf16) launch_rows<128, kBf16>(p, stream);
-    else if (format == kInt8) launch_rows<128, kInt8>(p, stream);
-    else launch_rows<128, kFp8>(p, stream);
-  } else {
-    if (format == kBf16) launch_rows<64, kBf16>(p, stream);
-    else if (format == kInt8) launch_rows<64, kInt8>(p, stream);
-    else launch_rows<64, kFp8>(p, stream);
+PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t heads, int64_t group, int64_t head_dim) {
+  PagedSize s;
+  s.step = rows * group <= 32 * sequences;
+  const int64_t R = s.step ? 32 : 128, TK = s.step && head_dim == 128 ? 32 : 64;
+  const int64_t tiles = rows * group / R + sequences;  // row tiles: sum ceil(n_s G / R) at most
+  const int64_t key_tiles = (keys + TK - 1) / TK;
+  s.min_tiles = s.step ? 8 : 4;
+  s.target = 0;
+  if (key_tiles > s.min_tiles) {
+    if (s.step)
+      s.target = (1536 + heads - 1) / heads;
+    else if (tiles * heads < 512)
+      s.target = (512 + heads - 1) / heads;
   }
+  s.grid = (s.target + tiles) * heads;
+  s.bytes = s.target ? s.grid * (int64_t(sizeof(Header)) + R * (head_dim + 4) * 4) : 0;
+  return s;
+}
+
+hipError_t launch_paged(const PagedParams& params, const PagedSize& size, int D, int format, hipStream_t stream) {
+  PagedParams p = params;
+  p.target = int(size.target);
+  p.min_tiles = int(size.min_tiles);
+  p.records = size.target ? size.grid : 0;
+  if (D == 128) launch_format<128>(p, size, format, stream);
+  else launch_format<64>(p, size, format, stream);
   return hipGetLastError();
 }
 

@@ -55,10 +55,25 @@ struct PagedParams {
   float scale_log2;
   int causal;
   int window, sinks;          // window 2^30: none
+  // Keys split over workgroups (take_item in paged.hip); target 0: not split.
+  int target, min_tiles;      // workgroups per head; key tiles of a part at least
+  int64_t records;            // workgroups of the launch with target, else 0
+  void* workspace;            // PagedSize::bytes
 };
+
+// The launch of a call, from what the host knows of it.
+struct PagedSize {
+  bool step;               // step_kernel, else wide_kernel
+  int64_t target, min_tiles;
+  int64_t grid;            // workgroups
+  int64_t bytes;           // workspace, 0 without target
+};
+
+// rows: new tokens in all; keys: a sequence's at most; group: query heads per head.
+PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t heads, int64_t group, int64_t head_dim);
 
 hipError_t launch_cache_write(const CacheParams& p, int D, int format, hipStream_t stream);
 hipError_t launch_cache_read(const CacheParams& p, int D, int format, hipStream_t stream);
-hipError_t launch_paged(const PagedParams& p, int D, int format, hipStream_t stream);
+hipError_t launch_paged(const PagedParams& p, const PagedSize& size, int D, int format, hipStream_t stream);
 
 }  // namespace sol

@@ -199,13 +199,15 @@ def test_c_abi_refuses_without_launching():
         return lib.sol_cache_read(fake, fake, scales, scales, fake, fake, 2, 2, 4, 16, 2, 64, fmt, start, tokens, out,
                                   fake, None)
 
-    def attend(q=fake, rows=3, hq=4, heads=2, scale=0.125, window=0, sinks=0, out=fake, offsets=fake):
-        return lib.sol_paged_attention(q, ok, rows, fake, fake, None, None, fake, fake, offsets, 2, 2, 4, 16, hq, heads,
-                                       64, 0, scale, 1, window, sinks, out, None)
+    def attend(q=fake, rows=3, hq=4, heads=2, scale=0.125, window=0, sinks=0, out=fake, offsets=fake, width=2,
+               ws=None, size=0):
+        return lib.sol_paged_attention(q, ok, rows, fake, fake, None, None, fake, fake, offsets, 2, width, 4, 16, hq,
+                                       heads, 64, 0, scale, 1, window, sinks, ws, size, out, None)
 
-    def plain(strides=ok, tq=3, tk=5, hq=4, heads=2, dim=64, out=fake):
+    def plain(strides=ok, tq=3, tk=5, hq=4, heads=2, dim=64, out=fake, ws=None):
         s = (ctypes.c_int64 * 3)(128 * 5, strides[1], strides[2])
-        return lib.sol_window_attention(fake, s, fake, s, fake, s, 1, tq, tk, hq, heads, dim, 0.125, 1, 0, 0, out, None)
+        return lib.sol_window_attention(fake, s, fake, s, fake, s, 1, tq, tk, hq, heads, dim, 0.125, 1, 0, 0, ws, 16,
+                                        out, None)
 
     refused = [
         (lambda: write(bad), b"aligned"),
@@ -238,7 +240,19 @@ def test_c_abi_refuses_without_launching():
         (lambda: plain(hq=5), b"multiple"),
         (lambda: plain(dim=32), b"head_dim"),
         (lambda: plain(out=odd), b"aligned"),
+        (lambda: attend(width=200), b"workspace"),
+        (lambda: attend(width=200, ws=odd, size=1 << 40), b"workspace"),
+        (lambda: attend(width=200, ws=fake, size=16), b"workspace"),
+        (lambda: plain(tk=5000, ws=fake), b"workspace"),
+        (lambda: plain((ctypes.c_int64 * 3)(0, 1 << 24, 64)), b"2^24"),
     ]
     for call, word in refused:
         assert call() < 0 and word in lib.sol_last_error(), (word, lib.sol_last_error())
     assert write(rows=0) == 0 and read(tokens=0) == 0 and attend(rows=0) == 0  # nothing to do, nothing launched
+    # Partial states of the calls that split their keys: none for short sequences.
+    paged, window = lib.sol_paged_attention_workspace_size, lib.sol_window_attention_workspace_size
+    assert paged(3, 2, 2, 16, 4, 2, 64, 1, 0, 0) == 0 and paged(0, 2, 200, 16, 4, 2, 64, 1, 0, 0) == 0
+    assert paged(3, 2, 200, 16, 4, 2, 64, 1, 0, 0) > 0 and paged(3, 2, 200, 16, 4, 2, 64, 1, 10, 0) == 0
+    assert paged(3, 2, 200, 16, 4, 2, 96, 1, 0, 0) == -1 and paged(3, 2, 200, 16, 3, 2, 64, 1, 0, 0) == -1
+    assert window(1, 3, 5, 4, 2, 64, 1, 0, 0) == 0 and window(1, 3, 5000, 4, 2, 64, 1, 0, 0) > 0
+    assert window(1, 0, 5, 4, 2, 64, 1, 0, 0) == -1 and window(1, 3, 5, 4, 2, 64, 1, -1, 0) == -1
