@@ -87,7 +87,10 @@ struct Item {
 // captured launch follows them and no launch or copy comes before this one.
 // With p.target, parts are of at most z key tiles, z such that about p.target
 // workgroups per head share all key tiles evenly: sum ceil(n_s / z) tiles_s is
-// at most target + sum tiles_s, the grid.  Without, one part each.
+// at most target + sum tiles_s, the grid.  Without, one part each.  No tile has
+// more than kMaxParts parts, which the merge reads one after another.
+constexpr int kMaxParts = 128;
+
 template <int R, int TK>
 __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item& it) {
   __shared__ int64_t s_total[kWaves];
@@ -125,7 +128,7 @@ __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item
     if (s < S) {
       int kt;
       sizes(s, rt, kt);
-      if (rt) parts = (kt - 1) / z + 1;
+      if (rt) parts = (kt - 1) / max(z, cdiv_i(kt, kMaxParts)) + 1;
     }
     const int64_t mine = int64_t(rt) * parts;
     int64_t end = mine;  // inclusive sum over the wave
@@ -351,9 +354,13 @@ __device__ __forceinline__ f32x16 key_factors(const float* half, int hh) {
 // hidden keys taking no part, whatever their score, value and scale hold.
 // `valid`: bits of the half's two groups of 16 rows that have a page.  scales:
 // the half's K scales in LDS (V's TK floats on), or null.
-template <int D, int TK>
+// PRECISE: the probabilities as two BF16 terms (16 significant bits): twice the
+// matrix products, which a kernel that waits for memory has time for.
+template <int D, int TK, bool PRECISE>
 __device__ __forceinline__ void attend_masked(State<D>& st, LaneRow& row, f32x16 s, const uint16_t* slot, int t, int j0,
-                                              uint32_t valid, int col, int hh, float c, const float* scales) {
+                                              uint32_t valid, int lane_col, int lane_hh, float c,
+                                              const float* scales) {
+  const int col = fresh(lane_col), hh = fresh(lane_hh);
   if (scales) {
     const f32x16 sk = key_factors(scales, hh);
 #pragma unroll
@@ -394,6 +401,17 @@ __device__ __forceinline__ void attend_masked(State<D>& st, LaneRow& row, f32x16
     for (int e = 0; e < 16; ++e) s[e] = (seen >> e) & 1u ? s[e] * sv[e] : 0.f;
   }
   const bf16x8 pb[2] = {pack8(s, 0), pack8(s, 8)};
+  bf16x8 rest[2];
+  if constexpr (PRECISE) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const u32x4 w = __builtin_bit_cast(u32x4, pb[e >> 3]);
+      const uint32_t b = w[(e & 7) >> 1];
+      s[e] -= __uint_as_float((e & 1) ? b & 0xFFFF0000u : b << 16);
+    }
+    rest[0] = pack8(s, 0);
+    rest[1] = pack8(s, 8);
+  }
   // Scheduled apart from the scores: V's operands are not held meanwhile.
   chunk_end();
   u32x4 v[2][Shape<D>::DT];
@@ -418,7 +436,10 @@ __device__ __forceinline__ void attend_masked(State<D>& st, LaneRow& row, f32x16
 #pragma unroll
   for (int c4 = 0; c4 < 2; ++c4)
 #pragma unroll
-    for (int dt = 0; dt < Shape<D>::DT; ++dt) st.acc[dt] = mfma32x32x16(as_bf16x8(v[c4][dt]), pb[c4], st.acc[dt]);
+    for (int dt = 0; dt < Shape<D>::DT; ++dt) {
+      st.acc[dt] = mfma32x32x16(as_bf16x8(v[c4][dt]), pb[c4], st.acc[dt]);
+      if constexpr (PRECISE) st.acc[dt] = mfma32x32x16(as_bf16x8(v[c4][dt]), rest[c4], st.acc[dt]);
+    }
   if (some) add_nonfinite<D, TK>(st, slot, t, hh, seen);
 }
 
@@ -457,35 +478,71 @@ __device__ __forceinline__ void store4(uint16_t* out, const f32x4& x, float den,
 }
 
 // Joins the parts of split tiles: m = max_s m_s, O = sum_s 2^(m_s - m) acc_s /
-// sum_s 2^(m_s - m) den_s over the parts in ascending order.  One workgroup per
-// record; those that begin a split tile work, a thread per row and 4 features.
+// sum_s 2^(m_s - m) den_s.  A wave per record and every kMergeRows-th row of it;
+// those of records that begin a split tile work.  D / 4 lanes take 4 features
+// each and 256 / D such groups of lanes every other (fourth) part, kMergeAhead
+// parts' loads in flight; their states join in a fixed order, so results do
+// not depend on the schedule.
+constexpr int kMergeAhead = 8;
+template <int R>
+constexpr int kMergeRows = R == 32 ? 8 : 16;
+
 template <int D, int R>
 __global__ __launch_bounds__(kNT) void merge_kernel(PagedParams p) {
-  Header hd = headers(p)[blockIdx.x];
+  constexpr int kLanes = D / 4, kGroups = kWave / kLanes;
+  const int64_t unit = int64_t(blockIdx.x) * kWaves + (threadIdx.x >> 6);
+  const int64_t rec = unit / kMergeRows<R>;
+  if (rec >= p.records) return;
+  Header hd = headers(p)[rec];
   if (hd.parts <= 1) return;
-  constexpr int kChunks = D / 4;
-  const int h = blockIdx.x % p.H;
   // Offsets that do not ascend can name more parts than the launch has.
-  hd.parts = min(hd.parts, int((p.records - 1 - blockIdx.x) / p.H) + 1);
-  for (int i = threadIdx.x; i < hd.rows * kChunks; i += kNT) {
-    const int r = i / kChunks, c = i % kChunks;
-    auto row = [&](int s) { return record<D, R>(p, int64_t(blockIdx.x) + int64_t(s) * p.H) + r * kRecordRow<D>; };
-    float m = kNegInf;
-    for (int s = 0; s < hd.parts; ++s) m = fmaxf(m, row(s)[D]);
-    float den = 0.f;
-    bool any = false;
+  hd.parts = min(hd.parts, int((p.records - 1 - rec) / p.H) + 1);
+  const int h = int(rec % p.H), lane = threadIdx.x & 63, c = lane % kLanes, group = lane / kLanes;
+  for (int r = int(unit % kMergeRows<R>); r < hd.rows; r += kMergeRows<R>) {
+    const float* base = record<D, R>(p, rec) + r * kRecordRow<D>;
+    const int64_t step = int64_t(p.H) * R * kRecordRow<D>;
+    float m = kNegInf, den = 0.f, any = 0.f;
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < hd.parts; ++s) {
-      const f32x4 tail = *reinterpret_cast<const f32x4*>(row(s) + D);
-      const f32x4 x = *reinterpret_cast<const f32x4*>(row(s) + 4 * c);
-      any |= tail[2] != 0.f;
-      if (tail[0] == kNegInf && tail[1] == 0.f) continue;
-      const float w = tail[0] == kNegInf ? 1.f : fast_exp2(tail[0] - m);
-      den += w * tail[1];
+    auto join = [&](float ms, float ds, float as, const f32x4& x) {
+      any += as;
+      const float mn = fmaxf(m, ms);
+      // Nothing scored on a side (or only -inf): it has no sums, but may have a
+      // NaN, which stays.
+      const float a = m == kNegInf ? 1.f : fast_exp2(m - mn), b = ms == kNegInf ? 1.f : fast_exp2(ms - mn);
+      m = mn;
+      den = den * a + ds * b;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) o[k] += w * x[k];
+      for (int k = 0; k < 4; ++k) o[k] = o[k] * a + x[k] * b;
+    };
+    for (int s0 = group; s0 < hd.parts; s0 += kGroups * kMergeAhead) {
+      f32x4 tail[kMergeAhead], x[kMergeAhead];
+#pragma unroll
+      for (int u = 0; u < kMergeAhead; ++u) {
+        const float* row = base + min(s0 + u * kGroups, hd.parts - 1) * step;
+        tail[u] = *reinterpret_cast<const f32x4*>(row + D);
+        x[u] = *reinterpret_cast<const f32x4*>(row + 4 * c);
+      }
+#pragma unroll
+      for (int u = 0; u < kMergeAhead; ++u)
+        if (s0 + u * kGroups < hd.parts) join(tail[u][0], tail[u][1], tail[u][2], x[u]);
     }
-    store4(p.out + output_row<D>(p, hd.off, hd.r0 + r, h) + 4 * c, o, den, any);
+#pragma unroll
+    for (int off = kLanes; off < kWave; off <<= 1) {
+      // The lower group's state first, in both.
+      const float m2 = __shfl_xor(m, off), d2 = __shfl_xor(den, off), a2 = __shfl_xor(any, off);
+      f32x4 x2;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x2[k] = __shfl_xor(o[k], off);
+      if (lane & off) {
+        const float m1 = m, d1 = den, a1 = any;
+        const f32x4 x1 = o;
+        m = m2, den = d2, any = a2, o = x2;
+        join(m1, d1, a1, x1);
+      } else {
+        join(m2, d2, a2, x2);
+      }
+    }
+    if (group == 0) store4(p.out + output_row<D>(p, hd.off, hd.r0 + r, h) + 4 * c, o, den, any != 0.f);
   }
 }
 
@@ -508,7 +565,8 @@ struct RawTile {
   u32x4 x[2][kLoads];
   float scale[2];
 
-  __device__ __forceinline__ void load(const Keys<D, F, PAGED>& keys, int t, const TilePages<TK>& pages, int lane) {
+  __device__ __forceinline__ void load(const Keys<D, F, PAGED>& keys, int t, const TilePages<TK>& pages, int lane_id) {
+    const int lane = fresh(lane_id);
     if constexpr (PAGED) {
       const uint32_t off = uint32_t(lane / kRowLanes) * keys.kRowBytes + 16u * (lane % kRowLanes);
       int64_t row[TK / 16];
@@ -536,8 +594,9 @@ struct RawTile {
     }
   }
 
-  __device__ __forceinline__ void put(uint16_t* slot, float* scales, int lane) const {
+  __device__ __forceinline__ void put(uint16_t* slot, float* scales, int lane_id) const {
     using Image = TileImage<D, TK>;
+    const int lane = fresh(lane_id);
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
 #pragma unroll
@@ -603,11 +662,12 @@ __global__ __launch_bounds__(kNT, 2) void step_kernel(PagedParams p) {
   auto attend = [&](int tile, uint32_t valid) {
 #pragma unroll 1
     for (int t = 0; t < TK / 32; ++t) {
+      const int fcol = fresh(col), fhh = fresh(hh);
       f32x16 s = zero16();
 #pragma unroll
-      for (int ks = 0; ks < S::KT; ++ks) s = mfma32x32x16(as_bf16x8(Image::k(slot, col, hh, t, ks)), qf[ks], s);
+      for (int ks = 0; ks < S::KT; ++ks) s = mfma32x32x16(as_bf16x8(Image::k(slot, fcol, fhh, t, ks)), qf[ks], s);
       chunk_end();
-      attend_masked<D, TK>(st, row, s, slot, t, tile * TK + 32 * t, valid >> (2 * t), col, hh, p.scale_log2,
+      attend_masked<D, TK, true>(st, row, s, slot, t, tile * TK + 32 * t, valid >> (2 * t), col, hh, p.scale_log2,
                            F == kBf16 ? nullptr : scales + 32 * t);
     }
   };
@@ -796,7 +856,9 @@ struct CodeTile {
   u32x4 x[2][kLoads];
   float scale;
 
-  __device__ __forceinline__ void load(const Keys<D, F, true>& keys, const TilePages<64>& pages, int tile, int wave, int l) {
+  __device__ __forceinline__ void load(const Keys<D, F, true>& keys, const TilePages<64>& pages, int tile, int wave,
+                                       int lane) {
+    const int l = fresh(lane);
     const uint32_t off = uint32_t(l / kRowLanes) * keys.kRowBytes + 16u * (l % kRowLanes);
     // A wave's 64 chunks are 8 (D = 128) or 16 rows of one group.
 #pragma unroll
@@ -813,8 +875,9 @@ struct CodeTile {
       scale = (wave ? keys.scale[1] : keys.scale[0])[keys.row(page, tile * 64 + l)];
     }
   }
-  __device__ __forceinline__ void put(uint16_t* slot, float* scales, int tid) const {
+  __device__ __forceinline__ void put(uint16_t* slot, float* scales, int thread) const {
     using Image = TileImage<D, 64>;
+    const int tid = fresh(thread);
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv)
 #pragma unroll
@@ -840,9 +903,12 @@ struct WideHalf : FastHalf<D> {
     }
   }
   __device__ static __forceinline__ void scale(f32x16& x, const float* factors, int hh) {
-    const f32x16 f = key_factors(factors, hh);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) x[e] *= f[e];
+    for (int q = 0; q < 4; ++q) {
+      const f32x4 f = *reinterpret_cast<const f32x4*>(factors + 8 * q + 4 * hh);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[4 * q + i] *= f[i];
+    }
   }
   template <typename Raw>
   __device__ __forceinline__ void finish(State<D>& st, float c, const float* sv, int hh, Raw raw) {
@@ -864,21 +930,23 @@ struct WideHalf : FastHalf<D> {
 // A key tile that every row of the wave sees whole, pipelined over its two
 // halves inside the wave so that the softmax's vector work runs beside the
 // matrix products:
-//   chunks 0 .. KT - 1  half 0's scores; half 1's K reads
-//   next KT             half 1's scores; half 0's softmax; half 0's V^T reads
-//   next 2 DT           half 0's P V; half 1's softmax; half 1's V^T reads
-//   next 2 DT           half 1's P V
-// The next tile's DMA rounds are spread over the score chunks.
+//   KT products    half 0's scores
+//   KT products    half 1's scores; half 0's softmax
+//   2 DT products  half 0's P V; half 1's softmax
+//   2 DT products  half 1's P V
+// Operands are read kAhead products before their use, and the next tile's DMA
+// rounds are spread over the score products.
 template <int D, bool SCALED, typename Refill>
 __device__ __forceinline__ void wide_tile(State<D>& st, const uint16_t* buf, const float* scales,
                                           const bf16x8 (&qf)[Shape<D>::KT], int col, int hh, float c,
                                           const Refill& refill) {
   constexpr int KT = Shape<D>::KT, DT = Shape<D>::DT;
+  constexpr int kAhead = SCALED ? 2 : 4;
   const FragLane<D> fl(fresh(col), fresh(hh));
   const uint32_t vbase = fl.v_base(buf);
-  u32x4 k0[KT], k1[KT];
-#pragma unroll
-  for (int ks = 0; ks < KT; ++ks) k0[ks] = fl.k(buf, 0, ks);
+  // Operand n of the tile's 2 KT K operands, and of its 4 DT V operands.
+  auto kfrag = [&](int n) { return fl.k(buf, n / KT, n % KT); };
+  auto vfrag = [&](int n) { return fl.v(vbase, n / (2 * DT), n / DT % 2, n % DT); };
   auto raw = [&](int t) {
     const FragLane<D> fr(fresh(col), fresh(hh));
     f32x16 s = zero16();
@@ -887,45 +955,42 @@ __device__ __forceinline__ void wide_tile(State<D>& st, const uint16_t* buf, con
     if (SCALED) WideHalf<D, SCALED>::scale(s, scales + 32 * t, hh);
     return s;
   };
+  u32x4 k[kAhead], v[kAhead];
+#pragma unroll
+  for (int n = 0; n < kAhead; ++n) k[n] = kfrag(n);
   WideHalf<D, SCALED> h0, h1;
   h0.s = zero16();
+  h1.s = zero16();
   chunk_end();
 #pragma unroll
-  for (int ks = 0; ks < KT; ++ks) {
-    h0.s = mfma32x32x16(as_bf16x8(k0[ks]), qf[ks], h0.s);
-    k1[ks] = fl.k(buf, 1, ks);
-    refill.template after_step<2 * KT>(ks);
+  for (int n = 0; n < KT; ++n) {
+    h0.s = mfma32x32x16(as_bf16x8(k[n % kAhead]), qf[n], h0.s);
+    k[n % kAhead] = kfrag(n + kAhead);
+    refill.template after_step<2 * KT>(n);
     chunk_end();
   }
   if (SCALED) h0.scale(h0.s, scales, hh);
-  u32x4 va[2][DT], vb[2][DT];
-  h1.s = zero16();
 #pragma unroll
-  for (int ks = 0; ks < KT; ++ks) {
-    h1.s = mfma32x32x16(as_bf16x8(k1[ks]), qf[ks], h1.s);
-    h0.template step<KT>(ks, st, c, scales + 64, hh);
-    if (ks >= KT / 2) {
-#pragma unroll
-      for (int f = 2 * (ks - KT / 2); f < 2 * (ks - KT / 2) + 2; ++f) va[f / DT][f % DT] = fl.v(vbase, 0, f / DT, f % DT);
-    }
-    refill.template after_step<2 * KT>(KT + ks);
+  for (int n = KT; n < 2 * KT; ++n) {
+    h1.s = mfma32x32x16(as_bf16x8(k[n % kAhead]), qf[n - KT], h1.s);
+    if (n + kAhead < 2 * KT)
+      k[n % kAhead] = kfrag(n + kAhead);
+    else
+      v[n + kAhead - 2 * KT] = vfrag(n + kAhead - 2 * KT);
+    h0.template step<KT>(n - KT, st, c, scales + 64, hh);
+    refill.template after_step<2 * KT>(n);
     chunk_end();
   }
   h0.finish(st, c, scales + 64, hh, [&] { return raw(0); });
   if (SCALED) h1.scale(h1.s, scales + 32, hh);
 #pragma unroll
-  for (int f = 0; f < 2 * DT; ++f) {
-    const int c4 = f / DT, dt = f % DT;
-    st.acc[dt] = mfma32x32x16(as_bf16x8(va[c4][dt]), h0.pb(c4), st.acc[dt]);
-    vb[c4][dt] = fl.v(vbase, 1, c4, dt);
-    h1.template step<2 * DT>(f, st, c, scales + 96, hh);
+  for (int n = 0; n < 4 * DT; ++n) {
+    const int f = n % (2 * DT);
+    if (n == 2 * DT) h1.finish(st, c, scales + 96, hh, [&] { return raw(1); });
+    st.acc[f % DT] = mfma32x32x16(as_bf16x8(v[n % kAhead]), n < 2 * DT ? h0.pb(f / DT) : h1.pb(f / DT), st.acc[f % DT]);
+    if (n + kAhead < 4 * DT) v[n % kAhead] = vfrag(n + kAhead);
+    if (n < 2 * DT) h1.template step<2 * DT>(f, st, c, scales + 96, hh);
     chunk_end();
-  }
-  h1.finish(st, c, scales + 96, hh, [&] { return raw(1); });
-#pragma unroll
-  for (int f = 0; f < 2 * DT; ++f) {
-    const int c4 = f / DT, dt = f % DT;
-    st.acc[dt] = mfma32x32x16(as_bf16x8(vb[c4][dt]), h1.pb(c4), st.acc[dt]);
   }
 }
 
@@ -971,24 +1036,48 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
   auto at = [&](int i) { return span.tile(min(i, t1 - 1)); };
   const uint32_t ring_lds = lds_address(ring[0]);
 
-  auto attend = [&](int tile, uint32_t valid, const uint16_t* buf, const float* scales, const auto& refill) {
+  // How the wave's rows see a tile: not at all, in part, or whole.
+  enum Kind { kHidden, kPart, kWhole };
+  auto kind_of = [&](int tile, uint32_t valid) {
     const int a = tile * TK, b = a + TK - 1;
-    if (wrows <= 0 || ((a > vb.hi || b < va.lo) && a >= vb.sink)) {
-      refill.all();  // hidden from every row of the wave
-    } else if (valid == kAllGroups && b <= va.hi && (a >= vb.lo || b < va.sink)) {
-      row.any = true;
-      wide_tile<D, SCALED>(st, buf, scales, qf, col, hh, p.scale_log2, refill);
-    } else {
-      refill.all();
+    if (wrows <= 0 || ((a > vb.hi || b < va.lo) && a >= vb.sink)) return kHidden;
+    return valid == kAllGroups && b <= va.hi && (a >= vb.lo || b < va.sink) ? kWhole : kPart;
+  };
+  auto hidden = [&](int, uint32_t, const uint16_t*, const float*, const auto& refill) { refill.all(); };
+  auto whole = [&](int, uint32_t, const uint16_t* buf, const float* scales, const auto& refill) {
+    wide_tile<D, SCALED>(st, buf, scales, qf, col, hh, p.scale_log2, refill);
+  };
+  auto part = [&](int tile, uint32_t valid, const uint16_t* buf, const float* scales, const auto& refill) {
+    refill.all();
 #pragma unroll 1
-      for (int t = 0; t < 2; ++t) {
-        f32x16 s = zero16();
+    for (int t = 0; t < 2; ++t) {
+      const int fcol = fresh(col), fhh = fresh(hh);
+      f32x16 s = zero16();
 #pragma unroll
-        for (int ks = 0; ks < S::KT; ++ks)
-          s = mfma32x32x16(as_bf16x8(TileImage<D, TK>::k(buf, col, hh, t, ks)), qf[ks], s);
-        chunk_end();
-        attend_masked<D, TK>(st, row, s, buf, t, a + 32 * t, valid >> (2 * t), col, hh, p.scale_log2,
-                             SCALED ? scales + 32 * t : nullptr);
+      for (int ks = 0; ks < S::KT; ++ks)
+        s = mfma32x32x16(as_bf16x8(TileImage<D, TK>::k(buf, fcol, fhh, t, ks)), qf[ks], s);
+      chunk_end();
+      attend_masked<D, TK, false>(st, row, s, buf, t, tile * TK + 32 * t, valid >> (2 * t), col, hh, p.scale_log2,
+                           SCALED ? scales + 32 * t : nullptr);
+    }
+  };
+  // One tile after another; consecutive tiles of a kind run in a loop of their
+  // own, so that the sums are not split across a branch per tile.  The waves of
+  // a workgroup may be in different loops: each meets one barrier per tile.
+  auto stream = [&](auto&& step, const uint32_t& valid) {
+    int i = t0;
+    while (i < t1) {
+      const Kind kind = kind_of(at(i), valid);
+      if (kind == kWhole) {
+        row.any = true;
+        do step(i, whole);
+        while (++i < t1 && kind_of(at(i), valid) == kWhole);
+      } else if (kind == kPart) {
+        do step(i, part);
+        while (++i < t1 && kind_of(at(i), valid) == kPart);
+      } else {
+        do step(i, hidden);
+        while (++i < t1 && kind_of(at(i), valid) == kHidden);
       }
     }
   };
@@ -999,7 +1088,7 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
       uint32_t lanes[2];
       DmaTile<D, PAGED>::lane_offsets(keys, wave, lane, lanes);
       DmaTile<D, PAGED>(keys, now, at(t0), ring_lds, wave, lane, lanes).all();
-      for (int i = t0; i < t1; ++i) {
+      stream([&](int i, auto&& attend) {
         wait_vmcnt<0>();
         lds_barrier();
         const int slot = (i - t0) & 1;
@@ -1009,14 +1098,14 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
         const uint32_t valid = now.valid;
         now = next;
         next = keys.template pages_of<TK>(at(i + 2));
-        attend(at(i), valid, ring[slot], nullptr, refill);
-      }
+        attend(at(i), valid, ring[slot], static_cast<const float*>(nullptr), refill);
+      }, now.valid);
       wait_vmcnt<0>();
     } else {
       CodeTile<D, F> code;
       code.load(keys, now, at(t0), wave, lane);
       code.put(ring[0], s_scale[0], tid);
-      for (int i = t0; i < t1; ++i) {
+      stream([&](int i, auto&& attend) {
         lds_barrier();
         const int slot = (i - t0) & 1;
         code.load(keys, next, at(i + 1), wave, lane);
@@ -1025,7 +1114,7 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
         next = keys.template pages_of<TK>(at(i + 2));
         attend(at(i), valid, ring[slot], s_scale[slot], NoStep{});
         code.put(ring[slot ^ 1], s_scale[slot ^ 1], tid);
-      }
+      }, now.valid);
     }
   }
 
@@ -1061,10 +1150,12 @@ void launch_variant(const PagedParams& p, const PagedSize& size, hipStream_t str
   else
     hipLaunchKernelGGL((wide_kernel<D, F, PAGED>), grid, dim3(kNT), 0, stream, p);
   if (size.target) {
+    const int rows = size.step ? kMergeRows<32> : kMergeRows<128>;
+    const dim3 merge(unsigned((size.grid * rows + kWaves - 1) / kWaves));
     if (size.step)
-      hipLaunchKernelGGL((merge_kernel<D, 32>), grid, dim3(kNT), 0, stream, p);
+      hipLaunchKernelGGL((merge_kernel<D, 32>), merge, dim3(kNT), 0, stream, p);
     else
-      hipLaunchKernelGGL((merge_kernel<D, 128>), grid, dim3(kNT), 0, stream, p);
+      hipLaunchKernelGGL((merge_kernel<D, 128>), merge, dim3(kNT), 0, stream, p);
   }
 }
 
@@ -1088,7 +1179,7 @@ PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t head
   s.target = 0;
   if (key_tiles > s.min_tiles) {
     if (s.step)
-      s.target = (1536 + heads - 1) / heads;
+      s.target = (1024 + heads - 1) / heads;
     else if (tiles * heads < 512)
       s.target = (512 + heads - 1) / heads;
   }
