@@ -13,7 +13,7 @@
 // r % G of the group.  They are cut into tiles of R rows; a tile's keys are the
 // union of what its rows see, in key tiles, and may be split over several
 // workgroups ("parts"), whose softmax states the merge kernel joins.
-//   step_kernel  R = 32, for few rows per sequence (single tokens): four waves,
+//   step_kernel  R = 16, for few rows per sequence (single tokens): four waves,
 //                each with key tiles of its own; bound by reading the cache
 //   wide_kernel  R = 128, for chunks: four waves of 32 rows share every key tile;
 //                bound by the matrix cores and the softmax's vector work
@@ -354,9 +354,7 @@ __device__ __forceinline__ f32x16 key_factors(const float* half, int hh) {
 // hidden keys taking no part, whatever their score, value and scale hold.
 // `valid`: bits of the half's two groups of 16 rows that have a page.  scales:
 // the half's K scales in LDS (V's TK floats on), or null.
-// PRECISE: the probabilities as two BF16 terms (16 significant bits): twice the
-// matrix products, which a kernel that waits for memory has time for.
-template <int D, int TK, bool PRECISE>
+template <int D, int TK>
 __device__ __forceinline__ void attend_masked(State<D>& st, LaneRow& row, f32x16 s, const uint16_t* slot, int t, int j0,
                                               uint32_t valid, int lane_col, int lane_hh, float c,
                                               const float* scales) {
@@ -401,17 +399,6 @@ __device__ __forceinline__ void attend_masked(State<D>& st, LaneRow& row, f32x16
     for (int e = 0; e < 16; ++e) s[e] = (seen >> e) & 1u ? s[e] * sv[e] : 0.f;
   }
   const bf16x8 pb[2] = {pack8(s, 0), pack8(s, 8)};
-  bf16x8 rest[2];
-  if constexpr (PRECISE) {
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const u32x4 w = __builtin_bit_cast(u32x4, pb[e >> 3]);
-      const uint32_t b = w[(e & 7) >> 1];
-      s[e] -= __uint_as_float((e & 1) ? b & 0xFFFF0000u : b << 16);
-    }
-    rest[0] = pack8(s, 0);
-    rest[1] = pack8(s, 8);
-  }
   // Scheduled apart from the scores: V's operands are not held meanwhile.
   chunk_end();
   u32x4 v[2][Shape<D>::DT];
@@ -436,10 +423,7 @@ __device__ __forceinline__ void attend_masked(State<D>& st, LaneRow& row, f32x16
 #pragma unroll
   for (int c4 = 0; c4 < 2; ++c4)
 #pragma unroll
-    for (int dt = 0; dt < Shape<D>::DT; ++dt) {
-      st.acc[dt] = mfma32x32x16(as_bf16x8(v[c4][dt]), pb[c4], st.acc[dt]);
-      if constexpr (PRECISE) st.acc[dt] = mfma32x32x16(as_bf16x8(v[c4][dt]), rest[c4], st.acc[dt]);
-    }
+    for (int dt = 0; dt < Shape<D>::DT; ++dt) st.acc[dt] = mfma32x32x16(as_bf16x8(v[c4][dt]), pb[c4], st.acc[dt]);
   if (some) add_nonfinite<D, TK>(st, slot, t, hh, seen);
 }
 
@@ -485,7 +469,7 @@ __device__ __forceinline__ void store4(uint16_t* out, const f32x4& x, float den,
 // not depend on the schedule.
 constexpr int kMergeAhead = 8;
 template <int R>
-constexpr int kMergeRows = R == 32 ? 8 : 16;
+constexpr int kMergeRows = R == 128 ? 16 : 8;
 
 template <int D, int R>
 __global__ __launch_bounds__(kNT) void merge_kernel(PagedParams p) {
@@ -547,6 +531,16 @@ __global__ __launch_bounds__(kNT) void merge_kernel(PagedParams p) {
 }
 
 // ---- few rows ---------------------------------------------------------------
+//
+// Matrix products of 16 x 16 x 32: S^T = K Q^T has a query per column and four
+// keys per lane, O^T = V^T P^T a query per column and four features per lane, so
+// the softmax's vector work per key is half of the 32 x 32 form's.  A operand:
+// lane l supplies row l % 16, k-slots 8 (l / 16) .. + 7; B operand: column l %
+// 16, the same slots; C: lane l holds column l % 16, rows 4 (l / 16) + e.
+
+__device__ __forceinline__ f32x4 mfma16x16x32(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
 
 // Keeps a wave's LDS writes and reads of its own slot in program order (the
 // hardware runs them in order; nothing is emitted).
@@ -554,6 +548,95 @@ __device__ __forceinline__ void wave_order() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
 }
+
+// Maximum / sum over the four lanes (l % 16 alike) that share a query.
+__device__ __forceinline__ float quad_max(float x) {
+  x = pair_max(x);
+  const auto sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+}
+
+__device__ __forceinline__ float quad_sum(float x) {
+  x = pair_sum(x);
+  const auto sw = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+}
+
+// A wave's LDS slot: TK rows of K, then of V, BF16, in 16-byte chunks.  K as in
+// TileLayout.  V in row quads, chunk c of row r at chunk (c >> 2) 16 + (r & 3) 4
+// + ((c & 3) ^ 2 (quad & 1)) of quad r >> 2: the two lane groups of a transpose
+// read, which take 16 features of neighbouring quads, meet different banks.
+template <int D, int TK>
+struct StepSlot {
+  static constexpr int CPR = D / 8;
+  static constexpr int kElems = TK * D;
+  static constexpr int kQuad = 64 * CPR;  // bytes of a V quad
+  int k_lane[D / 32];  // element offset of this lane's K operand, per k-step (key block 0)
+  uint32_t v_lane[2];  // byte offset of its V reads, for even and odd feature blocks
+
+  __device__ __forceinline__ StepSlot(const uint16_t* slot, int lane) {
+    const int r = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int ks = 0; ks < D / 32; ++ks) k_lane[ks] = r * D + ((8 * (g ^ TileLayout<D>::k_swizzle(r))) ^ (32 * ks));
+    // Lane j of a group reads row j >> 2 of the quad, features 4 (j & 3) .. + 3.
+    const uint32_t base = lds_address(slot) + 2u * kElems + g * kQuad + 64 * (r >> 2) + 16 * ((r >> 1) & 1) + 8 * (r & 1);
+#pragma unroll
+    for (int odd = 0; odd < 2; ++odd) v_lane[odd] = base + 32u * (odd ^ (g & 1));
+  }
+  __device__ __forceinline__ bf16x8 k(const uint16_t* slot, int kb, int ks) const {
+    return as_bf16x8(*reinterpret_cast<const u32x4*>(slot + k_lane[ks] + 16 * kb * D));
+  }
+  // V^T of feature block fb (16 features) for keys 32 h + 4 g + {0..3, 16..19}.
+  __device__ __forceinline__ u32x4 v(int h, int fb) const {
+    const uint32_t a = v_lane[fb & 1] + uint32_t(8 * h * kQuad + 256 * (fb >> 1));
+    const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SOL_LDS i16x4*)(uintptr_t)a);
+    const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SOL_LDS i16x4*)(uintptr_t)(a + 4u * kQuad));
+    const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
+    const u32x4 r = {x[0], x[1], y[0], y[1]};
+    return r;
+  }
+  // Element offset of chunk c of row r.
+  __device__ __forceinline__ static int v_offset(int r, int c) {
+    const int quad = r >> 2;
+    return kElems + 8 * (quad * 4 * CPR + (c >> 2) * 16 + (r & 3) * 4 + ((c & 3) ^ (2 * (quad & 1))));
+  }
+  __device__ __forceinline__ static int offset(int kv, int r, int c) {
+    return kv ? v_offset(r, c) : TileLayout<D>::k_offset(r, c);
+  }
+};
+
+// The pages of the next kTiles key tiles of a wave's list, one lane per group
+// of 16 rows; read once per kTiles tiles, and handed out through the scalar
+// registers.
+template <int D, int F, bool PAGED, int TK>
+struct PageWindow {
+  static constexpr int kGroups = TK / 16, kTiles = 64 / kGroups;
+  int page;
+  uint64_t ok;
+
+  // tile_of(i): tile i of the window.
+  template <typename TileOf>
+  __device__ __forceinline__ void fetch(const Keys<D, F, PAGED>& keys, TileOf tile_of, int lane) {
+    if constexpr (PAGED) {
+      const int pos = min(tile_of(lane / kGroups) * TK + 16 * (lane % kGroups), keys.last);
+      const int id = keys.table[pos >> keys.shift];
+      const bool in = uint32_t(id) < uint32_t(keys.pages);
+      page = in ? id : 0;
+      ok = __builtin_amdgcn_ballot_w64(in);
+    }
+  }
+  __device__ __forceinline__ TilePages<TK> get(int i) const {
+    TilePages<TK> t;
+    t.valid = kAllGroups;
+    if constexpr (PAGED) {
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) t.page[g] = __builtin_amdgcn_readlane(page, i * kGroups + g);
+      t.valid = uint32_t(ok >> (i * kGroups)) & ((1u << kGroups) - 1u);
+      if constexpr (kGroups == 2) t.valid |= t.valid << 2;
+    }
+    return t;
+  }
+};
 
 // A key tile on its way from memory to LDS, in registers.
 template <int D, int F, bool PAGED, int TK>
@@ -565,8 +648,7 @@ struct RawTile {
   u32x4 x[2][kLoads];
   float scale[2];
 
-  __device__ __forceinline__ void load(const Keys<D, F, PAGED>& keys, int t, const TilePages<TK>& pages, int lane_id) {
-    const int lane = fresh(lane_id);
+  __device__ __forceinline__ void load(const Keys<D, F, PAGED>& keys, int t, const TilePages<TK>& pages, int lane) {
     if constexpr (PAGED) {
       const uint32_t off = uint32_t(lane / kRowLanes) * keys.kRowBytes + 16u * (lane % kRowLanes);
       int64_t row[TK / 16];
@@ -594,19 +676,35 @@ struct RawTile {
     }
   }
 
-  __device__ __forceinline__ void put(uint16_t* slot, float* scales, int lane_id) const {
-    using Image = TileImage<D, TK>;
-    const int lane = fresh(lane_id);
+  // Where this lane's chunks go (StepSlot's image): the row of load i is kRows
+  // i + lane / kRowLanes, so its place is the lane's place of load 0, moved by
+  // whole rows and with a few chunk bits flipped, both known at compile time.
+  struct Puts {
+    uint32_t at[2];
+    __device__ __forceinline__ Puts(uint16_t* slot, int lane) {
+      const int r = lane / kRowLanes, c = (F == kBf16 ? 1 : 2) * (lane % kRowLanes);
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) at[kv] = lds_address(slot + StepSlot<D, TK>::offset(kv, r, c));
+    }
+    __device__ __forceinline__ SOL_LDS u32x4* place(int kv, int i, int second) const {
+      // K's swizzle: row & 15 (D = 128), (row / 2) & 7 (D = 64); V's: the quad's parity.
+      const uint32_t flip = kv ? 32u * (kRows == 4 ? i & 1 : 0)
+                               : 16u * ((D == 128 ? kRows * i & 15 : kRows * i / 2 & 7) ^ second);
+      const uint32_t move = kv ? kRows / 4 * i * StepSlot<D, TK>::kQuad + 16 * second : kRows * i * D * 2;
+      return (SOL_LDS u32x4*)(uintptr_t)((at[kv] ^ flip) + move);
+    }
+  };
+
+  __device__ __forceinline__ void put(const Puts& puts, float* scales, int lane) const {
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
-        const int row = kRows * i + lane / kRowLanes, c = lane % kRowLanes;
         if constexpr (F == kBf16) {
-          Image::put(slot, kv, row, c, x[kv][i]);
+          *puts.place(kv, i, 0) = x[kv][i];
         } else {
-          Image::put(slot, kv, row, 2 * c, codes_to_bf16<F>(x[kv][i][0], x[kv][i][1]));
-          Image::put(slot, kv, row, 2 * c + 1, codes_to_bf16<F>(x[kv][i][2], x[kv][i][3]));
+          *puts.place(kv, i, 0) = codes_to_bf16<F>(x[kv][i][0], x[kv][i][1]);
+          *puts.place(kv, i, 1) = codes_to_bf16<F>(x[kv][i][2], x[kv][i][3]);
         }
       }
       if constexpr (F != kBf16)
@@ -615,15 +713,150 @@ struct RawTile {
   }
 };
 
+// A wave's state for its 16 queries.
+template <int D>
+struct StepState {
+  f32x4 acc[D / 16];
+  float m, den;
+};
+
+// Adds V's elements that are not finite to the sums of the queries that see
+// their keys (as add_nonfinite: the products took zeros for them).  Bit 4 kb +
+// e of `seen`: this lane's query sees key 16 kb + 4 (lane / 16) + e.
+template <int D, int TK>
+__device__ __forceinline__ void step_nonfinite(StepState<D>& st, const uint16_t* slot, int lane, uint32_t seen) {
+  // Distance of the inline assembly below from the matrix instructions.
+#pragma unroll
+  for (int fb = 0; fb < D / 16; ++fb) asm volatile("s_nop 15\n\ts_nop 7" : "+v"(st.acc[fb]));
+  const int g = lane >> 4;
+#pragma unroll 1
+  for (int r = 0; r < TK; ++r) {
+    const uint32_t bits = uint32_t(__shfl(int(seen), (lane & 15) + 16 * ((r >> 2) & 3)));
+    const bool on = (bits >> (4 * (r >> 4) + (r & 3))) & 1u;
+#pragma unroll
+    for (int fb = 0; fb < D / 16; ++fb) {
+      const u32x2 x = *reinterpret_cast<const u32x2*>(slot + StepSlot<D, TK>::v_offset(r, 2 * fb + (g >> 1)) + 4 * (g & 1));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t b = (e & 1) ? x[e >> 1] >> 16 : x[e >> 1] & 0xFFFFu;
+        const float add = on && (b & 0x7F80u) == 0x7F80u ? bf16_bits_to_f32(b) : 0.f;
+        asm volatile("v_add_f32 %0, %0, %1" : "+v"(st.acc[fb][e]) : "v"(add));
+      }
+    }
+  }
+}
+
+// One key tile against the wave's queries.  MASKED: hidden keys take no part,
+// whatever their score, value and scale hold.
+template <int D, int TK, bool SCALED, bool MASKED>
+__device__ __forceinline__ void step_tile(StepState<D>& st, LaneRow& row, const bf16x8 (&qf)[D / 32],
+                                          const uint16_t* slot, const StepSlot<D, TK>& lane_at, const float* scales,
+                                          int tile, uint32_t valid, int lane, float c) {
+  constexpr int KB = TK / 16, FB = D / 16;
+  const int g = lane >> 4;
+  f32x4 s[KB];
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb) {
+    s[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < D / 32; ++ks) s[kb] = mfma16x16x32(lane_at.k(slot, kb, ks), qf[ks], s[kb]);
+  }
+  if constexpr (SCALED) {
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      const f32x4 sk = *reinterpret_cast<const f32x4*>(scales + 16 * kb + 4 * g);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[kb][e] *= sk[e];
+    }
+  }
+  uint32_t seen = 0;
+  if constexpr (MASKED) {
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int j = tile * TK + 16 * kb + 4 * g + e;
+        const bool in = (((j <= row.v.hi) & (j >= row.v.lo)) | (j < row.v.sink)) & (((valid >> kb) & 1u) != 0);
+        s[kb][e] = in ? s[kb][e] : kNegInf;
+        seen |= in ? 1u << (4 * kb + e) : 0u;
+      }
+    row.any |= seen != 0;
+  } else {
+    row.any = true;
+  }
+  float mx = s[0][0];
+#pragma unroll
+  for (int i = 1; i < 4 * KB; ++i) mx = fmaxf(mx, s[i / 4][i % 4]);
+  mx = quad_max(mx) * c;
+  if (__builtin_amdgcn_ballot_w64(mx > st.m)) {
+    const float mnew = fmaxf(st.m, mx);
+    const float alpha = mnew == kNegInf ? 1.f : fast_exp2(st.m - mnew);
+    st.m = mnew;
+    st.den *= alpha;
+#pragma unroll
+    for (int fb = 0; fb < FB; ++fb)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) st.acc[fb][e] *= alpha;
+  }
+  const float neg_m = st.m == kNegInf ? 0.f : -st.m;
+  float sum = 0.f;
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      s[kb][e] = fast_exp2(fmaf(s[kb][e], c, neg_m));
+      sum += s[kb][e];
+    }
+  st.den += sum;
+  if constexpr (SCALED) {
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      const f32x4 sv = *reinterpret_cast<const f32x4*>(scales + TK + 16 * kb + 4 * g);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[kb][e] = MASKED && !((seen >> (4 * kb + e)) & 1u) ? 0.f : s[kb][e] * sv[e];
+    }
+  }
+  // The probabilities as two BF16 terms (16 significant bits): the kernel waits
+  // for memory, and the products have time.
+  uint32_t bad = 0;
+#pragma unroll
+  for (int h = 0; h < TK / 32; ++h) {
+    u32x4 hi, lo;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x4& x = s[2 * h + (i >> 1)];
+      const float u = x[2 * (i & 1)], w = x[2 * (i & 1) + 1];
+      hi[i] = pack_bf16x2(u, w);
+      lo[i] = pack_bf16x2(u - __uint_as_float(hi[i] << 16), w - __uint_as_float(hi[i] & 0xFFFF0000u));
+    }
+#pragma unroll
+    for (int fb = 0; fb < FB; ++fb) {
+      u32x4 v = lane_at.v(h, fb);
+      if constexpr (MASKED) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t b = nonfinite(v[i]);
+          bad |= b;
+          v[i] &= ~((b >> 15) * 0xFFFFu);
+        }
+      }
+      st.acc[fb] = mfma16x16x32(as_bf16x8(v), as_bf16x8(hi), st.acc[fb]);
+      st.acc[fb] = mfma16x16x32(as_bf16x8(v), as_bf16x8(lo), st.acc[fb]);
+    }
+  }
+  if constexpr (MASKED) {
+    if (__builtin_amdgcn_ballot_w64(bad != 0)) step_nonfinite<D, TK>(st, slot, lane, seen);
+  }
+}
+
 template <int D, int F, bool PAGED>
 __global__ __launch_bounds__(kNT, 2) void step_kernel(PagedParams p) {
-  using S = Shape<D>;
-  constexpr int R = 32;
+  constexpr int R = 16;
   constexpr int TK = D == 128 ? 32 : 64;      // 16 KB of LDS per wave
   constexpr int kSets = F == kBf16 ? 1 : 2;   // tiles in flight per wave: 16 KB
-  using Image = TileImage<D, TK>;
+  constexpr bool SCALED = F != kBf16;
   __shared__ __align__(256) uint16_t s_tile[kWaves][2 * TK * D];
-  __shared__ __align__(16) float s_scale[kWaves][F == kBf16 ? 1 : 2 * TK];
+  __shared__ __align__(16) float s_scale[kWaves][SCALED ? 2 * TK : 1];
   __shared__ float s_md[kWaves][3][kWave];
 
   const int h = blockIdx.x % p.H;
@@ -634,7 +867,7 @@ __global__ __launch_bounds__(kNT, 2) void step_kernel(PagedParams p) {
   }
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int col = lane & 31, hh = lane >> 5;
+  const int col = lane & 15, g = lane >> 4;
 
   // This lane's query, straight into its operand registers.
   const int pos0 = it.length - it.n;
@@ -642,66 +875,76 @@ __global__ __launch_bounds__(kNT, 2) void step_kernel(PagedParams p) {
   const int token = r / p.G;
   const uint16_t* q = p.q + (PAGED ? (it.off + token) * p.q_st : it.s * p.q_sb + token * p.q_st) +
                       (h * p.G + r % p.G) * p.q_sh;
-  bf16x8 qf[S::KT];
+  bf16x8 qf[D / 32];
 #pragma unroll
-  for (int ks = 0; ks < S::KT; ++ks) qf[ks] = as_bf16x8(load16(q + 16 * ks + 8 * hh));
+  for (int ks = 0; ks < D / 32; ++ks) qf[ks] = as_bf16x8(load16(q + 32 * ks + 8 * g));
   LaneRow row;
   row.v = visible(p, pos0 + token, it.length);
   row.any = false;
-
   const int first = pos0 + it.r0 / p.G, last = pos0 + (it.r0 + it.rows - 1) / p.G;
   const Span span = span_of<TK>(p, first, last, it.length);
   const int t0 = int(int64_t(it.part) * span.n / it.parts), t1 = int(int64_t(it.part + 1) * span.n / it.parts);
-  State<D> st;
-  state_init(st);
+  // Tiles inside these bounds are seen whole by every row.
+  const Visible va = visible(p, first, it.length), vb = visible(p, last, it.length);
+
+  StepState<D> st;
+#pragma unroll
+  for (int fb = 0; fb < D / 16; ++fb) st.acc[fb] = f32x4{0.f, 0.f, 0.f, 0.f};
+  st.m = kNegInf;
+  st.den = 0.f;
   const Keys<D, F, PAGED> keys(p, it, h);
   uint16_t* slot = s_tile[wave];
   float* scales = s_scale[wave];
-  auto at = [&](int i) { return span.tile(min(i, t1 - 1)); };
+  const StepSlot<D, TK> lane_at(slot, lane);
 
-  auto attend = [&](int tile, uint32_t valid) {
-#pragma unroll 1
-    for (int t = 0; t < TK / 32; ++t) {
-      const int fcol = fresh(col), fhh = fresh(hh);
-      f32x16 s = zero16();
-#pragma unroll
-      for (int ks = 0; ks < S::KT; ++ks) s = mfma32x32x16(as_bf16x8(Image::k(slot, fcol, fhh, t, ks)), qf[ks], s);
-      chunk_end();
-      attend_masked<D, TK, true>(st, row, s, slot, t, tile * TK + 32 * t, valid >> (2 * t), col, hh, p.scale_log2,
-                           F == kBf16 ? nullptr : scales + 32 * t);
-    }
-  };
-
-  if (t0 + wave < t1) {
-    RawTile<D, F, PAGED, TK> raw[kSets];
+  // The wave's tiles are every kWaves-th of the part's: tile k of its list.
+  const int count = t1 - t0 > wave ? (t1 - t0 - wave - 1) / kWaves + 1 : 0;
+  auto tile_of = [&](int k) { return span.tile(t0 + wave + kWaves * min(k, count - 1)); };
+  if (count > 0) {
+    using Window = PageWindow<D, F, PAGED, TK>;
+    using Raw = RawTile<D, F, PAGED, TK>;
+    Window window;
+    Raw raw[kSets];
     uint32_t valid[kSets];
-    TilePages<TK> ahead[kSets];
-    int i = t0 + wave;
-#pragma unroll
-    for (int u = 0; u < kSets; ++u) {
-      const int n = at(i + u * kWaves);
-      const TilePages<TK> pages = keys.template pages_of<TK>(n);
+    const typename Raw::Puts puts(slot, lane);
+    // Starts the loads of tile k into set u.
+    auto load = [&](int k, int u) {
+      if (k % Window::kTiles == 0) window.fetch(keys, [&](int i) { return tile_of(k + i); }, lane);
+      const TilePages<TK> pages = window.get(k % Window::kTiles);
       valid[u] = pages.valid;
-      raw[u].load(keys, n, pages, lane);
-    }
+      raw[u].load(keys, tile_of(k), pages, lane);
+    };
+    auto step = [&](int k, int u, auto masked) {
+      wave_order();
+      raw[u].put(puts, scales, lane);
+      wave_order();
+      const uint32_t now = valid[u];
+      if (k + kSets < count) load(k + kSets, u);
+      step_tile<D, TK, SCALED, decltype(masked)::value>(st, row, qf, slot, lane_at, scales, tile_of(k), now, lane,
+                                                        p.scale_log2);
+    };
+    // Whole tiles, the common kind, run in a loop of their own.
+    auto whole = [&](int k, uint32_t pages) {
+      const int a = tile_of(k) * TK, b = a + TK - 1;
+      return k < count && pages == kAllGroups && b <= va.hi && (a >= vb.lo || b < va.sink);
+    };
 #pragma unroll
-    for (int u = 0; u < kSets; ++u) ahead[u] = keys.template pages_of<TK>(at(i + (kSets + u) * kWaves));
-    while (i < t1) {
-#pragma unroll
-      for (int u = 0; u < kSets; ++u) {
-        if (i < t1) {
-          wave_order();
-          raw[u].put(slot, scales, lane);
-          wave_order();
-          const uint32_t now = valid[u];
-          if (i + kSets * kWaves < t1) {
-            raw[u].load(keys, at(i + kSets * kWaves), ahead[u], lane);
-            valid[u] = ahead[u].valid;
-            ahead[u] = keys.template pages_of<TK>(at(i + 2 * kSets * kWaves));
-          }
-          attend(at(i), now);
+    for (int u = 0; u < kSets; ++u)
+      if (u < count) load(u, u);
+    int k = 0;
+    while (k < count) {
+      if constexpr (kSets == 1) {
+        while (whole(k, valid[0])) step(k++, 0, std::false_type{});
+        if (k < count) step(k++, 0, std::true_type{});
+      } else {
+        while (whole(k, valid[0]) && whole(k + 1, valid[1])) {
+          step(k, 0, std::false_type{});
+          step(k + 1, 1, std::false_type{});
+          k += 2;
         }
-        i += kWaves;
+        if (k < count) step(k, 0, std::true_type{});
+        if (k + 1 < count) step(k + 1, 1, std::true_type{});
+        k += 2;
       }
     }
   }
@@ -709,54 +952,49 @@ __global__ __launch_bounds__(kNT, 2) void step_kernel(PagedParams p) {
   // Join the four waves' states: each writes its sums over its own tiles.
   wave_order();
   f32x4* mine = reinterpret_cast<f32x4*>(slot);
-  constexpr int NC = D / 8;  // groups of 4 features per lane
+  constexpr int FB = D / 16;
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    const f32x4 x = {st.acc[c / 4][4 * (c % 4)], st.acc[c / 4][4 * (c % 4) + 1], st.acc[c / 4][4 * (c % 4) + 2],
-                     st.acc[c / 4][4 * (c % 4) + 3]};
-    mine[c * kWave + lane] = x;
-  }
+  for (int fb = 0; fb < FB; ++fb) mine[fb * kWave + lane] = st.acc[fb];
   s_md[wave][0][lane] = st.m;
   s_md[wave][1][lane] = st.den;
   s_md[wave][2][lane] = row.any ? 1.f : 0.f;
   __syncthreads();
-  float m = kNegInf, den = 0.f, w[kWaves], seen = 0.f;
-#pragma unroll
-  for (int g = 0; g < kWaves; ++g) m = fmaxf(m, s_md[g][0][lane]);
-#pragma unroll
-  for (int g = 0; g < kWaves; ++g) {
-    const float mg = s_md[g][0][lane];
-    w[g] = mg == kNegInf ? 1.f : fast_exp2(mg - m);
-    den += w[g] * s_md[g][1][lane];
-    seen += s_md[g][2][lane];
-  }
-  // Both lanes of a pair saw different keys of each tile.
-  den = pair_sum(den);
-  seen = pair_sum(seen);
   const int64_t rec = blockIdx.x;
   if (p.records && tid == 0)
     headers(p)[rec] = Header{it.part == 0 && it.parts > 1 ? it.parts : 0, it.off, it.r0, it.rows};
-  if (col >= it.rows) return;
+  float m = kNegInf, den = 0.f, w[kWaves], seen = 0.f;
 #pragma unroll
-  for (int c = wave; c < NC; c += kWaves) {
+  for (int i = 0; i < kWaves; ++i) m = fmaxf(m, s_md[i][0][lane]);
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    const float mi = s_md[i][0][lane];
+    w[i] = mi == kNegInf ? 1.f : fast_exp2(mi - m);
+    den += w[i] * s_md[i][1][lane];
+    seen += s_md[i][2][lane];
+  }
+  // The four lanes of a query saw different keys of each tile.
+  den = quad_sum(den);
+  seen = quad_sum(seen);
+  if (col >= it.rows) return;
+  float* row_out = record<D, R>(p, rec) + col * kRecordRow<D>;
+  uint16_t* out = p.out + output_row<D>(p, it.off, it.r0 + col, h);
+#pragma unroll
+  for (int fb = wave; fb < FB; fb += kWaves) {
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int g = 0; g < kWaves; ++g) {
-      const f32x4 x = reinterpret_cast<const f32x4*>(s_tile[g])[c * kWave + lane];
+    for (int i = 0; i < kWaves; ++i) {
+      const f32x4 x = reinterpret_cast<const f32x4*>(s_tile[i])[fb * kWave + lane];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] += w[g] * x[i];
+      for (int e = 0; e < 4; ++e) o[e] += w[i] * x[e];
     }
-    const int feature = 32 * (c / 4) + 8 * (c % 4) + 4 * hh;
-    if (it.parts > 1) {
-      float* row_out = record<D, R>(p, rec) + col * kRecordRow<D>;
-      *reinterpret_cast<f32x4*>(row_out + feature) = o;
-      if (c == 0 && hh == 0) {
-        const f32x4 tail = {m, den, seen, 0.f};
-        *reinterpret_cast<f32x4*>(row_out + D) = tail;
-      }
-    } else {
-      store4(p.out + output_row<D>(p, it.off, r, h) + feature, o, den, seen > 0.f);
-    }
+    if (it.parts > 1)
+      *reinterpret_cast<f32x4*>(row_out + 16 * fb + 4 * g) = o;
+    else
+      store4(out + 16 * fb + 4 * g, o, den, seen > 0.f);
+  }
+  if (it.parts > 1 && wave == 0 && g == 0) {
+    const f32x4 tail = {m, den, seen, 0.f};
+    *reinterpret_cast<f32x4*>(row_out + D) = tail;
   }
 }
 
@@ -1057,7 +1295,7 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
       for (int ks = 0; ks < S::KT; ++ks)
         s = mfma32x32x16(as_bf16x8(TileImage<D, TK>::k(buf, fcol, fhh, t, ks)), qf[ks], s);
       chunk_end();
-      attend_masked<D, TK, false>(st, row, s, buf, t, tile * TK + 32 * t, valid >> (2 * t), col, hh, p.scale_log2,
+      attend_masked<D, TK>(st, row, s, buf, t, tile * TK + 32 * t, valid >> (2 * t), col, hh, p.scale_log2,
                            SCALED ? scales + 32 * t : nullptr);
     }
   };
@@ -1142,20 +1380,21 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
 
 // ---- launches ---------------------------------------------------------------
 
+template <int D, int R>
+void launch_merge(const PagedParams& p, hipStream_t stream) {
+  const int64_t units = p.records * kMergeRows<R>;
+  hipLaunchKernelGGL((merge_kernel<D, R>), dim3(unsigned((units + kWaves - 1) / kWaves)), dim3(kNT), 0, stream, p);
+}
+
 template <int D, int F, bool PAGED>
 void launch_variant(const PagedParams& p, const PagedSize& size, hipStream_t stream) {
-  const dim3 grid(unsigned(size.grid));
-  if (size.step)
-    hipLaunchKernelGGL((step_kernel<D, F, PAGED>), grid, dim3(kNT), 0, stream, p);
-  else
-    hipLaunchKernelGGL((wide_kernel<D, F, PAGED>), grid, dim3(kNT), 0, stream, p);
-  if (size.target) {
-    const int rows = size.step ? kMergeRows<32> : kMergeRows<128>;
-    const dim3 merge(unsigned((size.grid * rows + kWaves - 1) / kWaves));
-    if (size.step)
-      hipLaunchKernelGGL((merge_kernel<D, 32>), merge, dim3(kNT), 0, stream, p);
-    else
-      hipLaunchKernelGGL((merge_kernel<D, 128>), merge, dim3(kNT), 0, stream, p);
+  const dim3 grid(unsigned(size.grid)), block(kNT);
+  if (size.rows == 16) {
+    hipLaunchKernelGGL((step_kernel<D, F, PAGED>), grid, block, 0, stream, p);
+    if (p.records) launch_merge<D, 16>(p, stream);
+  } else {
+    hipLaunchKernelGGL((wide_kernel<D, F, PAGED>), grid, block, 0, stream, p);
+    if (p.records) launch_merge<D, 128>(p, stream);
   }
 }
 
@@ -1171,20 +1410,21 @@ void launch_format(const PagedParams& p, const PagedSize& size, int format, hipS
 
 PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t heads, int64_t group, int64_t head_dim) {
   PagedSize s;
-  s.step = rows * group <= 32 * sequences;
-  const int64_t R = s.step ? 32 : 128, TK = s.step && head_dim == 128 ? 32 : 64;
-  const int64_t tiles = rows * group / R + sequences;  // row tiles: sum ceil(n_s G / R) at most
+  const bool step = rows * group <= 32 * sequences;
+  s.rows = step ? 16 : 128;
+  const int64_t TK = step && head_dim == 128 ? 32 : 64;
+  const int64_t tiles = rows * group / s.rows + sequences;  // row tiles: sum ceil(n_s G / R) at most
   const int64_t key_tiles = (keys + TK - 1) / TK;
-  s.min_tiles = s.step ? 8 : 4;
+  s.min_tiles = step ? 8 : 4;
   s.target = 0;
   if (key_tiles > s.min_tiles) {
-    if (s.step)
+    if (step)
       s.target = (1024 + heads - 1) / heads;
     else if (tiles * heads < 512)
       s.target = (512 + heads - 1) / heads;
   }
   s.grid = (s.target + tiles) * heads;
-  s.bytes = s.target ? s.grid * (int64_t(sizeof(Header)) + R * (head_dim + 4) * 4) : 0;
+  s.bytes = s.target ? s.grid * (int64_t(sizeof(Header)) + s.rows * (head_dim + 4) * 4) : 0;
   return s;
 }
 

@@ -63,7 +63,7 @@ struct PagedParams {
 
 // The launch of a call, from what the host knows of it.
 struct PagedSize {
-  bool step;               // step_kernel, else wide_kernel
+  int64_t rows;            // of a row tile: 16 (step_kernel) or 128 (wide_kernel)
   int64_t target, min_tiles;
   int64_t grid;            // workgroups
   int64_t bytes;           // workspace, 0 without target
