@@ -497,8 +497,8 @@ int sol_paged_attention(const void* q, const int64_t* q_strides, int64_t rows, c
                         int64_t head_dim, int format, double scale, int causal, int64_t window, int64_t sink_tokens,
                         void* workspace, int64_t workspace_bytes, void* out, void* stream);
 int64_t sol_paged_attention_workspace_size(int64_t rows, int64_t sequences, int64_t table_width, int64_t page_size,
-                                           int64_t query_heads, int64_t heads, int64_t head_dim, int causal,
-                                           int64_t window, int64_t sink_tokens);
+                                           int64_t query_heads, int64_t heads, int64_t head_dim, int format,
+                                           int causal, int64_t window, int64_t sink_tokens);
 
 /* The same over plain BF16 K and V [batch, key_tokens, heads, head_dim] and Q
  * [batch, query_tokens, query_heads, head_dim] by their {batch, token, head}

@@ -71,7 +71,7 @@ _SIGNATURES = {
                         _p, _p, _p], ctypes.c_int),
     "sol_paged_attention": ([_p, _i64p, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                              _int, _dbl, _int, _i64, _i64, _p, _i64, _p, _p], ctypes.c_int),
-    "sol_paged_attention_workspace_size": ([_i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _i64, _i64], _i64),
+    "sol_paged_attention_workspace_size": ([_i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _int, _i64, _i64], _i64),
     "sol_window_attention": ([_p, _i64p, _p, _i64p, _p, _i64p, _i64, _i64, _i64, _i64, _i64, _i64, _dbl, _int,
                               _i64, _i64, _p, _i64, _p, _p], ctypes.c_int),
     "sol_window_attention_workspace_size": ([_i64, _i64, _i64, _i64, _i64, _i64, _int, _i64, _i64], _i64),
@@ -762,8 +762,8 @@ def launch_cache_read(cache, plan, start, tokens):
 
 
 @functools.lru_cache(maxsize=1024)
-def _paged_size(n, s, width, page_size, hq, h, d, causal, window, sinks):
-    return library().sol_paged_attention_workspace_size(n, s, width, page_size, hq, h, d, causal, window, sinks)
+def _paged_size(n, s, width, page_size, hq, h, d, fmt, causal, window, sinks):
+    return library().sol_paged_attention_workspace_size(n, s, width, page_size, hq, h, d, fmt, causal, window, sinks)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -789,12 +789,13 @@ def launch_paged(q, cache, plan, scale, causal, window, sinks, out=None):
         return out
     q = _rows(q)
     table, lengths, offsets = _plan_args(plan)
-    size = _paged_size(n, s, width, page_size, hq, h, d, causal, window, sinks)
+    fmt = CACHE_FORMATS[cache.k.dtype]
+    size = _paged_size(n, s, width, page_size, hq, h, d, fmt, causal, window, sinks)
     ws = _workspace(size, dev)
     _check(library().sol_paged_attention(
         q.data_ptr(), _strides(q, True), n, cache.k.data_ptr(), cache.v.data_ptr(), _ptr(cache.k_scales),
         _ptr(cache.v_scales), table, lengths, offsets, s, width, pages, page_size, hq, h, d,
-        CACHE_FORMATS[cache.k.dtype], scale, causal, window, sinks, _ptr(ws), size, out.data_ptr(), _stream(dev)))
+        fmt, scale, causal, window, sinks, _ptr(ws), size, out.data_ptr(), _stream(dev)))
     return out
 
 

@@ -20,6 +20,9 @@
 //
 // Cached INT8 and FP8 codes are converted to BF16 (exact) on their way into
 // LDS; a key's scale multiplies its score, a value's scale its probability.
+#include <algorithm>
+#include <type_traits>
+
 #include "attn_common.h"
 #include "paged_internal.h"
 
@@ -81,6 +84,31 @@ struct Item {
   int part, parts;        // its share of the tile's keys
 };
 
+// What the merge kernel has to join: a header per (row tile, head), the tiles
+// in order of sequences.
+struct Header {
+  int parts;         // 0: nothing
+  int off, r0, rows; // Item's
+  uint32_t first;    // record of its first part; the next ones are p.H apart
+};
+
+// Partial states of split tiles, after the headers: per workgroup (record) and
+// row D sums, the maximum, the denominator and whether a key was seen.
+template <int D>
+constexpr int kRecordRow = D + 4;
+
+template <int D, int R>
+__device__ __forceinline__ float* record(const PagedParams& p, int64_t i) {
+  return reinterpret_cast<float*>(static_cast<uint8_t*>(p.workspace) + p.header_bytes) + i * R * kRecordRow<D>;
+}
+
+// Header of row tile `tile` for this workgroup's head (every thread writes the
+// same: no branch on the thread).  (Offsets that do not
+// ascend can name more tiles than there are headers.)
+__device__ __forceinline__ void write_header(const PagedParams& p, int64_t tile, const Header& hd) {
+  if (tile >= 0 && tile < p.tiles) static_cast<Header*>(p.workspace)[tile * p.H + blockIdx.x % p.H] = hd;
+}
+
 // Item `id` of the launch, in order of sequences, row tiles and parts; false
 // past the last one.  Every workgroup forms the whole plan from the lengths on
 // the device (two scans over the sequences, a few microseconds), so that a
@@ -94,7 +122,8 @@ constexpr int kMaxParts = 128;
 template <int R, int TK>
 __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item& it) {
   __shared__ int64_t s_total[kWaves];
-  __shared__ int s_found[4];
+  __shared__ int s_tiles[kWaves];
+  __shared__ int s_found[5];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int S = p.batch.S;
   // Row tiles and key tiles of sequence s.
@@ -118,10 +147,12 @@ __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item
     sum = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) sum += s_total[w];
+    sum = int64_t(uniform64(uint64_t(sum)));
     z = int(min(int64_t(1) << 30, max(int64_t(p.min_tiles), (sum + p.target - 1) / p.target)));
     __syncthreads();
   }
   int64_t base = 0;
+  int tiles = 0;  // row tiles of the sequences before s0
   for (int s0 = 0; s0 < S; s0 += kNT) {
     const int s = s0 + tid;
     int rt = 0, parts = 1;
@@ -131,19 +162,23 @@ __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item
       if (rt) parts = (kt - 1) / max(z, cdiv_i(kt, kMaxParts)) + 1;
     }
     const int64_t mine = int64_t(rt) * parts;
-    int64_t end = mine;  // inclusive sum over the wave
+    int64_t end = mine;  // inclusive sums over the wave
+    int tile_end = rt;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
       const int64_t x = __shfl_up(end, off);
-      if (lane >= off) end += x;
+      const int y = __shfl_up(tile_end, off);
+      if (lane >= off) end += x, tile_end += y;
     }
-    if (lane == 63) s_total[wave] = end;
+    if (lane == 63) s_total[wave] = end, s_tiles[wave] = tile_end;
     __syncthreads();
     int64_t all = 0;
+    int all_tiles = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      if (w == wave) end += all + base;
+      if (w == wave) end += all + base, tile_end += all_tiles + tiles;
       all += s_total[w];
+      all_tiles += s_tiles[w];
     }
     if (id >= end - mine && id < end) {
       const int k = int(id - (end - mine));
@@ -151,12 +186,19 @@ __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item
       s_found[1] = p.causal ? rt - 1 - k / parts : k / parts;  // the longest first
       s_found[2] = k % parts;
       s_found[3] = parts;
+      s_found[4] = tile_end - rt + k / parts;
     }
     __syncthreads();
-    base += all;
+    base += int64_t(uniform64(uint64_t(all)));
+    tiles += __builtin_amdgcn_readfirstlane(all_tiles);
     if (id < base) break;
   }
-  if (id >= base) return false;
+  if (id >= base) {
+    // The launch has as many workgroups without an item as headers without a
+    // tile, at least.
+    if (p.records) write_header(p, tiles + (id - base), Header{0, 0, 0, 0, 0});
+    return false;
+  }
   it.s = __builtin_amdgcn_readfirstlane(s_found[0]);
   it.off = __builtin_amdgcn_readfirstlane(entry_offset(p, it.s));
   it.n = __builtin_amdgcn_readfirstlane(entry_offset(p, it.s + 1)) - it.off;
@@ -165,6 +207,8 @@ __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item
   it.rows = min(R, it.n * p.G - it.r0);
   it.part = __builtin_amdgcn_readfirstlane(s_found[2]);
   it.parts = __builtin_amdgcn_readfirstlane(s_found[3]);
+  if (p.records && it.part == 0)
+    write_header(p, __builtin_amdgcn_readfirstlane(s_found[4]), Header{it.parts > 1 ? it.parts : 0, it.off, it.r0, it.rows, blockIdx.x});
   return true;
 }
 
@@ -178,7 +222,8 @@ struct TilePages {
   uint32_t valid;
 };
 
-constexpr uint32_t kAllGroups = 0xFu;
+template <int TK>
+constexpr uint32_t kAllGroups = (1u << (TK / 16)) - 1u;
 
 __device__ __forceinline__ int pick(bool second, int a, int b) { return second ? b : a; }
 
@@ -214,7 +259,7 @@ struct Keys {
   template <int TK>
   __device__ __forceinline__ TilePages<TK> pages_of(int tile) const {
     TilePages<TK> t;
-    t.valid = kAllGroups;
+    t.valid = kAllGroups<TK>;
     if constexpr (PAGED) {
       typedef const int32_t __attribute__((address_space(4)))* scalar_ptr;
       const scalar_ptr tab = (scalar_ptr)(uintptr_t)table;
@@ -226,7 +271,6 @@ struct Keys {
         t.page[g] = ok ? page : 0;
         t.valid |= ok ? 1u << g : 0u;
       }
-      if constexpr (TK == 32) t.valid |= t.valid << 2;
     }
     return t;
   }
@@ -429,22 +473,6 @@ __device__ __forceinline__ void attend_masked(State<D>& st, LaneRow& row, f32x16
 
 // ---- results ----------------------------------------------------------------
 
-// Partial states of split tiles: per workgroup (record) a header, and per row
-// D sums, the maximum, the denominator and whether a key was seen.
-struct Header {
-  int parts, off, r0, rows;  // parts 0: nothing to join at this record
-};
-
-template <int D>
-constexpr int kRecordRow = D + 4;
-
-__device__ __forceinline__ Header* headers(const PagedParams& p) { return static_cast<Header*>(p.workspace); }
-
-template <int D, int R>
-__device__ __forceinline__ float* record(const PagedParams& p, int64_t i) {
-  return reinterpret_cast<float*>(static_cast<Header*>(p.workspace) + p.records) + i * R * kRecordRow<D>;
-}
-
 // Element offset of row r (of a sequence's n G) of the output.
 template <int D>
 __device__ __forceinline__ int64_t output_row(const PagedParams& p, int off, int r, int h) {
@@ -462,71 +490,77 @@ __device__ __forceinline__ void store4(uint16_t* out, const f32x4& x, float den,
 }
 
 // Joins the parts of split tiles: m = max_s m_s, O = sum_s 2^(m_s - m) acc_s /
-// sum_s 2^(m_s - m) den_s.  A wave per record and every kMergeRows-th row of it;
-// those of records that begin a split tile work.  D / 4 lanes take 4 features
-// each and 256 / D such groups of lanes every other (fourth) part, kMergeAhead
-// parts' loads in flight; their states join in a fixed order, so results do
-// not depend on the schedule.
-constexpr int kMergeAhead = 8;
-template <int R>
-constexpr int kMergeRows = R == 128 ? 16 : 8;
+// sum_s 2^(m_s - m) den_s.  A workgroup per (row tile, head) and every
+// gridDim.y-th row of it.  D / 4 lanes take 4 features each; the waves and
+// their 256 / D such groups of lanes take the parts in turn, kMergeAhead each
+// in flight, and their states join in a fixed order.
+constexpr int kMergeAhead = 4;
+
+// A state of the merge: sums of 4 features, and the row's maximum, denominator
+// and whether a key was seen.
+struct Joined {
+  f32x4 o;
+  float m, den, any;
+  __device__ __forceinline__ void add(const Joined& x) {
+    any += x.any;
+    const float mn = fmaxf(m, x.m);
+    // A side that has scored nothing (or only -inf) has no sums, but may have a
+    // NaN, which stays.
+    const float a = m == kNegInf ? 1.f : fast_exp2(m - mn), b = x.m == kNegInf ? 1.f : fast_exp2(x.m - mn);
+    m = mn;
+    den = den * a + x.den * b;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] = o[k] * a + x.o[k] * b;
+  }
+};
 
 template <int D, int R>
 __global__ __launch_bounds__(kNT) void merge_kernel(PagedParams p) {
-  constexpr int kLanes = D / 4, kGroups = kWave / kLanes;
-  const int64_t unit = int64_t(blockIdx.x) * kWaves + (threadIdx.x >> 6);
-  const int64_t rec = unit / kMergeRows<R>;
-  if (rec >= p.records) return;
-  Header hd = headers(p)[rec];
-  if (hd.parts <= 1) return;
-  // Offsets that do not ascend can name more parts than the launch has.
-  hd.parts = min(hd.parts, int((p.records - 1 - rec) / p.H) + 1);
-  const int h = int(rec % p.H), lane = threadIdx.x & 63, c = lane % kLanes, group = lane / kLanes;
-  for (int r = int(unit % kMergeRows<R>); r < hd.rows; r += kMergeRows<R>) {
-    const float* base = record<D, R>(p, rec) + r * kRecordRow<D>;
-    const int64_t step = int64_t(p.H) * R * kRecordRow<D>;
-    float m = kNegInf, den = 0.f, any = 0.f;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    auto join = [&](float ms, float ds, float as, const f32x4& x) {
-      any += as;
-      const float mn = fmaxf(m, ms);
-      // Nothing scored on a side (or only -inf): it has no sums, but may have a
-      // NaN, which stays.
-      const float a = m == kNegInf ? 1.f : fast_exp2(m - mn), b = ms == kNegInf ? 1.f : fast_exp2(ms - mn);
-      m = mn;
-      den = den * a + ds * b;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) o[k] = o[k] * a + x[k] * b;
-    };
-    for (int s0 = group; s0 < hd.parts; s0 += kGroups * kMergeAhead) {
+  constexpr int kLanes = D / 4, kGroups = kWave / kLanes, kSlots = kWaves * kGroups;
+  __shared__ Joined s_state[kWaves][kLanes];
+  Header hd = static_cast<const Header*>(p.workspace)[blockIdx.x];
+  // Offsets that do not ascend can leave headers of another call here, and name
+  // more parts than the launch has: nothing outside the tensors is touched.
+  if (hd.parts <= 1 || int64_t(hd.first) >= p.records || hd.rows <= 0 || hd.rows > R || hd.off < 0 || hd.r0 < 0 ||
+      int64_t(hd.off) + (int64_t(hd.r0) + hd.rows - 1) / p.G >= p.new_rows)
+    return;
+  hd.parts = min(hd.parts, int((p.records - 1 - hd.first) / p.H) + 1);
+  const int h = blockIdx.x % p.H, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane % kLanes;
+  const int slot = wave * kGroups + lane / kLanes;
+  const int64_t step = int64_t(p.H) * R * kRecordRow<D>;
+  for (int r = blockIdx.y; r < hd.rows; r += gridDim.y) {
+    const float* base = record<D, R>(p, hd.first) + r * kRecordRow<D>;
+    Joined mine = {{0.f, 0.f, 0.f, 0.f}, kNegInf, 0.f, 0.f};
+    for (int s0 = slot; s0 < hd.parts; s0 += kSlots * kMergeAhead) {
       f32x4 tail[kMergeAhead], x[kMergeAhead];
 #pragma unroll
       for (int u = 0; u < kMergeAhead; ++u) {
-        const float* row = base + min(s0 + u * kGroups, hd.parts - 1) * step;
-        tail[u] = *reinterpret_cast<const f32x4*>(row + D);
-        x[u] = *reinterpret_cast<const f32x4*>(row + 4 * c);
+        const float* at = base + min(s0 + u * kSlots, hd.parts - 1) * step;
+        tail[u] = *reinterpret_cast<const f32x4*>(at + D);
+        x[u] = *reinterpret_cast<const f32x4*>(at + 4 * c);
       }
 #pragma unroll
       for (int u = 0; u < kMergeAhead; ++u)
-        if (s0 + u * kGroups < hd.parts) join(tail[u][0], tail[u][1], tail[u][2], x[u]);
+        if (s0 + u * kSlots < hd.parts) mine.add(Joined{x[u], tail[u][0], tail[u][1], tail[u][2]});
     }
 #pragma unroll
     for (int off = kLanes; off < kWave; off <<= 1) {
-      // The lower group's state first, in both.
-      const float m2 = __shfl_xor(m, off), d2 = __shfl_xor(den, off), a2 = __shfl_xor(any, off);
-      f32x4 x2;
+      Joined other;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) x2[k] = __shfl_xor(o[k], off);
-      if (lane & off) {
-        const float m1 = m, d1 = den, a1 = any;
-        const f32x4 x1 = o;
-        m = m2, den = d2, any = a2, o = x2;
-        join(m1, d1, a1, x1);
-      } else {
-        join(m2, d2, a2, x2);
-      }
+      for (int k = 0; k < 4; ++k) other.o[k] = __shfl_xor(mine.o[k], off);
+      other.m = __shfl_xor(mine.m, off);
+      other.den = __shfl_xor(mine.den, off);
+      other.any = __shfl_xor(mine.any, off);
+      mine.add(other);
     }
-    if (group == 0) store4(p.out + output_row<D>(p, hd.off, hd.r0 + r, h) + 4 * c, o, den, any != 0.f);
+    if (lane < kLanes) s_state[wave][lane] = mine;
+    __syncthreads();
+    if (wave == 0 && lane < kLanes) {
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) mine.add(s_state[w][lane]);
+      store4(p.out + output_row<D>(p, hd.off, hd.r0 + r, h) + 4 * c, mine.o, mine.den, mine.any != 0.f);
+    }
+    __syncthreads();
   }
 }
 
@@ -549,6 +583,9 @@ __device__ __forceinline__ void wave_order() {
   __builtin_amdgcn_wave_barrier();
 }
 
+// Every LDS read of the wave has returned: its slot may be written.
+__device__ __forceinline__ void lds_returned() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
 // Maximum / sum over the four lanes (l % 16 alike) that share a query.
 __device__ __forceinline__ float quad_max(float x) {
   x = pair_max(x);
@@ -562,46 +599,83 @@ __device__ __forceinline__ float quad_sum(float x) {
   return __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
 }
 
-// A wave's LDS slot: TK rows of K, then of V, BF16, in 16-byte chunks.  K as in
-// TileLayout.  V in row quads, chunk c of row r at chunk (c >> 2) 16 + (r & 3) 4
-// + ((c & 3) ^ 2 (quad & 1)) of quad r >> 2: the two lane groups of a transpose
-// read, which take 16 features of neighbouring quads, meet different banks.
-template <int D, int TK>
+// Key tiles of the step kernel: 16 KB of stored K and V rows each, which a wave
+// moves through its LDS slot as they are (8-bit codes are converted as they are
+// read).  Chunks are 16 bytes.
+//   K, row by row, chunk c of row r at c ^ k_swizzle(r): the 16 rows that a
+//      phase of an operand read takes meet different banks.
+//   V, BF16: row quads, chunk c of row r at chunk (c >> 2) 16 + (r & 3) 4 + ((c &
+//      3) ^ 2 (quad & 1)) of quad r >> 2; a 16-bit transpose read takes 16
+//      features of a quad per lane group, neighbouring quads from different
+//      banks.
+//   V, codes: row by row, chunk c of row r at c ^ v_swizzle(r); an 8-bit
+//      transpose read takes 16 features of 8 rows per lane group: lane j reads
+//      row j >> 1, bytes 8 (j & 1) .. + 7, and gets feature j of the 8 rows.
+// The scores of a pair of key blocks (32 keys from 32 h on) sit so that a lane's
+// eight are the keys of its V^T operand: element e of block 2 h + b in lane group
+// g is key 32 h + 16 b + 4 g + e with BF16, 32 h + 8 g + 4 b + e with codes.
+template <int D, int F>
 struct StepSlot {
-  static constexpr int CPR = D / 8;
-  static constexpr int kElems = TK * D;
-  static constexpr int kQuad = 64 * CPR;  // bytes of a V quad
-  int k_lane[D / 32];  // element offset of this lane's K operand, per k-step (key block 0)
-  uint32_t v_lane[2];  // byte offset of its V reads, for even and odd feature blocks
+  static constexpr bool kCodes = F != kBf16;
+  static constexpr int kRow = D * kElemBytes<F>;  // bytes
+  static constexpr int TK = 8192 / kRow;
+  static constexpr int kPlane = 8192;             // bytes of K, then of V
+  static constexpr int kQuad = 4 * kRow;
+  static constexpr int kReads = kCodes ? D / 64 : D / 32;  // K chunks per lane and key block
+  uint32_t k_lane;     // LDS address of this lane's K chunk 0 of key block 0
+  uint32_t v_lane[2];  // of its V reads (BF16: for even and odd feature blocks)
 
-  __device__ __forceinline__ StepSlot(const uint16_t* slot, int lane) {
-    const int r = lane & 15, g = lane >> 4;
-#pragma unroll
-    for (int ks = 0; ks < D / 32; ++ks) k_lane[ks] = r * D + ((8 * (g ^ TileLayout<D>::k_swizzle(r))) ^ (32 * ks));
-    // Lane j of a group reads row j >> 2 of the quad, features 4 (j & 3) .. + 3.
-    const uint32_t base = lds_address(slot) + 2u * kElems + g * kQuad + 64 * (r >> 2) + 16 * ((r >> 1) & 1) + 8 * (r & 1);
-#pragma unroll
-    for (int odd = 0; odd < 2; ++odd) v_lane[odd] = base + 32u * (odd ^ (g & 1));
+  __device__ __forceinline__ static int k_swizzle(int r) {
+    if (!kCodes) return TileLayout<D>::k_swizzle(r);
+    return D == 128 ? ((r >> 1) & 1) | ((r >> 3) & 3) << 1 : (r >> 3) & 3;
   }
-  __device__ __forceinline__ bf16x8 k(const uint16_t* slot, int kb, int ks) const {
-    return as_bf16x8(*reinterpret_cast<const u32x4*>(slot + k_lane[ks] + 16 * kb * D));
-  }
-  // V^T of feature block fb (16 features) for keys 32 h + 4 g + {0..3, 16..19}.
-  __device__ __forceinline__ u32x4 v(int h, int fb) const {
-    const uint32_t a = v_lane[fb & 1] + uint32_t(8 * h * kQuad + 256 * (fb >> 1));
-    const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SOL_LDS i16x4*)(uintptr_t)a);
-    const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SOL_LDS i16x4*)(uintptr_t)(a + 4u * kQuad));
-    const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
-    const u32x4 r = {x[0], x[1], y[0], y[1]};
-    return r;
-  }
-  // Element offset of chunk c of row r.
-  __device__ __forceinline__ static int v_offset(int r, int c) {
-    const int quad = r >> 2;
-    return kElems + 8 * (quad * 4 * CPR + (c >> 2) * 16 + (r & 3) * 4 + ((c & 3) ^ (2 * (quad & 1))));
-  }
+  __device__ __forceinline__ static int v_swizzle(int r) { return D == 128 ? (r >> 1) & 7 : (r >> 2) & 3; }
+  // Byte offset of chunk c of row r.
   __device__ __forceinline__ static int offset(int kv, int r, int c) {
-    return kv ? v_offset(r, c) : TileLayout<D>::k_offset(r, c);
+    if (!kv) return r * kRow + 16 * (c ^ k_swizzle(r));
+    if (kCodes) return kPlane + r * kRow + 16 * (c ^ v_swizzle(r));
+    const int quad = r >> 2;
+    return kPlane + quad * kQuad + 16 * ((c >> 2) * 16 + (r & 3) * 4 + ((c & 3) ^ (2 * (quad & 1))));
+  }
+  // Key of score element e of block kb in lane group g.
+  __device__ __forceinline__ static int key(int kb, int g, int e) {
+    return kCodes ? 32 * (kb >> 1) + 8 * g + 4 * (kb & 1) + e : 16 * kb + 4 * g + e;
+  }
+
+  __device__ __forceinline__ StepSlot(const uint8_t* slot, int lane) {
+    const int i = lane & 15, g = lane >> 4;
+    const uint32_t base = lds_address(slot);
+    const int r = kCodes ? 8 * (i >> 2) + (i & 3) : i;  // the K row of A operand row i
+    k_lane = base + r * kRow + 16 * (g ^ k_swizzle(r));
+    if constexpr (kCodes) {
+      const int vr = 8 * g + (i >> 1);
+      v_lane[0] = v_lane[1] = base + kPlane + vr * kRow + 16 * v_swizzle(vr) + 8 * (i & 1);
+    } else {
+      const uint32_t at = base + kPlane + g * kQuad + 64 * (i >> 2) + 16 * ((i >> 1) & 1) + 8 * (i & 1);
+#pragma unroll
+      for (int odd = 0; odd < 2; ++odd) v_lane[odd] = at + 32u * (odd ^ (g & 1));
+    }
+  }
+  // K chunk n of key block kb: features 32 n + 8 g .. + 7, or the codes 64 n + 16 g .. + 15.
+  __device__ __forceinline__ u32x4 k(int kb, int n) const {
+    const uint32_t block = kCodes ? (kb >> 1) * 32 * kRow + (kb & 1) * 4 * kRow : kb * 16 * kRow;
+    return *(const SOL_LDS u32x4*)(uintptr_t)((k_lane ^ (64u * n)) + block);
+  }
+  // V^T of feature block fb (16 features) for the 32 keys from 32 h on.
+  __device__ __forceinline__ u32x4 v(int h, int fb) const {
+    if constexpr (kCodes) {
+      typedef int i32x2 __attribute__((ext_vector_type(2)));
+      const i32x2 x = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+          (SOL_LDS i32x2*)(uintptr_t)((v_lane[0] ^ (16u * fb)) + 32 * h * kRow));
+      return codes_to_bf16<F>(x[0], x[1]);
+    } else {
+      const uint32_t a = v_lane[fb & 1] + uint32_t(8 * h * kQuad + 256 * (fb >> 1));
+      const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SOL_LDS i16x4*)(uintptr_t)a);
+      const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SOL_LDS i16x4*)(uintptr_t)(a + 4u * kQuad));
+      const u32x2 x = __builtin_bit_cast(u32x2, lo), y = __builtin_bit_cast(u32x2, hi);
+      const u32x4 r = {x[0], x[1], y[0], y[1]};
+      return r;
+    }
   }
 };
 
@@ -627,89 +701,105 @@ struct PageWindow {
   }
   __device__ __forceinline__ TilePages<TK> get(int i) const {
     TilePages<TK> t;
-    t.valid = kAllGroups;
+    t.valid = kAllGroups<TK>;
     if constexpr (PAGED) {
 #pragma unroll
       for (int g = 0; g < kGroups; ++g) t.page[g] = __builtin_amdgcn_readlane(page, i * kGroups + g);
-      t.valid = uint32_t(ok >> (i * kGroups)) & ((1u << kGroups) - 1u);
-      if constexpr (kGroups == 2) t.valid |= t.valid << 2;
+      t.valid = uint32_t(ok >> (i * kGroups)) & kAllGroups<TK>;
     }
     return t;
   }
 };
 
-// A key tile on its way from memory to LDS, in registers.
-template <int D, int F, bool PAGED, int TK>
-struct RawTile {
-  static constexpr int kRowLanes = F == kBf16 ? D / 8 : D / 16;  // 16 bytes each
-  static constexpr int kRows = 64 / kRowLanes;                   // rows per load
-  static constexpr int kLoads = TK / kRows;
-  static_assert(kRows <= 16, "the rows of a load lie in one page");
-  u32x4 x[2][kLoads];
-  float scale[2];
+// 4-byte global -> LDS DMA per lane, each from an address of its own; lane l's
+// bytes land at LDS address m + 4 l (dma16's notes).
+__device__ __forceinline__ void dma4(uint64_t address, uint32_t m) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "global_load_lds_dword %1, off"
+      :
+      : "s"(m), "v"(address)
+      : "memory", "m0");
+}
 
-  __device__ __forceinline__ void load(const Keys<D, F, PAGED>& keys, int t, const TilePages<TK>& pages, int lane) {
-    if constexpr (PAGED) {
-      const uint32_t off = uint32_t(lane / kRowLanes) * keys.kRowBytes + 16u * (lane % kRowLanes);
-      int64_t row[TK / 16];
-#pragma unroll
-      for (int g = 0; g < TK / 16; ++g) row[g] = keys.row(pages.page[g], t * TK + 16 * g);
-#pragma unroll
-      for (int kv = 0; kv < 2; ++kv)
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i)
-          x[kv][i] = load_chunk(keys.base[kv] + row[kRows * i / 16] * keys.kRowBytes + off + kRows * i % 16 * keys.kRowBytes);
-      if constexpr (F != kBf16) {
-        int64_t at = row[0] + (lane & 15);
-#pragma unroll
-        for (int g = 1; g < TK / 16; ++g) at = (lane % TK) >= 16 * g ? row[g] + (lane & 15) : at;
-        scale[0] = keys.scale[0][at];
-        scale[1] = keys.scale[1][at];
-      }
+// The DMA of a wave's next key tile into its slot, K and V apart: 1 KB pieces
+// of kRows rows each, whose rows lie in one page.  A lane's place in a piece
+// names the (row, chunk) it reads, the row's swizzle taken from the piece's
+// first row and the lane's by exclusive or.
+template <int D, int F, bool PAGED>
+struct StepDma {
+  using Slot = StepSlot<D, F>;
+  using Source = Keys<D, F, PAGED>;
+  static constexpr int TK = Slot::TK;
+  static constexpr int kPieces = 8;
+  static constexpr int kRows = TK / kPieces;
+  static_assert(kRows <= 16, "the rows of a piece lie in one page");
+  static constexpr int kScales = F == kBf16 ? 0 : TK / 64;
+  static constexpr int kLoads = kPieces + kScales;  // of K, and of V
+  int row[2];         // this lane's row of a piece
+  uint32_t chunk[2];  // its chunk, in bytes
+  uint32_t slot, scales;
+  int tile, lane;
+  uint32_t valid;
+  int64_t group[PAGED ? TK / 16 : 1];  // row of the cache that each group begins at
+  int page;                            // this lane's, for the scales (one lane per row of 64)
+  int page2;
+
+  __device__ __forceinline__ StepDma(uint32_t slot_lds, uint32_t scales_lds, int l) : slot(slot_lds), scales(scales_lds), lane(l) {
+    constexpr int kRowLanes = Slot::kRow / 16;
+    row[0] = l / kRowLanes;
+    chunk[0] = 16u * ((l % kRowLanes) ^ Slot::k_swizzle(row[0]));
+    if constexpr (Slot::kCodes) {
+      row[1] = row[0];
+      chunk[1] = 16u * ((l % kRowLanes) ^ Slot::v_swizzle(row[1]));
     } else {
-#pragma unroll
-      for (int kv = 0; kv < 2; ++kv)
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i)
-          x[kv][i] = load_chunk(keys.base[kv] + uint64_t(min(t * TK + kRows * i + lane / kRowLanes, keys.last)) * keys.st[kv] +
-                                16 * (lane % kRowLanes));
+      const int quad = D == 128 ? 0 : l >> 5, m = D == 128 ? l : l & 31;  // of the piece's quads
+      row[1] = 4 * quad + ((m >> 2) & 3);
+      chunk[1] = 16u * (4 * (m >> 4) + ((m & 3) ^ (2 * (quad & 1))));
     }
   }
 
-  // Where this lane's chunks go (StepSlot's image): the row of load i is kRows
-  // i + lane / kRowLanes, so its place is the lane's place of load 0, moved by
-  // whole rows and with a few chunk bits flipped, both known at compile time.
-  struct Puts {
-    uint32_t at[2];
-    __device__ __forceinline__ Puts(uint16_t* slot, int lane) {
-      const int r = lane / kRowLanes, c = (F == kBf16 ? 1 : 2) * (lane % kRowLanes);
+  __device__ __forceinline__ void prepare(const Source& keys, int t, const TilePages<TK>& pages) {
+    tile = t;
+    valid = pages.valid;
+    if constexpr (PAGED) {
 #pragma unroll
-      for (int kv = 0; kv < 2; ++kv) at[kv] = lds_address(slot + StepSlot<D, TK>::offset(kv, r, c));
-    }
-    __device__ __forceinline__ SOL_LDS u32x4* place(int kv, int i, int second) const {
-      // K's swizzle: row & 15 (D = 128), (row / 2) & 7 (D = 64); V's: the quad's parity.
-      const uint32_t flip = kv ? 32u * (kRows == 4 ? i & 1 : 0)
-                               : 16u * ((D == 128 ? kRows * i & 15 : kRows * i / 2 & 7) ^ second);
-      const uint32_t move = kv ? kRows / 4 * i * StepSlot<D, TK>::kQuad + 16 * second : kRows * i * D * 2;
-      return (SOL_LDS u32x4*)(uintptr_t)((at[kv] ^ flip) + move);
-    }
-  };
-
-  __device__ __forceinline__ void put(const Puts& puts, float* scales, int lane) const {
+      for (int g = 0; g < TK / 16; ++g) group[g] = keys.row(pages.page[g], t * TK + 16 * g);
+      if constexpr (kScales > 0) {
+        page = pages.page[0];
+        page2 = pages.page[kScales > 1 ? 4 : 0];
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        if constexpr (F == kBf16) {
-          *puts.place(kv, i, 0) = x[kv][i];
-        } else {
-          *puts.place(kv, i, 0) = codes_to_bf16<F>(x[kv][i][0], x[kv][i][1]);
-          *puts.place(kv, i, 1) = codes_to_bf16<F>(x[kv][i][2], x[kv][i][3]);
+        for (int g = 1; g < 4; ++g) {
+          page = lane >= 16 * g ? pages.page[g] : page;
+          if constexpr (kScales > 1) page2 = lane >= 16 * g ? pages.page[4 + g] : page2;
         }
       }
-      if constexpr (F != kBf16)
-        if (lane < TK) scales[kv * TK + lane] = scale[kv];
     }
+  }
+
+  // Starts K's (V's) loads of the prepared tile; the slot's reads have returned.
+  __device__ __forceinline__ void issue(const Source& keys, int kv) const {
+    const uint64_t base = reinterpret_cast<uint64_t>(keys.base[kv]);
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      const int r = kRows * i;
+      const uint32_t flip = kv ? (Slot::kCodes ? 16u * Slot::v_swizzle(r) : (D == 128 ? 32u * (i & 1) : 0u))
+                               : 16u * Slot::k_swizzle(r);
+      const uint32_t dst = slot + uint32_t(kv * Slot::kPlane + i * 1024);
+      if constexpr (PAGED) {
+        dma16(base + uint64_t(group[r / 16]) * Slot::kRow + round_offset(uint32_t(r % 16) * Slot::kRow),
+              row[kv] * Slot::kRow + (chunk[kv] ^ flip), dst);
+      } else {
+        const int first = min(tile * TK + r, keys.last);
+        const uint32_t off = uint32_t(min(tile * TK + r + row[kv], keys.last) - first) * keys.st[kv];
+        dma16(base + uint64_t(uint32_t(first)) * keys.st[kv] + round_offset(0u), off + (chunk[kv] ^ flip), dst);
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < kScales; ++n)
+      dma4(reinterpret_cast<uint64_t>(keys.scale[kv] + keys.row(n ? page2 : page, tile * TK + 64 * n + lane)),
+           scales + uint32_t(kv * TK + 64 * n) * 4u);
   }
 };
 
@@ -722,23 +812,36 @@ struct StepState {
 
 // Adds V's elements that are not finite to the sums of the queries that see
 // their keys (as add_nonfinite: the products took zeros for them).  Bit 4 kb +
-// e of `seen`: this lane's query sees key 16 kb + 4 (lane / 16) + e.
-template <int D, int TK>
-__device__ __forceinline__ void step_nonfinite(StepState<D>& st, const uint16_t* slot, int lane, uint32_t seen) {
+// e of `seen`: this lane's query sees that score element's key.
+template <int D, int F>
+__device__ __forceinline__ void step_nonfinite(StepState<D>& st, const uint8_t* slot, int lane, uint32_t seen) {
+  using Slot = StepSlot<D, F>;
   // Distance of the inline assembly below from the matrix instructions.
 #pragma unroll
   for (int fb = 0; fb < D / 16; ++fb) asm volatile("s_nop 15\n\ts_nop 7" : "+v"(st.acc[fb]));
   const int g = lane >> 4;
 #pragma unroll 1
-  for (int r = 0; r < TK; ++r) {
-    const uint32_t bits = uint32_t(__shfl(int(seen), (lane & 15) + 16 * ((r >> 2) & 3)));
-    const bool on = (bits >> (4 * (r >> 4) + (r & 3))) & 1u;
+  for (int r = 0; r < Slot::TK; ++r) {
+    // The lane group and element that hold key r.
+    const int rg = Slot::kCodes ? r >> 3 & 3 : r >> 2 & 3;
+    const int kb = Slot::kCodes ? 2 * (r >> 5) + (r >> 2 & 1) : r >> 4;
+    const uint32_t bits = uint32_t(__shfl(int(seen), (lane & 15) + 16 * rg));
+    const bool on = (bits >> (4 * kb + (r & 3))) & 1u;
 #pragma unroll
     for (int fb = 0; fb < D / 16; ++fb) {
-      const u32x2 x = *reinterpret_cast<const u32x2*>(slot + StepSlot<D, TK>::v_offset(r, 2 * fb + (g >> 1)) + 4 * (g & 1));
+      // Features 16 fb + 4 g .. + 3.
+      uint32_t w[2];
+      if constexpr (Slot::kCodes) {
+        const uint32_t c = *reinterpret_cast<const uint32_t*>(slot + Slot::offset(1, r, fb) + 4 * g);
+        const u32x4 x = codes_to_bf16<F>(c, 0u);
+        w[0] = x[0], w[1] = x[1];
+      } else {
+        const u32x2 x = *reinterpret_cast<const u32x2*>(slot + Slot::offset(1, r, 2 * fb + (g >> 1)) + 8 * (g & 1));
+        w[0] = x[0], w[1] = x[1];
+      }
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const uint32_t b = (e & 1) ? x[e >> 1] >> 16 : x[e >> 1] & 0xFFFFu;
+        const uint32_t b = (e & 1) ? w[e >> 1] >> 16 : w[e >> 1] & 0xFFFFu;
         const float add = on && (b & 0x7F80u) == 0x7F80u ? bf16_bits_to_f32(b) : 0.f;
         asm volatile("v_add_f32 %0, %0, %1" : "+v"(st.acc[fb][e]) : "v"(add));
       }
@@ -748,35 +851,49 @@ __device__ __forceinline__ void step_nonfinite(StepState<D>& st, const uint16_t*
 
 // One key tile against the wave's queries.  MASKED: hidden keys take no part,
 // whatever their score, value and scale hold.
-template <int D, int TK, bool SCALED, bool MASKED>
-__device__ __forceinline__ void step_tile(StepState<D>& st, LaneRow& row, const bf16x8 (&qf)[D / 32],
-                                          const uint16_t* slot, const StepSlot<D, TK>& lane_at, const float* scales,
-                                          int tile, uint32_t valid, int lane, float c) {
-  constexpr int KB = TK / 16, FB = D / 16;
+// keys_read() runs once K has been read, values_due() before V is, which starts
+// the next tile's K and waits for this one's V.
+template <int D, int F, bool MASKED, typename KeysRead, typename ValuesDue>
+__device__ __forceinline__ void step_tile(StepState<D>& st, LaneRow& row, const bf16x8 (&qf)[D / 32], const uint8_t* slot,
+                                          const StepSlot<D, F>& at, const float* scales, int tile, uint32_t valid,
+                                          int lane, float c, KeysRead keys_read, ValuesDue values_due) {
+  using Slot = StepSlot<D, F>;
+  constexpr int TK = Slot::TK, KB = TK / 16, FB = D / 16;
+  constexpr bool SCALED = F != kBf16;
   const int g = lane >> 4;
   f32x4 s[KB];
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb) {
     s[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int ks = 0; ks < D / 32; ++ks) s[kb] = mfma16x16x32(lane_at.k(slot, kb, ks), qf[ks], s[kb]);
+    for (int n = 0; n < Slot::kReads; ++n) {
+      const u32x4 x = at.k(kb, n);
+      if constexpr (Slot::kCodes) {
+        s[kb] = mfma16x16x32(as_bf16x8(codes_to_bf16<F>(x[0], x[1])), qf[2 * n], s[kb]);
+        s[kb] = mfma16x16x32(as_bf16x8(codes_to_bf16<F>(x[2], x[3])), qf[2 * n + 1], s[kb]);
+      } else {
+        s[kb] = mfma16x16x32(as_bf16x8(x), qf[n], s[kb]);
+      }
+    }
+    if constexpr (Slot::kCodes) chunk_end();  // few operands in flight: their conversions take registers
   }
   if constexpr (SCALED) {
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
-      const f32x4 sk = *reinterpret_cast<const f32x4*>(scales + 16 * kb + 4 * g);
+      const f32x4 sk = *reinterpret_cast<const f32x4*>(scales + Slot::key(kb, g, 0));
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[kb][e] *= sk[e];
     }
   }
+  keys_read();
   uint32_t seen = 0;
   if constexpr (MASKED) {
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int j = tile * TK + 16 * kb + 4 * g + e;
-        const bool in = (((j <= row.v.hi) & (j >= row.v.lo)) | (j < row.v.sink)) & (((valid >> kb) & 1u) != 0);
+        const int r = Slot::key(kb, g, e), j = tile * TK + r;
+        const bool in = (((j <= row.v.hi) & (j >= row.v.lo)) | (j < row.v.sink)) & (((valid >> (r >> 4)) & 1u) != 0);
         s[kb][e] = in ? s[kb][e] : kNegInf;
         seen |= in ? 1u << (4 * kb + e) : 0u;
       }
@@ -808,16 +925,18 @@ __device__ __forceinline__ void step_tile(StepState<D>& st, LaneRow& row, const 
       sum += s[kb][e];
     }
   st.den += sum;
+  values_due();
   if constexpr (SCALED) {
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
-      const f32x4 sv = *reinterpret_cast<const f32x4*>(scales + TK + 16 * kb + 4 * g);
+      const f32x4 sv = *reinterpret_cast<const f32x4*>(scales + TK + Slot::key(kb, g, 0));
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[kb][e] = MASKED && !((seen >> (4 * kb + e)) & 1u) ? 0.f : s[kb][e] * sv[e];
     }
   }
   // The probabilities as two BF16 terms (16 significant bits): the kernel waits
   // for memory, and the products have time.
+  constexpr bool kCheck = MASKED && F != kInt8;  // INT8 codes are finite
   uint32_t bad = 0;
 #pragma unroll
   for (int h = 0; h < TK / 32; ++h) {
@@ -831,8 +950,8 @@ __device__ __forceinline__ void step_tile(StepState<D>& st, LaneRow& row, const 
     }
 #pragma unroll
     for (int fb = 0; fb < FB; ++fb) {
-      u32x4 v = lane_at.v(h, fb);
-      if constexpr (MASKED) {
+      u32x4 v = at.v(h, fb);
+      if constexpr (kCheck) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const uint32_t b = nonfinite(v[i]);
@@ -842,34 +961,31 @@ __device__ __forceinline__ void step_tile(StepState<D>& st, LaneRow& row, const 
       }
       st.acc[fb] = mfma16x16x32(as_bf16x8(v), as_bf16x8(hi), st.acc[fb]);
       st.acc[fb] = mfma16x16x32(as_bf16x8(v), as_bf16x8(lo), st.acc[fb]);
+      if (Slot::kCodes && fb % 2) chunk_end();
     }
   }
-  if constexpr (MASKED) {
-    if (__builtin_amdgcn_ballot_w64(bad != 0)) step_nonfinite<D, TK>(st, slot, lane, seen);
+  if constexpr (kCheck) {
+    if (__builtin_amdgcn_ballot_w64(bad != 0)) step_nonfinite<D, F>(st, slot, lane, seen);
   }
 }
 
 template <int D, int F, bool PAGED>
 __global__ __launch_bounds__(kNT, 2) void step_kernel(PagedParams p) {
-  constexpr int R = 16;
-  constexpr int TK = D == 128 ? 32 : 64;      // 16 KB of LDS per wave
-  constexpr int kSets = F == kBf16 ? 1 : 2;   // tiles in flight per wave: 16 KB
+  using Slot = StepSlot<D, F>;
+  constexpr int R = 16, TK = Slot::TK;
   constexpr bool SCALED = F != kBf16;
-  __shared__ __align__(256) uint16_t s_tile[kWaves][2 * TK * D];
+  __shared__ __align__(256) uint8_t s_tile[kWaves][2 * Slot::kPlane];
   __shared__ __align__(16) float s_scale[kWaves][SCALED ? 2 * TK : 1];
   __shared__ float s_md[kWaves][3][kWave];
 
   const int h = blockIdx.x % p.H;
   Item it;
-  if (!take_item<R, TK>(p, blockIdx.x / p.H, it)) {
-    if (p.records && threadIdx.x == 0) headers(p)[blockIdx.x] = Header{0, 0, 0, 0};
-    return;
-  }
+  if (!take_item<R, TK>(p, blockIdx.x / p.H, it)) return;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, g = lane >> 4;
 
-  // This lane's query, straight into its operand registers.
+  // This lane's query, straight into its operand registers (StepSlot::k's features).
   const int pos0 = it.length - it.n;
   const int r = it.r0 + min(col, it.rows - 1);
   const int token = r / p.G;
@@ -877,7 +993,8 @@ __global__ __launch_bounds__(kNT, 2) void step_kernel(PagedParams p) {
                       (h * p.G + r % p.G) * p.q_sh;
   bf16x8 qf[D / 32];
 #pragma unroll
-  for (int ks = 0; ks < D / 32; ++ks) qf[ks] = as_bf16x8(load16(q + 32 * ks + 8 * g));
+  for (int ks = 0; ks < D / 32; ++ks)
+    qf[ks] = as_bf16x8(load16(q + (SCALED ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1) : 32 * ks + 8 * g)));
   LaneRow row;
   row.v = visible(p, pos0 + token, it.length);
   row.any = false;
@@ -893,59 +1010,60 @@ __global__ __launch_bounds__(kNT, 2) void step_kernel(PagedParams p) {
   st.m = kNegInf;
   st.den = 0.f;
   const Keys<D, F, PAGED> keys(p, it, h);
-  uint16_t* slot = s_tile[wave];
+  uint8_t* slot = s_tile[wave];
   float* scales = s_scale[wave];
-  const StepSlot<D, TK> lane_at(slot, lane);
+  const Slot at(slot, lane);
 
   // The wave's tiles are every kWaves-th of the part's: tile k of its list.
   const int count = t1 - t0 > wave ? (t1 - t0 - wave - 1) / kWaves + 1 : 0;
   auto tile_of = [&](int k) { return span.tile(t0 + wave + kWaves * min(k, count - 1)); };
   if (count > 0) {
     using Window = PageWindow<D, F, PAGED, TK>;
-    using Raw = RawTile<D, F, PAGED, TK>;
+    using Dma = StepDma<D, F, PAGED>;
     Window window;
-    Raw raw[kSets];
-    uint32_t valid[kSets];
-    const typename Raw::Puts puts(slot, lane);
-    // Starts the loads of tile k into set u.
-    auto load = [&](int k, int u) {
+    Dma dma(lds_address(slot), lds_address(scales), lane);
+    auto prepare = [&](int k) {
       if (k % Window::kTiles == 0) window.fetch(keys, [&](int i) { return tile_of(k + i); }, lane);
-      const TilePages<TK> pages = window.get(k % Window::kTiles);
-      valid[u] = pages.valid;
-      raw[u].load(keys, tile_of(k), pages, lane);
+      dma.prepare(keys, tile_of(k), window.get(k % Window::kTiles));
     };
-    auto step = [&](int k, int u, auto masked) {
-      wave_order();
-      raw[u].put(puts, scales, lane);
-      wave_order();
-      const uint32_t now = valid[u];
-      if (k + kSets < count) load(k + kSets, u);
-      step_tile<D, TK, SCALED, decltype(masked)::value>(st, row, qf, slot, lane_at, scales, tile_of(k), now, lane,
-                                                        p.scale_log2);
+    // Tile k: its K is awaited, then its V, with the next tile's K on its way
+    // meanwhile and its V from the end on (each wave on its own, no barrier).
+    auto step = [&](int k, auto masked) {
+      const bool more = k + 1 < count;
+      const uint32_t valid = dma.valid;
+      wait_vmcnt<Dma::kLoads>();
+      step_tile<D, F, decltype(masked)::value>(
+          st, row, qf, slot, at, scales, tile_of(k), valid, lane, p.scale_log2,
+          [&] {
+            if (more) {
+              prepare(k + 1);
+              lds_returned();
+              dma.issue(keys, 0);
+            }
+          },
+          [&] {
+            if (more)
+              wait_vmcnt<Dma::kLoads>();
+            else
+              wait_vmcnt<0>();
+          });
+      if (more) {
+        lds_returned();
+        dma.issue(keys, 1);
+      }
     };
-    // Whole tiles, the common kind, run in a loop of their own.
-    auto whole = [&](int k, uint32_t pages) {
+    auto whole = [&](int k) {
       const int a = tile_of(k) * TK, b = a + TK - 1;
-      return k < count && pages == kAllGroups && b <= va.hi && (a >= vb.lo || b < va.sink);
+      return k < count && dma.valid == kAllGroups<TK> && b <= va.hi && (a >= vb.lo || b < va.sink);
     };
-#pragma unroll
-    for (int u = 0; u < kSets; ++u)
-      if (u < count) load(u, u);
+    prepare(0);
+    dma.issue(keys, 0);
+    dma.issue(keys, 1);
     int k = 0;
     while (k < count) {
-      if constexpr (kSets == 1) {
-        while (whole(k, valid[0])) step(k++, 0, std::false_type{});
-        if (k < count) step(k++, 0, std::true_type{});
-      } else {
-        while (whole(k, valid[0]) && whole(k + 1, valid[1])) {
-          step(k, 0, std::false_type{});
-          step(k + 1, 1, std::false_type{});
-          k += 2;
-        }
-        if (k < count) step(k, 0, std::true_type{});
-        if (k + 1 < count) step(k + 1, 1, std::true_type{});
-        k += 2;
-      }
+      // Whole tiles, the common kind, run in a loop of their own.
+      while (whole(k)) step(k++, std::false_type{});
+      if (k < count) step(k++, std::true_type{});
     }
   }
 
@@ -959,9 +1077,6 @@ __global__ __launch_bounds__(kNT, 2) void step_kernel(PagedParams p) {
   s_md[wave][1][lane] = st.den;
   s_md[wave][2][lane] = row.any ? 1.f : 0.f;
   __syncthreads();
-  const int64_t rec = blockIdx.x;
-  if (p.records && tid == 0)
-    headers(p)[rec] = Header{it.part == 0 && it.parts > 1 ? it.parts : 0, it.off, it.r0, it.rows};
   float m = kNegInf, den = 0.f, w[kWaves], seen = 0.f;
 #pragma unroll
   for (int i = 0; i < kWaves; ++i) m = fmaxf(m, s_md[i][0][lane]);
@@ -976,7 +1091,7 @@ __global__ __launch_bounds__(kNT, 2) void step_kernel(PagedParams p) {
   den = quad_sum(den);
   seen = quad_sum(seen);
   if (col >= it.rows) return;
-  float* row_out = record<D, R>(p, rec) + col * kRecordRow<D>;
+  float* row_out = record<D, R>(p, blockIdx.x) + col * kRecordRow<D>;
   uint16_t* out = p.out + output_row<D>(p, it.off, it.r0 + col, h);
 #pragma unroll
   for (int fb = wave; fb < FB; fb += kWaves) {
@@ -1242,10 +1357,7 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
 
   const int h = blockIdx.x % p.H;
   Item it;
-  if (!take_item<R, TK>(p, blockIdx.x / p.H, it)) {
-    if (p.records && threadIdx.x == 0) headers(p)[blockIdx.x] = Header{0, 0, 0, 0};
-    return;
-  }
+  if (!take_item<R, TK>(p, blockIdx.x / p.H, it)) return;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, hh = lane >> 5;
@@ -1279,7 +1391,7 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
   auto kind_of = [&](int tile, uint32_t valid) {
     const int a = tile * TK, b = a + TK - 1;
     if (wrows <= 0 || ((a > vb.hi || b < va.lo) && a >= vb.sink)) return kHidden;
-    return valid == kAllGroups && b <= va.hi && (a >= vb.lo || b < va.sink) ? kWhole : kPart;
+    return valid == kAllGroups<TK> && b <= va.hi && (a >= vb.lo || b < va.sink) ? kWhole : kPart;
   };
   auto hidden = [&](int, uint32_t, const uint16_t*, const float*, const auto& refill) { refill.all(); };
   auto whole = [&](int, uint32_t, const uint16_t* buf, const float* scales, const auto& refill) {
@@ -1357,8 +1469,6 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
   }
 
   const float den = pair_sum(st.den), seen = pair_sum(row.any ? 1.f : 0.f);
-  if (p.records && tid == 0)
-    headers(p)[blockIdx.x] = Header{it.part == 0 && it.parts > 1 ? it.parts : 0, it.off, it.r0, it.rows};
   if (col >= wrows) return;
   float* row_out = record<D, R>(p, blockIdx.x) + (32 * wave + col) * kRecordRow<D>;
   uint16_t* out = p.out + output_row<D>(p, it.off, r, h);
@@ -1381,9 +1491,9 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
 // ---- launches ---------------------------------------------------------------
 
 template <int D, int R>
-void launch_merge(const PagedParams& p, hipStream_t stream) {
-  const int64_t units = p.records * kMergeRows<R>;
-  hipLaunchKernelGGL((merge_kernel<D, R>), dim3(unsigned((units + kWaves - 1) / kWaves)), dim3(kNT), 0, stream, p);
+void launch_merge(const PagedParams& p, const PagedSize& size, hipStream_t stream) {
+  hipLaunchKernelGGL((merge_kernel<D, R>), dim3(unsigned(size.tiles * p.H), unsigned(size.merge_rows)), dim3(kNT), 0,
+                     stream, p);
 }
 
 template <int D, int F, bool PAGED>
@@ -1391,10 +1501,10 @@ void launch_variant(const PagedParams& p, const PagedSize& size, hipStream_t str
   const dim3 grid(unsigned(size.grid)), block(kNT);
   if (size.rows == 16) {
     hipLaunchKernelGGL((step_kernel<D, F, PAGED>), grid, block, 0, stream, p);
-    if (p.records) launch_merge<D, 16>(p, stream);
+    if (p.records) launch_merge<D, 16>(p, size, stream);
   } else {
     hipLaunchKernelGGL((wide_kernel<D, F, PAGED>), grid, block, 0, stream, p);
-    if (p.records) launch_merge<D, 128>(p, stream);
+    if (p.records) launch_merge<D, 128>(p, size, stream);
   }
 }
 
@@ -1408,23 +1518,26 @@ void launch_format(const PagedParams& p, const PagedSize& size, int format, hipS
 
 }  // namespace
 
-PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t heads, int64_t group, int64_t head_dim) {
+PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t heads, int64_t group, int64_t head_dim,
+                     int format) {
   PagedSize s;
   const bool step = rows * group <= 32 * sequences;
   s.rows = step ? 16 : 128;
-  const int64_t TK = step && head_dim == 128 ? 32 : 64;
-  const int64_t tiles = rows * group / s.rows + sequences;  // row tiles: sum ceil(n_s G / R) at most
+  const int64_t TK = step ? 8192 / (head_dim * (format == kBf16 ? 2 : 1)) : 64;  // StepSlot::TK
+  s.tiles = rows * group / s.rows + sequences;  // row tiles: sum ceil(n_s G / R) at most
   const int64_t key_tiles = (keys + TK - 1) / TK;
   s.min_tiles = step ? 8 : 4;
   s.target = 0;
   if (key_tiles > s.min_tiles) {
     if (step)
       s.target = (1024 + heads - 1) / heads;
-    else if (tiles * heads < 512)
+    else if (s.tiles * heads < 512)
       s.target = (512 + heads - 1) / heads;
   }
-  s.grid = (s.target + tiles) * heads;
-  s.bytes = s.target ? s.grid * (int64_t(sizeof(Header)) + s.rows * (head_dim + 4) * 4) : 0;
+  s.grid = (s.target + s.tiles) * heads;
+  s.header_bytes = (s.tiles * heads * int64_t(sizeof(Header)) + 15) / 16 * 16;
+  s.merge_rows = std::min(s.rows, (rows * group + sequences - 1) / sequences);
+  s.bytes = s.target ? s.header_bytes + s.grid * s.rows * (head_dim + 4) * 4 : 0;
   return s;
 }
 
@@ -1433,6 +1546,9 @@ hipError_t launch_paged(const PagedParams& params, const PagedSize& size, int D,
   p.target = int(size.target);
   p.min_tiles = int(size.min_tiles);
   p.records = size.target ? size.grid : 0;
+  p.tiles = size.tiles;
+  p.header_bytes = size.header_bytes;
+  p.new_rows = p.batch.table ? p.batch.rows : int64_t(p.batch.S) * p.Tq;
   if (D == 128) launch_format<128>(p, size, format, stream);
   else launch_format<64>(p, size, format, stream);
   return hipGetLastError();

@@ -58,19 +58,24 @@ struct PagedParams {
   // Keys split over workgroups (take_item in paged.hip); target 0: not split.
   int target, min_tiles;      // workgroups per head; key tiles of a part at least
   int64_t records;            // workgroups of the launch with target, else 0
-  void* workspace;            // PagedSize::bytes
+  int64_t tiles, header_bytes, new_rows;
+  void* workspace;            // PagedSize::bytes: headers, then records
 };
 
 // The launch of a call, from what the host knows of it.
 struct PagedSize {
-  int64_t rows;            // of a row tile: 16 (step_kernel) or 128 (wide_kernel)
+  int64_t rows;               // of a row tile: 16 (step_kernel) or 128 (wide_kernel)
+  int64_t tiles;              // row tiles at most
   int64_t target, min_tiles;
-  int64_t grid;            // workgroups
-  int64_t bytes;           // workspace, 0 without target
+  int64_t grid;               // workgroups
+  int64_t merge_rows;         // rows of a tile that the merge's workgroups take side by side
+  int64_t header_bytes;
+  int64_t bytes;              // workspace, 0 without target
 };
 
 // rows: new tokens in all; keys: a sequence's at most; group: query heads per head.
-PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t heads, int64_t group, int64_t head_dim);
+PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t heads, int64_t group, int64_t head_dim,
+                     int format);
 
 hipError_t launch_cache_write(const CacheParams& p, int D, int format, hipStream_t stream);
 hipError_t launch_cache_read(const CacheParams& p, int D, int format, hipStream_t stream);

@@ -251,8 +251,8 @@ def test_c_abi_refuses_without_launching():
     assert write(rows=0) == 0 and read(tokens=0) == 0 and attend(rows=0) == 0  # nothing to do, nothing launched
     # Partial states of the calls that split their keys: none for short sequences.
     paged, window = lib.sol_paged_attention_workspace_size, lib.sol_window_attention_workspace_size
-    assert paged(3, 2, 2, 16, 4, 2, 64, 1, 0, 0) == 0 and paged(0, 2, 200, 16, 4, 2, 64, 1, 0, 0) == 0
-    assert paged(3, 2, 200, 16, 4, 2, 64, 1, 0, 0) > 0 and paged(3, 2, 200, 16, 4, 2, 64, 1, 10, 0) == 0
-    assert paged(3, 2, 200, 16, 4, 2, 96, 1, 0, 0) == -1 and paged(3, 2, 200, 16, 3, 2, 64, 1, 0, 0) == -1
+    assert paged(3, 2, 2, 16, 4, 2, 64, 0, 1, 0, 0) == 0 and paged(0, 2, 200, 16, 4, 2, 64, 0, 1, 0, 0) == 0
+    assert paged(3, 2, 200, 16, 4, 2, 64, 0, 1, 0, 0) > 0 and paged(3, 2, 200, 16, 4, 2, 64, 0, 1, 10, 0) == 0
+    assert paged(3, 2, 200, 16, 4, 2, 96, 0, 1, 0, 0) == -1 and paged(3, 2, 200, 16, 3, 2, 64, 0, 1, 0, 0) == -1
     assert window(1, 3, 5, 4, 2, 64, 1, 0, 0) == 0 and window(1, 3, 5000, 4, 2, 64, 1, 0, 0) > 0
     assert window(1, 0, 5, 4, 2, 64, 1, 0, 0) == -1 and window(1, 3, 5, 4, 2, 64, 1, -1, 0) == -1

@@ -31,7 +31,7 @@ def test_only_the_key_tile_dma_uses_m0(asm):
     for i, line in enumerate(code):
         if re.search(r"\bm0\b", line):
             assert re.fullmatch(r"s_mov_b32 m0, (s\d+|vcc_lo|vcc_hi)", line), f"unexpected use of M0: {line!r}"
-            assert code[i + 1] == "s_nop 0" and code[i + 2].startswith("global_load_lds_dwordx4")
+            assert code[i + 1] == "s_nop 0" and code[i + 2].startswith("global_load_lds_dword")
             writes += 1
     assert (writes > 0) == (source == "paged.hip")
 
