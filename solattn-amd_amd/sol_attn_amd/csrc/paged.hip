@@ -254,31 +254,48 @@ struct Keys {
     }
   }
 
-  // Through the scalar cache.  `tile` is uniform; groups past the last key
-  // take its page.
-  template <int TK>
-  __device__ __forceinline__ TilePages<TK> pages_of(int tile) const {
-    TilePages<TK> t;
-    t.valid = kAllGroups<TK>;
-    if constexpr (PAGED) {
-      typedef const int32_t __attribute__((address_space(4)))* scalar_ptr;
-      const scalar_ptr tab = (scalar_ptr)(uintptr_t)table;
-      t.valid = 0;
-#pragma unroll
-      for (int g = 0; g < TK / 16; ++g) {
-        const int page = tab[min(tile * TK + 16 * g, last) >> shift];
-        const bool ok = uint32_t(page) < uint32_t(pages);
-        t.page[g] = ok ? page : 0;
-        t.valid |= ok ? 1u << g : 0u;
-      }
-    }
-    return t;
-  }
-
   // Index in the cache of position pos, which lies in `page` (uniform).  The
   // rows of a group of 16 follow one another, those past the last key too.
   __device__ __forceinline__ int64_t row(int page, int pos) const {
     return ((int64_t(page) * H + h) << shift) + (pos & ((1 << shift) - 1));
+  }
+};
+
+// The pages of kTiles key tiles of a list, one lane per group of 16 rows, handed
+// out through the scalar registers (page numbers read one by one through the
+// scalar cache would make every wait for an LDS read wait for all of them).
+template <int D, int F, bool PAGED, int TK>
+struct PageWindow {
+  static constexpr int kGroups = TK / 16, kTiles = 64 / kGroups;
+  int id, page;
+  uint64_t ok;
+
+  // Starts the read of a window's page numbers; groups past the last key take
+  // its page.  tile_of(i): tile i of the window.
+  template <typename TileOf>
+  __device__ __forceinline__ void fetch(const Keys<D, F, PAGED>& keys, TileOf tile_of, int lane) {
+    if constexpr (PAGED) {
+      const int pos = min(tile_of(lane / kGroups) * TK + 16 * (lane % kGroups), keys.last);
+      id = keys.table[pos >> keys.shift];
+    }
+  }
+  // Makes the window read last the current one.
+  __device__ __forceinline__ void turn(const Keys<D, F, PAGED>& keys) {
+    if constexpr (PAGED) {
+      const bool in = uint32_t(id) < uint32_t(keys.pages);
+      page = in ? id : 0;
+      ok = __builtin_amdgcn_ballot_w64(in);
+    }
+  }
+  __device__ __forceinline__ TilePages<TK> get(int i) const {
+    TilePages<TK> t;
+    t.valid = kAllGroups<TK>;
+    if constexpr (PAGED) {
+#pragma unroll
+      for (int g = 0; g < kGroups; ++g) t.page[g] = __builtin_amdgcn_readlane(page, i * kGroups + g);
+      t.valid = uint32_t(ok >> (i * kGroups)) & kAllGroups<TK>;
+    }
+    return t;
   }
 };
 
@@ -374,9 +391,9 @@ __device__ __forceinline__ void add_nonfinite(State<D>& st, const uint16_t* slot
   }
 }
 
-// The rows of lane (col, hh): what its query sees, and whether it saw a key.
+// This lane's query: its position, and whether it saw a key.
 struct LaneRow {
-  Visible v;
+  int pos;
   bool any;
 };
 
@@ -399,10 +416,12 @@ __device__ __forceinline__ f32x16 key_factors(const float* half, int hh) {
 // `valid`: bits of the half's two groups of 16 rows that have a page.  scales:
 // the half's K scales in LDS (V's TK floats on), or null.
 template <int D, int TK>
-__device__ __forceinline__ void attend_masked(State<D>& st, LaneRow& row, f32x16 s, const uint16_t* slot, int t, int j0,
-                                              uint32_t valid, int lane_col, int lane_hh, float c,
-                                              const float* scales) {
+__device__ __forceinline__ void attend_masked(const PagedParams& p, int length, State<D>& st, LaneRow& row, f32x16 s,
+                                              const uint16_t* slot, int t, int j0, uint32_t valid, int lane_col,
+                                              int lane_hh, const float* scales) {
   const int col = fresh(lane_col), hh = fresh(lane_hh);
+  const float c = p.scale_log2;
+  const Visible v = visible(p, fresh(row.pos), length);  // not held in registers over the stream
   if (scales) {
     const f32x16 sk = key_factors(scales, hh);
 #pragma unroll
@@ -413,7 +432,7 @@ __device__ __forceinline__ void attend_masked(State<D>& st, LaneRow& row, f32x16
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
     const int j = a + 8 * (e >> 2) + (e & 3);
-    const bool in = (((j <= row.v.hi) & (j >= row.v.lo)) | (j < row.v.sink)) & (((valid >> (e >> 3)) & 1u) != 0);
+    const bool in = (((j <= v.hi) & (j >= v.lo)) | (j < v.sink)) & (((valid >> (e >> 3)) & 1u) != 0);
     s[e] = in ? s[e] : kNegInf;
     seen |= in ? 1u << e : 0u;
   }
@@ -445,15 +464,15 @@ __device__ __forceinline__ void attend_masked(State<D>& st, LaneRow& row, f32x16
   const bf16x8 pb[2] = {pack8(s, 0), pack8(s, 8)};
   // Scheduled apart from the scores: V's operands are not held meanwhile.
   chunk_end();
-  u32x4 v[2][Shape<D>::DT];
+  u32x4 vt[2][Shape<D>::DT];
   uint32_t bad = 0;
 #pragma unroll
   for (int c4 = 0; c4 < 2; ++c4)
 #pragma unroll
     for (int dt = 0; dt < Shape<D>::DT; ++dt) {
-      v[c4][dt] = TileImage<D, TK>::v(slot, col, hh, t, c4, dt);
+      vt[c4][dt] = TileImage<D, TK>::v(slot, col, hh, t, c4, dt);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) bad |= nonfinite(v[c4][dt][i]);
+      for (int i = 0; i < 4; ++i) bad |= nonfinite(vt[c4][dt][i]);
     }
   const bool some = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
   if (some) {
@@ -462,12 +481,12 @@ __device__ __forceinline__ void attend_masked(State<D>& st, LaneRow& row, f32x16
 #pragma unroll
       for (int dt = 0; dt < Shape<D>::DT; ++dt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[c4][dt][i] &= ~((nonfinite(v[c4][dt][i]) >> 15) * 0xFFFFu);
+        for (int i = 0; i < 4; ++i) vt[c4][dt][i] &= ~((nonfinite(vt[c4][dt][i]) >> 15) * 0xFFFFu);
   }
 #pragma unroll
   for (int c4 = 0; c4 < 2; ++c4)
 #pragma unroll
-    for (int dt = 0; dt < Shape<D>::DT; ++dt) st.acc[dt] = mfma32x32x16(as_bf16x8(v[c4][dt]), pb[c4], st.acc[dt]);
+    for (int dt = 0; dt < Shape<D>::DT; ++dt) st.acc[dt] = mfma32x32x16(as_bf16x8(vt[c4][dt]), pb[c4], st.acc[dt]);
   if (some) add_nonfinite<D, TK>(st, slot, t, hh, seen);
 }
 
@@ -679,38 +698,6 @@ struct StepSlot {
   }
 };
 
-// The pages of the next kTiles key tiles of a wave's list, one lane per group
-// of 16 rows; read once per kTiles tiles, and handed out through the scalar
-// registers.
-template <int D, int F, bool PAGED, int TK>
-struct PageWindow {
-  static constexpr int kGroups = TK / 16, kTiles = 64 / kGroups;
-  int page;
-  uint64_t ok;
-
-  // tile_of(i): tile i of the window.
-  template <typename TileOf>
-  __device__ __forceinline__ void fetch(const Keys<D, F, PAGED>& keys, TileOf tile_of, int lane) {
-    if constexpr (PAGED) {
-      const int pos = min(tile_of(lane / kGroups) * TK + 16 * (lane % kGroups), keys.last);
-      const int id = keys.table[pos >> keys.shift];
-      const bool in = uint32_t(id) < uint32_t(keys.pages);
-      page = in ? id : 0;
-      ok = __builtin_amdgcn_ballot_w64(in);
-    }
-  }
-  __device__ __forceinline__ TilePages<TK> get(int i) const {
-    TilePages<TK> t;
-    t.valid = kAllGroups<TK>;
-    if constexpr (PAGED) {
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g) t.page[g] = __builtin_amdgcn_readlane(page, i * kGroups + g);
-      t.valid = uint32_t(ok >> (i * kGroups)) & kAllGroups<TK>;
-    }
-    return t;
-  }
-};
-
 // 4-byte global -> LDS DMA per lane, each from an address of its own; lane l's
 // bytes land at LDS address m + 4 l (dma16's notes).
 __device__ __forceinline__ void dma4(uint64_t address, uint32_t m) {
@@ -854,12 +841,14 @@ __device__ __forceinline__ void step_nonfinite(StepState<D>& st, const uint8_t* 
 // keys_read() runs once K has been read, values_due() before V is, which starts
 // the next tile's K and waits for this one's V.
 template <int D, int F, bool MASKED, typename KeysRead, typename ValuesDue>
-__device__ __forceinline__ void step_tile(StepState<D>& st, LaneRow& row, const bf16x8 (&qf)[D / 32], const uint8_t* slot,
-                                          const StepSlot<D, F>& at, const float* scales, int tile, uint32_t valid,
-                                          int lane, float c, KeysRead keys_read, ValuesDue values_due) {
+__device__ __forceinline__ void step_tile(const PagedParams& p, int length, StepState<D>& st, LaneRow& row,
+                                          const bf16x8 (&qf)[D / 32], const uint8_t* slot, const StepSlot<D, F>& at,
+                                          const float* scales, int tile, uint32_t valid, int lane, KeysRead keys_read,
+                                          ValuesDue values_due) {
   using Slot = StepSlot<D, F>;
   constexpr int TK = Slot::TK, KB = TK / 16, FB = D / 16;
   constexpr bool SCALED = F != kBf16;
+  const float c = p.scale_log2;
   const int g = lane >> 4;
   f32x4 s[KB];
 #pragma unroll
@@ -888,12 +877,13 @@ __device__ __forceinline__ void step_tile(StepState<D>& st, LaneRow& row, const 
   keys_read();
   uint32_t seen = 0;
   if constexpr (MASKED) {
+    const Visible v = visible(p, fresh(row.pos), length);  // not held in registers over the stream
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int r = Slot::key(kb, g, e), j = tile * TK + r;
-        const bool in = (((j <= row.v.hi) & (j >= row.v.lo)) | (j < row.v.sink)) & (((valid >> (r >> 4)) & 1u) != 0);
+        const bool in = (((j <= v.hi) & (j >= v.lo)) | (j < v.sink)) & (((valid >> (r >> 4)) & 1u) != 0);
         s[kb][e] = in ? s[kb][e] : kNegInf;
         seen |= in ? 1u << (4 * kb + e) : 0u;
       }
@@ -996,7 +986,7 @@ __global__ __launch_bounds__(kNT, 2) void step_kernel(PagedParams p) {
   for (int ks = 0; ks < D / 32; ++ks)
     qf[ks] = as_bf16x8(load16(q + (SCALED ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1) : 32 * ks + 8 * g)));
   LaneRow row;
-  row.v = visible(p, pos0 + token, it.length);
+  row.pos = pos0 + token;
   row.any = false;
   const int first = pos0 + it.r0 / p.G, last = pos0 + (it.r0 + it.rows - 1) / p.G;
   const Span span = span_of<TK>(p, first, last, it.length);
@@ -1023,7 +1013,10 @@ __global__ __launch_bounds__(kNT, 2) void step_kernel(PagedParams p) {
     Window window;
     Dma dma(lds_address(slot), lds_address(scales), lane);
     auto prepare = [&](int k) {
-      if (k % Window::kTiles == 0) window.fetch(keys, [&](int i) { return tile_of(k + i); }, lane);
+      if (k % Window::kTiles == 0) {
+        window.fetch(keys, [&](int i) { return tile_of(k + i); }, lane);
+        window.turn(keys);
+      }
       dma.prepare(keys, tile_of(k), window.get(k % Window::kTiles));
     };
     // Tile k: its K is awaited, then its V, with the next tile's K on its way
@@ -1033,7 +1026,7 @@ __global__ __launch_bounds__(kNT, 2) void step_kernel(PagedParams p) {
       const uint32_t valid = dma.valid;
       wait_vmcnt<Dma::kLoads>();
       step_tile<D, F, decltype(masked)::value>(
-          st, row, qf, slot, at, scales, tile_of(k), valid, lane, p.scale_log2,
+          p, it.length, st, row, qf, slot, at, scales, tile_of(k), valid, lane,
           [&] {
             if (more) {
               prepare(k + 1);
@@ -1372,7 +1365,7 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
 #pragma unroll
   for (int ks = 0; ks < S::KT; ++ks) qf[ks] = as_bf16x8(load16(q + 16 * ks + 8 * hh));
   LaneRow row;
-  row.v = visible(p, pos0 + token, it.length);
+  row.pos = pos0 + token;
   row.any = false;
 
   const Span span = span_of<TK>(p, pos0 + it.r0 / p.G, pos0 + (it.r0 + it.rows - 1) / p.G, it.length);
@@ -1407,7 +1400,7 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
       for (int ks = 0; ks < S::KT; ++ks)
         s = mfma32x32x16(as_bf16x8(TileImage<D, TK>::k(buf, fcol, fhh, t, ks)), qf[ks], s);
       chunk_end();
-      attend_masked<D, TK>(st, row, s, buf, t, tile * TK + 32 * t, valid >> (2 * t), col, hh, p.scale_log2,
+      attend_masked<D, TK>(p, it.length, st, row, s, buf, t, tile * TK + 32 * t, valid >> (2 * t), col, hh,
                            SCALED ? scales + 32 * t : nullptr);
     }
   };
@@ -1433,38 +1426,51 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
   };
 
   if (t0 < t1) {
-    TilePages<TK> now = keys.template pages_of<TK>(at(t0)), next = keys.template pages_of<TK>(at(t0 + 1));
+    using Window = PageWindow<D, F, PAGED, TK>;
+    Window window;
+    auto fetch = [&](int i) { window.fetch(keys, [&](int k) { return at(i + k); }, lane); };
+    // The pages of tile i, asked for in order of i.  The next window is read half
+    // a window ahead.
+    auto pages_of = [&](int i) {
+      const int k = (i - t0) % Window::kTiles;
+      if (k == 0) window.turn(keys);
+      if (k == Window::kTiles / 2) fetch(i + Window::kTiles / 2);
+      return window.get(k);
+    };
+    fetch(t0);
+    TilePages<TK> next = pages_of(t0);
+    uint32_t valid = next.valid;  // of the tile at hand
     if constexpr (!SCALED) {
       uint32_t lanes[2];
       DmaTile<D, PAGED>::lane_offsets(keys, wave, lane, lanes);
-      DmaTile<D, PAGED>(keys, now, at(t0), ring_lds, wave, lane, lanes).all();
+      DmaTile<D, PAGED>(keys, next, at(t0), ring_lds, wave, lane, lanes).all();
       stream([&](int i, auto&& attend) {
         wait_vmcnt<0>();
         lds_barrier();
         const int slot = (i - t0) & 1;
+        const uint32_t now = valid;
+        next = pages_of(i + 1);
+        valid = next.valid;
         // Past the last tile that tile again, into the slot nobody reads.
         const DmaTile<D, PAGED> refill(keys, next, at(i + 1), ring_lds + uint32_t((slot ^ 1) * S::TILE * 2), wave, lane,
                                        lanes);
-        const uint32_t valid = now.valid;
-        now = next;
-        next = keys.template pages_of<TK>(at(i + 2));
-        attend(at(i), valid, ring[slot], static_cast<const float*>(nullptr), refill);
-      }, now.valid);
+        attend(at(i), now, ring[slot], static_cast<const float*>(nullptr), refill);
+      }, valid);
       wait_vmcnt<0>();
     } else {
       CodeTile<D, F> code;
-      code.load(keys, now, at(t0), wave, lane);
+      code.load(keys, next, at(t0), wave, lane);
       code.put(ring[0], s_scale[0], tid);
       stream([&](int i, auto&& attend) {
         lds_barrier();
         const int slot = (i - t0) & 1;
+        const uint32_t now = valid;
+        next = pages_of(i + 1);
+        valid = next.valid;
         code.load(keys, next, at(i + 1), wave, lane);
-        const uint32_t valid = now.valid;
-        now = next;
-        next = keys.template pages_of<TK>(at(i + 2));
-        attend(at(i), valid, ring[slot], s_scale[slot], NoStep{});
+        attend(at(i), now, ring[slot], s_scale[slot], NoStep{});
         code.put(ring[slot ^ 1], s_scale[slot ^ 1], tid);
-      }, now.valid);
+      }, valid);
     }
   }
 
@@ -1518,6 +1524,29 @@ void launch_format(const PagedParams& p, const PagedSize& size, int format, hipS
 
 }  // namespace
 
+namespace {
+
+constexpr int64_t kResident = 512;  // workgroups of either kernel that the card holds at once (two per CU)
+
+// Workgroups per head that the wide kernel's keys are split for, or 0.  `tiles`
+// row tiles per head of `key_tiles` key tiles each run in rounds of kResident
+// workgroups; in q parts each they take ceil(q tiles heads / kResident) rounds of
+// key_tiles / q key tiles, and kPartCost more for every part (its set-up, its
+// partial state written and joined).
+int64_t wide_target(int64_t tiles, int64_t heads, int64_t key_tiles, int64_t min_tiles) {
+  constexpr double kPartCost = 6.0;
+  auto cost = [&](int64_t q) {
+    const int64_t rounds = (q * tiles * heads + kResident - 1) / kResident;
+    return double(rounds) * (double(key_tiles) / double(q) + (q > 1 ? 2.0 : 1.0) * kPartCost);
+  };
+  int64_t best = 1;
+  for (int64_t q = 2; q <= 64 && key_tiles / q >= min_tiles; ++q)
+    if (cost(q) < cost(best)) best = q;
+  return best > 1 && cost(best) < 0.95 * cost(1) ? best * tiles : 0;
+}
+
+}  // namespace
+
 PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t heads, int64_t group, int64_t head_dim,
                      int format) {
   PagedSize s;
@@ -1527,13 +1556,12 @@ PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t head
   s.tiles = rows * group / s.rows + sequences;  // row tiles: sum ceil(n_s G / R) at most
   const int64_t key_tiles = (keys + TK - 1) / TK;
   s.min_tiles = step ? 8 : 4;
-  s.target = 0;
-  if (key_tiles > s.min_tiles) {
-    if (step)
-      s.target = (1024 + heads - 1) / heads;
-    else if (s.tiles * heads < 512)
-      s.target = (512 + heads - 1) / heads;
-  }
+  if (key_tiles <= s.min_tiles)
+    s.target = 0;
+  else if (step)
+    s.target = (2 * kResident + heads - 1) / heads;
+  else
+    s.target = wide_target((rows * group + s.rows - 1) / s.rows + (sequences - 1) / 2, heads, key_tiles, s.min_tiles);
   s.grid = (s.target + s.tiles) * heads;
   s.header_bytes = (s.tiles * heads * int64_t(sizeof(Header)) + 15) / 16 * 16;
   s.merge_rows = std::min(s.rows, (rows * group + sequences - 1) / sequences);
