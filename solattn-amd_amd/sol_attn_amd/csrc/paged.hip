@@ -214,18 +214,10 @@ __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item
 
 // ---- where the keys lie -----------------------------------------------------
 
-// The pages of a key tile's groups of 16 rows (a page holds at least 16), and
-// a bit for each group that has one.
-template <int TK>
-struct TilePages {
-  int page[TK / 16];
-  uint32_t valid;
-};
-
+// Key tiles are cut into groups of 16 rows, each of which lies in one page (a
+// page holds at least 16); a bit for each group that has a page.
 template <int TK>
 constexpr uint32_t kAllGroups = (1u << (TK / 16)) - 1u;
-
-__device__ __forceinline__ int pick(bool second, int a, int b) { return second ? b : a; }
 
 // K and V rows of one (sequence, head): in a cache, rows of kRowBytes that
 // both operands (and their scales) have at the same index; or plain, at strides
@@ -253,21 +245,19 @@ struct Keys {
       st[kv] = PAGED ? kRowBytes : uint32_t(p.st[kv]);
     }
   }
-
-  // Index in the cache of position pos, which lies in `page` (uniform).  The
-  // rows of a group of 16 follow one another, those past the last key too.
-  __device__ __forceinline__ int64_t row(int page, int pos) const {
-    return ((int64_t(page) * H + h) << shift) + (pos & ((1 << shift) - 1));
-  }
 };
 
-// The pages of kTiles key tiles of a list, one lane per group of 16 rows, handed
-// out through the scalar registers (page numbers read one by one through the
-// scalar cache would make every wait for an LDS read wait for all of them).
+// Where the groups of kTiles key tiles of a list begin, one lane per group:
+// byte offsets from the cache's first K (V) row, handed out through the scalar
+// registers.  (Page numbers read one by one through the scalar cache made every
+// wait for an LDS read wait for all of them, and their address arithmetic came
+// before each tile's products.)
 template <int D, int F, bool PAGED, int TK>
 struct PageWindow {
   static constexpr int kGroups = TK / 16, kTiles = 64 / kGroups;
-  int id, page;
+  static constexpr uint32_t kRowBytes = D * kElemBytes<F>;
+  int id, pos;
+  uint32_t lo, hi;
   uint64_t ok;
 
   // Starts the read of a window's page numbers; groups past the last key take
@@ -275,27 +265,36 @@ struct PageWindow {
   template <typename TileOf>
   __device__ __forceinline__ void fetch(const Keys<D, F, PAGED>& keys, TileOf tile_of, int lane) {
     if constexpr (PAGED) {
-      const int pos = min(tile_of(lane / kGroups) * TK + 16 * (lane % kGroups), keys.last);
-      id = keys.table[pos >> keys.shift];
+      pos = tile_of(lane / kGroups) * TK + 16 * (lane % kGroups);
+      id = keys.table[min(pos, keys.last) >> keys.shift];
     }
   }
   // Makes the window read last the current one.
   __device__ __forceinline__ void turn(const Keys<D, F, PAGED>& keys) {
     if constexpr (PAGED) {
       const bool in = uint32_t(id) < uint32_t(keys.pages);
-      page = in ? id : 0;
       ok = __builtin_amdgcn_ballot_w64(in);
+      const uint64_t row = ((uint64_t(in ? uint32_t(id) : 0u) * uint32_t(keys.H) + uint32_t(keys.h)) << keys.shift) +
+                           uint32_t(pos & ((1 << keys.shift) - 1));
+      lo = uint32_t(row * kRowBytes);
+      hi = uint32_t(row * kRowBytes >> 32);
     }
   }
-  __device__ __forceinline__ TilePages<TK> get(int i) const {
-    TilePages<TK> t;
-    t.valid = kAllGroups<TK>;
-    if constexpr (PAGED) {
-#pragma unroll
-      for (int g = 0; g < kGroups; ++g) t.page[g] = __builtin_amdgcn_readlane(page, i * kGroups + g);
-      t.valid = uint32_t(ok >> (i * kGroups)) & kAllGroups<TK>;
-    }
-    return t;
+  // Group g of tile i.
+  __device__ __forceinline__ uint64_t offset(int i, int g) const {
+    if constexpr (!PAGED) return 0;
+    const uint32_t l = uint32_t(__builtin_amdgcn_readlane(lo, i * kGroups + g));
+    const uint32_t h = uint32_t(__builtin_amdgcn_readlane(hi, i * kGroups + g));
+    return uint64_t(h) << 32 | l;
+  }
+  // Row of the cache (of both operands and their scales) of row `row` of tile i, per lane.
+  __device__ __forceinline__ uint64_t row(int i, int row) const {
+    const int from = i * kGroups + (row >> 4);
+    return (uint64_t(uint32_t(__shfl(int(hi), from))) << 32 | uint32_t(__shfl(int(lo), from))) / kRowBytes + (row & 15);
+  }
+  __device__ __forceinline__ uint32_t valid(int i) const {
+    if constexpr (!PAGED) return kAllGroups<TK>;
+    return uint32_t(ok >> (i * kGroups)) & kAllGroups<TK>;
   }
 };
 
@@ -729,9 +728,8 @@ struct StepDma {
   uint32_t slot, scales;
   int tile, lane;
   uint32_t valid;
-  int64_t group[PAGED ? TK / 16 : 1];  // row of the cache that each group begins at
-  int page;                            // this lane's, for the scales (one lane per row of 64)
-  int page2;
+  uint64_t group[PAGED ? TK / 16 : 1];  // where each group begins
+  uint64_t scale_row[kScales ? kScales : 1];
 
   __device__ __forceinline__ StepDma(uint32_t slot_lds, uint32_t scales_lds, int l) : slot(slot_lds), scales(scales_lds), lane(l) {
     constexpr int kRowLanes = Slot::kRow / 16;
@@ -747,21 +745,16 @@ struct StepDma {
     }
   }
 
-  __device__ __forceinline__ void prepare(const Source& keys, int t, const TilePages<TK>& pages) {
+  // Tile t, the window's tile i.
+  template <typename Window>
+  __device__ __forceinline__ void prepare(const Window& window, int i, int t) {
     tile = t;
-    valid = pages.valid;
+    valid = window.valid(i);
     if constexpr (PAGED) {
 #pragma unroll
-      for (int g = 0; g < TK / 16; ++g) group[g] = keys.row(pages.page[g], t * TK + 16 * g);
-      if constexpr (kScales > 0) {
-        page = pages.page[0];
-        page2 = pages.page[kScales > 1 ? 4 : 0];
+      for (int g = 0; g < TK / 16; ++g) group[g] = window.offset(i, g);
 #pragma unroll
-        for (int g = 1; g < 4; ++g) {
-          page = lane >= 16 * g ? pages.page[g] : page;
-          if constexpr (kScales > 1) page2 = lane >= 16 * g ? pages.page[4 + g] : page2;
-        }
-      }
+      for (int n = 0; n < kScales; ++n) scale_row[n] = window.row(i, 64 * n + lane);
     }
   }
 
@@ -775,7 +768,7 @@ struct StepDma {
                                : 16u * Slot::k_swizzle(r);
       const uint32_t dst = slot + uint32_t(kv * Slot::kPlane + i * 1024);
       if constexpr (PAGED) {
-        dma16(base + uint64_t(group[r / 16]) * Slot::kRow + round_offset(uint32_t(r % 16) * Slot::kRow),
+        dma16(base + group[r / 16] + uint32_t(r % 16) * Slot::kRow,
               row[kv] * Slot::kRow + (chunk[kv] ^ flip), dst);
       } else {
         const int first = min(tile * TK + r, keys.last);
@@ -785,7 +778,7 @@ struct StepDma {
     }
 #pragma unroll
     for (int n = 0; n < kScales; ++n)
-      dma4(reinterpret_cast<uint64_t>(keys.scale[kv] + keys.row(n ? page2 : page, tile * TK + 64 * n + lane)),
+      dma4(reinterpret_cast<uint64_t>(keys.scale[kv] + scale_row[n]),
            scales + uint32_t(kv * TK + 64 * n) * 4u);
   }
 };
@@ -1017,7 +1010,7 @@ __global__ __launch_bounds__(kNT, 2) void step_kernel(PagedParams p) {
         window.fetch(keys, [&](int i) { return tile_of(k + i); }, lane);
         window.turn(keys);
       }
-      dma.prepare(keys, tile_of(k), window.get(k % Window::kTiles));
+      dma.prepare(window, k % Window::kTiles, tile_of(k));
     };
     // Tile k: its K is awaited, then its V, with the next tile's K on its way
     // meanwhile and its V from the end on (each wave on its own, no barrier).
@@ -1137,7 +1130,9 @@ struct DmaTile {
                     : (l % (D / 8)) ^ TileLayout<D>::k_swizzle(wave * kPieceRows + l / (D / 8)));
   }
 
-  __device__ __forceinline__ DmaTile(const Source& keys, const TilePages<64>& pages, int tile, uint32_t dst, int w,
+  // Tile `tile`, the window's tile i.
+  template <typename Window>
+  __device__ __forceinline__ DmaTile(const Source& keys, const Window& window, int i, int tile, uint32_t dst, int w,
                                      int lane_id, const uint32_t (&lanes)[2])
       : l(lane_id), wave(w) {
     last = keys.last;
@@ -1150,24 +1145,23 @@ struct DmaTile {
       lane[kv] = lanes[kv];
     }
     if constexpr (PAGED) {
+      // The piece begins w kPieceRows % 16 rows into its group (lane_offsets).
 #pragma unroll
-      for (int r = 0; r < kHalf; ++r) {
-        const int page = D == 128 ? pages.page[r] : pick(w >= 2, pages.page[2 * r], pages.page[2 * r + 1]);
-        off[r] = uint64_t(keys.row(page, pos0 + r * kRoundRows)) * Source::kRowBytes;
-      }
+      for (int r = 0; r < kHalf; ++r) off[r] = window.offset(i, D == 128 ? r : 2 * r + (w >> 1));
     }
     lds = dst + uint32_t(w) * 1024u;
   }
   // This lane's offsets in whole tiles.
   __device__ __forceinline__ static void lane_offsets(const Source& keys, int w, int lane_id, uint32_t (&lanes)[2]) {
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv) lanes[kv] = lane_row(kv, lane_id) * keys.st[kv] + lane_byte(kv, lane_id, w);
+    for (int kv = 0; kv < 2; ++kv)
+      lanes[kv] = ((PAGED ? w * kPieceRows % 16 : 0) + lane_row(kv, lane_id)) * keys.st[kv] + lane_byte(kv, lane_id, w);
   }
   __device__ __forceinline__ void round(int i) const {
     const int kv = i / kHalf, r = i % kHalf;
     const uint32_t dst = lds + uint32_t(kv * 64 * D * 2 + r * kNT * 16);
     if constexpr (PAGED) {
-      dma16(base[kv] + off[r] + round_offset(0u), lane[kv], dst);
+      dma16(base[kv] + off[r], lane[kv], dst);
     } else {
       const int pos = pos0 + r * kRoundRows, first = min(pos, last);
       uint32_t at = lane[kv];
@@ -1202,24 +1196,20 @@ struct CodeTile {
   u32x4 x[2][kLoads];
   float scale;
 
-  __device__ __forceinline__ void load(const Keys<D, F, true>& keys, const TilePages<64>& pages, int tile, int wave,
-                                       int lane) {
+  // The window's tile i.
+  template <typename Window>
+  __device__ __forceinline__ void load(const Keys<D, F, true>& keys, const Window& window, int i, int wave, int lane) {
     const int l = fresh(lane);
-    const uint32_t off = uint32_t(l / kRowLanes) * keys.kRowBytes + 16u * (l % kRowLanes);
     // A wave's 64 chunks are 8 (D = 128) or 16 rows of one group.
+    const uint32_t off = uint32_t(wave * kWave / kRowLanes % 16 + l / kRowLanes) * keys.kRowBytes + 16u * (l % kRowLanes);
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int page = D == 128 ? pick(wave >= 2, pages.page[2 * i], pages.page[2 * i + 1])
-                                : pick(wave >= 2, pick(wave & 1, pages.page[0], pages.page[1]),
-                                       pick(wave & 1, pages.page[2], pages.page[3]));
-      const int64_t at = keys.row(page, tile * 64 + (i * kNT + wave * kWave) / kRowLanes) * keys.kRowBytes;
+    for (int n = 0; n < kLoads; ++n) {
+      const uint64_t at = window.offset(i, D == 128 ? 2 * n + (wave >> 1) : wave);
 #pragma unroll
-      for (int kv = 0; kv < 2; ++kv) x[kv][i] = load_chunk(keys.base[kv] + at + off);
+      for (int kv = 0; kv < 2; ++kv) x[kv][n] = load_chunk(keys.base[kv] + at + off);
     }
-    if (wave < 2) {  // wave 0 the keys' scales, wave 1 the values'
-      const int page = pick(l >= 32, pick(l & 16, pages.page[0], pages.page[1]), pick(l & 16, pages.page[2], pages.page[3]));
-      scale = (wave ? keys.scale[1] : keys.scale[0])[keys.row(page, tile * 64 + l)];
-    }
+    // Wave 0 the keys' scales, wave 1 the values'.
+    if (wave < 2) scale = (wave ? keys.scale[1] : keys.scale[0])[window.row(i, l)];
   }
   __device__ __forceinline__ void put(uint16_t* slot, float* scales, int thread) const {
     using Image = TileImage<D, 64>;
@@ -1287,12 +1277,14 @@ __device__ __forceinline__ void wide_tile(State<D>& st, const uint16_t* buf, con
                                           const bf16x8 (&qf)[Shape<D>::KT], int col, int hh, float c,
                                           const Refill& refill) {
   constexpr int KT = Shape<D>::KT, DT = Shape<D>::DT;
-  constexpr int kAhead = SCALED ? 2 : 4;
+  constexpr int kAhead = SCALED ? 2 : (D == 64 ? 8 : 4);
   const FragLane<D> fl(fresh(col), fresh(hh));
   const uint32_t vbase = fl.v_base(buf);
-  // Operand n of the tile's 2 KT K operands, and of its 4 DT V operands.
-  auto kfrag = [&](int n) { return fl.k(buf, n / KT, n % KT); };
-  auto vfrag = [&](int n) { return fl.v(vbase, n / (2 * DT), n / DT % 2, n % DT); };
+  // Operand n of the tile's 2 KT K and 4 DT V operands.
+  auto operand = [&](int n) {
+    const int f = n - 2 * KT;
+    return n < 2 * KT ? fl.k(buf, n / KT, n % KT) : fl.v(vbase, f / (2 * DT), f / DT % 2, f % DT);
+  };
   auto raw = [&](int t) {
     const FragLane<D> fr(fresh(col), fresh(hh));
     f32x16 s = zero16();
@@ -1301,41 +1293,48 @@ __device__ __forceinline__ void wide_tile(State<D>& st, const uint16_t* buf, con
     if (SCALED) WideHalf<D, SCALED>::scale(s, scales + 32 * t, hh);
     return s;
   };
-  u32x4 k[kAhead], v[kAhead];
+  u32x4 o[kAhead];
 #pragma unroll
-  for (int n = 0; n < kAhead; ++n) k[n] = kfrag(n);
+  for (int n = 0; n < kAhead; ++n) o[n] = operand(n);
   WideHalf<D, SCALED> h0, h1;
   h0.s = zero16();
   h1.s = zero16();
   chunk_end();
+  // Operand n is taken, then the one kAhead on asked for in its place.
+  auto next = [&](int n) { return as_bf16x8(o[n % kAhead]); };
+  auto ask = [&](int n) {
+    if (n + kAhead < 2 * KT + 4 * DT) o[n % kAhead] = operand(n + kAhead);
+  };
 #pragma unroll
   for (int n = 0; n < KT; ++n) {
-    h0.s = mfma32x32x16(as_bf16x8(k[n % kAhead]), qf[n], h0.s);
-    k[n % kAhead] = kfrag(n + kAhead);
+    h0.s = mfma32x32x16(next(n), qf[n], h0.s);
+    ask(n);
     refill.template after_step<2 * KT>(n);
     chunk_end();
   }
   if (SCALED) h0.scale(h0.s, scales, hh);
 #pragma unroll
-  for (int n = KT; n < 2 * KT; ++n) {
-    h1.s = mfma32x32x16(as_bf16x8(k[n % kAhead]), qf[n - KT], h1.s);
-    if (n + kAhead < 2 * KT)
-      k[n % kAhead] = kfrag(n + kAhead);
-    else
-      v[n + kAhead - 2 * KT] = vfrag(n + kAhead - 2 * KT);
-    h0.template step<KT>(n - KT, st, c, scales + 64, hh);
-    refill.template after_step<2 * KT>(n);
+  for (int n = 0; n < KT; ++n) {
+    h1.s = mfma32x32x16(next(KT + n), qf[n], h1.s);
+    ask(KT + n);
+    h0.template step<KT>(n, st, c, scales + 64, hh);
+    refill.template after_step<2 * KT>(KT + n);
     chunk_end();
   }
   h0.finish(st, c, scales + 64, hh, [&] { return raw(0); });
   if (SCALED) h1.scale(h1.s, scales + 32, hh);
 #pragma unroll
-  for (int n = 0; n < 4 * DT; ++n) {
-    const int f = n % (2 * DT);
-    if (n == 2 * DT) h1.finish(st, c, scales + 96, hh, [&] { return raw(1); });
-    st.acc[f % DT] = mfma32x32x16(as_bf16x8(v[n % kAhead]), n < 2 * DT ? h0.pb(f / DT) : h1.pb(f / DT), st.acc[f % DT]);
-    if (n + kAhead < 4 * DT) v[n % kAhead] = vfrag(n + kAhead);
-    if (n < 2 * DT) h1.template step<2 * DT>(f, st, c, scales + 96, hh);
+  for (int f = 0; f < 2 * DT; ++f) {
+    st.acc[f % DT] = mfma32x32x16(next(2 * KT + f), h0.pb(f / DT), st.acc[f % DT]);
+    ask(2 * KT + f);
+    h1.template step<2 * DT>(f, st, c, scales + 96, hh);
+    chunk_end();
+  }
+  h1.finish(st, c, scales + 96, hh, [&] { return raw(1); });
+#pragma unroll
+  for (int f = 0; f < 2 * DT; ++f) {
+    st.acc[f % DT] = mfma32x32x16(next(2 * KT + 2 * DT + f), h1.pb(f / DT), st.acc[f % DT]);
+    ask(2 * KT + 2 * DT + f);
     chunk_end();
   }
 }
@@ -1429,45 +1428,45 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
     using Window = PageWindow<D, F, PAGED, TK>;
     Window window;
     auto fetch = [&](int i) { window.fetch(keys, [&](int k) { return at(i + k); }, lane); };
-    // The pages of tile i, asked for in order of i.  The next window is read half
-    // a window ahead.
-    auto pages_of = [&](int i) {
+    // Makes tile i's pages current, in order of i; returns its place in the
+    // window.  The next window is read half a window ahead.
+    auto turn_to = [&](int i) {
       const int k = (i - t0) % Window::kTiles;
       if (k == 0) window.turn(keys);
       if (k == Window::kTiles / 2) fetch(i + Window::kTiles / 2);
-      return window.get(k);
+      return k;
     };
     fetch(t0);
-    TilePages<TK> next = pages_of(t0);
-    uint32_t valid = next.valid;  // of the tile at hand
+    int k = turn_to(t0);
+    uint32_t valid = window.valid(k);  // of the tile at hand
     if constexpr (!SCALED) {
       uint32_t lanes[2];
       DmaTile<D, PAGED>::lane_offsets(keys, wave, lane, lanes);
-      DmaTile<D, PAGED>(keys, next, at(t0), ring_lds, wave, lane, lanes).all();
+      DmaTile<D, PAGED>(keys, window, k, at(t0), ring_lds, wave, lane, lanes).all();
       stream([&](int i, auto&& attend) {
         wait_vmcnt<0>();
         lds_barrier();
         const int slot = (i - t0) & 1;
         const uint32_t now = valid;
-        next = pages_of(i + 1);
-        valid = next.valid;
+        k = turn_to(i + 1);
+        valid = window.valid(k);
         // Past the last tile that tile again, into the slot nobody reads.
-        const DmaTile<D, PAGED> refill(keys, next, at(i + 1), ring_lds + uint32_t((slot ^ 1) * S::TILE * 2), wave, lane,
-                                       lanes);
+        const DmaTile<D, PAGED> refill(keys, window, k, at(i + 1), ring_lds + uint32_t((slot ^ 1) * S::TILE * 2), wave,
+                                       lane, lanes);
         attend(at(i), now, ring[slot], static_cast<const float*>(nullptr), refill);
       }, valid);
       wait_vmcnt<0>();
     } else {
       CodeTile<D, F> code;
-      code.load(keys, next, at(t0), wave, lane);
+      code.load(keys, window, k, wave, lane);
       code.put(ring[0], s_scale[0], tid);
       stream([&](int i, auto&& attend) {
         lds_barrier();
         const int slot = (i - t0) & 1;
         const uint32_t now = valid;
-        next = pages_of(i + 1);
-        valid = next.valid;
-        code.load(keys, next, at(i + 1), wave, lane);
+        k = turn_to(i + 1);
+        valid = window.valid(k);
+        code.load(keys, window, k, wave, lane);
         attend(at(i), now, ring[slot], s_scale[slot], NoStep{});
         code.put(ring[slot ^ 1], s_scale[slot ^ 1], tid);
       }, valid);
