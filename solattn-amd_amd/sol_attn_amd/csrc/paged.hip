@@ -1103,11 +1103,11 @@ __global__ __launch_bounds__(kNT, 2) void step_kernel(PagedParams p) {
 
 // The DMA of a BF16 key tile into an LDS slot, in kRounds rounds per wave of 1
 // KB each: round r of K (then of V) moves rows R0 = r kRoundRows + wave
-// kPieceRows on, all in one group of 16, so its address is one uniform row
-// address and a per-lane offset that is the same in every round (the swizzles
-// repeat).  Plain keys' tail tile repeats the last key instead of reading past
-// it (its lanes' offsets are formed per round); a page's rows past the last key
-// exist.
+// kPieceRows on, all in one group of 16.  In a cache a round's address is its
+// group's, and a lane's offset the same in every round (the swizzles repeat; a
+// page's rows past the last key exist).  Plain keys take the tile's first row
+// and a lane's own, which stops at the last key: no branch for the tail tile
+// (one per round took 5% of the kernel's time).
 template <int D, bool PAGED>
 struct DmaTile {
   using Source = Keys<D, kBf16, PAGED>;
@@ -1115,58 +1115,54 @@ struct DmaTile {
   static constexpr int kRounds = 2 * kHalf;
   static constexpr int kRoundRows = kNT * 16 / (2 * D);
   static constexpr int kPieceRows = kRoundRows / kWaves;
-  uint64_t base[2], off[PAGED ? kHalf : 1];
-  uint32_t lane[2];  // per-lane offsets in a whole tile
+  // What a lane keeps over the stream, per operand: paged, its offset; plain,
+  // its row and its chunk of the row.
+  struct Lane {
+    uint32_t off[2];
+    uint32_t row[2];
+    __device__ __forceinline__ Lane(int w, int l) {
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        const int m = D == 128 ? l : l % 32;  // of a quad (V)
+        const int r = kv ? (D == 128 ? 0 : 4 * (l / 32)) + ((m >> 2) & 3) : l / (D / 8);
+        const int c = kv ? 4 * (m >> 4) + (m & 3) : (l % (D / 8)) ^ TileLayout<D>::k_swizzle(w * kPieceRows + r);
+        row[kv] = w * kPieceRows + r;
+        off[kv] = PAGED ? (w * kPieceRows % 16 + r) * Source::kRowBytes + 16 * c : c;
+      }
+    }
+  };
+  const Lane& lane;
+  uint64_t src[2], off[PAGED ? kHalf : 1];
   uint32_t lds, st[2];
-  int pos0, last, l, wave;
-  bool tail;
-
-  __device__ __forceinline__ static int lane_row(int kv, int l) {
-    return kv ? (D == 128 ? 0 : 4 * (l / 32)) + ((l >> 2) & 3) : l / (D / 8);
-  }
-  __device__ __forceinline__ static int lane_byte(int kv, int l, int wave) {
-    const int m = D == 128 ? l : l % 32;
-    return 16 * (kv ? 4 * (m >> 4) + (m & 3)
-                    : (l % (D / 8)) ^ TileLayout<D>::k_swizzle(wave * kPieceRows + l / (D / 8)));
-  }
+  int last;  // plain: the last key's row of the tile
 
   // Tile `tile`, the window's tile i.
   template <typename Window>
   __device__ __forceinline__ DmaTile(const Source& keys, const Window& window, int i, int tile, uint32_t dst, int w,
-                                     int lane_id, const uint32_t (&lanes)[2])
-      : l(lane_id), wave(w) {
-    last = keys.last;
-    tail = !PAGED && tile * 64 + 63 > last;
-    pos0 = tile * 64 + w * kPieceRows;
+                                     const Lane& lanes)
+      : lane(lanes) {
+    last = keys.last - tile * 64;
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
-      base[kv] = reinterpret_cast<uint64_t>(keys.base[kv]);
-      st[kv] = keys.st[kv];
-      lane[kv] = lanes[kv];
+      src[kv] = reinterpret_cast<uint64_t>(keys.base[kv]);
+      if constexpr (!PAGED) src[kv] += uint64_t(uint32_t(tile * 64)) * keys.st[kv];
+      st[kv] = keys.st[kv] / 16;  // below 2^21: token strides are below 2^24 elements
     }
     if constexpr (PAGED) {
-      // The piece begins w kPieceRows % 16 rows into its group (lane_offsets).
+      // The wave's piece begins w kPieceRows % 16 rows into its group (Lane).
 #pragma unroll
       for (int r = 0; r < kHalf; ++r) off[r] = window.offset(i, D == 128 ? r : 2 * r + (w >> 1));
     }
     lds = dst + uint32_t(w) * 1024u;
   }
-  // This lane's offsets in whole tiles.
-  __device__ __forceinline__ static void lane_offsets(const Source& keys, int w, int lane_id, uint32_t (&lanes)[2]) {
-#pragma unroll
-    for (int kv = 0; kv < 2; ++kv)
-      lanes[kv] = ((PAGED ? w * kPieceRows % 16 : 0) + lane_row(kv, lane_id)) * keys.st[kv] + lane_byte(kv, lane_id, w);
-  }
   __device__ __forceinline__ void round(int i) const {
     const int kv = i / kHalf, r = i % kHalf;
     const uint32_t dst = lds + uint32_t(kv * 64 * D * 2 + r * kNT * 16);
     if constexpr (PAGED) {
-      dma16(base[kv] + off[r], lane[kv], dst);
+      dma16(src[kv] + off[r], lane.off[kv], dst);
     } else {
-      const int pos = pos0 + r * kRoundRows, first = min(pos, last);
-      uint32_t at = lane[kv];
-      if (tail) at = uint32_t(min(pos + lane_row(kv, fresh(l)), last) - first) * st[kv] + lane_byte(kv, fresh(l), wave);
-      dma16(base[kv] + uint64_t(uint32_t(first)) * st[kv] + round_offset(0u), at, dst);
+      const uint32_t row = min(int(lane.row[kv]) + r * kRoundRows, last);
+      dma16(src[kv] + round_offset(0u), (__umul24(row, st[kv]) + lane.off[kv]) * 16u, dst);
     }
   }
   __device__ __forceinline__ void all() const {
@@ -1440,9 +1436,8 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
     int k = turn_to(t0);
     uint32_t valid = window.valid(k);  // of the tile at hand
     if constexpr (!SCALED) {
-      uint32_t lanes[2];
-      DmaTile<D, PAGED>::lane_offsets(keys, wave, lane, lanes);
-      DmaTile<D, PAGED>(keys, window, k, at(t0), ring_lds, wave, lane, lanes).all();
+      const typename DmaTile<D, PAGED>::Lane lanes(wave, lane);
+      DmaTile<D, PAGED>(keys, window, k, at(t0), ring_lds, wave, lanes).all();
       stream([&](int i, auto&& attend) {
         wait_vmcnt<0>();
         lds_barrier();
@@ -1452,7 +1447,7 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
         valid = window.valid(k);
         // Past the last tile that tile again, into the slot nobody reads.
         const DmaTile<D, PAGED> refill(keys, window, k, at(i + 1), ring_lds + uint32_t((slot ^ 1) * S::TILE * 2), wave,
-                                       lane, lanes);
+                                       lanes);
         attend(at(i), now, ring[slot], static_cast<const float*>(nullptr), refill);
       }, valid);
       wait_vmcnt<0>();
