@@ -413,13 +413,13 @@ __device__ __forceinline__ f32x16 key_factors(const float* half, int hh) {
 // and O^T += V^T P^T,
 // hidden keys taking no part, whatever their score, value and scale hold.
 // `valid`: bits of the half's two groups of 16 rows that have a page.  scales:
-// the half's K scales in LDS (V's TK floats on), or null.
+// the half's K scales times c in LDS (V's scales TK floats on), or null.
 template <int D, int TK>
 __device__ __forceinline__ void attend_masked(const PagedParams& p, int length, State<D>& st, LaneRow& row, f32x16 s,
                                               const uint16_t* slot, int t, int j0, uint32_t valid, int lane_col,
                                               int lane_hh, const float* scales) {
   const int col = fresh(lane_col), hh = fresh(lane_hh);
-  const float c = p.scale_log2;
+  const float c = scales ? 1.f : p.scale_log2;
   const Visible v = visible(p, fresh(row.pos), length);  // not held in registers over the stream
   if (scales) {
     const f32x16 sk = key_factors(scales, hh);
@@ -1174,13 +1174,9 @@ struct DmaTile {
 #pragma unroll
     for (int r = k * kRounds / N; r < (k + 1) * kRounds / N; ++r) round(r);
   }
-};
-
-// Nothing to move beside a tile's products.
-struct NoStep {
-  __device__ __forceinline__ void all() const {}
+  __device__ __forceinline__ void late() const {}
   template <int N>
-  __device__ __forceinline__ void after_step(int) const {}
+  __device__ __forceinline__ void late_step(int) const {}
 };
 
 // An 8-bit key tile on its way, in the workgroup's registers: loaded while
@@ -1207,31 +1203,67 @@ struct CodeTile {
     // Wave 0 the keys' scales, wave 1 the values'.
     if (wave < 2) scale = (wave ? keys.scale[1] : keys.scale[0])[window.row(i, l)];
   }
-  __device__ __forceinline__ void put(uint16_t* slot, float* scales, int thread) const {
+  // Converts piece n of kPieces (16 codes of a row) into its place.
+  static constexpr int kPieces = 2 * kLoads;
+  __device__ __forceinline__ void put(uint16_t* slot, int n, int thread) const {
     using Image = TileImage<D, 64>;
-    const int tid = fresh(thread);
-#pragma unroll
-    for (int kv = 0; kv < 2; ++kv)
-#pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const int row = (i * kNT + tid) / kRowLanes, c = tid % kRowLanes;
-        Image::put(slot, kv, row, 2 * c, codes_to_bf16<F>(x[kv][i][0], x[kv][i][1]));
-        Image::put(slot, kv, row, 2 * c + 1, codes_to_bf16<F>(x[kv][i][2], x[kv][i][3]));
-      }
-    if (tid < 128) scales[tid] = scale;
+    const int tid = fresh(thread), kv = n / kLoads, i = n % kLoads;
+    const int row = (i * kNT + tid) / kRowLanes, c = tid % kRowLanes;
+    Image::put(slot, kv, row, 2 * c, codes_to_bf16<F>(x[kv][i][0], x[kv][i][1]));
+    Image::put(slot, kv, row, 2 * c + 1, codes_to_bf16<F>(x[kv][i][2], x[kv][i][3]));
   }
 };
 
-// FastHalf with the values' scales (SCALED): the probabilities are multiplied
-// by them before they are packed.
+// The next tile's codes beside a tile's products: they are converted beside
+// half 1's P V, which has no other vector work, or at the end.  K's scales are
+// kept times c.
+template <int D, int F>
+struct CodeRefill {
+  const CodeTile<D, F>& code;
+  uint16_t* slot;
+  float* scales;
+  int tid;
+  float c;
+  __device__ __forceinline__ void all() const {}
+  template <int N>
+  __device__ __forceinline__ void after_step(int) const {}
+  // Step k of N.
+  template <int N>
+  __device__ __forceinline__ void late_step(int k) const {
+    constexpr int P = CodeTile<D, F>::kPieces;
+    static_assert(N % P == 0, "a piece every N / P steps");
+    if (k % (N / P) == 0) code.put(slot, k / (N / P), tid);
+    if (k == N - 1 && tid < 128) scales[tid] = tid < 64 ? code.scale * c : code.scale;
+  }
+  __device__ __forceinline__ void late() const {
+#pragma unroll
+    for (int n = 0; n < CodeTile<D, F>::kPieces; ++n) late_step<CodeTile<D, F>::kPieces>(n);
+  }
+};
+
+// FastHalf with per-key factors (SCALED): the scores take K's scales (times c)
+// in the place of c, four at a time, and the probabilities V's before they are
+// packed.
 template <int D, bool SCALED>
 struct WideHalf : FastHalf<D> {
+  f32x4 factor;  // of the next four scores
+
+  // half: the half's K factors in LDS, V's 64 floats on.
+  __device__ __forceinline__ void ask(const float* half, int q, int hh) {
+    if constexpr (SCALED) factor = *reinterpret_cast<const f32x4*>(half + 8 * q + 4 * hh);
+  }
   template <int N>
-  __device__ __forceinline__ void step(int k, State<D>& st, float c, const float* sv, int hh) {
+  __device__ __forceinline__ void step(int k, State<D>& st, float c, const float* half, int hh) {
 #pragma unroll
     for (int i = k * 8 / N; i < (k + 1) * 8 / N; ++i) {
-      if (SCALED && i == 5) scale(this->s, sv, hh);
-      this->stage(i, st, c);
+      if (SCALED && i < 4) {
+        const f32x4 f = factor;
+        if (i < 3) ask(half, i + 1, hh);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) this->s[4 * i + e] *= f[e];
+      }
+      if (SCALED && i == 5) scale(this->s, half + 64, hh);
+      this->stage(i, st, SCALED ? 1.f : c);
     }
   }
   __device__ static __forceinline__ void scale(f32x16& x, const float* factors, int hh) {
@@ -1243,15 +1275,20 @@ struct WideHalf : FastHalf<D> {
     }
   }
   template <typename Raw>
-  __device__ __forceinline__ void finish(State<D>& st, float c, const float* sv, int hh, Raw raw) {
+  __device__ __forceinline__ void finish(State<D>& st, float c, const float* half, int hh, Raw raw) {
     if (this->redo) {
       HalfSoftmax<D> full;
       full.s = raw();
+      const int fh = fresh(hh);
+      if (SCALED) scale(full.s, half, fh);
+      const float cs = SCALED ? 1.f : c;
+      chunk_end();
 #pragma unroll
-      for (int i = 0; i < 6; ++i) full.stage(i, st, c);
-      if (SCALED) scale(full.s, sv, hh);
-      full.stage(6, st, c);
-      full.stage(7, st, c);
+      for (int i = 0; i < 6; ++i) full.stage(i, st, cs);
+      chunk_end();
+      if (SCALED) scale(full.s, half + 64, fh);
+      full.stage(6, st, cs);
+      full.stage(7, st, cs);
       if (full.rescale) rescale_acc<D>(st, full.alpha);
       this->pw[0] = full.pw[0];
       this->pw[1] = full.pw[1];
@@ -1285,8 +1322,10 @@ __device__ __forceinline__ void wide_tile(State<D>& st, const uint16_t* buf, con
     const FragLane<D> fr(fresh(col), fresh(hh));
     f32x16 s = zero16();
 #pragma unroll
-    for (int ks = 0; ks < KT; ++ks) s = mfma32x32x16(as_bf16x8(fr.k(buf, t, ks)), qf[ks], s);
-    if (SCALED) WideHalf<D, SCALED>::scale(s, scales + 32 * t, hh);
+    for (int ks = 0; ks < KT; ++ks) {
+      s = mfma32x32x16(as_bf16x8(fr.k(buf, t, ks)), qf[ks], s);
+      chunk_end();
+    }
     return s;
   };
   u32x4 o[kAhead];
@@ -1308,29 +1347,30 @@ __device__ __forceinline__ void wide_tile(State<D>& st, const uint16_t* buf, con
     refill.template after_step<2 * KT>(n);
     chunk_end();
   }
-  if (SCALED) h0.scale(h0.s, scales, hh);
+  h0.ask(scales, 0, hh);
 #pragma unroll
   for (int n = 0; n < KT; ++n) {
     h1.s = mfma32x32x16(next(KT + n), qf[n], h1.s);
     ask(KT + n);
-    h0.template step<KT>(n, st, c, scales + 64, hh);
+    h0.template step<KT>(n, st, c, scales, hh);
     refill.template after_step<2 * KT>(KT + n);
     chunk_end();
   }
-  h0.finish(st, c, scales + 64, hh, [&] { return raw(0); });
-  if (SCALED) h1.scale(h1.s, scales + 32, hh);
+  h0.finish(st, c, scales, hh, [&] { return raw(0); });
+  h1.ask(scales + 32, 0, hh);
 #pragma unroll
   for (int f = 0; f < 2 * DT; ++f) {
     st.acc[f % DT] = mfma32x32x16(next(2 * KT + f), h0.pb(f / DT), st.acc[f % DT]);
     ask(2 * KT + f);
-    h1.template step<2 * DT>(f, st, c, scales + 96, hh);
+    h1.template step<2 * DT>(f, st, c, scales + 32, hh);
     chunk_end();
   }
-  h1.finish(st, c, scales + 96, hh, [&] { return raw(1); });
+  h1.finish(st, c, scales + 32, hh, [&] { return raw(1); });
 #pragma unroll
   for (int f = 0; f < 2 * DT; ++f) {
     st.acc[f % DT] = mfma32x32x16(next(2 * KT + 2 * DT + f), h1.pb(f / DT), st.acc[f % DT]);
     ask(2 * KT + 2 * DT + f);
+    refill.template late_step<2 * DT>(f);
     chunk_end();
   }
 }
@@ -1381,7 +1421,10 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
     if (wrows <= 0 || ((a > vb.hi || b < va.lo) && a >= vb.sink)) return kHidden;
     return valid == kAllGroups<TK> && b <= va.hi && (a >= vb.lo || b < va.sink) ? kWhole : kPart;
   };
-  auto hidden = [&](int, uint32_t, const uint16_t*, const float*, const auto& refill) { refill.all(); };
+  auto hidden = [&](int, uint32_t, const uint16_t*, const float*, const auto& refill) {
+    refill.all();
+    refill.late();
+  };
   auto whole = [&](int, uint32_t, const uint16_t* buf, const float* scales, const auto& refill) {
     wide_tile<D, SCALED>(st, buf, scales, qf, col, hh, p.scale_log2, refill);
   };
@@ -1398,6 +1441,7 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
       attend_masked<D, TK>(p, it.length, st, row, s, buf, t, tile * TK + 32 * t, valid >> (2 * t), col, hh,
                            SCALED ? scales + 32 * t : nullptr);
     }
+    refill.late();
   };
   // One tile after another; consecutive tiles of a kind run in a loop of their
   // own, so that the sums are not split across a branch per tile.  The waves of
@@ -1454,7 +1498,7 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
     } else {
       CodeTile<D, F> code;
       code.load(keys, window, k, wave, lane);
-      code.put(ring[0], s_scale[0], tid);
+      CodeRefill<D, F>{code, ring[0], s_scale[0], tid, p.scale_log2}.late();
       stream([&](int i, auto&& attend) {
         lds_barrier();
         const int slot = (i - t0) & 1;
@@ -1462,8 +1506,8 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
         k = turn_to(i + 1);
         valid = window.valid(k);
         code.load(keys, window, k, wave, lane);
-        attend(at(i), now, ring[slot], s_scale[slot], NoStep{});
-        code.put(ring[slot ^ 1], s_scale[slot ^ 1], tid);
+        attend(at(i), now, ring[slot], s_scale[slot],
+               CodeRefill<D, F>{code, ring[slot ^ 1], s_scale[slot ^ 1], tid, p.scale_log2});
       }, valid);
     }
   }
