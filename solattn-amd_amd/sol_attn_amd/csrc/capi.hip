@@ -1056,7 +1056,7 @@ int sol_paged_attention(const void* q, const int64_t* q_strides, int64_t rows, c
     return fail(SOL_ERR_UNSUPPORTED, "sol_paged_attention: grid too large");
   const sol::PagedSize size =
       sol::paged_size(rows, sequences, window_keys(rows, table_width * page_size, causal, window, sink_tokens), heads,
-                      query_heads / heads, head_dim, format);
+                      query_heads / heads, head_dim, format, causal != 0, true);
   rc = paged_workspace_ok(what, size, workspace, workspace_bytes);
   if (rc != SOL_OK) return rc;
   p.q = static_cast<const uint16_t*>(q);
@@ -1084,7 +1084,7 @@ int64_t sol_paged_attention_workspace_size(int64_t rows, int64_t sequences, int6
     return -1;
   if (rows == 0) return 0;
   return sol::paged_size(rows, sequences, window_keys(rows, table_width * page_size, causal, window, sink_tokens), heads,
-                         query_heads / heads, head_dim, format).bytes;
+                         query_heads / heads, head_dim, format, causal != 0, true).bytes;
 }
 
 int sol_window_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
@@ -1106,7 +1106,7 @@ int sol_window_attention(const void* q, const int64_t* q_strides, const void* k,
     return fail(SOL_ERR_UNSUPPORTED, "sol_window_attention: K and V token strides must be below 2^24 elements");
   const sol::PagedSize size =
       sol::paged_size(batch * query_tokens, batch, window_keys(query_tokens, key_tokens, causal, window, sink_tokens),
-                      heads, query_heads / heads, head_dim, SOL_CACHE_BF16);
+                      heads, query_heads / heads, head_dim, SOL_CACHE_BF16, causal != 0, false);
   rc = paged_workspace_ok(what, size, workspace, workspace_bytes);
   if (rc != SOL_OK) return rc;
   sol::PagedParams p;
@@ -1134,7 +1134,7 @@ int64_t sol_window_attention_workspace_size(int64_t batch, int64_t query_tokens,
     return -1;
   return sol::paged_size(batch * query_tokens, batch,
                          window_keys(query_tokens, key_tokens, causal, window, sink_tokens), heads,
-                         query_heads / heads, head_dim, SOL_CACHE_BF16).bytes;
+                         query_heads / heads, head_dim, SOL_CACHE_BF16, causal != 0, false).bytes;
 }
 
 }  // extern "C"

@@ -89,7 +89,7 @@ struct Item {
 struct Header {
   int parts;         // 0: nothing
   int off, r0, rows; // Item's
-  uint32_t first;    // record of its first part; the next ones are p.H apart
+  uint32_t first, step;  // record of its first part, and from one part to the next
 };
 
 // Partial states of split tiles, after the headers: per workgroup (record) and
@@ -123,7 +123,7 @@ template <int R, int TK>
 __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item& it) {
   __shared__ int64_t s_total[kWaves];
   __shared__ int s_tiles[kWaves];
-  __shared__ int s_found[5];
+  __shared__ int s_found[6];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int S = p.batch.S;
   // Row tiles and key tiles of sequence s.
@@ -181,12 +181,14 @@ __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item
       all_tiles += s_tiles[w];
     }
     if (id >= end - mine && id < end) {
+      // Row tile by row tile of a part (they read the same keys), the longest first.
       const int k = int(id - (end - mine));
       s_found[0] = s;
-      s_found[1] = p.causal ? rt - 1 - k / parts : k / parts;  // the longest first
-      s_found[2] = k % parts;
+      s_found[1] = p.causal ? rt - 1 - k % rt : k % rt;
+      s_found[2] = k / rt;
       s_found[3] = parts;
-      s_found[4] = tile_end - rt + k / parts;
+      s_found[4] = tile_end - rt + k % rt;
+      s_found[5] = rt;
     }
     __syncthreads();
     base += int64_t(uniform64(uint64_t(all)));
@@ -196,7 +198,7 @@ __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item
   if (id >= base) {
     // The launch has as many workgroups without an item as headers without a
     // tile, at least.
-    if (p.records) write_header(p, tiles + (id - base), Header{0, 0, 0, 0, 0});
+    if (p.records) write_header(p, tiles + (id - base), Header{0, 0, 0, 0, 0, 0});
     return false;
   }
   it.s = __builtin_amdgcn_readfirstlane(s_found[0]);
@@ -208,7 +210,9 @@ __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item
   it.part = __builtin_amdgcn_readfirstlane(s_found[2]);
   it.parts = __builtin_amdgcn_readfirstlane(s_found[3]);
   if (p.records && it.part == 0)
-    write_header(p, __builtin_amdgcn_readfirstlane(s_found[4]), Header{it.parts > 1 ? it.parts : 0, it.off, it.r0, it.rows, blockIdx.x});
+    write_header(p, __builtin_amdgcn_readfirstlane(s_found[4]),
+                 Header{it.parts > 1 ? it.parts : 0, it.off, it.r0, it.rows, blockIdx.x,
+                        uint32_t(__builtin_amdgcn_readfirstlane(s_found[5])) * uint32_t(p.H)});
   return true;
 }
 
@@ -508,11 +512,12 @@ __device__ __forceinline__ void store4(uint16_t* out, const f32x4& x, float den,
 }
 
 // Joins the parts of split tiles: m = max_s m_s, O = sum_s 2^(m_s - m) acc_s /
-// sum_s 2^(m_s - m) den_s.  A workgroup per (row tile, head) and every
-// gridDim.y-th row of it.  D / 4 lanes take 4 features each; the waves and
-// their 256 / D such groups of lanes take the parts in turn, kMergeAhead each
-// in flight, and their states join in a fixed order.
-constexpr int kMergeAhead = 4;
+// sum_s 2^(m_s - m) den_s.  A workgroup per (row tile, head) and some of its
+// rows.  D / 4 lanes take 4 features each.  Tiles of 16 rows have many parts
+// and few rows: a row at a time, the 1,024 / D such groups of lanes take the
+// parts in turn, kMergeAhead each in flight, and their states join in a fixed
+// order.  Tiles of 128 rows have few parts: each group takes a row of its own.
+constexpr int kMergeAhead = 8;
 
 // A state of the merge: sums of 4 features, and the row's maximum, denominator
 // and whether a key was seen.
@@ -532,53 +537,73 @@ struct Joined {
   }
 };
 
+// Joins every `stride`-th part of a row from part `first` on; `row`: its record
+// in part 0, `step` floats on the next part's.
+template <int D>
+__device__ __forceinline__ Joined join_parts(const float* row, int64_t step, int parts, int first, int stride, int c) {
+  Joined mine = {{0.f, 0.f, 0.f, 0.f}, kNegInf, 0.f, 0.f};
+  for (int s0 = first; s0 < parts; s0 += stride * kMergeAhead) {
+    f32x4 tail[kMergeAhead], x[kMergeAhead];
+#pragma unroll
+    for (int u = 0; u < kMergeAhead; ++u) {
+      const float* at = row + min(s0 + u * stride, parts - 1) * step;
+      tail[u] = *reinterpret_cast<const f32x4*>(at + D);
+      x[u] = *reinterpret_cast<const f32x4*>(at + 4 * c);
+    }
+#pragma unroll
+    for (int u = 0; u < kMergeAhead; ++u)
+      if (s0 + u * stride < parts) mine.add(Joined{x[u], tail[u][0], tail[u][1], tail[u][2]});
+  }
+  return mine;
+}
+
+// Rows that a workgroup of the merge takes at once.
+template <int D, int R>
+constexpr int kMergeRows = R == 16 ? 1 : kNT / (D / 4);
+
 template <int D, int R>
 __global__ __launch_bounds__(kNT) void merge_kernel(PagedParams p) {
-  constexpr int kLanes = D / 4, kGroups = kWave / kLanes, kSlots = kWaves * kGroups;
+  constexpr int kLanes = D / 4, kSlots = kNT / kLanes;
   __shared__ Joined s_state[kWaves][kLanes];
   Header hd = static_cast<const Header*>(p.workspace)[blockIdx.x];
   // Offsets that do not ascend can leave headers of another call here, and name
   // more parts than the launch has: nothing outside the tensors is touched.
-  if (hd.parts <= 1 || int64_t(hd.first) >= p.records || hd.rows <= 0 || hd.rows > R || hd.off < 0 || hd.r0 < 0 ||
-      int64_t(hd.off) + (int64_t(hd.r0) + hd.rows - 1) / p.G >= p.new_rows)
+  if (hd.parts <= 1 || int64_t(hd.first) >= p.records || hd.step == 0 || hd.rows <= 0 || hd.rows > R || hd.off < 0 ||
+      hd.r0 < 0 || int64_t(hd.off) + (int64_t(hd.r0) + hd.rows - 1) / p.G >= p.new_rows)
     return;
-  hd.parts = min(hd.parts, int((p.records - 1 - hd.first) / p.H) + 1);
+  hd.parts = int(min(int64_t(hd.parts), (p.records - 1 - hd.first) / hd.step + 1));
   const int h = blockIdx.x % p.H, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane % kLanes;
-  const int slot = wave * kGroups + lane / kLanes;
-  const int64_t step = int64_t(p.H) * R * kRecordRow<D>;
-  for (int r = blockIdx.y; r < hd.rows; r += gridDim.y) {
-    const float* base = record<D, R>(p, hd.first) + r * kRecordRow<D>;
-    Joined mine = {{0.f, 0.f, 0.f, 0.f}, kNegInf, 0.f, 0.f};
-    for (int s0 = slot; s0 < hd.parts; s0 += kSlots * kMergeAhead) {
-      f32x4 tail[kMergeAhead], x[kMergeAhead];
+  const int slot = threadIdx.x / kLanes;
+  const int64_t step = int64_t(hd.step) * R * kRecordRow<D>;
+  const float* base = record<D, R>(p, hd.first);
+  auto store = [&](int r, const Joined& x) {
+    store4(p.out + output_row<D>(p, hd.off, hd.r0 + r, h) + 4 * c, x.o, x.den, x.any != 0.f);
+  };
+  if constexpr (kMergeRows<D, R> > 1) {
+    for (int r = blockIdx.y * kSlots + slot; r < hd.rows; r += gridDim.y * kSlots)
+      store(r, join_parts<D>(base + r * kRecordRow<D>, step, hd.parts, 0, 1, c));
+  } else {
+    for (int r = blockIdx.y; r < hd.rows; r += gridDim.y) {
+      Joined mine = join_parts<D>(base + r * kRecordRow<D>, step, hd.parts, slot, kSlots, c);
 #pragma unroll
-      for (int u = 0; u < kMergeAhead; ++u) {
-        const float* at = base + min(s0 + u * kSlots, hd.parts - 1) * step;
-        tail[u] = *reinterpret_cast<const f32x4*>(at + D);
-        x[u] = *reinterpret_cast<const f32x4*>(at + 4 * c);
+      for (int off = kLanes; off < kWave; off <<= 1) {
+        Joined other;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) other.o[k] = __shfl_xor(mine.o[k], off);
+        other.m = __shfl_xor(mine.m, off);
+        other.den = __shfl_xor(mine.den, off);
+        other.any = __shfl_xor(mine.any, off);
+        mine.add(other);
       }
+      if (lane < kLanes) s_state[wave][lane] = mine;
+      __syncthreads();
+      if (wave == 0 && lane < kLanes) {
 #pragma unroll
-      for (int u = 0; u < kMergeAhead; ++u)
-        if (s0 + u * kSlots < hd.parts) mine.add(Joined{x[u], tail[u][0], tail[u][1], tail[u][2]});
+        for (int w = 1; w < kWaves; ++w) mine.add(s_state[w][lane]);
+        store(r, mine);
+      }
+      __syncthreads();
     }
-#pragma unroll
-    for (int off = kLanes; off < kWave; off <<= 1) {
-      Joined other;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) other.o[k] = __shfl_xor(mine.o[k], off);
-      other.m = __shfl_xor(mine.m, off);
-      other.den = __shfl_xor(mine.den, off);
-      other.any = __shfl_xor(mine.any, off);
-      mine.add(other);
-    }
-    if (lane < kLanes) s_state[wave][lane] = mine;
-    __syncthreads();
-    if (wave == 0 && lane < kLanes) {
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) mine.add(s_state[w][lane]);
-      store4(p.out + output_row<D>(p, hd.off, hd.r0 + r, h) + 4 * c, mine.o, mine.den, mine.any != 0.f);
-    }
-    __syncthreads();
   }
 }
 
@@ -1536,8 +1561,8 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
 
 template <int D, int R>
 void launch_merge(const PagedParams& p, const PagedSize& size, hipStream_t stream) {
-  hipLaunchKernelGGL((merge_kernel<D, R>), dim3(unsigned(size.tiles * p.H), unsigned(size.merge_rows)), dim3(kNT), 0,
-                     stream, p);
+  const unsigned rows = unsigned((size.merge_rows - 1) / kMergeRows<D, R> + 1);
+  hipLaunchKernelGGL((merge_kernel<D, R>), dim3(unsigned(size.tiles * p.H), rows), dim3(kNT), 0, stream, p);
 }
 
 template <int D, int F, bool PAGED>
@@ -1566,11 +1591,13 @@ namespace {
 
 constexpr int64_t kResident = 512;  // workgroups of either kernel that the card holds at once (two per CU)
 
-// Workgroups per head that the wide kernel's keys are split for, or 0.  `tiles`
-// row tiles per head of `key_tiles` key tiles each run in rounds of kResident
-// workgroups; in q parts each they take ceil(q tiles heads / kResident) rounds of
-// key_tiles / q key tiles, and kPartCost more for every part (its set-up, its
-// partial state written and joined).
+// Workgroups per head that the wide kernel's keys are split for, or 0, where all
+// row tiles have as many key tiles.  `tiles` row tiles per head of `key_tiles` key
+// tiles each run in rounds of kResident workgroups; in q parts each they take
+// ceil(q tiles heads / kResident) rounds of key_tiles / q key tiles, and kPartCost
+// more for every part (its set-up, its partial state written and joined).  (128
+// queries of 8 heads over 32,768 keys: 46 us in 32 parts, 54 in 64, 561 in one.
+// 2,048 queries over themselves, 32 heads: 54 us in one part, 59 in two.)
 int64_t wide_target(int64_t tiles, int64_t heads, int64_t key_tiles, int64_t min_tiles) {
   constexpr double kPartCost = 6.0;
   auto cost = [&](int64_t q) {
@@ -1578,7 +1605,7 @@ int64_t wide_target(int64_t tiles, int64_t heads, int64_t key_tiles, int64_t min
     return double(rounds) * (double(key_tiles) / double(q) + (q > 1 ? 2.0 : 1.0) * kPartCost);
   };
   int64_t best = 1;
-  for (int64_t q = 2; q <= 64 && key_tiles / q >= min_tiles; ++q)
+  for (int64_t q = 2; q <= 32 && key_tiles / q >= min_tiles; ++q)
     if (cost(q) < cost(best)) best = q;
   return best > 1 && cost(best) < 0.95 * cost(1) ? best * tiles : 0;
 }
@@ -1586,20 +1613,40 @@ int64_t wide_target(int64_t tiles, int64_t heads, int64_t key_tiles, int64_t min
 }  // namespace
 
 PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t heads, int64_t group, int64_t head_dim,
-                     int format) {
+                     int format, bool causal, bool ragged) {
   PagedSize s;
+  // Few rows per sequence: the step kernel, whose tiles are 16 rows.
   const bool step = rows * group <= 32 * sequences;
   s.rows = step ? 16 : 128;
   const int64_t TK = step ? 8192 / (head_dim * (format == kBf16 ? 2 : 1)) : 64;  // StepSlot::TK
   s.tiles = rows * group / s.rows + sequences;  // row tiles: sum ceil(n_s G / R) at most
+  const int64_t likely = (rows * group + s.rows - 1) / s.rows + (sequences - 1) / 2;
   const int64_t key_tiles = (keys + TK - 1) / TK;
-  s.min_tiles = step ? 8 : 4;
-  if (key_tiles <= s.min_tiles)
-    s.target = 0;
-  else if (step)
-    s.target = (2 * kResident + heads - 1) / heads;
-  else
-    s.target = wide_target((rows * group + s.rows - 1) / s.rows + (sequences - 1) / 2, heads, key_tiles, s.min_tiles);
+  // Row tiles that differ in their keys: other sequences, or the rows of a triangle.
+  const bool uneven = (ragged && sequences > 1) || (causal && 2 * rows > keys * sequences);
+  s.target = 0;
+  if (step) {
+    // A second launch costs 5 us, as much as 16 queries over 48 BF16 key tiles or
+    // 20 of codes take alone (16 sequences, 4 heads: 1,024 BF16 keys 13.6 us whole,
+    // 18.3 split; 4,096 33.5 and 30.7; INT8 1,024 18.0 and 19.8, 2,048 29 and 20).
+    // One round of workgroups (one sequence of 84,672 INT8 keys, 8 heads: 44 us,
+    // 51 in two rounds), but two where the sequences alone fill half the card
+    // and may differ (48 of 300 .. 19,003 keys: 318 us, 330 in one round; 64 of
+    // 8,192: 373 and 361).
+    s.min_tiles = 8;
+    const int64_t rounds = ragged && 2 * sequences * heads >= kResident ? 2 : 1;
+    if (key_tiles > (format == kBf16 ? 48 : 20)) s.target = (rounds * kResident + heads - 1) / heads;
+  } else if (uneven && 2 * likely * heads * key_tiles >= 3 * kResident * 24) {
+    // Enough keys for one and a half rounds of parts of 24 tiles: those even the
+    // lengths out (8 sequences of 600 .. 12,000 keys, 512 new tokens of 8 x 4
+    // heads: 505 us, 687 with the rule below; 8,192 queries over themselves, 4
+    // heads: 116 and 135).
+    s.min_tiles = 24;
+    if (key_tiles > s.min_tiles) s.target = (3 * kResident / 2 + heads - 1) / heads;
+  } else {
+    s.min_tiles = 4;
+    if (key_tiles > s.min_tiles) s.target = wide_target(likely, heads, key_tiles, s.min_tiles);
+  }
   s.grid = (s.target + s.tiles) * heads;
   s.header_bytes = (s.tiles * heads * int64_t(sizeof(Header)) + 15) / 16 * 16;
   s.merge_rows = std::min(s.rows, (rows * group + sequences - 1) / sequences);

@@ -75,7 +75,7 @@ struct PagedSize {
 
 // rows: new tokens in all; keys: a sequence's at most; group: query heads per head.
 PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t heads, int64_t group, int64_t head_dim,
-                     int format);
+                     int format, bool causal, bool ragged);
 
 hipError_t launch_cache_write(const CacheParams& p, int D, int format, hipStream_t stream);
 hipError_t launch_cache_read(const CacheParams& p, int D, int format, hipStream_t stream);
