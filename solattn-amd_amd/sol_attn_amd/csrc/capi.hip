@@ -875,6 +875,7 @@ namespace {
 
 constexpr int64_t kRowsStrideMax = int64_t(1) << 24;  // elements between plain keys
 constexpr int64_t kMaxPositions = int64_t(1) << 30;  // positions of one sequence, and new rows of one call
+constexpr int64_t kMaxGrid = (int64_t(1) << 24) - 1;  // workgroups: a launch has fewer than 2^32 threads
 
 // Checks a sequence batch over a cache (its arrays' contents the kernels
 // check themselves) and its sizes, and fills `b`.
@@ -945,7 +946,7 @@ int64_t window_keys(int64_t rows, int64_t keys, int causal, int64_t window, int6
 }
 
 int paged_workspace_ok(const char* what, const sol::PagedSize& size, const void* workspace, int64_t workspace_bytes) {
-  if (size.grid >= (int64_t(1) << 31)) {
+  if (size.grid > kMaxGrid) {
     g_last_error = std::string(what) + ": grid too large";
     return SOL_ERR_UNSUPPORTED;
   }
@@ -988,7 +989,9 @@ int sol_cache_write(const void* k, const int64_t* k_strides, const void* v, cons
   if (rows == 0) return SOL_OK;
   if (!operand_ok(k, k_strides, true) || !operand_ok(v, v_strides, true))
     return fail(SOL_ERR_INVALID, "sol_cache_write: K and V need 16-byte aligned rows and positive strides");
-  if (rows * heads >= (int64_t(1) << 33)) return fail(SOL_ERR_UNSUPPORTED, "sol_cache_write: grid too large");
+  // A workgroup takes 2,048 / head_dim rows of a head.
+  if (cdiv(rows, 512 / head_dim) * heads > 4 * kMaxGrid)
+    return fail(SOL_ERR_UNSUPPORTED, "sol_cache_write: grid too large");
   p.rows[0] = static_cast<const uint16_t*>(k);
   p.rows[1] = static_cast<const uint16_t*>(v);
   p.st[0] = k_strides[1], p.sh[0] = k_strides[2];
@@ -1018,7 +1021,7 @@ int sol_cache_read(const void* cache_k, const void* cache_v, const float* k_scal
   if (tokens == 0) return SOL_OK;
   if (!k_out || !v_out || !aligned16(k_out) || !aligned16(v_out))
     return fail(SOL_ERR_INVALID, "sol_cache_read: the outputs must be 16-byte aligned");
-  if (sequences * cdiv(tokens, 4) * heads >= (int64_t(1) << 33))
+  if (sequences * cdiv(tokens, 512 / head_dim) > 4 * kMaxGrid / heads)
     return fail(SOL_ERR_UNSUPPORTED, "sol_cache_read: grid too large");
   p.store[0] = const_cast<uint8_t*>(static_cast<const uint8_t*>(cache_k));
   p.store[1] = const_cast<uint8_t*>(static_cast<const uint8_t*>(cache_v));

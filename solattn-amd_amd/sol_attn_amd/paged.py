@@ -153,6 +153,8 @@ def _validate(cache, plan, device):
             or min(shape) <= 0 or not k.is_contiguous() or not v.is_contiguous()
             or (k.data_ptr() | v.data_ptr()) & 15):
         raise ValueError("Invalid cache tensors; use PagedCache.create")
+    if k.requires_grad or v.requires_grad:
+        raise ValueError("Inference only: the cache must not require gradients")
     if shape[3] not in (64, 128):
         raise ValueError("Only head dimensions 64 and 128 are implemented")
     _page_size(shape[2])
@@ -253,6 +255,8 @@ def paged_attention(q, cache, plan, *, causal=True, window=None, sink_tokens=0, 
     if out is not None and (out.dtype != torch.bfloat16 or out.shape != q.shape or not out.is_contiguous()
                             or out.device != q.device or out.data_ptr() & 15):
         raise ValueError("out must be a contiguous BF16 tensor shaped like Q on its device")
+    if out is not None and out.requires_grad:
+        raise ValueError("Inference only: out must not require gradients")
     if out is not None and (_overlap(out, q) or _overlap(out, cache.k) or _overlap(out, cache.v)):
         raise ValueError("out must not share memory with Q or the cache")
     with _on(q.device):

@@ -256,3 +256,48 @@ def test_c_abi_refuses_without_launching():
     assert paged(3, 2, 200, 16, 4, 2, 96, 0, 1, 0, 0) == -1 and paged(3, 2, 200, 16, 3, 2, 64, 0, 1, 0, 0) == -1
     assert window(1, 3, 5, 4, 2, 64, 1, 0, 0) == 0 and window(1, 3, 5000, 4, 2, 64, 1, 0, 0) > 0
     assert window(1, 0, 5, 4, 2, 64, 1, 0, 0) == -1 and window(1, 3, 5, 4, 2, 64, 1, -1, 0) == -1
+
+
+def test_c_abi_refuses_launches_of_too_many_threads():
+    # 2^24 workgroups of 256 threads and more.
+    if not os.path.exists(_native.LIB_PATH):
+        pytest.skip("libsol_attn_amd.so not built")
+    lib = _native.library()
+    fake, odd = ctypes.c_void_p(1 << 20), ctypes.c_void_p((1 << 20) + 8)  # never dereferenced
+    ok = (ctypes.c_int64 * 3)(1 << 40, 128, 64)
+
+    def write(rows, heads, dim):
+        return lib.sol_cache_write(fake, ok, fake, ok, rows, fake, fake, fake, 2, 2, 4, 16, heads, dim, 0, fake, fake,
+                                   None, None, None)
+
+    def read(seqs, tokens, heads, dim):
+        return lib.sol_cache_read(fake, fake, None, None, fake, fake, seqs, 2, 4, 16, heads, dim, 0, 0, tokens, fake,
+                                  fake, None)
+
+    def attend(rows, seqs, heads, width=2, ws=None):
+        return lib.sol_paged_attention(fake, ok, rows, fake, fake, None, None, fake, fake, fake, seqs, width, 4, 16,
+                                       heads, heads, 64, 0, 0.125, 1, 0, 0, ws, 16, fake, None)
+
+    def plain(batch, tq, heads):
+        return lib.sol_window_attention(fake, ok, fake, ok, fake, ok, batch, tq, 20, heads, heads, 64, 0.125, 1, 0, 0,
+                                        odd, 16, fake, None)
+
+    for call in (lambda: write(1 << 24, 16, 128), lambda: write(1 << 24, 32, 64), lambda: read(1 << 14, 1 << 10, 16, 128),
+                 lambda: read(1 << 14, 1 << 10, 32, 64), lambda: read(1 << 20, (1 << 30) - 1, (1 << 16) - 1, 128),
+                 lambda: attend(1 << 20, 1 << 20, 16), lambda: attend(1, 1 << 20, (1 << 16) - 1),
+                 lambda: plain(1 << 20, 32, 15)):
+        assert call() == -2 and b"grid too large" in lib.sol_last_error()
+
+
+@pytest.mark.parametrize("name", ["k", "v", "out"])
+def test_gradients_of_the_cache_and_the_output_are_refused(name, monkeypatch):
+    from sol_attn_amd import paged
+    cache, plan = parts()
+    q, out = bf16(3, 4, 64), bf16(3, 4, 64)
+    if name == "out":
+        monkeypatch.setattr(paged, "_validate", lambda c, p, d: (2, 64))
+        out.requires_grad_()
+    else:
+        getattr(cache, name).requires_grad_()
+    with pytest.raises(ValueError, match="Inference only"):
+        paged_attention(q, cache, plan, out=out)

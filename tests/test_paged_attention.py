@@ -80,6 +80,63 @@ def test_many_sequences():
     check(seqs, rows(sum(new), 1, 64, seed=17, device="cuda"))
 
 
+def check_sampled(out, q, ks, vs, new, picks, **how):
+    """Some rows of each sequence against the 64-bit form: row i of a causal sequence is the last of its first keys."""
+    at = 0
+    for k, v, n in zip(ks, vs, new):
+        for i in sorted({min(x, n - 1) for x in picks} if n else ()):
+            end = len(k) - n + i + 1
+            assert_within(out[at + i:at + i + 1], *attend(q[at + i:at + i + 1], k[:end], v[:end], **how))
+        at += n
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_chunks_split_by_lengths_that_differ(fmt):
+    # Enough keys that parts of one size even the sequences out: one, two or no parts a row tile.
+    lengths, new = [2600, 700, 0, 1900, 300, 2300, 1200], [300, 250, 0, 310, 300, 1, 299]
+    seqs = Sequences(lengths, new, heads=16, dim=64, fmt=fmt, page_size=16, seed=84)
+    q = rows(sum(new), 32, 64, seed=85, device="cuda")
+    out = paged_attention(q, seqs.cache, seqs.plan)
+    from paged_testlib import values
+    check_sampled(out, q, [values(x, fmt) for x in seqs.k], [values(x, fmt) for x in seqs.v], new, (0, 63, 64, 200, 309))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_one_chunk_split_into_many_parts(dim):
+    # Several row tiles, up to 32 parts each; the last tile is not full.
+    seqs = Sequences([9000], [300], heads=2, dim=dim, page_size=64, seed=86)
+    q = rows(300, 2, dim, seed=87, device="cuda")
+    check_sampled(paged_attention(q, seqs.cache, seqs.plan), q, seqs.k, seqs.v, [300], (0, 127, 128, 256, 299))
+    out = paged_attention(q, seqs.cache, seqs.plan, causal=False)
+    for i in (0, 128, 299):  # without a mask a row's place does not matter
+        assert_within(out[i:i + 1], *attend(q[i:i + 1], seqs.k[0], seqs.v[0], causal=False))
+
+
+def test_a_plain_triangle_split_into_parts():
+    q, k, v = (rows(1, 2600, 32, 64, seed=s, device="cuda") for s in (88, 89, 90))
+    out = window_attention(q, k, v)
+    check_sampled(out[0], q[0], k, v, [2600], (0, 1, 127, 1000, 2047, 2048, 2599))
+
+
+def test_two_streams_at_once():
+    # Calls that split their keys, side by side on two streams, each with partial states of its own.
+    seqs = [Sequences(n, m, heads=2, dim=64, page_size=16, seed=91 + i)
+            for i, (n, m) in enumerate((([4000, 90], [130, 1]), ([5000, 3800], [1, 1])))]
+    q = [rows(sum(s.new), 4, 64, seed=93, device="cuda") for s in seqs]
+    good = [check(s, x) for s, x in zip(seqs, q)]
+    streams = [torch.cuda.Stream() for _ in seqs]
+    outs = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                outs[i].append(paged_attention(q[i], seqs[i].cache, seqs[i].plan))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, good[i]) for x in outs[i])
+
+
 def test_scale_strides_and_misaligned_queries():
     seqs = Sequences([100, 30], [20, 3], heads=2, dim=64, seed=18)
     wide = rows(23, 8, 64, seed=19, device="cuda")
