@@ -937,7 +937,7 @@ int window_args_ok(const char* what, int64_t query_heads, int64_t heads, double 
   return SOL_OK;
 }
 
-// Keys that the new tokens of one sequence see at most.
+// Keys that `rows` neighbouring new tokens of one sequence see at most.
 int64_t window_keys(int64_t rows, int64_t keys, int causal, int64_t window, int64_t sink_tokens) {
   if (window == 0) return keys;
   window = std::min(window, kMaxPositions);
@@ -1058,8 +1058,8 @@ int sol_paged_attention(const void* q, const int64_t* q_strides, int64_t rows, c
   if (rows * query_heads >= (int64_t(1) << 31))
     return fail(SOL_ERR_UNSUPPORTED, "sol_paged_attention: grid too large");
   const sol::PagedSize size =
-      sol::paged_size(rows, sequences, window_keys(rows, table_width * page_size, causal, window, sink_tokens), heads,
-                      query_heads / heads, head_dim, format, causal != 0, true);
+      sol::paged_size(rows, sequences, window_keys(rows, table_width * page_size, causal, window, sink_tokens),
+                      window_keys(16, table_width * page_size, causal, window, sink_tokens), heads, query_heads / heads, head_dim, format, causal != 0, true);
   rc = paged_workspace_ok(what, size, workspace, workspace_bytes);
   if (rc != SOL_OK) return rc;
   p.q = static_cast<const uint16_t*>(q);
@@ -1086,8 +1086,8 @@ int64_t sol_paged_attention_workspace_size(int64_t rows, int64_t sequences, int6
       format > SOL_CACHE_FP8 || window < 0 || sink_tokens < 0)
     return -1;
   if (rows == 0) return 0;
-  return sol::paged_size(rows, sequences, window_keys(rows, table_width * page_size, causal, window, sink_tokens), heads,
-                         query_heads / heads, head_dim, format, causal != 0, true).bytes;
+  return sol::paged_size(rows, sequences, window_keys(rows, table_width * page_size, causal, window, sink_tokens),
+                         window_keys(16, table_width * page_size, causal, window, sink_tokens), heads, query_heads / heads, head_dim, format, causal != 0, true).bytes;
 }
 
 int sol_window_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
@@ -1109,7 +1109,7 @@ int sol_window_attention(const void* q, const int64_t* q_strides, const void* k,
     return fail(SOL_ERR_UNSUPPORTED, "sol_window_attention: K and V token strides must be below 2^24 elements");
   const sol::PagedSize size =
       sol::paged_size(batch * query_tokens, batch, window_keys(query_tokens, key_tokens, causal, window, sink_tokens),
-                      heads, query_heads / heads, head_dim, SOL_CACHE_BF16, causal != 0, false);
+                      window_keys(16, key_tokens, causal, window, sink_tokens), heads, query_heads / heads, head_dim, SOL_CACHE_BF16, causal != 0, false);
   rc = paged_workspace_ok(what, size, workspace, workspace_bytes);
   if (rc != SOL_OK) return rc;
   sol::PagedParams p;
@@ -1136,8 +1136,8 @@ int64_t sol_window_attention_workspace_size(int64_t batch, int64_t query_tokens,
       heads <= 0 || heads >= (1 << 16) || query_heads % heads || window < 0 || sink_tokens < 0)
     return -1;
   return sol::paged_size(batch * query_tokens, batch,
-                         window_keys(query_tokens, key_tokens, causal, window, sink_tokens), heads,
-                         query_heads / heads, head_dim, SOL_CACHE_BF16, causal != 0, false).bytes;
+                         window_keys(query_tokens, key_tokens, causal, window, sink_tokens),
+                         window_keys(16, key_tokens, causal, window, sink_tokens), heads, query_heads / heads, head_dim, SOL_CACHE_BF16, causal != 0, false).bytes;
 }
 
 }  // extern "C"

@@ -1612,16 +1612,25 @@ int64_t wide_target(int64_t tiles, int64_t heads, int64_t key_tiles, int64_t min
 
 }  // namespace
 
-PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t heads, int64_t group, int64_t head_dim,
-                     int format, bool causal, bool ragged) {
+PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t tile_keys, int64_t heads, int64_t group,
+                     int64_t head_dim, int format, bool causal, bool ragged) {
   PagedSize s;
-  // Few rows per sequence: the step kernel, whose tiles are 16 rows.
-  const bool step = rows * group <= 32 * sequences;
+  auto likely_tiles = [&](int64_t R) { return (rows * group + R - 1) / R + (sequences - 1) / 2; };
+  // The step kernel, whose tiles are 16 rows, for few rows per sequence; and for
+  // small calls, which its tiles spread over more of the card: up to two rounds of
+  // workgroups that read 128 MB of BF16 keys and values, some of them again and
+  // again.  (Heads of 128: 193 queries of 2 heads, 317 keys 11.8 us, 17.8 with tiles
+  // of 128; 256 of 16 heads, 1,024 keys, 128 MB: 16 and 21; 1,000 of 16 heads
+  // under a window of 100, 1,008 workgroups: 18 and 27, 2,000: 46 and 36; 4 x 12
+  // x 4 of 8 heads, 9,000 keys, 440 MB: 48 and 40.)
+  const int64_t small = likely_tiles(16) * heads;
+  const bool step = rows * group <= 32 * sequences ||
+                    (small <= 2 * kResident && small * tile_keys <= (int64_t(128) << 20) / (4 * head_dim));
   s.rows = step ? 16 : 128;
   const int64_t TK = step ? 8192 / (head_dim * (format == kBf16 ? 2 : 1)) : 64;  // StepSlot::TK
   s.tiles = rows * group / s.rows + sequences;  // row tiles: sum ceil(n_s G / R) at most
-  const int64_t likely = (rows * group + s.rows - 1) / s.rows + (sequences - 1) / 2;
-  const int64_t key_tiles = (keys + TK - 1) / TK;
+  const int64_t likely = likely_tiles(s.rows);
+  const int64_t key_tiles = ((step ? tile_keys : keys) + TK - 1) / TK;
   // Row tiles that differ in their keys: other sequences, or the rows of a triangle.
   const bool uneven = (ragged && sequences > 1) || (causal && 2 * rows > keys * sequences);
   s.target = 0;

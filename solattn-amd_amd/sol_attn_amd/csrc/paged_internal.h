@@ -73,9 +73,11 @@ struct PagedSize {
   int64_t bytes;              // workspace, 0 without target
 };
 
-// rows: new tokens in all; keys: a sequence's at most; group: query heads per head.
-PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t heads, int64_t group, int64_t head_dim,
-                     int format, bool causal, bool ragged);
+// rows: new tokens in all; keys: what a sequence's see at most; tile_keys: what 16
+// neighbouring ones see; group: query heads per head; ragged: sequences may
+// differ in length.
+PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t tile_keys, int64_t heads, int64_t group,
+                     int64_t head_dim, int format, bool causal, bool ragged);
 
 hipError_t launch_cache_write(const CacheParams& p, int D, int format, hipStream_t stream);
 hipError_t launch_cache_read(const CacheParams& p, int D, int format, hipStream_t stream);

