@@ -749,8 +749,7 @@ def launch_cache_read(cache, plan, start, tokens):
     pages, h, page_size, d = cache.k.shape
     s, width = plan.page_table.shape
     dev = cache.k.device
-    out = torch.empty((2, s, tokens, h, d), device=dev, dtype=torch.bfloat16)
-    k, v = out[0], out[1]
+    k, v = torch.empty((2, s, tokens, h, d), device=dev, dtype=torch.bfloat16).unbind()
     if s == 0 or tokens == 0:
         return k, v
     table, lengths, _ = _plan_args(plan)
@@ -784,7 +783,7 @@ def launch_paged(q, cache, plan, scale, causal, window, sinks, out=None):
     s, width = plan.page_table.shape
     dev = q.device
     if out is None:
-        out = torch.empty((n, hq, d), device=dev, dtype=torch.bfloat16)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if n == 0 or s == 0:
         return out
     q = _rows(q)
@@ -809,7 +808,7 @@ def launch_window(q, k, v, scale, causal, window, sinks):
     v, v_ptr, v_strides = _bthd_rows(v)
     b, tq, hq, d = q.shape
     tk, h = k.shape[1:3]
-    out = torch.empty((b, tq, hq, d), device=q.device, dtype=torch.bfloat16)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     size = _window_size(b, tq, tk, hq, h, d, causal, window, sinks)
     ws = _workspace(size, q.device)
     _check(library().sol_window_attention(q_ptr, q_strides, k_ptr, k_strides, v_ptr, v_strides, b, tq, tk, hq, h, d,

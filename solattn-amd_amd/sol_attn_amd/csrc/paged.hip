@@ -1630,7 +1630,7 @@ PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t tile
   const int64_t TK = step ? 8192 / (head_dim * (format == kBf16 ? 2 : 1)) : 64;  // StepSlot::TK
   s.tiles = rows * group / s.rows + sequences;  // row tiles: sum ceil(n_s G / R) at most
   const int64_t likely = likely_tiles(s.rows);
-  const int64_t key_tiles = ((step ? tile_keys : keys) + TK - 1) / TK;
+  const int64_t key_tiles = (std::min(keys, tile_keys + (step ? 0 : 128)) + TK - 1) / TK;  // of a row tile, at most
   // Row tiles that differ in their keys: other sequences, or the rows of a triangle.
   const bool uneven = (ragged && sequences > 1) || (causal && 2 * rows > keys * sequences);
   s.target = 0;
@@ -1650,8 +1650,11 @@ PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t tile
     // lengths out (8 sequences of 600 .. 12,000 keys, 512 new tokens of 8 x 4
     // heads: 505 us, 687 with the rule below; 8,192 queries over themselves, 4
     // heads: 116 and 135).
+    // A triangle of more row tiles than that holds no part (19,003 queries
+    // under a window, 16 heads: the second launch took 10 of 700 us).
     s.min_tiles = 24;
-    if (key_tiles > s.min_tiles) s.target = (3 * kResident / 2 + heads - 1) / heads;
+    const int64_t target = (3 * kResident / 2 + heads - 1) / heads;
+    if (key_tiles > s.min_tiles && ((ragged && sequences > 1) || likely < 2 * target)) s.target = target;
   } else {
     s.min_tiles = 4;
     if (key_tiles > s.min_tiles) s.target = wide_target(likely, heads, key_tiles, s.min_tiles);
