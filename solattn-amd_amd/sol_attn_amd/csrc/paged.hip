@@ -123,22 +123,31 @@ template <int R, int TK>
 __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item& it) {
   __shared__ int64_t s_total[kWaves];
   __shared__ int s_tiles[kWaves];
-  __shared__ int s_found[6];
+  __shared__ int s_found[9];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int S = p.batch.S;
-  // Row tiles and key tiles of sequence s.
-  auto sizes = [&](int s, int& row_tiles, int& key_tiles) {
-    const int n = entry_offset(p, s + 1) - entry_offset(p, s), length = entry_length(p, s);
-    row_tiles = n > 0 ? (n * p.G - 1) / R + 1 : 0;
-    key_tiles = n > 0 ? max(1, span_of<TK>(p, length - n, length - 1, length).n) : 0;
+  // A sequence's first row, new tokens and keys, and its row tiles and key tiles.
+  struct Sizes {
+    int off, n, length, row_tiles, key_tiles;
   };
+  auto sizes = [&](int s) {
+    Sizes x = {0, 0, 0, 0, 0};
+    if (s < S) {
+      x.off = entry_offset(p, s);
+      x.n = entry_offset(p, s + 1) - x.off;
+      x.length = entry_length(p, s);
+      x.row_tiles = x.n > 0 ? (x.n * p.G - 1) / R + 1 : 0;
+      x.key_tiles = x.n > 0 ? max(1, span_of<TK>(p, x.length - x.n, x.length - 1, x.length).n) : 0;
+    }
+    return x;
+  };
+  const Sizes mine0 = sizes(tid);  // read once where there are no more sequences than threads
   int z = 1 << 30;
   if (p.target) {
     int64_t sum = 0;
     for (int s = tid; s < S; s += kNT) {
-      int rt, kt;
-      sizes(s, rt, kt);
-      sum += int64_t(rt) * kt;
+      const Sizes x = s == tid ? mine0 : sizes(s);
+      sum += int64_t(x.row_tiles) * x.key_tiles;
     }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
@@ -155,20 +164,17 @@ __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item
   int tiles = 0;  // row tiles of the sequences before s0
   for (int s0 = 0; s0 < S; s0 += kNT) {
     const int s = s0 + tid;
-    int rt = 0, parts = 1;
-    if (s < S) {
-      int kt;
-      sizes(s, rt, kt);
-      if (rt) parts = (kt - 1) / max(z, cdiv_i(kt, kMaxParts)) + 1;
-    }
+    const Sizes x = s0 ? sizes(s) : mine0;
+    const int rt = x.row_tiles, kt = x.key_tiles;
+    const int parts = rt ? (kt - 1) / max(z, cdiv_i(kt, kMaxParts)) + 1 : 1;
     const int64_t mine = int64_t(rt) * parts;
     int64_t end = mine;  // inclusive sums over the wave
     int tile_end = rt;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
-      const int64_t x = __shfl_up(end, off);
-      const int y = __shfl_up(tile_end, off);
-      if (lane >= off) end += x, tile_end += y;
+      const int64_t a = __shfl_up(end, off);
+      const int b = __shfl_up(tile_end, off);
+      if (lane >= off) end += a, tile_end += b;
     }
     if (lane == 63) s_total[wave] = end, s_tiles[wave] = tile_end;
     __syncthreads();
@@ -189,6 +195,9 @@ __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item
       s_found[3] = parts;
       s_found[4] = tile_end - rt + k % rt;
       s_found[5] = rt;
+      s_found[6] = x.off;
+      s_found[7] = x.n;
+      s_found[8] = x.length;
     }
     __syncthreads();
     base += int64_t(uniform64(uint64_t(all)));
@@ -202,9 +211,9 @@ __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item
     return false;
   }
   it.s = __builtin_amdgcn_readfirstlane(s_found[0]);
-  it.off = __builtin_amdgcn_readfirstlane(entry_offset(p, it.s));
-  it.n = __builtin_amdgcn_readfirstlane(entry_offset(p, it.s + 1)) - it.off;
-  it.length = __builtin_amdgcn_readfirstlane(entry_length(p, it.s));
+  it.off = __builtin_amdgcn_readfirstlane(s_found[6]);
+  it.n = __builtin_amdgcn_readfirstlane(s_found[7]);
+  it.length = __builtin_amdgcn_readfirstlane(s_found[8]);
   it.r0 = __builtin_amdgcn_readfirstlane(s_found[1]) * R;
   it.rows = min(R, it.n * p.G - it.r0);
   it.part = __builtin_amdgcn_readfirstlane(s_found[2]);
