@@ -5,21 +5,23 @@
 // j < L is visible iff (j <= p or not causal) and (|p - j| < window or j <
 // sinks).  O = sum_j softmax_j(scale q . k_j) v_j over the visible keys, 0 for
 // a query that sees none.  Scores, softmax statistics and sums are FP32; the
-// probabilities are rounded to BF16 for their product with V, as everywhere in
-// this library (the denominator sums the unrounded ones).
+// probabilities are rounded to BF16 for their product with V on the matrix
+// cores, as everywhere in this library (half a step each, 2^-9, which averages
+// out over the keys; the denominator sums the unrounded ones), where few rows
+// leave them time as two BF16 terms.
 //
 // The rows of a (sequence, K/V head) are its new tokens times the G query
 // heads that share the head, token by token: row r is token r / G, query head
 // r % G of the group.  They are cut into tiles of R rows; a tile's keys are the
 // union of what its rows see, in key tiles, and may be split over several
 // workgroups ("parts"), whose softmax states the merge kernel joins.
-//   step_kernel  R = 16, for few rows per sequence (single tokens): four waves,
-//                each with key tiles of its own; bound by reading the cache
-//   wide_kernel  R = 128, for chunks: four waves of 32 rows share every key tile;
-//                bound by the matrix cores and the softmax's vector work
+//   step_kernel  R = 16, for few rows per sequence (single tokens) and small
+//                calls: four waves, each with key tiles of its own
+//   wide_kernel  R = 128, for chunks: four waves of 32 rows share every key tile
+// paged_size() at the end chooses and says what both sides took.
 //
-// Cached INT8 and FP8 codes are converted to BF16 (exact) on their way into
-// LDS; a key's scale multiplies its score, a value's scale its probability.
+// Cached INT8 and FP8 codes are converted to BF16 (exact); a key's scale
+// multiplies its score, a value's scale its probability.
 #include <algorithm>
 #include <type_traits>
 
@@ -102,8 +104,9 @@ __device__ __forceinline__ float* record(const PagedParams& p, int64_t i) {
   return reinterpret_cast<float*>(static_cast<uint8_t*>(p.workspace) + p.header_bytes) + i * R * kRecordRow<D>;
 }
 
-// Header of row tile `tile` for this workgroup's head (every thread writes the
-// same: no branch on the thread).  (Offsets that do not
+// Header of row tile `tile` for this workgroup's head.  Every thread writes the
+// same: a branch on the thread made the compiler hold the keys' addresses, which
+// the DMA takes from scalar registers, in vector ones.  (Offsets that do not
 // ascend can name more tiles than there are headers.)
 __device__ __forceinline__ void write_header(const PagedParams& p, int64_t tile, const Header& hd) {
   if (tile >= 0 && tile < p.tiles) static_cast<Header*>(p.workspace)[tile * p.H + blockIdx.x % p.H] = hd;
@@ -116,7 +119,7 @@ __device__ __forceinline__ void write_header(const PagedParams& p, int64_t tile,
 // With p.target, parts are of at most z key tiles, z such that about p.target
 // workgroups per head share all key tiles evenly: sum ceil(n_s / z) tiles_s is
 // at most target + sum tiles_s, the grid.  Without, one part each.  No tile has
-// more than kMaxParts parts, which the merge reads one after another.
+// more than kMaxParts parts: the merge's time grows with them.
 constexpr int kMaxParts = 128;
 
 template <int R, int TK>
@@ -423,8 +426,8 @@ __device__ __forceinline__ f32x16 key_factors(const float* half, int hh) {
 }
 
 // Online softmax of raw scores s (half t of the tile in `slot`, keys from j0 on)
-// and O^T += V^T P^T,
-// hidden keys taking no part, whatever their score, value and scale hold.
+// and O^T += V^T P^T, hidden keys taking no part, whatever their score, value
+// and scale hold.
 // `valid`: bits of the half's two groups of 16 rows that have a page.  scales:
 // the half's K scales times c in LDS (V's scales TK floats on), or null.
 template <int D, int TK>
@@ -526,6 +529,8 @@ __device__ __forceinline__ void store4(uint16_t* out, const f32x4& x, float den,
 // and few rows: a row at a time, the 1,024 / D such groups of lanes take the
 // parts in turn, kMergeAhead each in flight, and their states join in a fixed
 // order.  Tiles of 128 rows have few parts: each group takes a row of its own.
+// Bound by its launch (5 us with its reads' latency) or by memory: two parts of
+// 4,032 rows of 24 heads of 128, 129 MB, 27 us, 4.7 TB/s (148 us a row at a time).
 constexpr int kMergeAhead = 8;
 
 // A state of the merge: sums of 4 features, and the row's maximum, denominator
@@ -986,6 +991,15 @@ __device__ __forceinline__ void step_tile(const PagedParams& p, int length, Step
   }
 }
 
+// Bound by reading the keys, so that bytes in flight count: every wave moves
+// tiles of its own into its own slot, without a barrier, the next tile's keys
+// under way while this one's values are, and two workgroups per CU keep 128 KB
+// asked for.  Heads of 128, four query heads each: 64 sequences of 8,192 keys of
+// 8 heads, BF16 2.15 GB in 363 us, 5.9 TB/s; INT8 1.11 GB 218 us, 5.1 TB/s; FP8
+// 210 us.  (BF16 tiles through registers, 32 x 32 products: 48 sequences of up to
+// 19,003 keys 256 us, 183 now.)  One sequence of 84,672 INT8 keys: 179 MB in 38
+// us and the merge's 5.  Small calls are a chain of latencies: three single
+// tokens over up to 317 keys 7.8 us.
 template <int D, int F, bool PAGED>
 __global__ __launch_bounds__(kNT, 2) void step_kernel(PagedParams p) {
   using Slot = StepSlot<D, F>;
@@ -1338,7 +1352,9 @@ struct WideHalf : FastHalf<D> {
 //   2 DT products  half 0's P V; half 1's softmax
 //   2 DT products  half 1's P V
 // Operands are read kAhead products before their use, and the next tile's DMA
-// rounds are spread over the score products.
+// rounds are spread over the score products.  (More ahead spills with heads of
+// 128, where codes under way leave registers for two; heads of 64 have some for
+// eight.)
 template <int D, bool SCALED, typename Refill>
 __device__ __forceinline__ void wide_tile(State<D>& st, const uint16_t* buf, const float* scales,
                                           const bf16x8 (&qf)[Shape<D>::KT], int col, int hh, float c,
@@ -1409,6 +1425,14 @@ __device__ __forceinline__ void wide_tile(State<D>& st, const uint16_t* buf, con
   }
 }
 
+// Bound by the softmax's vector work beside the products: a half's 16 products
+// are 512 cycles of the matrix core, its exponentials, sums and packing about
+// 420 of the vector unit, of each of two waves.  4,096 queries of 16 heads of 128
+// over 16,384 keys, 550 GFLOP: BF16 502 us, 1.10 PFLOP/s (dense_attention_kernel
+// 486); heads of 64 323 us, 0.85 PFLOP/s.  8-bit codes add a conversion of 64
+// codes and 64 multiplications by scales per lane and tile: FP8 650 us, INT8
+// 690.  Two workgroups per CU hold 256 registers a wave and a ring of two tiles
+// each.
 template <int D, int F, bool PAGED>
 __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
   using S = Shape<D>;
