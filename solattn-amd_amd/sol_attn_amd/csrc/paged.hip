@@ -370,6 +370,8 @@ struct TileImage {
 
 // ---- the softmax and P V of 32 keys -----------------------------------------
 
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+
 // Bit 15 of every 16-bit half that is an infinity or a NaN.
 __device__ __forceinline__ uint32_t nonfinite(uint32_t x) { return ((x & 0x7F807F80u) + 0x00800080u) & 0x80008000u; }
 
@@ -430,7 +432,7 @@ __device__ __forceinline__ f32x16 key_factors(const float* half, int hh) {
 // and scale hold.
 // `valid`: bits of the half's two groups of 16 rows that have a page.  scales:
 // the half's K scales times c in LDS (V's scales TK floats on), or null.
-template <int D, int TK>
+template <int D, int TK, int F>
 __device__ __forceinline__ void attend_masked(const PagedParams& p, int length, State<D>& st, LaneRow& row, f32x16 s,
                                               const uint16_t* slot, int t, int j0, uint32_t valid, int lane_col,
                                               int lane_hh, const float* scales) {
@@ -480,16 +482,18 @@ __device__ __forceinline__ void attend_masked(const PagedParams& p, int length, 
   // Scheduled apart from the scores: V's operands are not held meanwhile.
   chunk_end();
   u32x4 vt[2][Shape<D>::DT];
-  uint32_t bad = 0;
+  u16x2 most = {0, 0};  // magnitudes compare like their bits
 #pragma unroll
   for (int c4 = 0; c4 < 2; ++c4)
 #pragma unroll
     for (int dt = 0; dt < Shape<D>::DT; ++dt) {
       vt[c4][dt] = TileImage<D, TK>::v(slot, col, hh, t, c4, dt);
+      if constexpr (F != kInt8)  // INT8 codes are finite
 #pragma unroll
-      for (int i = 0; i < 4; ++i) bad |= nonfinite(vt[c4][dt][i]);
+        for (int i = 0; i < 4; ++i)
+          most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, vt[c4][dt][i] & 0x7FFF7FFFu));
     }
-  const bool some = __builtin_amdgcn_ballot_w64(bad != 0) != 0;
+  const bool some = F != kInt8 && __builtin_amdgcn_ballot_w64(nonfinite(__builtin_bit_cast(uint32_t, most)) != 0) != 0;
   if (some) {
 #pragma unroll
     for (int c4 = 0; c4 < 2; ++c4)
@@ -1496,7 +1500,7 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
       for (int ks = 0; ks < S::KT; ++ks)
         s = mfma32x32x16(as_bf16x8(TileImage<D, TK>::k(buf, fcol, fhh, t, ks)), qf[ks], s);
       chunk_end();
-      attend_masked<D, TK>(p, it.length, st, row, s, buf, t, tile * TK + 32 * t, valid >> (2 * t), col, hh,
+      attend_masked<D, TK, F>(p, it.length, st, row, s, buf, t, tile * TK + 32 * t, valid >> (2 * t), col, hh,
                            SCALED ? scales + 32 * t : nullptr);
     }
     refill.late();
