@@ -204,7 +204,9 @@ def cache_write(k, v, cache, plan):
     read, and everything else in the cache is left as it was.  Per token and
     head, INT8 stores ``round(x * 127 / max|x|)`` (half to even) and FP8 the
     e4m3 value nearest ``x * 448 / max|x|``, with the scale ``max|x| / 127``
-    (``/ 448``); a row with an infinity or a NaN reads back as NaN.
+    (``/ 448``); a row with an infinity or a NaN reads back as NaN.  ``k`` and
+    ``v`` may be views of a BF16 cache (a page copied to another), but not of
+    rows that the call writes.
     """
     _check_rows("K/V", k)
     _check_rows("K/V", v)
@@ -212,6 +214,8 @@ def cache_write(k, v, cache, plan):
         raise ValueError("K and V must have the same shape and device")
     if k.shape[1:] != _validate(cache, plan, k.device):
         raise ValueError("K/V heads and head dimension must be the cache's")
+    if abs(cache.k.data_ptr() - cache.v.data_ptr()) < cache.k.numel() * cache.k.element_size():
+        raise ValueError("The cache's K and V must not share memory")
     with _on(k.device):
         _native.launch_cache_write(k, v, cache, plan)
 

@@ -252,3 +252,16 @@ def test_values_stand_for_the_rows():
         most = x.double().abs().amax(-1, keepdim=True)
         limit = tol * most if tol else 2 ** -4 * x.double().abs() + 2 ** -10 / LEVELS["fp8"] * most
         assert (off <= limit * (1 + 2 ** -16)).all()
+
+
+def test_a_page_copied_to_another():
+    # Rows read from the cache's own pages: a shared page that two sequences go on to write differently.
+    seqs = Sequences([30], [30], heads=2, dim=64, page_size=16, seed=50)
+    src, dst = seqs.table[0][0], next(p for p in range(seqs.pages) if p not in seqs.table[0])
+    k, v = (x[src].transpose(0, 1) for x in (seqs.cache.k, seqs.cache.v))
+    copy = PagedPlan.create([[dst]], [16], [16], pages=seqs.pages, page_size=16).to("cuda")
+    before = [x.clone() for x in (seqs.cache.k, seqs.cache.v)]
+    cache_write(k, v, seqs.cache, copy)
+    for x, b in zip((seqs.cache.k, seqs.cache.v), before):
+        b[dst] = b[src]
+        assert torch.equal(x, b)

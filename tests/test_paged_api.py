@@ -289,6 +289,17 @@ def test_c_abi_refuses_launches_of_too_many_threads():
         assert call() == -2 and b"grid too large" in lib.sol_last_error()
 
 
+@pytest.mark.parametrize("shift", [0, 64])
+def test_write_refuses_a_cache_whose_sides_share_memory(shift, monkeypatch):
+    from sol_attn_amd import paged
+    _, plan = parts()
+    monkeypatch.setattr(paged, "_validate", lambda c, p, d: (2, 64))
+    store = bf16(4 * 2 * 16 * 64 + shift)
+    cache = PagedCache(*(x.view(4, 2, 16, 64) for x in (store[:8192], store[shift:])))
+    with pytest.raises(ValueError, match="share memory"):
+        cache_write(bf16(3, 2, 64), bf16(3, 2, 64), cache, plan)
+
+
 @pytest.mark.parametrize("name", ["k", "v", "out"])
 def test_gradients_of_the_cache_and_the_output_are_refused(name, monkeypatch):
     from sol_attn_amd import paged
