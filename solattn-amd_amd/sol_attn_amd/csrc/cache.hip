@@ -15,9 +15,10 @@
 // then row), and the BF16 side is read or written in whole rows.  A copy of 4
 // GiB reaches 4.9 TB/s on this card.  Writing 4,032 tokens of 24 heads of 128 in
 // BF16, 99 MB: 21 us a call, 4.7 TB/s; nine prompts of up to 4,801 tokens, 12
-// heads of 64, FP8, 111 MB: 28 us, 4.0 TB/s.  Reading 19,003 tokens of 16 heads
-// of 128 from INT8, 236 MB: 57 us, 4.2 TB/s, 36 where the caches hold them.
-// Small calls are 5 us, less than the 12 that the host takes to make one.
+// heads of 64, FP8, 111 MB: 28 us, 4.0 TB/s (more rows per wave: 29 and 30).
+// Reading 40,320 tokens of 24 heads of 128 from INT8, 501 MB: 145 us, 3.5 TB/s;
+// 19,003 of 16 heads, 236 MB: 39 us where the caches hold a part.  Small calls
+// are 5 us, less than the 12 that the host takes to make one.
 #include "paged_internal.h"
 #include "sol_device.h"
 
@@ -173,36 +174,66 @@ __device__ __forceinline__ u32x4 dequantised(u32x2 codes, float scale) {
   return o;
 }
 
-// A wave reads kWaveRows consecutive positions of one sequence and head, K and V.
+// Groups of kWaveRows positions that a wave reads.  Rows of codes are half as
+// long: two groups, all of whose codes and scales are on their way together
+// (40,320 tokens of 24 heads of 128 from FP8 173 us with one whose K is stored
+// before V is asked for, 149 with one, 141 with two, 143 with four; BF16 169, 170,
+// 182, 186).
+template <int F>
+constexpr int kReadGroups = F == kBf16 ? 1 : 2;
+
+// A wave reads consecutive positions of one sequence and head, K and V.
 template <int D, int F>
 __global__ __launch_bounds__(kCacheThreads) void cache_read_kernel(CacheParams p) {
+  constexpr int U = kReadGroups<F>, kRows = U * kWaveRows<D>;
   const PagedBatch& bt = p.batch;
   const int lane = threadIdx.x & 63, c = lane % kRowLanes<D>;
   const int64_t unit = int64_t(blockIdx.x) * (kCacheThreads / 64) + (threadIdx.x >> 6);
-  const int groups = (p.tokens + kWaveRows<D> - 1) / kWaveRows<D>;
+  const int groups = (p.tokens + kRows - 1) / kRows;
   const int h = int(unit % p.H);
   const int64_t sg = unit / p.H;
   const int s = int(sg / groups);
-  const int t = int(sg % groups) * kWaveRows<D> + lane / kRowLanes<D>;
-  if (s >= bt.S || t >= p.tokens) return;
-  const int64_t pos = int64_t(p.start) + t;
-  int page = -1;
-  if (pos < bt.length(s)) page = bt.table[int64_t(s) * bt.width + (pos >> bt.page_shift)];
-  const bool there = page >= 0 && page < bt.pages;
-  const int64_t row = there ? ((int64_t(page) * p.H + h) << bt.page_shift) + (pos & ((1 << bt.page_shift) - 1)) : 0;
-  const int64_t dst = ((int64_t(s) * p.tokens + t) * p.H + h) * D + 8 * c;
+  if (s >= bt.S) return;
+  const int t0 = int(sg % groups) * kRows + lane / kRowLanes<D>;
+  const int length = bt.length(s);
+  int64_t row[U];  // -1: not there
 #pragma unroll
-  for (int kv = 0; kv < 2; ++kv) {
-    u32x4 o = zero_u32x4();
-    if (there) {
-      if constexpr (F == kBf16) {
-        o = *reinterpret_cast<const u32x4*>(p.store[kv] + row * D * 2 + 16 * c);
-      } else {
-        const u32x2 codes = *reinterpret_cast<const u32x2*>(p.store[kv] + row * D + 8 * c);
-        o = dequantised<F>(codes, p.scale[kv][row]);
-      }
+  for (int u = 0; u < U; ++u) {
+    const int64_t pos = int64_t(p.start) + t0 + u * kWaveRows<D>;
+    int page = -1;
+    if (pos < length) page = bt.table[int64_t(s) * bt.width + (pos >> bt.page_shift)];
+    row[u] = page >= 0 && page < bt.pages
+                 ? ((int64_t(page) * p.H + h) << bt.page_shift) + (pos & ((1 << bt.page_shift) - 1))
+                 : -1;
+  }
+  auto out = [&](int u, int kv) {
+    return reinterpret_cast<u32x4*>(p.out[kv] + ((int64_t(s) * p.tokens + t0 + u * kWaveRows<D>) * p.H + h) * D + 8 * c);
+  };
+  if constexpr (F == kBf16) {
+    if (t0 >= p.tokens) return;
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      u32x4 o = zero_u32x4();
+      if (row[0] >= 0) o = *reinterpret_cast<const u32x4*>(p.store[kv] + row[0] * D * 2 + 16 * c);
+      *out(0, kv) = o;
     }
-    *reinterpret_cast<u32x4*>(p.out[kv] + dst) = o;
+  } else {
+    u32x2 x[U][2];
+    float scale[U][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        const int64_t at = max(row[u], int64_t(0));  // row 0 for what is not there
+        x[u][kv] = *reinterpret_cast<const u32x2*>(p.store[kv] + at * D + 8 * c);
+        scale[u][kv] = p.scale[kv][at];
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (t0 + u * kWaveRows<D> >= p.tokens) return;
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) *out(u, kv) = row[u] >= 0 ? dequantised<F>(x[u][kv], scale[u][kv]) : zero_u32x4();
+    }
   }
 }
 
@@ -214,7 +245,8 @@ void write_variant(const CacheParams& p, hipStream_t stream) {
 
 template <int D, int F>
 void read_variant(const CacheParams& p, hipStream_t stream) {
-  const int64_t units = int64_t(p.batch.S) * ((p.tokens + kWaveRows<D> - 1) / kWaveRows<D>) * p.H;
+  constexpr int kRows = kReadGroups<F> * kWaveRows<D>;
+  const int64_t units = int64_t(p.batch.S) * ((p.tokens + kRows - 1) / kRows) * p.H;
   hipLaunchKernelGGL((cache_read_kernel<D, F>), dim3(unsigned((units + 3) / 4)), dim3(kCacheThreads), 0, stream, p);
 }
 
