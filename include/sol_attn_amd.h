@@ -489,7 +489,8 @@ int sol_cache_read(const void* cache_k, const void* cache_v, const float* k_scal
  * result, infinities and NaN included.  out: contiguous BF16 [rows,
  * query_heads, head_dim].  workspace: 16-byte aligned device memory of at least
  * sol_paged_attention_workspace_size() bytes for the same sizes (NULL when that
- * is 0): the partial states of calls that split their keys over workgroups. */
+ * is 0): the partial states of calls that split their keys over workgroups.  At
+ * most 65,536 sequences. */
 int sol_paged_attention(const void* q, const int64_t* q_strides, int64_t rows, const void* cache_k,
                         const void* cache_v, const float* k_scales, const float* v_scales, const int32_t* page_table,
                         const int32_t* context_lengths, const int32_t* query_offsets, int64_t sequences,

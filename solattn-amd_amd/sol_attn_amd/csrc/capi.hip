@@ -875,6 +875,7 @@ namespace {
 
 constexpr int64_t kRowsStrideMax = int64_t(1) << 24;  // elements between plain keys
 constexpr int64_t kMaxPositions = int64_t(1) << 30;  // positions of one sequence, and new rows of one call
+constexpr int64_t kMaxAttended = int64_t(1) << 16;  // sequences of one paged attention call: every workgroup looks at all
 constexpr int64_t kMaxGrid = (int64_t(1) << 24) - 1;  // workgroups: a launch has fewer than 2^32 threads
 
 // Checks a sequence batch over a cache (its arrays' contents the kernels
@@ -1055,6 +1056,8 @@ int sol_paged_attention(const void* q, const int64_t* q_strides, int64_t rows, c
   if (rc != SOL_OK) return rc;
   if (!operand_ok(q, q_strides, true))
     return fail(SOL_ERR_INVALID, "sol_paged_attention: Q needs 16-byte aligned rows and positive strides");
+  if (sequences > kMaxAttended)
+    return fail(SOL_ERR_UNSUPPORTED, "sol_paged_attention: at most 65,536 sequences in one call");
   if (rows * query_heads >= (int64_t(1) << 31))
     return fail(SOL_ERR_UNSUPPORTED, "sol_paged_attention: grid too large");
   const sol::PagedSize size =
@@ -1080,10 +1083,10 @@ int sol_paged_attention(const void* q, const int64_t* q_strides, int64_t rows, c
 int64_t sol_paged_attention_workspace_size(int64_t rows, int64_t sequences, int64_t table_width, int64_t page_size,
                                            int64_t query_heads, int64_t heads, int64_t head_dim, int format,
                                            int causal, int64_t window, int64_t sink_tokens) {
-  if (rows < 0 || rows >= kMaxPositions || sequences <= 0 || sequences > (1 << 20) || table_width <= 0 ||
+  if (rows < 0 || rows >= kMaxPositions || sequences <= 0 || sequences > kMaxAttended || table_width <= 0 ||
       page_size <= 0 || table_width > kMaxPositions / page_size || heads <= 0 || heads >= (1 << 16) || query_heads <= 0 ||
       query_heads % heads || query_heads >= (1 << 16) || (head_dim != 64 && head_dim != 128) || format < SOL_CACHE_BF16 ||
-      format > SOL_CACHE_FP8 || window < 0 || sink_tokens < 0)
+      format > SOL_CACHE_FP8 || window < 0 || sink_tokens < 0 || rows * query_heads >= (int64_t(1) << 31))
     return -1;
   if (rows == 0) return 0;
   return sol::paged_size(rows, sequences, window_keys(rows, table_width * page_size, causal, window, sink_tokens),
@@ -1133,7 +1136,8 @@ int64_t sol_window_attention_workspace_size(int64_t batch, int64_t query_tokens,
                                             int64_t query_heads, int64_t heads, int64_t head_dim, int causal,
                                             int64_t window, int64_t sink_tokens) {
   if (!shape_ok(batch, query_tokens, query_heads, head_dim) || key_tokens <= 0 || key_tokens >= kMaxPositions ||
-      heads <= 0 || heads >= (1 << 16) || query_heads % heads || window < 0 || sink_tokens < 0)
+      heads <= 0 || heads >= (1 << 16) || query_heads % heads || window < 0 || sink_tokens < 0 ||
+      batch * query_tokens * query_heads >= (int64_t(1) << 31))
     return -1;
   return sol::paged_size(batch * query_tokens, batch,
                          window_keys(query_tokens, key_tokens, causal, window, sink_tokens),

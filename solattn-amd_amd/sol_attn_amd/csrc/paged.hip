@@ -72,14 +72,6 @@ __device__ __forceinline__ Span span_of(const PagedParams& p, int first, int las
 
 // ---- which rows and keys a workgroup takes ----------------------------------
 
-__device__ __forceinline__ int entry_offset(const PagedParams& p, int s) {
-  return p.batch.table ? p.batch.offset(s) : s * p.Tq;
-}
-
-__device__ __forceinline__ int entry_length(const PagedParams& p, int s) {
-  return p.batch.table ? p.batch.length(s) : p.Tk;
-}
-
 struct Item {
   int s, off, n, length;  // the sequence: first row, new tokens, keys
   int r0, rows;           // the tile's rows r0 .. r0 + rows - 1 of the sequence's n G
@@ -112,7 +104,7 @@ __device__ __forceinline__ void write_header(const PagedParams& p, int64_t tile,
   if (tile >= 0 && tile < p.tiles) static_cast<Header*>(p.workspace)[tile * p.H + blockIdx.x % p.H] = hd;
 }
 
-// Item `id` of the launch, in order of sequences, row tiles and parts; false
+// Item `id` of the launch, in order of sequences, parts and row tiles; false
 // past the last one.  Every workgroup forms the whole plan from the lengths on
 // the device (two scans over the sequences, a few microseconds), so that a
 // captured launch follows them and no launch or copy comes before this one.
@@ -122,8 +114,40 @@ __device__ __forceinline__ void write_header(const PagedParams& p, int64_t tile,
 // more than kMaxParts parts: the merge's time grows with them.
 constexpr int kMaxParts = 128;
 
+// A tile's key tiles at most in a part, of `sum` key tiles per head.
+__device__ __forceinline__ int part_tiles(const PagedParams& p, int64_t sum) {
+  return int(min(int64_t(1) << 30, max(int64_t(p.min_tiles), (sum + p.target - 1) / p.target)));
+}
+
+// Entries of plain K / V are all alike: the item by divisions alone.
 template <int R, int TK>
+__device__ __forceinline__ bool take_plain_item(const PagedParams& p, int id, Item& it) {
+  const int rt = (p.Tq * p.G - 1) / R + 1, kt = max(1, span_of<TK>(p, p.Tk - p.Tq, p.Tk - 1, p.Tk).n);
+  const int z = p.target ? part_tiles(p, int64_t(p.batch.S) * rt * kt) : 1 << 30;
+  it.parts = __builtin_amdgcn_readfirstlane((kt - 1) / max(z, cdiv_i(kt, kMaxParts)) + 1);
+  const int items = rt * it.parts;  // of an entry; all of them are fewer than 2^24 (the grid)
+  it.s = __builtin_amdgcn_readfirstlane(id / items);
+  if (it.s >= p.batch.S) {
+    if (p.records) write_header(p, int64_t(p.batch.S) * rt + (id - p.batch.S * items), Header{0, 0, 0, 0, 0, 0});
+    return false;
+  }
+  const int k = id - it.s * items;
+  it.part = __builtin_amdgcn_readfirstlane(k / rt);
+  const int tile = k - it.part * rt, row_tile = p.causal ? rt - 1 - tile : tile;
+  it.off = it.s * p.Tq;
+  it.n = p.Tq;
+  it.length = p.Tk;
+  it.r0 = row_tile * R;
+  it.rows = min(R, it.n * p.G - it.r0);
+  if (p.records && it.part == 0)
+    write_header(p, int64_t(it.s) * rt + tile,
+                 Header{it.parts > 1 ? it.parts : 0, it.off, it.r0, it.rows, blockIdx.x, uint32_t(rt) * uint32_t(p.H)});
+  return true;
+}
+
+template <int R, int TK, bool PAGED>
 __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item& it) {
+  if constexpr (!PAGED) return take_plain_item<R, TK>(p, int(id), it);
   __shared__ int64_t s_total[kWaves];
   __shared__ int s_tiles[kWaves];
   __shared__ int s_found[9];
@@ -136,9 +160,9 @@ __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item
   auto sizes = [&](int s) {
     Sizes x = {0, 0, 0, 0, 0};
     if (s < S) {
-      x.off = entry_offset(p, s);
-      x.n = entry_offset(p, s + 1) - x.off;
-      x.length = entry_length(p, s);
+      x.off = p.batch.offset(s);
+      x.n = p.batch.offset(s + 1) - x.off;
+      x.length = p.batch.length(s);
       x.row_tiles = x.n > 0 ? (x.n * p.G - 1) / R + 1 : 0;
       x.key_tiles = x.n > 0 ? max(1, span_of<TK>(p, x.length - x.n, x.length - 1, x.length).n) : 0;
     }
@@ -160,7 +184,7 @@ __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) sum += s_total[w];
     sum = int64_t(uniform64(uint64_t(sum)));
-    z = int(min(int64_t(1) << 30, max(int64_t(p.min_tiles), (sum + p.target - 1) / p.target)));
+    z = part_tiles(p, sum);
     __syncthreads();
   }
   int64_t base = 0;
@@ -1015,7 +1039,7 @@ __global__ __launch_bounds__(kNT, 2) void step_kernel(PagedParams p) {
 
   const int h = blockIdx.x % p.H;
   Item it;
-  if (!take_item<R, TK>(p, blockIdx.x / p.H, it)) return;
+  if (!take_item<R, TK, PAGED>(p, blockIdx.x / p.H, it)) return;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, g = lane >> 4;
@@ -1447,7 +1471,7 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
 
   const int h = blockIdx.x % p.H;
   Item it;
-  if (!take_item<R, TK>(p, blockIdx.x / p.H, it)) return;
+  if (!take_item<R, TK, PAGED>(p, blockIdx.x / p.H, it)) return;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, hh = lane >> 5;

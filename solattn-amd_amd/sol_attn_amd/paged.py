@@ -19,6 +19,7 @@ from .attention import _nonnegative_integer, _on, _visibility
 
 CACHE_FORMATS = {"bf16": torch.bfloat16, "int8": torch.int8, "fp8": torch.float8_e4m3fn}
 MAX_POSITIONS = 1 << 30  # positions of one sequence that a page table may name
+MAX_ATTENDED = 1 << 16  # sequences of one attention call: every workgroup finds its place among all of them by itself
 
 
 @dataclass(frozen=True)
@@ -253,6 +254,8 @@ def paged_attention(q, cache, plan, *, causal=True, window=None, sink_tokens=0, 
     heads, dim = _validate(cache, plan, q.device)
     if q.shape[2] != dim or q.shape[1] == 0 or q.shape[1] % heads:
         raise ValueError("Q heads must be a multiple of the cache's, of its head dimension")
+    if plan.context_lengths.shape[0] > MAX_ATTENDED:
+        raise ValueError(f"More than {MAX_ATTENDED} sequences in one call are not supported")
     window = _visibility(causal, window, sink_tokens)
     scale = dim ** -0.5 if scale is None else float(scale)
     if not math.isfinite(scale) or scale <= 0:

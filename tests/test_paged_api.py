@@ -284,9 +284,25 @@ def test_c_abi_refuses_launches_of_too_many_threads():
 
     for call in (lambda: write(1 << 24, 16, 128), lambda: write(1 << 24, 32, 64), lambda: read(1 << 14, 1 << 10, 16, 128),
                  lambda: read(1 << 14, 1 << 10, 32, 64), lambda: read(1 << 20, (1 << 30) - 1, (1 << 16) - 1, 128),
-                 lambda: attend(1 << 20, 1 << 20, 16), lambda: attend(1, 1 << 20, (1 << 16) - 1),
+                 lambda: attend(1 << 21, 1 << 16, 192), lambda: attend(1, 1 << 16, (1 << 16) - 1),
                  lambda: plain(1 << 20, 32, 15)):
         assert call() == -2 and b"grid too large" in lib.sol_last_error()
+    assert attend(1, (1 << 16) + 1, 2) == -2 and b"65,536 sequences" in lib.sol_last_error()
+    paged, window = lib.sol_paged_attention_workspace_size, lib.sol_window_attention_workspace_size
+    assert paged(3, 1 << 16, 2, 16, 4, 2, 64, 0, 1, 0, 0) == 0 and paged(3, (1 << 16) + 1, 2, 16, 4, 2, 64, 0, 1, 0, 0) == -1
+    assert paged((1 << 30) - 1, 2, 1 << 25, 16, 65534, 2, 64, 0, 1, 0, 0) == -1
+    assert window(1 << 20, 1 << 10, 5, 4, 2, 64, 1, 0, 0) == -1
+
+
+def test_too_many_sequences_are_refused(monkeypatch):
+    from sol_attn_amd import paged
+    monkeypatch.setattr(paged, "_validate", lambda c, p, d: (2, 64))
+    cache, _ = parts()
+    n = paged.MAX_ATTENDED + 1
+    plan = PagedPlan(torch.zeros(n, 1, dtype=torch.int32), torch.zeros(n, dtype=torch.int32),
+                     torch.zeros(n + 1, dtype=torch.int32))
+    with pytest.raises(ValueError, match="More than 65536 sequences"):
+        paged_attention(bf16(3, 4, 64), cache, plan)
 
 
 @pytest.mark.parametrize("shift", [0, 64])

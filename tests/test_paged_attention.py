@@ -137,6 +137,25 @@ def test_two_streams_at_once():
         assert all(torch.equal(x, good[i]) for x in outs[i])
 
 
+def test_thousands_of_sequences():
+    # More than the workgroup's threads, several times; single tokens, then some of two.
+    lengths = [1 + (11 * i) % 40 for i in range(5000)]
+    for new in ([1] * 5000, [1 + (i % 7 == 3) * (lengths[i] > 1) for i in range(5000)]):
+        seqs = Sequences(lengths, new, heads=1, dim=64, page_size=16, seed=95)
+        check(seqs, rows(sum(new), 1, 64, seed=96, device="cuda"))
+
+
+@pytest.mark.parametrize("tq,tk", [(1, 40), (3, 9000), (70, 6000)])
+@pytest.mark.parametrize("batch", [1, 5, 300])
+def test_window_over_many_entries(batch, tq, tk):
+    if batch == 300:
+        tk = min(tk, 700)
+    q, k, v = rows(batch, tq, 2, 64, seed=97), rows(batch, tk, 1, 64, seed=98), rows(batch, tk, 1, 64, seed=99)
+    out = window_attention(q.cuda(), k.cuda(), v.cuda())
+    for b in sorted({0, batch // 2, batch - 1}):
+        assert_within(out[b], *attend(q[b], k[b], v[b]))
+
+
 def test_scale_strides_and_misaligned_queries():
     seqs = Sequences([100, 30], [20, 3], heads=2, dim=64, seed=18)
     wide = rows(23, 8, 64, seed=19, device="cuda")
