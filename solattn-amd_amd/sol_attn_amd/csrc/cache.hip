@@ -59,7 +59,8 @@ __device__ __forceinline__ uint32_t row_max(uint32_t x) {
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ uint32_t pk_max_u16(uint32_t a, uint32_t b) {
-  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+  const u16x2 x = __builtin_bit_cast(u16x2, a), y = __builtin_bit_cast(u16x2, b);
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(x, y));
 }
 
 // x / a, correctly rounded in all but rare cases and exact wherever the
@@ -207,7 +208,8 @@ __global__ __launch_bounds__(kCacheThreads) void cache_read_kernel(CacheParams p
                  : -1;
   }
   auto out = [&](int u, int kv) {
-    return reinterpret_cast<u32x4*>(p.out[kv] + ((int64_t(s) * p.tokens + t0 + u * kWaveRows<D>) * p.H + h) * D + 8 * c);
+    const int64_t token = int64_t(s) * p.tokens + t0 + u * kWaveRows<D>;
+    return reinterpret_cast<u32x4*>(p.out[kv] + (token * p.H + h) * D + 8 * c);
   };
   if constexpr (F == kBf16) {
     if (t0 >= p.tokens) return;

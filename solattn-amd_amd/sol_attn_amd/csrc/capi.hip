@@ -1062,18 +1062,15 @@ int sol_paged_attention(const void* q, const int64_t* q_strides, int64_t rows, c
     return fail(SOL_ERR_UNSUPPORTED, "sol_paged_attention: grid too large");
   const sol::PagedSize size =
       sol::paged_size(rows, sequences, window_keys(rows, table_width * page_size, causal, window, sink_tokens),
-                      window_keys(16, table_width * page_size, causal, window, sink_tokens), heads, query_heads / heads, head_dim, format, causal != 0, true);
+                      window_keys(16, table_width * page_size, causal, window, sink_tokens), heads,
+                      query_heads / heads, head_dim, format, causal != 0, true);
   rc = paged_workspace_ok(what, size, workspace, workspace_bytes);
   if (rc != SOL_OK) return rc;
   p.q = static_cast<const uint16_t*>(q);
   p.q_st = q_strides[1], p.q_sh = q_strides[2];
-  const int64_t row_bytes = head_dim * (format == SOL_CACHE_BF16 ? 2 : 1);
   for (int i = 0; i < 2; ++i) {
     p.store[i] = static_cast<const uint8_t*>(i ? cache_v : cache_k);
     p.scale[i] = i ? v_scales : k_scales;
-    p.st[i] = row_bytes;
-    p.sh[i] = row_bytes * page_size;
-    p.sb[i] = p.sh[i] * heads;
   }
   window_params(&p, query_heads, heads, scale, causal, window, sink_tokens, out);
   p.workspace = workspace;
@@ -1090,7 +1087,8 @@ int64_t sol_paged_attention_workspace_size(int64_t rows, int64_t sequences, int6
     return -1;
   if (rows == 0) return 0;
   return sol::paged_size(rows, sequences, window_keys(rows, table_width * page_size, causal, window, sink_tokens),
-                         window_keys(16, table_width * page_size, causal, window, sink_tokens), heads, query_heads / heads, head_dim, format, causal != 0, true).bytes;
+                         window_keys(16, table_width * page_size, causal, window, sink_tokens), heads,
+                         query_heads / heads, head_dim, format, causal != 0, true).bytes;
 }
 
 int sol_window_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,

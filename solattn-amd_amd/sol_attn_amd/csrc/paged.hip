@@ -404,7 +404,8 @@ struct TileImage {
   }
   // This lane's K operand of half t, k-step ks.
   __device__ static __forceinline__ u32x4 k(const uint16_t* slot, int col, int hh, int t, int ks) {
-    return *reinterpret_cast<const u32x4*>(slot + (32 * t + col) * D + (TileLayout<D>::k_lane_xor(col, hh) ^ (16 * ks)));
+    const int at = (32 * t + col) * D + (TileLayout<D>::k_lane_xor(col, hh) ^ (16 * ks));
+    return *reinterpret_cast<const u32x4*>(slot + at);
   }
   // This lane's V^T operand (FragLane's addresses): feature 32 dt + col, keys
   // 32 t + 16 c4 + 4 hh + {0..3, 8..11}.
@@ -826,7 +827,8 @@ struct StepDma {
   uint64_t group[PAGED ? TK / 16 : 1];  // where each group begins
   uint64_t scale_row[kScales ? kScales : 1];
 
-  __device__ __forceinline__ StepDma(uint32_t slot_lds, uint32_t scales_lds, int l) : slot(slot_lds), scales(scales_lds), lane(l) {
+  __device__ __forceinline__ StepDma(uint32_t slot_lds, uint32_t scales_lds, int l)
+      : slot(slot_lds), scales(scales_lds), lane(l) {
     constexpr int kRowLanes = Slot::kRow / 16;
     row[0] = l / kRowLanes;
     chunk[0] = 16u * ((l % kRowLanes) ^ Slot::k_swizzle(row[0]));
@@ -1297,7 +1299,8 @@ struct CodeTile {
   __device__ __forceinline__ void load(const Keys<D, F, true>& keys, const Window& window, int i, int wave, int lane) {
     const int l = fresh(lane);
     // A wave's 64 chunks are 8 (D = 128) or 16 rows of one group.
-    const uint32_t off = uint32_t(wave * kWave / kRowLanes % 16 + l / kRowLanes) * keys.kRowBytes + 16u * (l % kRowLanes);
+    const uint32_t row = uint32_t(wave * kWave / kRowLanes % 16 + l / kRowLanes);
+    const uint32_t off = row * keys.kRowBytes + 16u * (l % kRowLanes);
 #pragma unroll
     for (int n = 0; n < kLoads; ++n) {
       const uint64_t at = window.offset(i, D == 128 ? 2 * n + (wave >> 1) : wave);

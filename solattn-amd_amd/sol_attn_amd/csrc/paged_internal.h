@@ -48,7 +48,7 @@ struct PagedParams {
   int64_t q_sb, q_st, q_sh;   // element strides
   const uint8_t* store[2];    // K, V
   const float* scale[2];      // or null
-  int64_t sb[2], st[2], sh[2];  // byte strides {page or entry, row, head}
+  int64_t sb[2], st[2], sh[2];  // plain: byte strides {entry, row, head}
   uint16_t* out;              // contiguous [rows, Hq, D] (plain: [S, Tq, Hq, D])
   int Tq, Tk;
   int H, G;                   // K / V heads, query heads of each
