@@ -14,8 +14,8 @@
 // rows of neighbouring tokens of a page are contiguous (page-major, then head,
 // then row), and the BF16 side is read or written in whole rows.  A copy of 4
 // GiB reaches 4.9 TB/s on this card.  Writing 4,032 tokens of 24 heads of 128 in
-// BF16, 99 MB: 21 us a call, 4.7 TB/s; nine prompts of up to 4,801 tokens, 12
-// heads of 64, FP8, 111 MB: 28 us, 4.0 TB/s (more rows per wave: 29 and 30).
+// BF16, 99 MB: 19 us a call, 5.2 TB/s; nine prompts of up to 4,801 tokens, 12
+// heads of 64, FP8, 111 MB: 28 us, 4.0 TB/s (more rows per wave: 29 to 30).
 // Reading 40,320 tokens of 24 heads of 128 from INT8, 501 MB: 145 us, 3.5 TB/s;
 // 19,003 of 16 heads, 236 MB: 39 us where the caches hold a part.  Small calls
 // are 5 us, less than the 12 that the host takes to make one.
@@ -120,8 +120,8 @@ __device__ __forceinline__ void write_row(const CacheParams& p, int kv, const u3
   }
 }
 
-// A wave writes kWaveRows consecutive new rows of one head, K and V.
-template <int D, int F>
+// A wave writes U kWaveRows consecutive new rows of one head, K and V.
+template <int D, int F, int U>
 __global__ __launch_bounds__(kCacheThreads) void cache_write_kernel(CacheParams p) {
   __shared__ int32_t s_off[kOffsetsMax];
   const PagedBatch& bt = p.batch;
@@ -133,26 +133,37 @@ __global__ __launch_bounds__(kCacheThreads) void cache_write_kernel(CacheParams 
   const int lane = threadIdx.x & 63;
   const int64_t unit = int64_t(blockIdx.x) * (kCacheThreads / 64) + (threadIdx.x >> 6);
   const int h = int(unit % p.H);
-  const int64_t group = unit / p.H;
-  const int64_t i64 = group * kWaveRows<D> + lane / kRowLanes<D>;
-  if (group * kWaveRows<D> >= bt.rows) return;
-  const int i = int(min(i64, int64_t(bt.rows - 1)));
-  u32x4 x[2];
+  const int64_t start = unit / p.H * (U * kWaveRows<D>);
+  if (start >= bt.rows) return;
+  // Rows past the last read that one and are not written.
+  auto place = [&](int u) { return start + u * kWaveRows<D> + lane / kRowLanes<D>; };
+  u32x4 x[U][2];
 #pragma unroll
-  for (int kv = 0; kv < 2; ++kv)
-    x[kv] = load16(p.rows[kv] + i * p.st[kv] + h * p.sh[kv] + 8 * (lane % kRowLanes<D>));
+  for (int u = 0; u < U; ++u) {
+    const int i = int(min(place(u), int64_t(bt.rows - 1)));
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv)
+      x[u][kv] = load16(p.rows[kv] + i * p.st[kv] + h * p.sh[kv] + 8 * (lane % kRowLanes<D>));
+  }
   auto offset = [&](int s) { return in_lds ? s_off[s] : bt.offset(s); };
-  const int s = sequence_of(offset, bt.S, i);
-  const int first = offset(s), end = offset(s + 1);
-  const int pos = bt.length(s) - (end - i);
-  int64_t row = -1;
-  if (i64 < bt.rows && i >= first && i < end && pos >= 0) {
-    const int page = bt.table[int64_t(s) * bt.width + (pos >> bt.page_shift)];
-    if (page >= 0 && page < bt.pages)
-      row = ((int64_t(page) * p.H + h) << bt.page_shift) + (pos & ((1 << bt.page_shift) - 1));
+  int64_t row[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int i = int(min(place(u), int64_t(bt.rows - 1)));
+    const int s = sequence_of(offset, bt.S, i);
+    const int first = offset(s), end = offset(s + 1);
+    const int pos = bt.length(s) - (end - i);
+    row[u] = -1;
+    if (place(u) < bt.rows && i >= first && i < end && pos >= 0) {
+      const int page = bt.table[int64_t(s) * bt.width + (pos >> bt.page_shift)];
+      if (page >= 0 && page < bt.pages)
+        row[u] = ((int64_t(page) * p.H + h) << bt.page_shift) + (pos & ((1 << bt.page_shift) - 1));
+    }
   }
 #pragma unroll
-  for (int kv = 0; kv < 2; ++kv) write_row<D, F>(p, kv, x[kv], row, lane);
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) write_row<D, F>(p, kv, x[u][kv], row[u], lane);
 }
 
 template <int F>
@@ -239,10 +250,24 @@ __global__ __launch_bounds__(kCacheThreads) void cache_read_kernel(CacheParams p
   }
 }
 
+template <int D, int F, int U>
+void write_rows(const CacheParams& p, hipStream_t stream) {
+  const int64_t units = (int64_t(p.batch.rows) + U * kWaveRows<D> - 1) / (U * kWaveRows<D>) * p.H;
+  hipLaunchKernelGGL((cache_write_kernel<D, F, U>), dim3(unsigned((units + 3) / 4)), dim3(kCacheThreads), 0, stream, p);
+}
+
 template <int D, int F>
 void write_variant(const CacheParams& p, hipStream_t stream) {
-  const int64_t units = (int64_t(p.batch.rows) + kWaveRows<D> - 1) / kWaveRows<D> * p.H;
-  hipLaunchKernelGGL((cache_write_kernel<D, F>), dim3(unsigned((units + 3) / 4)), dim3(kCacheThreads), 0, stream, p);
+  // BF16 rows, which need no arithmetic, four groups to a wave where that makes
+  // one round of waves of up to four (4,032 tokens of 24 heads of 128, 24,192
+  // waves: 17 us, 20 with one group; 20,000 of 8 heads, 40,000 waves: 38 and 33;
+  // 1,024 of 8, 2,048 waves, out of the caches: 9.1 and 8.0).
+  constexpr int64_t kCardWaves = 8192;  // 256 CUs of 32
+  const int64_t waves = (int64_t(p.batch.rows) + kWaveRows<D> - 1) / kWaveRows<D> * p.H;
+  if constexpr (F == kBf16) {
+    if (waves > kCardWaves && waves <= 4 * kCardWaves) return write_rows<D, F, 4>(p, stream);
+  }
+  write_rows<D, F, 1>(p, stream);
 }
 
 template <int D, int F>

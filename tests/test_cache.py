@@ -54,6 +54,16 @@ def test_write_equals_plain_indexing(fmt, dim, page, heads, lengths, new):
     assert_same_cache(got, whole)
 
 
+@pytest.mark.parametrize("lengths,new,heads,dim", [
+    ([1511], [1503], 24, 128), ([900, 0, 1400, 5], [897, 0, 1301, 1], 40, 64), ([5600], [5589], 24, 128),
+])
+def test_write_of_a_frame(lengths, new, heads, dim):
+    # From one round of waves up, and past four.
+    seqs = Sequences(lengths, new, heads=heads, dim=dim, page_size=64, seed=51)
+    whole = seqs.cache
+    assert_same_cache(written(seqs, new_rows(seqs, seqs.k), new_rows(seqs, seqs.v)), whole)
+
+
 def test_write_takes_many_sequences():
     # More sequences than one workgroup keeps offsets of.
     lengths = [1 + i % 3 for i in range(1500)]
