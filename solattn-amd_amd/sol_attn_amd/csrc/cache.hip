@@ -14,7 +14,7 @@
 // rows of neighbouring tokens of a page are contiguous (page-major, then head,
 // then row), and the BF16 side is read or written in whole rows.  A copy of 4
 // GiB reaches 4.9 TB/s on this card.  Writing 4,032 tokens of 24 heads of 128 in
-// BF16, 99 MB: 19 us a call, 5.2 TB/s; nine prompts of up to 4,801 tokens, 12
+// BF16, 99 MB: 18 us a call, 5.5 TB/s; nine prompts of up to 4,801 tokens, 12
 // heads of 64, FP8, 111 MB: 28 us, 4.0 TB/s (more rows per wave: 29 to 30).
 // Reading 40,320 tokens of 24 heads of 128 from INT8, 501 MB: 145 us, 3.5 TB/s;
 // 19,003 of 16 heads, 236 MB: 39 us where the caches hold a part.  Small calls
