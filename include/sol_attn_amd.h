@@ -452,11 +452,13 @@ int sol_attention_noalloc(const void* q, const int64_t* q_strides,
  *   context_lengths [sequences]: keys of each sequence, its new tokens included;
  *   query_offsets [sequences + 1]: rows query_offsets[s] .. [s + 1] - 1 of the
  *     call's K, V or Q are sequence s's new tokens, its last positions.
- * They are not validated on the host.  Lengths are clamped into the table's
- * range and offsets into [0, rows]; a page outside [0, pages) is no page: not
- * written, read as zeros, not attended; a new token whose position is
- * negative is not written.  So no content makes a kernel leave the given
- * tensors.  Offsets have to ascend, and no two new tokens may name one row of
+ * They are not validated on the host.  Rows outside [0, rows) do not exist
+ * (the write counts positions from the offsets as they are, attention from the
+ * offsets clamped into that range); a page outside [0, pages) is no page: not
+ * written, read as zeros, not attended; and neither is a position past the
+ * table, whatever the lengths say, or a negative one.  So no content makes a
+ * kernel leave the given tensors, and a length past the table moves no new
+ * token onto stored ones.  Offsets have to ascend, and no two new tokens may name one row of
  * one page: which of them stays, or a mix of both, is not defined then.  Rows
  * at and past query_offsets[sequences] are not read, and their outputs are
  * left as they were. */

@@ -127,7 +127,7 @@ __global__ __launch_bounds__(kCacheThreads) void cache_write_kernel(CacheParams 
   const PagedBatch& bt = p.batch;
   const bool in_lds = bt.S < kOffsetsMax;
   if (in_lds) {
-    for (int s = threadIdx.x; s <= bt.S; s += kCacheThreads) s_off[s] = bt.offset(s);
+    for (int s = threadIdx.x; s <= bt.S; s += kCacheThreads) s_off[s] = bt.offsets[s];
     __syncthreads();
   }
   const int lane = threadIdx.x & 63;
@@ -145,16 +145,17 @@ __global__ __launch_bounds__(kCacheThreads) void cache_write_kernel(CacheParams 
     for (int kv = 0; kv < 2; ++kv)
       x[u][kv] = load16(p.rows[kv] + i * p.st[kv] + h * p.sh[kv] + 8 * (lane % kRowLanes<D>));
   }
-  auto offset = [&](int s) { return in_lds ? s_off[s] : bt.offset(s); };
+  auto offset = [&](int s) { return in_lds ? s_off[s] : bt.offsets[s]; };
   int64_t row[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const int i = int(min(place(u), int64_t(bt.rows - 1)));
     const int s = sequence_of(offset, bt.S, i);
     const int first = offset(s), end = offset(s + 1);
-    const int pos = bt.length(s) - (end - i);
+    // From the length as it is: clamped to the table it would move the row to the place of a stored one.
+    const int64_t pos = int64_t(bt.lengths[s]) - (int64_t(end) - i);
     row[u] = -1;
-    if (place(u) < bt.rows && i >= first && i < end && pos >= 0) {
+    if (place(u) < bt.rows && i >= first && i < end && pos >= 0 && pos < bt.positions()) {
       const int page = bt.table[int64_t(s) * bt.width + (pos >> bt.page_shift)];
       if (page >= 0 && page < bt.pages)
         row[u] = ((int64_t(page) * p.H + h) << bt.page_shift) + (pos & ((1 << bt.page_shift) - 1));

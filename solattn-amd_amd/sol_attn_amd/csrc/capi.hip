@@ -965,7 +965,7 @@ void window_params(sol::PagedParams* p, int64_t query_heads, int64_t heads, doub
   p->G = int(query_heads / heads);
   p->scale_log2 = float(scale * 1.4426950408889634);
   p->causal = causal != 0;
-  p->window = int(window == 0 ? kMaxPositions : std::min(window, kMaxPositions));
+  p->window = window == 0 || window >= kMaxPositions ? INT32_MAX : int(window);  // (no key is further away)
   p->sinks = window == 0 ? 0 : int(std::min(sink_tokens, kMaxPositions));
 }
 

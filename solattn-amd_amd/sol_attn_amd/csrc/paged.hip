@@ -1,8 +1,9 @@
 // Attention of new tokens over a paged cache, and over plain K / V under a
 // sliding window with first tokens that stay visible.
 //
-// Query i of an entry with n queries and L keys has position p = L - n + i; key
-// j < L is visible iff (j <= p or not causal) and (|p - j| < window or j <
+// Query i of an entry with n queries and L keys has position p = L - n + i (L as
+// the caller gives it, also past the keys that a page table names); key j < L is
+// visible iff (j <= p or not causal) and (|p - j| < window or j <
 // sinks).  O = sum_j softmax_j(scale q . k_j) v_j over the visible keys, 0 for
 // a query that sees none.  Scores, softmax statistics and sums are FP32; the
 // probabilities are rounded to BF16 for their product with V on the matrix
@@ -44,11 +45,13 @@ struct Visible {
   int lo, hi, sink;
 };
 
+// Positions lie from -2^30 on and may be past every key, windows reach 2^31 - 1
+// (none).
 __device__ __forceinline__ Visible visible(const PagedParams& p, int pos, int length) {
   Visible v;
-  v.lo = max(0, pos - p.window + 1);
-  v.hi = p.causal ? pos : min(length - 1, pos + p.window - 1);
-  v.sink = min(p.sinks, p.causal ? pos + 1 : length);
+  v.lo = max(pos, p.window - 1) - (p.window - 1);
+  v.hi = p.causal ? min(pos, length - 1) : min(pos, length - p.window) + p.window - 1;
+  v.sink = min(p.sinks, p.causal ? v.hi + 1 : length);
   return v;
 }
 
@@ -74,6 +77,7 @@ __device__ __forceinline__ Span span_of(const PagedParams& p, int first, int las
 
 struct Item {
   int s, off, n, length;  // the sequence: first row, new tokens, keys
+  int pos0;               // position of its first new token
   int r0, rows;           // the tile's rows r0 .. r0 + rows - 1 of the sequence's n G
   int part, parts;        // its share of the tile's keys
 };
@@ -137,6 +141,7 @@ __device__ __forceinline__ bool take_plain_item(const PagedParams& p, int id, It
   it.off = it.s * p.Tq;
   it.n = p.Tq;
   it.length = p.Tk;
+  it.pos0 = p.Tk - p.Tq;
   it.r0 = row_tile * R;
   it.rows = min(R, it.n * p.G - it.r0);
   if (p.records && it.part == 0)
@@ -150,21 +155,22 @@ __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item
   if constexpr (!PAGED) return take_plain_item<R, TK>(p, int(id), it);
   __shared__ int64_t s_total[kWaves];
   __shared__ int s_tiles[kWaves];
-  __shared__ int s_found[9];
+  __shared__ int s_found[10];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int S = p.batch.S;
-  // A sequence's first row, new tokens and keys, and its row tiles and key tiles.
+  // A sequence's first row, new tokens, end and keys, and its row tiles and key tiles.
   struct Sizes {
-    int off, n, length, row_tiles, key_tiles;
+    int off, n, end, length, row_tiles, key_tiles;
   };
   auto sizes = [&](int s) {
-    Sizes x = {0, 0, 0, 0, 0};
+    Sizes x = {0, 0, 0, 0, 0, 0};
     if (s < S) {
       x.off = p.batch.offset(s);
       x.n = p.batch.offset(s + 1) - x.off;
-      x.length = p.batch.length(s);
+      x.end = p.batch.end(s);
+      x.length = min(x.end, p.batch.positions());
       x.row_tiles = x.n > 0 ? (x.n * p.G - 1) / R + 1 : 0;
-      x.key_tiles = x.n > 0 ? max(1, span_of<TK>(p, x.length - x.n, x.length - 1, x.length).n) : 0;
+      x.key_tiles = x.n > 0 ? max(1, span_of<TK>(p, x.end - x.n, x.end - 1, x.length).n) : 0;
     }
     return x;
   };
@@ -253,6 +259,7 @@ __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item
       s_found[6] = x.off;
       s_found[7] = x.n;
       s_found[8] = x.length;
+      s_found[9] = x.end - x.n;
     }
     __syncthreads();
     base += int64_t(uniform64(uint64_t(all)));
@@ -269,6 +276,7 @@ __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item
   it.off = __builtin_amdgcn_readfirstlane(s_found[6]);
   it.n = __builtin_amdgcn_readfirstlane(s_found[7]);
   it.length = __builtin_amdgcn_readfirstlane(s_found[8]);
+  it.pos0 = __builtin_amdgcn_readfirstlane(s_found[9]);
   it.r0 = __builtin_amdgcn_readfirstlane(s_found[1]) * R;
   it.rows = min(R, it.n * p.G - it.r0);
   it.part = __builtin_amdgcn_readfirstlane(s_found[2]);
@@ -1075,7 +1083,7 @@ __global__ __launch_bounds__(kNT, 2) void step_kernel(PagedParams p) {
   const int col = lane & 15, g = lane >> 4;
 
   // This lane's query, straight into its operand registers (StepSlot::k's features).
-  const int pos0 = it.length - it.n;
+  const int pos0 = it.pos0;
   const int r = it.r0 + min(col, it.rows - 1);
   const int token = r / p.G;
   const uint16_t* q = p.q + (PAGED ? (it.off + token) * p.q_st : it.s * p.q_sb + token * p.q_st) +
@@ -1508,7 +1516,7 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
   const int col = lane & 31, hh = lane >> 5;
   const int wrows = min(32, it.rows - 32 * wave);  // this wave's rows (none: it only moves tiles)
 
-  const int pos0 = it.length - it.n;
+  const int pos0 = it.pos0;
   const int r = it.r0 + min(32 * wave + col, it.rows - 1);
   const int token = r / p.G;
   const uint16_t* q = p.q + (PAGED ? (it.off + token) * p.q_st : it.s * p.q_sb + token * p.q_st) +

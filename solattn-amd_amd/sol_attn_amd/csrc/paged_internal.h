@@ -17,9 +17,11 @@ constexpr int kElemBytes = F == kBf16 ? 2 : 1;
 // new tokens belong to sequence s, whose keys (the new ones included) are
 // positions 0 .. context_lengths[s] - 1; position p is row p % page_size of
 // page page_table[s][p / page_size].  The arrays are the caller's device
-// memory and may hold anything: offsets are clamped into [0, rows], lengths
-// into [0, width page_size], and a page outside [0, pages) is no page (not
-// written, read as zeros, not attended).
+// memory and may hold anything: rows outside [0, rows) do not exist (attention
+// clamps the offsets, the write looks rows up), a page outside [0, pages) is no
+// page (not written, read as zeros, not attended), and neither is there anything
+// past the table's last position.  (A length past the table must not move the
+// new tokens to the places of stored ones.)
 struct PagedBatch {
   const int32_t* table;    // [S, width]
   const int32_t* lengths;  // [S]
@@ -29,7 +31,10 @@ struct PagedBatch {
   int rows;                // new rows there are
 
   __device__ __forceinline__ int offset(int s) const { return min(max(offsets[s], 0), rows); }
-  __device__ __forceinline__ int length(int s) const { return min(max(lengths[s], 0), width << page_shift); }
+  // The position after sequence s's last new token, and how many keys it has in the table.
+  __device__ __forceinline__ int end(int s) const { return max(lengths[s], 0); }
+  __device__ __forceinline__ int positions() const { return width << page_shift; }
+  __device__ __forceinline__ int length(int s) const { return min(end(s), positions()); }
 };
 
 struct CacheParams {
@@ -54,7 +59,7 @@ struct PagedParams {
   int H, G;                   // K / V heads, query heads of each
   float scale_log2;
   int causal;
-  int window, sinks;          // window 2^30: none
+  int window, sinks;          // window 2^31 - 1: none
   // Keys split over workgroups (take_item in paged.hip); target 0: not split.
   int target, min_tiles;      // workgroups per head; key tiles of a part at least
   int64_t records;            // workgroups of the launch with target, else 0

@@ -87,8 +87,9 @@ class PagedPlan:
     captured launch follows what they hold at replay); the kernels read them
     there and check every entry against the tensors they address, so that no
     content makes them leave those: a page number outside the cache is no page
-    (not written, read as zeros, not attended).  What :meth:`create` refuses
-    is then up to the program: offsets that do not ascend, and new tokens that
+    (not written, read as zeros, not attended), and a new token whose position
+    is past the table (a length that has outgrown it) is not written.  What
+    else :meth:`create` refuses is then up to the program: offsets that do not ascend, and new tokens that
     name one row of one page twice, of which either one or a mix stays.
     """
 

@@ -275,3 +275,27 @@ def test_a_page_copied_to_another():
     for x, b in zip((seqs.cache.k, seqs.cache.v), before):
         b[dst] = b[src]
         assert torch.equal(x, b)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("lengths", [[33, 20], [35, 40], [64, 2 ** 31 - 1]])
+def test_a_length_past_the_table_leaves_stored_rows_alone(fmt, lengths):
+    # Two sequences of two pages: a step whose lengths have outgrown the table (a captured one replayed too often) drops
+    # the tokens past it, and those before keep their places.
+    cache = PagedCache.create(4, 16, 2, 64, format=fmt)
+    full = PagedPlan.create([[0, 1], [2, 3]], [32, 32], [32, 32], pages=4, page_size=16).to("cuda")
+    fill, new = rows(64, 2, 64, seed=60, device="cuda"), rows(6, 2, 64, seed=61, device="cuda")
+    cache_write(fill, fill, cache, full)
+    want = cache_read(cache, full, 32)[0]
+    full.context_lengths.copy_(torch.tensor(lengths, dtype=torch.int32))
+    full.query_offsets.copy_(torch.tensor([0, 2, 6], dtype=torch.int32))
+    cache_write(new, new, cache, full)
+    codes, scale = stored(new, fmt)
+    now = (codes if scale is None else codes.float() * scale[..., None]).to(torch.bfloat16).cuda()
+    for s, (length, first, n) in enumerate(zip(lengths, (0, 2), (2, 4))):
+        for i in range(n):
+            if length - n + i < 32:
+                want[s, length - n + i] = now[first + i]
+    full.context_lengths.fill_(32)
+    for got in cache_read(cache, full, 32):
+        assert torch.equal(got, want)
