@@ -488,7 +488,9 @@ int sol_cache_read(const void* cache_k, const void* cache_v, const float* k_scal
  * at position p sees key j of its sequence iff (j <= p, or causal is 0) and
  * (window is 0, or |p - j| < window, or j < sink_tokens); a query that sees no
  * key gets zeros.  Values at positions a query does not see never reach its
- * result, infinities and NaN included.  out: contiguous BF16 [rows,
+ * result, infinities and NaN included; an infinite value that it sees makes its
+ * feature infinite, or NaN beside one of the other sign or where FP32 leaves the
+ * key no weight.  out: contiguous BF16 [rows,
  * query_heads, head_dim].  workspace: 16-byte aligned device memory of at least
  * sol_paged_attention_workspace_size() bytes for the same sizes (NULL when that
  * is 0): the partial states of calls that split their keys over workgroups.  At

@@ -122,7 +122,9 @@ def window_attention(q, k, v, *, causal=True, window=None, sink_tokens=0, scale=
     ``window``, if ``abs(p - j) < window`` or ``j < sink_tokens`` (first tokens
     that stay visible).  ``window=None`` limits nothing.  A query that sees no
     key gets zeros; what a query does not see never reaches its result,
-    infinities and NaN included.  FP32 scores, softmax and accumulation; keys
+    infinities and NaN included.  An infinite value that it sees makes its
+    feature infinite, or NaN beside one of the other sign or where FP32 leaves
+    the key no weight.  FP32 scores, softmax and accumulation; keys
     outside every window are not read.  Not in the reference, whose attention
     is noncausal over all keys (:func:`dense_attention`).
     """

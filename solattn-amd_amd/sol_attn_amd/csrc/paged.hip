@@ -1022,9 +1022,14 @@ __device__ __forceinline__ void step_tile(const PagedParams& p, int length, Step
       for (int e = 0; e < 4; ++e) s[kb][e] = MASKED && !((seen >> (4 * kb + e)) & 1u) ? 0.f : s[kb][e] * sv[e];
     }
   }
-  // The probabilities as two BF16 terms (16 significant bits): the kernel waits
-  // for memory, and the products have time.
+  // The probabilities as two BF16 terms, the upper half and the rest (16
+  // significant bits, 2^-16 at most): the kernel waits for memory, and the
+  // products have time.  Neither term is negative.  In a whole BF16 tile neither
+  // is 0, so that an infinite value stays one: 2^-126 is added at most, of the
+  // largest probability's 1.  In a masked tile hidden keys have 0, and values that
+  // are not finite are added apart.
   constexpr bool kCheck = MASKED && F != kInt8;  // INT8 codes are finite
+  constexpr float kLeast = !MASKED && F == kBf16 ? 0x1p-126f : 0.f;
   uint32_t bad = 0;
 #pragma unroll
   for (int h = 0; h < TK / 32; ++h) {
@@ -1032,9 +1037,17 @@ __device__ __forceinline__ void step_tile(const PagedParams& p, int length, Step
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const f32x4& x = s[2 * h + (i >> 1)];
-      const float u = x[2 * (i & 1)], w = x[2 * (i & 1) + 1];
-      hi[i] = pack_bf16x2(u, w);
-      lo[i] = pack_bf16x2(u - __uint_as_float(hi[i] << 16), w - __uint_as_float(hi[i] & 0xFFFF0000u));
+      uint32_t u[2];
+      float rest[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float y = kLeast > 0.f ? fmaxf(x[2 * (i & 1) + j], kLeast) : x[2 * (i & 1) + j];
+        u[j] = __float_as_uint(y);
+        rest[j] = y - __uint_as_float(u[j] & 0xFFFF0000u);
+        if (kLeast > 0.f) rest[j] = fmaxf(rest[j], kLeast);
+      }
+      hi[i] = __builtin_amdgcn_perm(u[1], u[0], 0x07060302u);
+      lo[i] = pack_bf16x2(rest[0], rest[1]);
     }
 #pragma unroll
     for (int fb = 0; fb < FB; ++fb) {
