@@ -80,18 +80,19 @@ struct Item {
   int pos0;               // position of its first new token
   int r0, rows;           // the tile's rows r0 .. r0 + rows - 1 of the sequence's n G
   int part, parts;        // its share of the tile's keys
+  int record;             // where its partial state goes, if there are several parts
 };
 
-// What the merge kernel has to join: a header per (row tile, head), the tiles
-// in order of sequences.
+// What the merge kernel has to join: a header per (split row tile, head), the
+// tiles in order of sequences.
 struct Header {
   int parts;         // 0: nothing
   int off, r0, rows; // Item's
   uint32_t first, step;  // record of its first part, and from one part to the next
 };
 
-// Partial states of split tiles, after the headers: per workgroup (record) and
-// row D sums, the maximum, the denominator and whether a key was seen.
+// Partial states of split tiles, after the headers: per part (record) and row D
+// sums, the maximum, the denominator and whether a key was seen.
 template <int D>
 constexpr int kRecordRow = D + 4;
 
@@ -100,12 +101,24 @@ __device__ __forceinline__ float* record(const PagedParams& p, int64_t i) {
   return reinterpret_cast<float*>(static_cast<uint8_t*>(p.workspace) + p.header_bytes) + i * R * kRecordRow<D>;
 }
 
-// Header of row tile `tile` for this workgroup's head.  Every thread writes the
-// same: a branch on the thread made the compiler hold the keys' addresses, which
-// the DMA takes from scalar registers, in vector ones.  (Offsets that do not
-// ascend can name more tiles than there are headers.)
+// Header of split row tile `tile` for this workgroup's head.  Every thread writes
+// the same: a branch on the thread made the compiler hold the keys' addresses,
+// which the DMA takes from scalar registers, in vector ones.
 __device__ __forceinline__ void write_header(const PagedParams& p, int64_t tile, const Header& hd) {
-  if (tile >= 0 && tile < p.tiles) static_cast<Header*>(p.workspace)[tile * p.H + blockIdx.x % p.H] = hd;
+  if (tile >= 0 && tile < p.headers) static_cast<Header*>(p.workspace)[tile * p.H + blockIdx.x % p.H] = hd;
+}
+
+// Marks the headers past the last split tile as nothing, by the workgroups
+// that have no item: the launch's last `idle` ones per head, of which this is
+// number i.
+__device__ __forceinline__ void clear_headers(const PagedParams& p, int64_t split_tiles, int64_t i, int64_t idle) {
+  for (int64_t t = split_tiles + i; t < p.headers; t += idle) write_header(p, t, Header{0, 0, 0, 0, 0, 0});
+}
+
+// Record `part` of this workgroup's head.  (Lengths that change while the launch
+// reads them could name one that there is not.)
+__device__ __forceinline__ int record_of(const PagedParams& p, int64_t part) {
+  return int(min(max(part, int64_t(0)) * p.H, p.records - p.H)) + int(blockIdx.x % p.H);
 }
 
 // Item `id` of the launch, in order of sequences, parts and row tiles; false
@@ -114,8 +127,11 @@ __device__ __forceinline__ void write_header(const PagedParams& p, int64_t tile,
 // captured launch follows them and no launch or copy comes before this one.
 // With p.target, parts are of at most z key tiles, z such that about p.target
 // workgroups per head share all key tiles evenly: sum ceil(n_s / z) tiles_s is
-// at most target + sum tiles_s, the grid.  Without, one part each.  No tile has
+// below target + sum tiles_s, the grid.  Without, one part each.  No tile has
 // more than kMaxParts parts: the merge's time grows with them.
+// A split tile has more than z >= sum / target key tiles, so there are fewer than
+// target of them, and ceil(n / z) < 2 n / z makes their parts fewer than 2
+// target: the headers and records of a launch, however many row tiles it has.
 constexpr int kMaxParts = 128;
 
 // A tile's key tiles at most in a part, of `sum` key tiles per head.
@@ -132,7 +148,8 @@ __device__ __forceinline__ bool take_plain_item(const PagedParams& p, int id, It
   const int items = rt * it.parts;  // of an entry; all of them are fewer than 2^24 (the grid)
   it.s = __builtin_amdgcn_readfirstlane(id / items);
   if (it.s >= p.batch.S) {
-    if (p.records) write_header(p, int64_t(p.batch.S) * rt + (id - p.batch.S * items), Header{0, 0, 0, 0, 0, 0});
+    const int all = p.batch.S * items;
+    if (p.records) clear_headers(p, it.parts > 1 ? p.batch.S * rt : 0, id - all, int(gridDim.x) / p.H - all);
     return false;
   }
   const int k = id - it.s * items;
@@ -144,9 +161,12 @@ __device__ __forceinline__ bool take_plain_item(const PagedParams& p, int id, It
   it.pos0 = p.Tk - p.Tq;
   it.r0 = row_tile * R;
   it.rows = min(R, it.n * p.G - it.r0);
-  if (p.records && it.part == 0)
-    write_header(p, int64_t(it.s) * rt + tile,
-                 Header{it.parts > 1 ? it.parts : 0, it.off, it.r0, it.rows, blockIdx.x, uint32_t(rt) * uint32_t(p.H)});
+  if (it.parts > 1) {
+    it.record = record_of(p, id);
+    if (it.part == 0)
+      write_header(p, int64_t(it.s) * rt + tile,
+                   Header{it.parts, it.off, it.r0, it.rows, uint32_t(it.record), uint32_t(rt) * uint32_t(p.H)});
+  }
   return true;
 }
 
@@ -154,23 +174,24 @@ template <int R, int TK, bool PAGED>
 __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item& it) {
   if constexpr (!PAGED) return take_plain_item<R, TK>(p, int(id), it);
   __shared__ int64_t s_total[kWaves];
-  __shared__ int s_tiles[kWaves];
+  __shared__ uint64_t s_split[kWaves];
   __shared__ int s_found[10];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int S = p.batch.S;
-  // A sequence's first row, new tokens, end and keys, and its row tiles and key tiles.
+  // A sequence's first row, new tokens and end, and its row tiles and key tiles
+  // (which matter with p.target alone).
   struct Sizes {
-    int off, n, end, length, row_tiles, key_tiles;
+    int off, n, end, row_tiles, key_tiles;
   };
   auto sizes = [&](int s) {
-    Sizes x = {0, 0, 0, 0, 0, 0};
+    Sizes x = {0, 0, 0, 0, 0};
     if (s < S) {
       x.off = p.batch.offset(s);
       x.n = p.batch.offset(s + 1) - x.off;
       x.end = p.batch.end(s);
-      x.length = min(x.end, p.batch.positions());
       x.row_tiles = x.n > 0 ? (x.n * p.G - 1) / R + 1 : 0;
-      x.key_tiles = x.n > 0 ? max(1, span_of<TK>(p, x.end - x.n, x.end - 1, x.length).n) : 0;
+      if (p.target && x.n > 0)
+        x.key_tiles = max(1, span_of<TK>(p, x.end - x.n, x.end - 1, min(x.end, p.batch.positions())).n);
     }
     return x;
   };
@@ -195,9 +216,12 @@ __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item
     __syncthreads();
   }
   int64_t base = 0;
-  int tiles = 0;  // row tiles of the sequences before s0
+  uint64_t split = 0;  // of the sequences before s0: parts of split tiles, times 2^32, and the tiles
   auto parts_of = [&](const Sizes& x) {
-    return x.row_tiles ? (x.key_tiles - 1) / max(z, cdiv_i(x.key_tiles, kMaxParts)) + 1 : 1;
+    return p.target && x.row_tiles ? (x.key_tiles - 1) / max(z, cdiv_i(x.key_tiles, kMaxParts)) + 1 : 1;
+  };
+  auto split_of = [&](const Sizes& x, int64_t items) {
+    return items > x.row_tiles ? (uint64_t(items) << 32) + uint32_t(x.row_tiles) : 0ull;
   };
   // Larger batches: kEach consecutive sequences per thread, as a step of the scan
   // costs two barriers (4,096 sequences of 256 keys, 8 heads: 1,172 us, 1,297
@@ -208,44 +232,48 @@ __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item
     int s = s0 + tid * each;
     Sizes mine_of[kEach] = {mine0};
     int64_t mine = 0;
-    int mine_tiles = 0;
+    uint64_t mine_split = 0;
 #pragma unroll
     for (int j = 0; j < kEach; ++j) {
       if (j && each == 1) break;
       if (each > 1) mine_of[j] = sizes(s + j);
-      mine += int64_t(mine_of[j].row_tiles) * parts_of(mine_of[j]);
-      mine_tiles += mine_of[j].row_tiles;
+      const int64_t items = int64_t(mine_of[j].row_tiles) * parts_of(mine_of[j]);
+      mine += items;
+      mine_split += split_of(mine_of[j], items);
     }
     int64_t end = mine;  // inclusive sums over the wave
-    int tile_end = mine_tiles;
+    uint64_t split_end = mine_split;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
       const int64_t a = __shfl_up(end, off);
-      const int b = __shfl_up(tile_end, off);
-      if (lane >= off) end += a, tile_end += b;
+      if (lane >= off) end += a;
+      if (p.target) {
+        const uint64_t b = uint64_t(__shfl_up(int64_t(split_end), off));
+        if (lane >= off) split_end += b;
+      }
     }
-    if (lane == 63) s_total[wave] = end, s_tiles[wave] = tile_end;
+    if (lane == 63) s_total[wave] = end, s_split[wave] = split_end;
     __syncthreads();
     int64_t all = 0;
-    int all_tiles = 0;
+    uint64_t all_split = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      if (w == wave) end += all + base, tile_end += all_tiles + tiles;
+      if (w == wave) end += all + base, split_end += all_split + split;
       all += s_total[w];
-      all_tiles += s_tiles[w];
+      all_split += s_split[w];
     }
     if (id >= end - mine && id < end) {
       // Row tile by row tile of a part (they read the same keys), the longest first.
       int64_t first = end - mine;
-      int tile = tile_end - mine_tiles;
+      uint64_t before = split_end - mine_split;
       Sizes x = mine_of[0];
 #pragma unroll
       for (int j = 1; j < kEach; ++j) {
         if (each == 1) break;
-        const int64_t next = first + int64_t(x.row_tiles) * parts_of(x);
-        if (id < next) break;
-        first = next;
-        tile += x.row_tiles;
+        const int64_t items = int64_t(x.row_tiles) * parts_of(x);
+        if (id < first + items) break;
+        first += items;
+        before += split_of(x, items);
         x = mine_of[j];
         s += 1;
       }
@@ -254,37 +282,39 @@ __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item
       s_found[1] = p.causal ? rt - 1 - k % rt : k % rt;
       s_found[2] = k / rt;
       s_found[3] = parts_of(x);
-      s_found[4] = tile + k % rt;
+      s_found[4] = int(uint32_t(before)) + k % rt;
       s_found[5] = rt;
       s_found[6] = x.off;
       s_found[7] = x.n;
-      s_found[8] = x.length;
-      s_found[9] = x.end - x.n;
+      s_found[8] = x.end;
+      s_found[9] = int(before >> 32) + k;
     }
     __syncthreads();
     base += int64_t(uniform64(uint64_t(all)));
-    tiles += __builtin_amdgcn_readfirstlane(all_tiles);
+    split += uniform64(all_split);
     if (id < base) break;
   }
   if (id >= base) {
-    // The launch has as many workgroups without an item as headers without a
-    // tile, at least.
-    if (p.records) write_header(p, tiles + (id - base), Header{0, 0, 0, 0, 0, 0});
+    if (p.records) clear_headers(p, uint32_t(split), id - base, int(gridDim.x) / p.H - base);
     return false;
   }
   it.s = __builtin_amdgcn_readfirstlane(s_found[0]);
   it.off = __builtin_amdgcn_readfirstlane(s_found[6]);
   it.n = __builtin_amdgcn_readfirstlane(s_found[7]);
-  it.length = __builtin_amdgcn_readfirstlane(s_found[8]);
-  it.pos0 = __builtin_amdgcn_readfirstlane(s_found[9]);
+  const int end = __builtin_amdgcn_readfirstlane(s_found[8]);
+  it.length = min(end, p.batch.positions());
+  it.pos0 = end - it.n;
   it.r0 = __builtin_amdgcn_readfirstlane(s_found[1]) * R;
   it.rows = min(R, it.n * p.G - it.r0);
   it.part = __builtin_amdgcn_readfirstlane(s_found[2]);
   it.parts = __builtin_amdgcn_readfirstlane(s_found[3]);
-  if (p.records && it.part == 0)
-    write_header(p, __builtin_amdgcn_readfirstlane(s_found[4]),
-                 Header{it.parts > 1 ? it.parts : 0, it.off, it.r0, it.rows, blockIdx.x,
-                        uint32_t(__builtin_amdgcn_readfirstlane(s_found[5])) * uint32_t(p.H)});
+  if (it.parts > 1) {
+    it.record = record_of(p, __builtin_amdgcn_readfirstlane(s_found[9]));
+    if (it.part == 0)
+      write_header(p, __builtin_amdgcn_readfirstlane(s_found[4]),
+                   Header{it.parts, it.off, it.r0, it.rows, uint32_t(it.record),
+                          uint32_t(__builtin_amdgcn_readfirstlane(s_found[5])) * uint32_t(p.H)});
+  }
   return true;
 }
 
@@ -1204,7 +1234,7 @@ __global__ __launch_bounds__(kNT, 2) void step_kernel(PagedParams p) {
   den = quad_sum(den);
   seen = quad_sum(seen);
   if (col >= it.rows) return;
-  float* row_out = record<D, R>(p, blockIdx.x) + col * kRecordRow<D>;
+  float* row_out = it.parts > 1 ? record<D, R>(p, it.record) + col * kRecordRow<D> : nullptr;
   uint16_t* out = p.out + output_row<D>(p, it.off, it.r0 + col, h);
 #pragma unroll
   for (int fb = wave; fb < FB; fb += kWaves) {
@@ -1652,7 +1682,7 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
 
   const float den = pair_sum(st.den), seen = pair_sum(row.any ? 1.f : 0.f);
   if (col >= wrows) return;
-  float* row_out = record<D, R>(p, blockIdx.x) + (32 * wave + col) * kRecordRow<D>;
+  float* row_out = it.parts > 1 ? record<D, R>(p, it.record) + (32 * wave + col) * kRecordRow<D> : nullptr;
   uint16_t* out = p.out + output_row<D>(p, it.off, r, h);
 #pragma unroll
   for (int c = 0; c < D / 8; ++c) {
@@ -1675,7 +1705,7 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
 template <int D, int R>
 void launch_merge(const PagedParams& p, const PagedSize& size, hipStream_t stream) {
   const unsigned rows = unsigned((size.merge_rows - 1) / kMergeRows<D, R> + 1);
-  hipLaunchKernelGGL((merge_kernel<D, R>), dim3(unsigned(size.tiles * p.H), rows), dim3(kNT), 0, stream, p);
+  hipLaunchKernelGGL((merge_kernel<D, R>), dim3(unsigned(p.headers * p.H), rows), dim3(kNT), 0, stream, p);
 }
 
 template <int D, int F, bool PAGED>
@@ -1773,9 +1803,11 @@ PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t tile
     if (key_tiles > s.min_tiles) s.target = wide_target(likely, heads, key_tiles, s.min_tiles);
   }
   s.grid = (s.target + s.tiles) * heads;
-  s.header_bytes = (s.tiles * heads * int64_t(sizeof(Header)) + 15) / 16 * 16;
+  s.headers = std::min(s.target, s.tiles);  // (take_item's bounds)
+  s.records = std::min(2 * s.target, s.target ? s.target + s.tiles : 0) * heads;
+  s.header_bytes = (s.headers * heads * int64_t(sizeof(Header)) + 15) / 16 * 16;
   s.merge_rows = std::min(s.rows, (rows * group + sequences - 1) / sequences);
-  s.bytes = s.target ? s.header_bytes + s.grid * s.rows * (head_dim + 4) * 4 : 0;
+  s.bytes = s.header_bytes + s.records * s.rows * (head_dim + 4) * 4;
   return s;
 }
 
@@ -1783,8 +1815,8 @@ hipError_t launch_paged(const PagedParams& params, const PagedSize& size, int D,
   PagedParams p = params;
   p.target = int(size.target);
   p.min_tiles = int(size.min_tiles);
-  p.records = size.target ? size.grid : 0;
-  p.tiles = size.tiles;
+  p.headers = size.headers;
+  p.records = size.records;
   p.header_bytes = size.header_bytes;
   p.new_rows = p.batch.table ? p.batch.rows : int64_t(p.batch.S) * p.Tq;
   if (D == 128) launch_format<128>(p, size, format, stream);

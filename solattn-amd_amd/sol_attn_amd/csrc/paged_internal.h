@@ -62,8 +62,8 @@ struct PagedParams {
   int window, sinks;          // window 2^31 - 1: none
   // Keys split over workgroups (take_item in paged.hip); target 0: not split.
   int target, min_tiles;      // workgroups per head; key tiles of a part at least
-  int64_t records;            // workgroups of the launch with target, else 0
-  int64_t tiles, header_bytes, new_rows;
+  int64_t headers, records;   // PagedSize's
+  int64_t header_bytes, new_rows;
   void* workspace;            // PagedSize::bytes: headers, then records
 };
 
@@ -73,6 +73,8 @@ struct PagedSize {
   int64_t tiles;              // row tiles at most
   int64_t target, min_tiles;
   int64_t grid;               // workgroups
+  int64_t headers;            // split row tiles per head at most, 0 without target
+  int64_t records;            // their parts over all heads at most
   int64_t merge_rows;         // rows of a tile that the merge's workgroups take side by side
   int64_t header_bytes;
   int64_t bytes;              // workspace, 0 without target

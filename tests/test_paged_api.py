@@ -328,3 +328,25 @@ def test_gradients_of_the_cache_and_the_output_are_refused(name, monkeypatch):
         getattr(cache, name).requires_grad_()
     with pytest.raises(ValueError, match="Inference only"):
         paged_attention(q, cache, plan, out=out)
+
+
+def test_partial_states_do_not_grow_with_the_rows():
+    # At most 2 target records (parts of split row tiles) per head, target 1.5 x 512 workgroups over all heads for chunks
+    # and 512, or twice that, for single tokens, a little more by rounding up per head.
+    if not os.path.exists(_native.LIB_PATH):
+        pytest.skip("libsol_attn_amd.so not built")
+    lib = _native.library()
+    paged, window = lib.sol_paged_attention_workspace_size, lib.sol_window_attention_workspace_size
+    for dim in (64, 128):
+        for heads, group in ((8, 4), (1, 1), (24, 1)):
+            record = heads * 128 * (dim + 4) * 4
+            for rows, seqs, keys in ((8192, 2, 131072), (262144, 2, 131072), (1 << 19, 64, 8192), (1 << 19, 4096, 65536)):
+                for fmt in (0, 1, 2):
+                    size = paged(rows, seqs, keys // 64, 64, heads * group, heads, dim, fmt, 1, 0, 0)
+                    target = -(-3 * 256 // heads)
+                    assert 0 <= size <= 2 * target * (record + 32 * heads) + 16, (rows, seqs, keys, heads, dim, fmt)
+            step = heads * 16 * (dim + 4) * 4
+            for seqs in (64, 4096, 65536):
+                size = paged(seqs, seqs, 1024, 64, heads * group, heads, dim, 0, 1, 0, 0)
+                assert 0 < size <= 2 * -(-1024 // heads) * (step + 32 * heads) + 16
+            assert window(1, 131072, 131072, heads * group, heads, dim, 1, 0, 0) <= 2 * target * (record + 32 * heads) + 16
