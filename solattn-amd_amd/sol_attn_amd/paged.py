@@ -187,6 +187,11 @@ def _overlap(x, y):
     return x.numel() > 0 and y.numel() > 0 and ends[0][0] < ends[1][1] and ends[1][0] < ends[0][1]
 
 
+def _alike_overlap(x, y):
+    """The same of two contiguous tensors of one shape and type."""
+    return abs(x.data_ptr() - y.data_ptr()) < x.numel() * x.element_size()
+
+
 def _check_rows(name, x):
     if x.ndim != 3:
         raise ValueError(f"{name} must have NHD rank-3 layout")
@@ -216,8 +221,9 @@ def cache_write(k, v, cache, plan):
         raise ValueError("K and V must have the same shape and device")
     if k.shape[1:] != _validate(cache, plan, k.device):
         raise ValueError("K/V heads and head dimension must be the cache's")
-    if abs(cache.k.data_ptr() - cache.v.data_ptr()) < cache.k.numel() * cache.k.element_size():
-        raise ValueError("The cache's K and V must not share memory")
+    if _alike_overlap(cache.k, cache.v) or (cache.k.dtype != torch.bfloat16
+                                            and _alike_overlap(cache.k_scales, cache.v_scales)):
+        raise ValueError("The cache's K and V, and their scales, must not share memory")
     with _on(k.device):
         _native.launch_cache_write(k, v, cache, plan)
 
@@ -267,7 +273,9 @@ def paged_attention(q, cache, plan, *, causal=True, window=None, sink_tokens=0, 
         raise ValueError("out must be a contiguous BF16 tensor shaped like Q on its device")
     if out is not None and out.requires_grad:
         raise ValueError("Inference only: out must not require gradients")
-    if out is not None and (_overlap(out, q) or _overlap(out, cache.k) or _overlap(out, cache.v)):
-        raise ValueError("out must not share memory with Q or the cache")
+    if out is not None:
+        scales = () if cache.k.dtype == torch.bfloat16 else (cache.k_scales, cache.v_scales)
+        if any(_overlap(out, x) for x in (q, cache.k, cache.v, *scales)):
+            raise ValueError("out must not share memory with Q or the cache")
     with _on(q.device):
         return _native.launch_paged(q, cache, plan, scale, causal, window, min(sink_tokens, MAX_POSITIONS), out)

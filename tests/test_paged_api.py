@@ -350,3 +350,27 @@ def test_partial_states_do_not_grow_with_the_rows():
                 size = paged(seqs, seqs, 1024, 64, heads * group, heads, dim, 0, 1, 0, 0)
                 assert 0 < size <= 2 * -(-1024 // heads) * (step + 32 * heads) + 16
             assert window(1, 131072, 131072, heads * group, heads, dim, 1, 0, 0) <= 2 * target * (record + 32 * heads) + 16
+
+
+@pytest.mark.parametrize("shift", [0, 16])
+def test_write_refuses_a_cache_whose_scales_share_memory(shift, monkeypatch):
+    from sol_attn_amd import paged
+    cache, plan = parts("int8")
+    monkeypatch.setattr(paged, "_validate", lambda c, p, d: (2, 64))
+    scales = torch.zeros(4 * 2 * 16 + shift)
+    shared = PagedCache(cache.k, cache.v, *(x.view(4, 2, 16) for x in (scales[:128], scales[shift:])))
+    with pytest.raises(ValueError, match="share memory"):
+        cache_write(bf16(3, 2, 64), bf16(3, 2, 64), shared, plan)
+
+
+@pytest.mark.parametrize("side", [0, 1])
+def test_attention_refuses_an_output_in_the_scales(side, monkeypatch):
+    from sol_attn_amd import paged
+    cache, plan = parts("int8")
+    monkeypatch.setattr(paged, "_validate", lambda c, p, d: (2, 64))
+    store = torch.zeros(1024)
+    scales = [cache.k_scales, cache.v_scales]
+    scales[side] = store[:128].view(4, 2, 16)
+    with pytest.raises(ValueError, match="share memory"):
+        paged_attention(bf16(3, 4, 64), PagedCache(cache.k, cache.v, *scales), plan,
+                        out=store.view(torch.bfloat16)[:768].view(3, 4, 64))
