@@ -460,8 +460,8 @@ int sol_attention_noalloc(const void* q, const int64_t* q_strides,
  * kernel leave the given tensors, and a length past the table moves no new
  * token onto stored ones.  Offsets have to ascend, and no two new tokens may name one row of
  * one page: which of them stays, or a mix of both, is not defined then.  Rows
- * at and past query_offsets[sequences] are not read, and their outputs are
- * left as they were. */
+ * at and past query_offsets[sequences] exist (a write may read them), but they
+ * are not stored, and their outputs are left as they were. */
 #define SOL_CACHE_BF16 0
 #define SOL_CACHE_INT8 1
 #define SOL_CACHE_FP8 2

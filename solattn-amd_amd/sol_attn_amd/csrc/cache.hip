@@ -14,11 +14,11 @@
 // rows of neighbouring tokens of a page are contiguous (page-major, then head,
 // then row), and the BF16 side is read or written in whole rows.  A copy of 4
 // GiB reaches 4.9 TB/s on this card.  Writing 4,032 tokens of 24 heads of 128 in
-// BF16, 99 MB: 18 us a call, 5.5 TB/s; nine prompts of up to 4,801 tokens, 12
-// heads of 64, FP8, 111 MB: 28 us, 4.0 TB/s (more rows per wave: 29 to 30).
-// Reading 40,320 tokens of 24 heads of 128 from INT8, 501 MB: 145 us, 3.5 TB/s;
-// 19,003 of 16 heads, 236 MB: 39 us where the caches hold a part.  Small calls
-// are 5 us, less than the 12 that the host takes to make one.
+// BF16, 99 MB: 17 us where the caches hold them, 23 where not, 4.3 TB/s; nine
+// prompts of up to 4,801 tokens, 12 heads of 64, FP8, 111 MB: 28 us, 4.0 TB/s (more
+// rows per wave: 29 to 30).  Reading 40,320 tokens of 24 heads of 128 from INT8, 751
+// MB: 145 us, 5.2 TB/s; 19,003 of 16 heads, 236 MB: 39 us where the caches hold a
+// part.  Small calls are 5 us, less than the 12 that the host takes to make one.
 #include "paged_internal.h"
 #include "sol_device.h"
 
@@ -260,13 +260,17 @@ void write_rows(const CacheParams& p, hipStream_t stream) {
 template <int D, int F>
 void write_variant(const CacheParams& p, hipStream_t stream) {
   // BF16 rows, which need no arithmetic, four groups to a wave where that makes
-  // one round of waves of up to four (4,032 tokens of 24 heads of 128, 24,192
-  // waves: 17 us, 20 with one group; 20,000 of 8 heads, 40,000 waves: 38 and 33;
-  // 1,024 of 8, 2,048 waves, out of the caches: 9.1 and 8.0).
+  // one round of waves of one and a half to four.  Kernel time with one group and
+  // with four, rows and pages out of the caches (in them), 24 heads of 128; 8
+  // heads, and heads of 64, are within 3% of these:
+  //    8,300 waves  11.4 and 11.8 us (7.2 and 7.7)     24,000  24.0 and 23.2 (17.9 and 17.1)
+  //   10,000        12.7 and 12.7 (8.0 and 8.8)        28,000  26.2 and 27.4 (19.7 and 19.0)
+  //   12,000        14.5 and 13.8 (10.1 and 10.1)      32,000  29.7 and 26.2 (22.1 and 21.2)
+  //   16,000        17.2 and 15.8 (12.9 and 12.6)      40,000  35.7 and 39.5 (26.8 and 26.0)
   constexpr int64_t kCardWaves = 8192;  // 256 CUs of 32
   const int64_t waves = (int64_t(p.batch.rows) + kWaveRows<D> - 1) / kWaveRows<D> * p.H;
   if constexpr (F == kBf16) {
-    if (waves > kCardWaves && waves <= 4 * kCardWaves) return write_rows<D, F, 4>(p, stream);
+    if (waves > kCardWaves * 3 / 2 && waves <= 4 * kCardWaves) return write_rows<D, F, 4>(p, stream);
   }
   write_rows<D, F, 1>(p, stream);
 }

@@ -208,7 +208,7 @@ def cache_write(k, v, cache, plan):
 
     Row ``plan.query_offsets[s] + i`` goes to sequence s's position
     ``context_lengths[s] - new + i``; rows at and past the last offset are not
-    read, and everything else in the cache is left as it was.  Per token and
+    stored, and everything else in the cache is left as it was.  Per token and
     head, INT8 stores ``round(x * 127 / max|x|)`` (half to even) and FP8 the
     e4m3 value nearest ``x * 448 / max|x|``, with the scale ``max|x| / 127``
     (``/ 448``); a row with an infinity or a NaN reads back as NaN.  ``k`` and

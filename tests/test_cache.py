@@ -64,6 +64,16 @@ def test_write_of_a_frame(lengths, new, heads, dim):
     assert_same_cache(written(seqs, new_rows(seqs, seqs.k), new_rows(seqs, seqs.v)), whole)
 
 
+@pytest.mark.parametrize("lengths,new,heads,dim", [
+    ([2250], [2243], 24, 128), ([1500, 0, 2400, 5], [1497, 0, 2301, 1], 40, 64), ([2100], [2070], 24, 128),
+])
+def test_write_of_a_frame_in_one_round(lengths, new, heads, dim):
+    # From one and a half rounds of waves up to four, which take four groups of rows each, and just below.
+    seqs = Sequences(lengths, new, heads=heads, dim=dim, page_size=64, seed=52)
+    whole = seqs.cache
+    assert_same_cache(written(seqs, new_rows(seqs, seqs.k), new_rows(seqs, seqs.v)), whole)
+
+
 def test_write_takes_many_sequences():
     # More sequences than one workgroup keeps offsets of.
     lengths = [1 + i % 3 for i in range(1500)]
