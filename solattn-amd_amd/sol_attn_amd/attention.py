@@ -100,8 +100,11 @@ def dense_attention(q, k, v, *, scale=None):
         return _native.launch_dense(q, k, v, scale)
 
 
-def _visibility(causal, window, sink_tokens):
-    """Checks the arguments that say which keys a query sees; returns the window, 0 for none."""
+def _visibility(scale, causal, window, sink_tokens):
+    """Checks the scale, which is an FP32 factor, and the arguments that say
+    which keys a query sees; returns the window, 0 for none."""
+    if not 0 < scale < 2.0 ** 127:
+        raise ValueError("scale must be finite and positive, below 2^127")
     if not isinstance(causal, bool):
         raise ValueError("causal must be True or False")
     _nonnegative_integer("sink_tokens", sink_tokens)
@@ -129,7 +132,7 @@ def window_attention(q, k, v, *, causal=True, window=None, sink_tokens=0, scale=
     is noncausal over all keys (:func:`dense_attention`).
     """
     scale = _validate(q, k, v, scale, grouped=True)
-    window = _visibility(causal, window, sink_tokens)
+    window = _visibility(scale, causal, window, sink_tokens)
     with _on(q.device):
         return _native.launch_window(q, k, v, scale, causal, window, min(sink_tokens, k.shape[1]))
 

@@ -932,7 +932,8 @@ int window_args_ok(const char* what, int64_t query_heads, int64_t heads, double 
   };
   if (query_heads <= 0 || query_heads >= (1 << 16) || query_heads % heads)
     return bad("query heads must be a positive multiple of the key heads");
-  if (!std::isfinite(scale) || scale <= 0) return bad("scale must be finite and positive");
+  // (Times log2 e it is an FP32 factor of the scores.)
+  if (!(scale > 0 && scale < 0x1p127)) return bad("scale must be finite and positive, below 2^127");
   if (window < 0 || sink_tokens < 0) return bad("window and sink_tokens must not be negative");
   if (!out || !aligned16(out)) return bad("out must be 16-byte aligned");
   return SOL_OK;

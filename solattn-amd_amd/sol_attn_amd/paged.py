@@ -10,8 +10,6 @@ stored rows back into plain BTHD tensors, as :func:`sol_attention` and
 """
 
 from dataclasses import dataclass
-import math
-
 import torch
 
 from . import _native
@@ -264,10 +262,8 @@ def paged_attention(q, cache, plan, *, causal=True, window=None, sink_tokens=0, 
         raise ValueError("Q heads must be a multiple of the cache's, of its head dimension")
     if plan.context_lengths.shape[0] > MAX_ATTENDED:
         raise ValueError(f"More than {MAX_ATTENDED} sequences in one call are not supported")
-    window = _visibility(causal, window, sink_tokens)
     scale = dim ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale) or scale <= 0:
-        raise ValueError("scale must be finite and positive")
+    window = _visibility(scale, causal, window, sink_tokens)
     if out is not None and (out.dtype != torch.bfloat16 or out.shape != q.shape or not out.is_contiguous()
                             or out.device != q.device or out.data_ptr() & 15):
         raise ValueError("out must be a contiguous BF16 tensor shaped like Q on its device")

@@ -374,3 +374,22 @@ def test_attention_refuses_an_output_in_the_scales(side, monkeypatch):
     with pytest.raises(ValueError, match="share memory"):
         paged_attention(bf16(3, 4, 64), PagedCache(cache.k, cache.v, *scales), plan,
                         out=store.view(torch.bfloat16)[:768].view(3, 4, 64))
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 127, 1e39, 1e300, float("inf")])
+def test_scales_past_fp32_are_refused(scale, monkeypatch):
+    from sol_attn_amd import attention, paged
+    cache, plan = parts()
+    monkeypatch.setattr(paged, "_validate", lambda c, p, d: (2, 64))
+    with pytest.raises(ValueError, match="scale must be"):
+        paged_attention(bf16(3, 4, 64), cache, plan, scale=scale)
+    monkeypatch.setattr(attention, "_validate", lambda q, k, v, scale, grouped: scale)
+    with pytest.raises(ValueError, match="scale must be"):
+        window_attention(bf16(1, 3, 4, 64), bf16(1, 5, 2, 64), bf16(1, 5, 2, 64), scale=scale)
+    if not os.path.exists(_native.LIB_PATH):
+        pytest.skip("libsol_attn_amd.so not built")
+    lib, fake, ok = _native.library(), ctypes.c_void_p(1 << 20), (ctypes.c_int64 * 3)(640, 128, 64)
+    assert lib.sol_paged_attention(fake, ok, 3, fake, fake, None, None, fake, fake, fake, 2, 2, 4, 16, 4, 2, 64, 0, scale,
+                                   1, 0, 0, None, 0, None, None) < 0 and b"scale" in lib.sol_last_error()
+    assert lib.sol_window_attention(fake, ok, fake, ok, fake, ok, 1, 3, 5, 4, 2, 64, scale, 1, 0, 0, None, 0, None,
+                                    None) < 0 and b"scale" in lib.sol_last_error()
