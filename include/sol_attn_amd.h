@@ -482,7 +482,9 @@ int sol_cache_read(const void* cache_k, const void* cache_v, const float* k_scal
                    int64_t pages, int64_t page_size, int64_t heads, int64_t head_dim, int format, int64_t start,
                    int64_t tokens, void* k_out, void* v_out, void* stream);
 
-/* Attention of the new tokens over the cache, FP32 scores, softmax and sums.
+/* Attention of the new tokens over the cache, FP32 scores, softmax and sums; a
+ * probability (times its value's scale) is rounded to BF16 for its product with
+ * the value, by at most 2^-8 of itself, or, in calls of few rows, to 16 bits.
  * q: BF16 [rows, query_heads, head_dim] by its {batch (ignored), token, head}
  * strides; query head h attends key head h / (query_heads / heads).  The query
  * at position p sees key j of its sequence iff (j <= p, or causal is 0) and

@@ -127,7 +127,9 @@ def window_attention(q, k, v, *, causal=True, window=None, sink_tokens=0, scale=
     key gets zeros; what a query does not see never reaches its result,
     infinities and NaN included.  An infinite value that it sees makes its
     feature infinite, or NaN beside one of the other sign or where FP32 leaves
-    the key no weight.  FP32 scores, softmax and accumulation; keys
+    the key no weight.  FP32 scores, softmax and accumulation; for its product
+    with the values a probability is rounded to BF16, by at most 2^-8 of itself,
+    as in :func:`dense_attention` (calls of few rows keep 16 bits of it).  Keys
     outside every window are not read.  Not in the reference, whose attention
     is noncausal over all keys (:func:`dense_attention`).
     """

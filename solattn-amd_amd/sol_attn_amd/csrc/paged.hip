@@ -6,10 +6,12 @@
 // visible iff (j <= p or not causal) and (|p - j| < window or j <
 // sinks).  O = sum_j softmax_j(scale q . k_j) v_j over the visible keys, 0 for
 // a query that sees none.  Scores, softmax statistics and sums are FP32; the
-// probabilities are rounded to BF16 for their product with V on the matrix
-// cores, as everywhere in this library (half a step each, 2^-9, which averages
-// out over the keys; the denominator sums the unrounded ones), where few rows
-// leave them time as two BF16 terms.
+// probabilities (times V's scales) are rounded to BF16 for their product with V
+// on the matrix cores, as everywhere in this library (half a step each, 2^-8 at
+// most, which averages out over the keys; the denominator sums the unrounded
+// ones), where few rows leave them time as two BF16 terms.  (Two terms in
+// wide_kernel would be half as many products again in a kernel whose matrix
+// cores are busy for half of its time and more.)
 //
 // The rows of a (sequence, K/V head) are its new tokens times the G query
 // heads that share the head, token by token: row r is token r / G, query head

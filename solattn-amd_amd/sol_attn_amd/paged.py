@@ -249,8 +249,11 @@ def paged_attention(q, cache, plan, *, causal=True, window=None, sink_tokens=0, 
     :func:`window_attention`: with ``causal=False`` the new tokens see one
     another (a video frame), with one new token per sequence the call is a
     decoding step.  FP32 scores, softmax and accumulation on the stored values
-    (code times scale).  A query that sees no key gets zeros; infinities and
-    NaN as in :func:`window_attention`.
+    (code times scale).  For its product with a value (a code) a probability
+    (times the value's scale) is rounded to BF16, by at most 2^-8 of itself, in
+    calls of chunks, and keeps 16 bits in decoding steps and small calls.  A
+    query that sees no key gets zeros; infinities and NaN as in
+    :func:`window_attention`.
 
     ``out``: an optional contiguous BF16 tensor shaped like ``q``.  Rows at and
     past the last offset are not computed: they are left as they were in
