@@ -627,7 +627,8 @@ __device__ __forceinline__ void store4(uint16_t* out, const f32x4& x, float den,
 // parts in turn, kMergeAhead each in flight, and their states join in a fixed
 // order.  Tiles of 128 rows have few parts: each group takes a row of its own.
 // Bound by its launch (5 us with its reads' latency) or by memory: two parts of
-// 4,032 rows of 24 heads of 128, 129 MB, 27 us, 4.7 TB/s (148 us a row at a time).
+// 4,032 rows of 24 heads of 128, 129 MB, 43 us after the attention, 3.0 TB/s (148
+// us a row at a time).
 constexpr int kMergeAhead = 8;
 
 // A state of the merge: sums of 4 features, and the row's maximum, denominator
@@ -1106,7 +1107,7 @@ __device__ __forceinline__ void step_tile(const PagedParams& p, int length, Step
 // tiles of its own into its own slot, without a barrier, the next tile's keys
 // under way while this one's values are, and two workgroups per CU keep 128 KB
 // asked for.  Heads of 128, four query heads each: 64 sequences of 8,192 keys of
-// 8 heads, BF16 2.15 GB in 363 us, 5.9 TB/s; INT8 1.11 GB 218 us, 5.1 TB/s; FP8
+// 8 heads, BF16 2.15 GB in 371 us, 5.8 TB/s; INT8 1.11 GB 211 us, 5.3 TB/s; FP8
 // 210 us.  (BF16 tiles through registers, 32 x 32 products: 48 sequences of up to
 // 19,003 keys 256 us, 183 now.)  One sequence of 84,672 INT8 keys: 179 MB in 38
 // us and the merge's 5.  Small calls are a chain of latencies: three single
@@ -1540,11 +1541,11 @@ __device__ __forceinline__ void wide_tile(State<D>& st, const uint16_t* buf, con
 // Bound by the softmax's vector work beside the products: a half's 16 products
 // are 512 cycles of the matrix core, its exponentials, sums and packing about
 // 420 of the vector unit, of each of two waves.  4,096 queries of 16 heads of 128
-// over 16,384 keys, 550 GFLOP: BF16 502 us, 1.10 PFLOP/s (dense_attention_kernel
-// 486); heads of 64 323 us, 0.85 PFLOP/s.  8-bit codes add a conversion of 64
-// codes and 64 multiplications by scales per lane and tile: FP8 650 us, INT8
-// 690.  Two workgroups per CU hold 256 registers a wave and a ring of two tiles
-// each.
+// over 16,384 keys, 550 GFLOP: BF16 494 us, 1.11 PFLOP/s (dense_attention_kernel
+// 485); heads of 64 317 us, 0.87 PFLOP/s.  8-bit codes add a conversion of 64
+// codes and 64 multiplications by scales per lane and tile: FP8 645 us, INT8
+// 688.  Two workgroups per CU hold 256 registers a wave and a ring of two tiles
+// each; with heads of 128 that leaves 6 (BF16) to 17 (codes) registers spilled.
 template <int D, int F, bool PAGED>
 __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
   using S = Shape<D>;
