@@ -458,10 +458,11 @@ int sol_attention_noalloc(const void* q, const int64_t* q_strides,
  * written, read as zeros, not attended; and neither is a position past the
  * table, whatever the lengths say, or a negative one.  So no content makes a
  * kernel leave the given tensors, and a length past the table moves no new
- * token onto stored ones.  Offsets have to ascend, and no two new tokens may name one row of
- * one page: which of them stays, or a mix of both, is not defined then.  Rows
- * at and past query_offsets[sequences] exist (a write may read them), but they
- * are not stored, and their outputs are left as they were. */
+ * token onto stored ones.  Offsets have to ascend, and no two new tokens may
+ * name one row of one page: which of them stays, or a mix of both, is not
+ * defined then.  Rows at and past query_offsets[sequences] exist (a write may
+ * read them), but they are not stored, and their outputs are left as they
+ * were. */
 #define SOL_CACHE_BF16 0
 #define SOL_CACHE_INT8 1
 #define SOL_CACHE_FP8 2
@@ -491,8 +492,8 @@ int sol_cache_read(const void* cache_k, const void* cache_v, const float* k_scal
  * (window is 0, or |p - j| < window, or j < sink_tokens); a query that sees no
  * key gets zeros.  Values at positions a query does not see never reach its
  * result, infinities and NaN included; an infinite value that it sees makes its
- * feature infinite, or NaN beside one of the other sign or where FP32 leaves the
- * key no weight.  out: contiguous BF16 [rows,
+ * feature infinite, or NaN beside one of the other sign or where FP32 leaves
+ * the key no weight.  out: contiguous BF16 [rows,
  * query_heads, head_dim].  workspace: 16-byte aligned device memory of at least
  * sol_paged_attention_workspace_size() bytes for the same sizes (NULL when that
  * is 0): the partial states of calls that split their keys over workgroups.  At

@@ -87,8 +87,9 @@ class PagedPlan:
     content makes them leave those: a page number outside the cache is no page
     (not written, read as zeros, not attended), and a new token whose position
     is past the table (a length that has outgrown it) is not written.  What
-    else :meth:`create` refuses is then up to the program: offsets that do not ascend, and new tokens that
-    name one row of one page twice, of which either one or a mix stays.
+    else :meth:`create` refuses is then up to the program: offsets that do not
+    ascend, and new tokens that name one row of one page twice, of which either
+    one or a mix stays.
     """
 
     page_table: torch.Tensor
