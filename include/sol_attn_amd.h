@@ -524,6 +524,27 @@ int64_t sol_window_attention_workspace_size(int64_t batch, int64_t query_tokens,
                                             int64_t query_heads, int64_t heads, int64_t head_dim, int causal,
                                             int64_t window, int64_t sink_tokens);
 
+/* Norms of the heads' rows of Q and K, and their rotation by the tokens'
+ * positions, in one pass, FP32 (angles FP64), rounded once.
+ * q, k: BF16 [batch, tokens, query_heads / heads, head_dim] by their {batch,
+ * token, head} element strides; query_heads or heads 0: no such operand.  q_out,
+ * k_out: the same shapes by strides of their own; an output may be its input
+ * (same pointer and strides), but not meet it otherwise.
+ * positions: int32 [batch, tokens, axes], the axes contiguous, by
+ * position_strides {batch, token} (0: shared).  Pair j of a row is elements j and
+ * j + head_dim / 2, or (pairs != 0) 2 j and 2 j + 1; it turns by the angle
+ * positions[.., pair_axes[j]] * frequencies[j] (radians), (a, b) -> (a cos - b
+ * sin, a sin + b cos), and not at all where pair_axes[j] is outside [0, axes).
+ * frequencies: fp64 [head_dim / 2]; pair_axes: int32 [head_dim / 2].
+ * q_norm, k_norm: NULL, or weights w [head_dim], fp32 or (norms_bf16 != 0) BF16: a
+ * row x becomes x w / sqrt(mean x^2 + eps) before it turns. */
+int sol_rotate_heads(const void* q, const int64_t* q_strides, int64_t query_heads, void* q_out,
+                     const int64_t* q_out_strides, const void* k, const int64_t* k_strides, int64_t heads, void* k_out,
+                     const int64_t* k_out_strides, const int32_t* positions, const int64_t* position_strides,
+                     int64_t axes, const double* frequencies, const int32_t* pair_axes, int pairs, const void* q_norm,
+                     const void* k_norm, int norms_bf16, double eps, int64_t batch, int64_t tokens, int64_t head_dim,
+                     void* stream);
+
 #ifdef __cplusplus
 }
 #endif

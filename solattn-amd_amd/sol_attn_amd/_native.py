@@ -74,6 +74,8 @@ _SIGNATURES = {
     "sol_paged_attention_workspace_size": ([_i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _int, _i64, _i64], _i64),
     "sol_window_attention": ([_p, _i64p, _p, _i64p, _p, _i64p, _i64, _i64, _i64, _i64, _i64, _i64, _dbl, _int,
                               _i64, _i64, _p, _i64, _p, _p], ctypes.c_int),
+    "sol_rotate_heads": ([_p, _i64p, _i64, _p, _i64p, _p, _i64p, _i64, _p, _i64p, _p, _i64p, _i64, _p, _p, _int, _p, _p,
+                          _int, _dbl, _i64, _i64, _i64, _p], ctypes.c_int),
     "sol_window_attention_workspace_size": ([_i64, _i64, _i64, _i64, _i64, _i64, _int, _i64, _i64], _i64),
 }
 
@@ -815,3 +817,33 @@ def launch_window(q, k, v, scale, causal, window, sinks):
                                           scale, causal, window, sinks, _ptr(ws), size, out.data_ptr(),
                                           _stream(q.device)))
     return out
+
+
+def launch_rotate(q, k, positions, rotary, q_norm, k_norm, eps, outs):
+    """Norms and rotation of Q's and K's heads, BTHD or NHD (``sol_rotate_heads``); ``k`` may be None.  ``outs``: where
+    the results go, None for new tensors; returns them."""
+    args, results = [], []
+    for x, out in zip((q, k), outs):
+        if x is None:
+            args += [None, None, 0, None, None]
+            results.append(None)
+            continue
+        if out is None or out.data_ptr() != x.data_ptr():
+            x = _rows(x)
+        if out is None:
+            out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        results.append(out)
+        s, o = x.stride(), out.stride()
+        # (An NHD tensor is one entry, whose stride is not used.)
+        args += [x.data_ptr(), _stride_array(s[0], s[-3], s[-2]), x.shape[-2], out.data_ptr(),
+                 _stride_array(o[0], o[-3], o[-2])]
+    batched = q.dim() == 4
+    if q.shape[-3] == 0:
+        return results
+    at, norm = positions.stride(), q_norm if q_norm is not None else k_norm
+    _check(library().sol_rotate_heads(
+        *args, positions.data_ptr(), _stride_array(at[0] if batched else 0, at[-2], 0), positions.shape[-1],
+        rotary.frequencies.data_ptr(), rotary.axes.data_ptr(), rotary.layout == "pairs", _ptr(q_norm), _ptr(k_norm),
+        norm is not None and norm.dtype == torch.bfloat16, eps, q.shape[0] if batched else 1, q.shape[-3], q.shape[-1],
+        _stream(q.device)))
+    return results

@@ -7,6 +7,7 @@
 #include <string>
 
 #include "paged_internal.h"
+#include "rotate_internal.h"
 #include "sol_attn_amd.h"
 #include "sol_internal.h"
 
@@ -1141,6 +1142,53 @@ int64_t sol_window_attention_workspace_size(int64_t batch, int64_t query_tokens,
   return sol::paged_size(batch * query_tokens, batch,
                          window_keys(query_tokens, key_tokens, causal, window, sink_tokens),
                          window_keys(16, key_tokens, causal, window, sink_tokens), heads, query_heads / heads, head_dim, SOL_CACHE_BF16, causal != 0, false).bytes;
+}
+
+int sol_rotate_heads(const void* q, const int64_t* q_strides, int64_t query_heads, void* q_out,
+                     const int64_t* q_out_strides, const void* k, const int64_t* k_strides, int64_t heads, void* k_out,
+                     const int64_t* k_out_strides, const int32_t* positions, const int64_t* position_strides,
+                     int64_t axes, const double* frequencies, const int32_t* pair_axes, int pairs, const void* q_norm,
+                     const void* k_norm, int norms_bf16, double eps, int64_t batch, int64_t tokens, int64_t head_dim,
+                     void* stream) {
+  if (head_dim != 64 && head_dim != 128)
+    return fail(SOL_ERR_INVALID, "sol_rotate_heads: unsupported shape (head_dim must be 64 or 128)");
+  if (batch < 0 || batch >= (1 << 24) || tokens < 0 || tokens >= kMaxPositions || query_heads < 0 || heads < 0 ||
+      query_heads >= (1 << 16) || heads >= (1 << 16) || axes <= 0 || axes >= (1 << 16))
+    return fail(SOL_ERR_INVALID, "sol_rotate_heads: invalid shape");
+  if ((q_norm || k_norm) && !(eps >= 0x1p-126 && eps < 0x1p127))
+    return fail(SOL_ERR_INVALID, "sol_rotate_heads: eps must be a positive FP32 number");
+  if (batch == 0 || tokens == 0 || query_heads + heads == 0) return SOL_OK;
+  if (!positions || !position_strides || position_strides[0] < 0 || position_strides[1] < 0 || !frequencies ||
+      !pair_axes)
+    return fail(SOL_ERR_INVALID, "sol_rotate_heads: positions, frequencies and pair_axes are required");
+  sol::RotateParams p;
+  std::memset(&p, 0, sizeof(p));
+  for (int i = 0; i < 2; ++i) {
+    sol::RotateOperand& x = p.x[i];
+    x.heads = int(i ? heads : query_heads);
+    if (x.heads == 0) continue;
+    const int64_t* from = i ? k_strides : q_strides;
+    const int64_t* to = i ? k_out_strides : q_out_strides;
+    if (!operand_ok(i ? k : q, from, false) || !operand_ok(i ? k_out : q_out, to, false))
+      return fail(SOL_ERR_INVALID, "sol_rotate_heads: the rows need 16-byte alignment and positive strides");
+    x.rows = static_cast<const uint16_t*>(i ? k : q);
+    x.out = static_cast<uint16_t*>(i ? k_out : q_out);
+    x.sb = from[0], x.st = from[1], x.sh = from[2];
+    x.ob = to[0], x.ot = to[1], x.oh = to[2];
+    x.weight = i ? k_norm : q_norm;
+  }
+  if (cdiv(batch * tokens, 1024 / head_dim) * (query_heads + heads) > 4 * kMaxGrid)
+    return fail(SOL_ERR_UNSUPPORTED, "sol_rotate_heads: grid too large");
+  p.positions = positions;
+  p.pb = position_strides[0], p.pt = position_strides[1];
+  p.frequencies = frequencies;
+  p.axis = pair_axes;
+  p.axes = int(axes);
+  p.tokens = int(tokens);
+  p.rows = batch * tokens;
+  p.weights_bf16 = norms_bf16 != 0;
+  p.eps = float(eps);
+  return hip_status(sol::launch_rotate(p, int(head_dim), pairs != 0, static_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"

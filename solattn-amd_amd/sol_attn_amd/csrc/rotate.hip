@@ -1,0 +1,208 @@
+// Norms of the heads' rows of Q and K, and their rotation by the tokens'
+// positions, in one pass.
+//
+// A row x of D elements, w its norm's weight (no norm: y = x):
+//   y = x w / sqrt(mean x^2 + eps)
+// Pair j is elements j and j + D / 2 (halves) or 2 j and 2 j + 1 (pairs); its
+// angle is a = position[axis_j] f_j, and
+//   (y0, y1) -> (y0 cos a - y1 sin a, y0 sin a + y1 cos a)
+// rounded once to BF16; everything before is FP32.  An angle is formed and
+// reduced to a part of a turn in FP64: position 2^31 times f = 1 still leaves an
+// error of 2^-22, where FP32 would leave hundreds of turns.
+#include "rotate_internal.h"
+#include "sol_device.h"
+
+namespace sol {
+
+namespace {
+
+constexpr int kRotateThreads = 256;
+
+// D / 16 lanes hold a row, two 16-byte chunks each: chunk c and chunk c + D / 16,
+// so that both elements of a pair of halves lie in one lane, and eight pairs in
+// either layout.  A wave holds one head's rows of 1024 / D consecutive tokens and
+// goes from head to head, so the angles are formed once per token and wave.
+template <int D>
+constexpr int kRotateLanes = D / 16;
+template <int D>
+constexpr int kRotateTokens = 64 / kRotateLanes<D>;
+
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float x) {
+  return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, false));
+}
+
+// Sum over the lanes that hold a row.
+template <int D>
+__device__ __forceinline__ float row_sum(float x) {
+  x = dpp_add<0xB1>(x);  // lane ^ 1
+  x = dpp_add<0x4E>(x);  // lane ^ 2
+  if constexpr (kRotateLanes<D> == 8) x = dpp_add<0x141>(x);  // the row's other four
+  return x;
+}
+
+// Pair i (of a lane's eight) of the row.
+template <int D, bool PAIRS>
+__device__ __forceinline__ int pair_of(int c, int i) {
+  return PAIRS ? (i < 4 ? 4 * c + i : D / 4 + 4 * c + i - 4) : 8 * c + i;
+}
+
+// A lane's elements of one row: pair i is a[i], b[i].
+struct LanePairs {
+  float a[8], b[8];
+};
+
+template <bool PAIRS>
+__device__ __forceinline__ LanePairs unpack(const u32x4 (&x)[2]) {
+  LanePairs y;
+#pragma unroll
+  for (int n = 0; n < 2; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float lo = bf16_bits_to_f32(x[n][i] & 0xFFFFu), hi = __uint_as_float(x[n][i] & 0xFFFF0000u);
+      if constexpr (PAIRS) {
+        y.a[4 * n + i] = lo, y.b[4 * n + i] = hi;
+      } else {
+        (n ? y.b : y.a)[2 * i] = lo, (n ? y.b : y.a)[2 * i + 1] = hi;
+      }
+    }
+  return y;
+}
+
+template <bool PAIRS>
+__device__ __forceinline__ void pack(const LanePairs& y, u32x4 (&x)[2]) {
+#pragma unroll
+  for (int n = 0; n < 2; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (PAIRS)
+        x[n][i] = pack_bf16x2(y.a[4 * n + i], y.b[4 * n + i]);
+      else
+        x[n][i] = n ? pack_bf16x2(y.b[2 * i], y.b[2 * i + 1]) : pack_bf16x2(y.a[2 * i], y.a[2 * i + 1]);
+    }
+}
+
+// Divides a row by sqrt(mean x^2 + eps).  Squares of very large or very small
+// rows leave FP32's range: those rows are moved by a power of two first.
+template <int D>
+__device__ __forceinline__ void normalise(LanePairs& y, float eps) {
+  auto squares = [&](float f) {
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float a = y.a[i] * f, b = y.b[i] * f;
+      s = fmaf(a, a, fmaf(b, b, s));
+    }
+    return row_sum<D>(s);
+  };
+  float s = squares(1.f), f = 1.f;
+  const bool out = !(s < 0x1p100f) || (s < 0x1p-90f && eps < 0x1p-90f);
+  if (__builtin_amdgcn_ballot_w64(out)) {
+    const float f2 = s < 1.f ? 0x1p100f : 0x1p-70f;
+    const float s2 = squares(f2);
+    if (out) s = s2, f = f2, eps = eps * f2 * f2;
+  }
+  const float r = __fdiv_rn(1.f, __fsqrt_rn(fmaf(s, 1.f / D, eps)));
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y.a[i] = y.a[i] * f * r, y.b[i] = y.b[i] * f * r;
+}
+
+template <int D, bool PAIRS>
+__global__ __launch_bounds__(kRotateThreads) void rotate_kernel(RotateParams p, int heads_each) {
+  constexpr int U = 4;  // heads on their way together
+  const int lane = threadIdx.x & 63, c = lane % kRotateLanes<D>;
+  const int heads = p.x[0].heads + p.x[1].heads;
+  const int groups = (heads + heads_each - 1) / heads_each;
+  const int64_t unit = int64_t(blockIdx.x) * (kRotateThreads / 64) + (threadIdx.x >> 6);
+  const int64_t first = unit / groups * kRotateTokens<D>;
+  if (first >= p.rows) return;
+  const int h0 = int(unit % groups) * heads_each, h1 = min(h0 + heads_each, heads);
+  // Tokens past the last one read that one and store nothing.
+  const bool mine = first + lane / kRotateLanes<D> < p.rows;
+  const int64_t row = min(first + lane / kRotateLanes<D>, p.rows - 1);
+  const int64_t b = row / p.tokens, t = row % p.tokens;
+
+  float cs[8], sn[8];
+  const int32_t* at = p.positions + b * p.pb + t * p.pt;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int j = pair_of<D, PAIRS>(c, i);
+    const int axis = p.axis[j];
+    const int position = axis >= 0 && axis < p.axes ? at[axis] : 0;  // a pair of no axis stays as it is
+    const double turns = double(position) * p.frequencies[j] * 0.15915494309189533577;
+    sincospif(2.f * float(turns - rint(turns)), &sn[i], &cs[i]);
+  }
+
+#pragma unroll
+  for (int n = 0; n < 2; ++n) {
+    const RotateOperand& x = p.x[n];
+    const int from = max(h0 - (n ? p.x[0].heads : 0), 0), to = min(h1 - (n ? p.x[0].heads : 0), x.heads);
+    if (from >= to) continue;
+    LanePairs w;
+    if (x.weight) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int j = pair_of<D, PAIRS>(c, i), ja = PAIRS ? 2 * j : j, jb = PAIRS ? 2 * j + 1 : j + D / 2;
+        if (p.weights_bf16) {
+          const uint16_t* v = static_cast<const uint16_t*>(x.weight);
+          w.a[i] = bf16_bits_to_f32(v[ja]), w.b[i] = bf16_bits_to_f32(v[jb]);
+        } else {
+          const float* v = static_cast<const float*>(x.weight);
+          w.a[i] = v[ja], w.b[i] = v[jb];
+        }
+      }
+    }
+    const uint16_t* in = x.rows + b * x.sb + t * x.st + 8 * c;
+    uint16_t* out = x.out + b * x.ob + t * x.ot + 8 * c;
+    for (int h = from; h < to; h += U) {
+      u32x4 v[U][2];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) v[u][k] = load16(in + min(h + u, to - 1) * x.sh + k * (D / 2));
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        LanePairs y = unpack<PAIRS>(v[u]);
+        if (x.weight) {
+          normalise<D>(y, p.eps);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) y.a[i] *= w.a[i], y.b[i] *= w.b[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float a = y.a[i], bb = y.b[i];
+          y.a[i] = a * cs[i] - bb * sn[i];
+          y.b[i] = a * sn[i] + bb * cs[i];
+        }
+        pack<PAIRS>(y, v[u]);
+        if (mine && h + u < to) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) *reinterpret_cast<u32x4*>(out + (h + u) * x.oh + k * (D / 2)) = v[u][k];
+        }
+      }
+    }
+  }
+}
+
+template <int D, bool PAIRS>
+void rotate_variant(const RotateParams& p, hipStream_t stream) {
+  const int64_t groups = (p.rows + kRotateTokens<D> - 1) / kRotateTokens<D>;
+  const int heads = p.x[0].heads + p.x[1].heads;
+  int each = 4;
+  while (each < heads && groups * ((heads + each - 1) / each) > 16384) each *= 2;
+  const int64_t units = groups * ((heads + each - 1) / each);
+  hipLaunchKernelGGL((rotate_kernel<D, PAIRS>), dim3(unsigned((units + 3) / 4)), dim3(kRotateThreads), 0, stream, p,
+                     each);
+}
+
+}  // namespace
+
+hipError_t launch_rotate(const RotateParams& p, int D, bool pairs, hipStream_t stream) {
+  if (D == 128)
+    pairs ? rotate_variant<128, true>(p, stream) : rotate_variant<128, false>(p, stream);
+  else
+    pairs ? rotate_variant<64, true>(p, stream) : rotate_variant<64, false>(p, stream);
+  return hipGetLastError();
+}
+
+}  // namespace sol
