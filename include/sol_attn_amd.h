@@ -545,6 +545,48 @@ int sol_rotate_heads(const void* q, const int64_t* q_strides, int64_t query_head
                      const void* k_norm, int norms_bf16, double eps, int64_t batch, int64_t tokens, int64_t head_dim,
                      void* stream);
 
+/* Moves kept new tokens of a paged cache together (the accepted ones of a tree of
+ * drafts).  Of sequence s's n = query_offsets[s + 1] - query_offsets[s] new
+ * tokens, at positions base = context_lengths[s] - n on, those whose numbers
+ * kept[s][0] < kept[s][1] < ... (int32 [sequences, most]) ascend inside [0, n): the
+ * first entry that does not ends the list.  Row base + kept[s][j] goes to row base
+ * + j, K, V and scales of every head, as if all were read before any is written;
+ * lengths_out[s] (int32 [sequences]) receives base + their count, at least 0.
+ * Everything else is left as it was, as are rows whose source or target is in
+ * no page. */
+int sol_cache_keep(const int32_t* page_table, const int32_t* context_lengths, const int32_t* query_offsets,
+                   int64_t sequences, int64_t table_width, int64_t pages, int64_t page_size, int64_t heads,
+                   int64_t head_dim, int format, void* cache_k, void* cache_v, float* k_scales, float* v_scales,
+                   const int32_t* kept, int64_t most, int32_t* lengths_out, void* stream);
+
+/* The next plan of sequences over a paged cache: they go on, branch, end or begin,
+ * and their pages are shared, copied, freed and taken, all on the device.
+ * Old plan: page_table [sequences, table_width] and context_lengths (sequences
+ * may be 0); continued (int32 [sequences], NULL: context_lengths): how many of
+ * a sequence's tokens are continued from, clamped into [0, its length].
+ * refs: int32 [pages], how many tables name each page among their sequence's
+ * pages; a page of 0 (or less) is free.
+ * New sequence i of new_sequences: parents[i] is the old sequence it continues
+ * (outside [0, sequences): none, it begins empty), new_tokens[i] (at least 0) how
+ * many tokens come behind.  Its pages: the parent's whole pages; for the first
+ * child of a parent, those of its further pages that no other table names; for
+ * the others and behind them free ones, lowest first, in order of sequences and
+ * places, whose first takes a copy of the parent's rows in it (its tokens
+ * behind the last whole page).  Pages that become free are taken by later calls.
+ * Outputs: new_table [new_sequences, new_width] (-1 past a sequence's pages, and
+ * where no page was free), new_lengths, new_offsets [new_sequences + 1] (its
+ * new tokens are its last), new_refs [pages] (memory of its own), missing [1]: how
+ * many pages were not to be had.  Sequences that are no one's parent end; refs of
+ * their pages fall.  workspace: 16-byte aligned, of
+ * sol_cache_fork_workspace_size() bytes. */
+int64_t sol_cache_fork_workspace_size(int64_t sequences, int64_t new_sequences, int64_t pages);
+int sol_cache_fork(const int32_t* page_table, const int32_t* context_lengths, const int32_t* continued,
+                   int64_t sequences, int64_t table_width, const int32_t* parents, const int32_t* new_tokens,
+                   int64_t new_sequences, int64_t new_width, const int32_t* refs, int64_t pages, int64_t page_size,
+                   int64_t heads, int64_t head_dim, int format, void* cache_k, void* cache_v, float* k_scales,
+                   float* v_scales, int32_t* new_table, int32_t* new_lengths, int32_t* new_offsets, int32_t* new_refs,
+                   int32_t* missing, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -74,6 +74,11 @@ _SIGNATURES = {
     "sol_paged_attention_workspace_size": ([_i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _int, _i64, _i64], _i64),
     "sol_window_attention": ([_p, _i64p, _p, _i64p, _p, _i64p, _i64, _i64, _i64, _i64, _i64, _i64, _dbl, _int,
                               _i64, _i64, _p, _i64, _p, _p], ctypes.c_int),
+    "sol_cache_keep": ([_p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _int, _p, _p, _p, _p, _p, _i64, _p, _p],
+                       ctypes.c_int),
+    "sol_cache_fork_workspace_size": ([_i64, _i64, _i64], _i64),
+    "sol_cache_fork": ([_p, _p, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _int, _p, _p, _p, _p,
+                        _p, _p, _p, _p, _p, _p, _i64, _p], ctypes.c_int),
     "sol_rotate_heads": ([_p, _i64p, _i64, _p, _i64p, _p, _i64p, _i64, _p, _i64p, _p, _i64p, _i64, _p, _p, _int, _p, _p,
                           _int, _dbl, _i64, _i64, _i64, _p], ctypes.c_int),
     "sol_window_attention_workspace_size": ([_i64, _i64, _i64, _i64, _i64, _i64, _int, _i64, _i64], _i64),
@@ -847,3 +852,42 @@ def launch_rotate(q, k, positions, rotary, q_norm, k_norm, eps, outs):
         norm is not None and norm.dtype == torch.bfloat16, eps, q.shape[0] if batched else 1, q.shape[-3], q.shape[-1],
         _stream(q.device)))
     return results
+
+
+def _store_args(cache):
+    return cache.k.data_ptr(), cache.v.data_ptr(), _ptr(cache.k_scales), _ptr(cache.v_scales)
+
+
+def launch_cache_keep(cache, plan, kept):
+    """Moves kept rows together (``sol_cache_keep``); the sequences' lengths then."""
+    pages, h, page_size, d = cache.k.shape
+    s, width = plan.page_table.shape
+    lengths = torch.empty((s,), device=cache.k.device, dtype=torch.int32)
+    if s == 0:
+        return lengths
+    _check(library().sol_cache_keep(
+        *_plan_args(plan), s, width, pages, page_size, h, d, CACHE_FORMATS[cache.k.dtype], *_store_args(cache),
+        kept.data_ptr(), kept.shape[1], lengths.data_ptr(), _stream(cache.k.device)))
+    return lengths
+
+
+@functools.lru_cache(maxsize=1024)
+def _fork_size(s, n, pages):
+    return library().sol_cache_fork_workspace_size(s, n, pages)
+
+
+def launch_cache_fork(cache, refs, plan, parents, new_tokens, lengths, width):
+    """``(table, lengths, offsets, refs, missing)`` of the next plan and pool (``sol_cache_fork``)."""
+    pages, h, page_size, d = cache.k.shape
+    s, old_width = plan.page_table.shape
+    n, dev = parents.shape[0], cache.k.device
+    table, *rest = torch.empty(n * width + 2 * n + 2 + pages, device=dev, dtype=torch.int32).split(
+        (n * width, n, n + 1, pages, 1))
+    table = table.view(n, width)
+    ws = _workspace(_fork_size(s, n, pages), dev)
+    old_table, old_lengths, _ = _plan_args(plan)
+    _check(library().sol_cache_fork(
+        old_table, old_lengths, _ptr(lengths), s, old_width, parents.data_ptr(), new_tokens.data_ptr(), n, width,
+        refs.data_ptr(), pages, page_size, h, d, CACHE_FORMATS[cache.k.dtype], *_store_args(cache), table.data_ptr(),
+        *(x.data_ptr() for x in rest), ws.data_ptr(), ws.shape[0], _stream(dev)))
+    return table, *rest

@@ -6,6 +6,7 @@
 #include <mutex>
 #include <string>
 
+#include "fork_internal.h"
 #include "paged_internal.h"
 #include "rotate_internal.h"
 #include "sol_attn_amd.h"
@@ -1189,6 +1190,104 @@ int sol_rotate_heads(const void* q, const int64_t* q_strides, int64_t query_head
   p.weights_bf16 = norms_bf16 != 0;
   p.eps = float(eps);
   return hip_status(sol::launch_rotate(p, int(head_dim), pairs != 0, static_cast<hipStream_t>(stream)));
+}
+
+int sol_cache_keep(const int32_t* page_table, const int32_t* context_lengths, const int32_t* query_offsets,
+                   int64_t sequences, int64_t table_width, int64_t pages, int64_t page_size, int64_t heads,
+                   int64_t head_dim, int format, void* cache_k, void* cache_v, float* k_scales, float* v_scales,
+                   const int32_t* kept, int64_t most, int32_t* lengths_out, void* stream) {
+  const char* what = "sol_cache_keep";
+  sol::KeepParams p;
+  std::memset(&p, 0, sizeof(p));
+  int rc = paged_batch_ok(what, page_table, context_lengths, query_offsets, 0, sequences, table_width, pages, page_size,
+                          heads, head_dim, format, &p.batch);
+  if (rc != SOL_OK) return rc;
+  if (!query_offsets) return fail(SOL_ERR_INVALID, "sol_cache_keep: query_offsets is required");
+  rc = store_ok(what, cache_k, cache_v, k_scales, v_scales, format);
+  if (rc != SOL_OK) return rc;
+  if (most < 0 || most >= kMaxPositions || (most && !kept) || !lengths_out)
+    return fail(SOL_ERR_INVALID, "sol_cache_keep: kept and lengths_out are required");
+  if (sequences * heads > kMaxGrid / 8) return fail(SOL_ERR_UNSUPPORTED, "sol_cache_keep: grid too large");  // of 1,024 threads
+  p.kept = kept;
+  p.most = int(most);
+  p.store[0] = static_cast<uint8_t*>(cache_k);
+  p.store[1] = static_cast<uint8_t*>(cache_v);
+  p.scale[0] = k_scales;
+  p.scale[1] = v_scales;
+  p.H = int(heads);
+  p.lengths_out = lengths_out;
+  return hip_status(sol::launch_keep(p, int(head_dim), format, static_cast<hipStream_t>(stream)));
+}
+
+int64_t sol_cache_fork_workspace_size(int64_t sequences, int64_t new_sequences, int64_t pages) {
+  if (sequences < 0 || sequences > (1 << 20) || new_sequences < 0 || new_sequences > (1 << 20) || pages <= 0 ||
+      pages >= (int64_t(1) << 31))
+    return -1;
+  return sol::fork_size(sequences, new_sequences, pages).bytes;
+}
+
+int sol_cache_fork(const int32_t* page_table, const int32_t* context_lengths, const int32_t* continued,
+                   int64_t sequences, int64_t table_width, const int32_t* parents, const int32_t* new_tokens,
+                   int64_t new_sequences, int64_t new_width, const int32_t* refs, int64_t pages, int64_t page_size,
+                   int64_t heads, int64_t head_dim, int format, void* cache_k, void* cache_v, float* k_scales,
+                   float* v_scales, int32_t* new_table, int32_t* new_lengths, int32_t* new_offsets, int32_t* new_refs,
+                   int32_t* missing, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* what = "sol_cache_fork";
+  sol::PagedBatch shape;
+  int rc = paged_batch_ok(what, sequences ? page_table : refs, sequences ? context_lengths : refs, nullptr, 0,
+                          sequences ? sequences : 1, sequences ? table_width : 1, pages, page_size, heads, head_dim,
+                          format, &shape);
+  if (rc != SOL_OK) return rc;
+  rc = store_ok(what, cache_k, cache_v, k_scales, v_scales, format);
+  if (rc != SOL_OK) return rc;
+  const int64_t bytes = sol_cache_fork_workspace_size(sequences, new_sequences, pages);
+  if (bytes < 0 || new_width <= 0 || new_width > kMaxPositions / page_size)
+    return fail(SOL_ERR_INVALID, "sol_cache_fork: invalid shape");
+  if ((new_sequences && (!parents || !new_tokens || !new_table || !new_lengths)) || !refs || !new_offsets ||
+      !new_refs || !missing || refs == new_refs)
+    return fail(SOL_ERR_INVALID, "sol_cache_fork: parents, new_tokens, refs and outputs of their own are required");
+  if (!workspace || !aligned16(workspace) || workspace_bytes < bytes)
+    return fail(SOL_ERR_INVALID,
+                "sol_cache_fork: needs a 16-byte aligned workspace of the size its size function returns");
+  const int64_t row_bytes = head_dim * (format == SOL_CACHE_BF16 ? 2 : 1);
+  // (A copied page takes a workgroup per 32 KB of each head's K and V.)
+  if (new_sequences * heads * 2 * cdiv(page_size * row_bytes, 32768) + new_sequences + sequences > kMaxGrid)
+    return fail(SOL_ERR_UNSUPPORTED, "sol_cache_fork: grid too large");
+  const sol::ForkSize size = sol::fork_size(sequences, new_sequences, pages);
+  sol::ForkParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.table = page_table;
+  p.lengths = context_lengths;
+  p.continued = continued ? continued : context_lengths;
+  p.S = int(sequences);
+  p.width = int(table_width);
+  p.parents = parents;
+  p.new_tokens = new_tokens;
+  p.N = int(new_sequences);
+  p.new_width = int(new_width);
+  p.refs = refs;
+  p.pages = int(pages);
+  p.page_shift = shape.page_shift;
+  p.store[0] = static_cast<uint8_t*>(cache_k);
+  p.store[1] = static_cast<uint8_t*>(cache_v);
+  p.scale[0] = k_scales;
+  p.scale[1] = v_scales;
+  p.H = int(heads);
+  p.row_bytes = int(row_bytes);
+  p.new_table = new_table;
+  p.new_lengths = new_lengths;
+  p.new_offsets = new_offsets;
+  p.new_refs = new_refs;
+  p.missing = missing;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.slices = int(size.slices);
+  p.slice_pages = int(size.slice_pages);
+  p.first = reinterpret_cast<int32_t*>(ws + size.first);
+  p.children = reinterpret_cast<int32_t*>(ws + size.children);
+  p.start = reinterpret_cast<int64_t*>(ws + size.start);
+  p.free_count = reinterpret_cast<int32_t*>(ws + size.free_count);
+  p.free_list = reinterpret_cast<int32_t*>(ws + size.free_list);
+  return hip_status(sol::launch_fork(p, static_cast<hipStream_t>(stream)));
 }
 
 }  // extern "C"

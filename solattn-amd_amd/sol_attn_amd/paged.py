@@ -142,6 +142,38 @@ class PagedPlan:
         return PagedPlan(self.page_table.to(device), self.context_lengths.to(device), self.query_offsets.to(device))
 
 
+@dataclass(frozen=True)
+class PagePool:
+    """How many sequences hold each page of a cache; pages of none are free.
+
+    ``refs``: contiguous int32 ``[pages]``, how many of the plan's tables name the
+    page among their sequence's first ``ceil(context_lengths / page_size)``
+    pages; ``missing``: int32 ``[1]``, the pages that the call which made the pool
+    had to do without.  :func:`cache_fork` takes a pool and returns the next.
+    """
+
+    refs: torch.Tensor
+    missing: torch.Tensor
+
+    @classmethod
+    def create(cls, cache, plan=None):
+        """The pool of a cache whose pages are all free, or held by ``plan``, a
+        :class:`PagedPlan` on any device."""
+        if not isinstance(cache, PagedCache):
+            raise ValueError("An explicit PagedCache is required")
+        pages, _, page_size, _ = cache.k.shape
+        refs = torch.zeros(pages, dtype=torch.int32)
+        if plan is not None:
+            if not isinstance(plan, PagedPlan):
+                raise ValueError("An explicit PagedPlan is required")
+            for row, length in zip(plan.page_table.tolist(), plan.context_lengths.tolist()):
+                for page in row[:-(-max(length, 0) // page_size)]:
+                    if not 0 <= page < pages:
+                        raise ValueError("page_table names a page outside the cache")
+                    refs[page] += 1
+        return cls(refs.to(cache.k.device), torch.zeros(1, dtype=torch.int32, device=cache.k.device))
+
+
 def _validate(cache, plan, device):
     """Checks a cache and a plan, and that they lie on ``device``; returns the cache's ``(heads, head_dim)``."""
     if not isinstance(cache, PagedCache):
@@ -191,6 +223,13 @@ def _alike_overlap(x, y):
     return abs(x.data_ptr() - y.data_ptr()) < x.numel() * x.element_size()
 
 
+def _separate(cache):
+    """Refuses a cache that a call writes, where K and V are one."""
+    if _alike_overlap(cache.k, cache.v) or (cache.k.dtype != torch.bfloat16
+                                            and _alike_overlap(cache.k_scales, cache.v_scales)):
+        raise ValueError("The cache's K and V, and their scales, must not share memory")
+
+
 def _check_rows(name, x):
     if x.ndim != 3:
         raise ValueError(f"{name} must have NHD rank-3 layout")
@@ -220,9 +259,7 @@ def cache_write(k, v, cache, plan):
         raise ValueError("K and V must have the same shape and device")
     if k.shape[1:] != _validate(cache, plan, k.device):
         raise ValueError("K/V heads and head dimension must be the cache's")
-    if _alike_overlap(cache.k, cache.v) or (cache.k.dtype != torch.bfloat16
-                                            and _alike_overlap(cache.k_scales, cache.v_scales)):
-        raise ValueError("The cache's K and V, and their scales, must not share memory")
+    _separate(cache)
     with _on(k.device):
         _native.launch_cache_write(k, v, cache, plan)
 
@@ -279,3 +316,86 @@ def paged_attention(q, cache, plan, *, causal=True, window=None, sink_tokens=0, 
             raise ValueError("out must not share memory with Q or the cache")
     with _on(q.device):
         return _native.launch_paged(q, cache, plan, scale, causal, window, min(sink_tokens, MAX_POSITIONS), out)
+
+
+def _check_integers(name, x, shape, device):
+    if not isinstance(x, torch.Tensor) or x.dtype != torch.int32 or not x.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor")
+    if x.ndim != len(shape) or any(n is not None and n != m for n, m in zip(shape, x.shape)):
+        raise ValueError(f"{name} must have an entry for each sequence")
+    if x.get_device() != device.index:
+        raise ValueError(f"{name} must be on the cache's device")
+
+
+def cache_keep(cache, plan, kept):
+    """Moves the kept ones of the new tokens together: the accepted drafts of a tree
+    (:func:`tree_attention`), or what is left of a frame that is thinned out.
+
+    ``kept``: int32 ``[sequences, most]``: which of sequence s's new tokens stay,
+    their numbers (0 .. new - 1) in ascending order; the first entry that does
+    not ascend or is not one of them (-1, say) ends the list.  The K and V rows
+    of new token ``kept[s, j]`` (of position ``context_lengths[s] - new +
+    kept[s, j]``) move to that of new token j, in place; rows behind the kept
+    ones stay as they are.  Stored values move as they are: keys that were
+    turned by their positions keep those (:func:`rotate_heads` turns a draft by
+    its depth, which is its place once it is kept).
+
+    Returns the sequences' lengths then, int32 ``[sequences]``: what
+    :func:`cache_fork` continues from, or the lengths of a plan of your own.
+    """
+    device = cache.k.device if isinstance(cache, PagedCache) else None
+    _validate(cache, plan, device)
+    _separate(cache)
+    _check_integers("kept", kept, (plan.page_table.shape[0], None), device)
+    with _on(device):
+        return _native.launch_cache_keep(cache, plan, kept)
+
+
+def cache_fork(cache, pool, plan, parents, new_tokens, *, lengths=None, width=None):
+    """``(plan, pool)`` of the next call: sequences go on, branch, end or begin, on the GPU.
+
+    New sequence i continues sequence ``parents[i]`` of ``plan`` (int32
+    ``[new_sequences]``; outside of it, -1 say: none, the sequence begins) and has
+    ``new_tokens[i]`` (int32, too) more tokens behind, whose rows
+    :func:`cache_write` stores next.  A sequence that is no one's parent ends,
+    and one that several continue branches: beams, samples of one prompt.
+    ``lengths`` (int32 ``[sequences]``, from :func:`cache_keep`) continues from the
+    first so many of a sequence's tokens instead of all.
+
+    Whole pages are shared; a sequence's first child goes on in the pages behind
+    them that no other sequence holds; the other children take pages of their
+    own, and a copy of the rows that the first one begins with.  Pages are taken
+    from those that ``pool`` has free, the lowest first, and freed pages are
+    free for the next call.  Where none is left a table has -1, which is no page
+    (not written, not attended), and ``missing`` of the new pool counts them.
+
+    ``width``: pages that a new table has room for, by default the old one's.
+    ``plan`` and ``pool`` stay as they were, but the sequences they describe must
+    not be written any more: their pages have new owners.
+    """
+    device = cache.k.device if isinstance(cache, PagedCache) else None
+    _validate(cache, plan, device)
+    _separate(cache)
+    sequences, page_size = plan.page_table.shape[0], cache.k.shape[2]
+    if not isinstance(pool, PagePool):
+        raise ValueError("An explicit PagePool is required")
+    _check_integers("parents", parents, (None,), device)
+    _check_integers("new_tokens", new_tokens, (parents.shape[0],), device)
+    if lengths is not None:
+        _check_integers("lengths", lengths, (sequences,), device)
+    refs = pool.refs
+    if refs.dtype != torch.int32 or refs.shape != cache.k.shape[:1] or not refs.is_contiguous():
+        raise ValueError("Invalid pool; use PagePool.create with this cache")
+    if refs.get_device() != device.index:
+        raise ValueError("The pool must be on the cache's device")
+    if width is None:
+        width = plan.page_table.shape[1]
+    _nonnegative_integer("width", width)
+    if not 0 < width <= MAX_POSITIONS // page_size:
+        raise ValueError(f"width must name 1 to {MAX_POSITIONS} positions of each sequence")
+    if max(sequences, parents.shape[0]) > MAX_ATTENDED:
+        raise ValueError(f"More than {MAX_ATTENDED} sequences in one call are not supported")
+    with _on(device):
+        table, lengths, offsets, refs, missing = _native.launch_cache_fork(cache, refs, plan, parents, new_tokens,
+                                                                           lengths, width)
+    return PagedPlan(table, lengths, offsets), PagePool(refs, missing)
