@@ -72,6 +72,8 @@ _SIGNATURES = {
     "sol_paged_attention": ([_p, _i64p, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                              _int, _dbl, _int, _i64, _i64, _p, _i64, _p, _p], ctypes.c_int),
     "sol_paged_attention_workspace_size": ([_i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _int, _i64, _i64], _i64),
+    "sol_tree_attention": ([_p, _i64p, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
+                            _int, _dbl, _i64, _i64, _p, _i64, _p, _p], ctypes.c_int),
     "sol_window_attention": ([_p, _i64p, _p, _i64p, _p, _i64p, _i64, _i64, _i64, _i64, _i64, _i64, _dbl, _int,
                               _i64, _i64, _p, _i64, _p, _p], ctypes.c_int),
     "sol_cache_keep": ([_p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _int, _p, _p, _p, _p, _p, _i64, _p, _p],
@@ -783,8 +785,9 @@ def _workspace(size, device):
     return torch.empty(size, device=device, dtype=torch.uint8) if size else None
 
 
-def launch_paged(q, cache, plan, scale, causal, window, sinks, out=None):
-    """Attention of new tokens (NHD) over a paged cache (``sol_paged_attention``); ``window`` 0: none."""
+def launch_paged(q, cache, plan, scale, causal, window, sinks, out=None, parents=None):
+    """Attention of new tokens (NHD) over a paged cache (``sol_paged_attention``), or of trees of them
+    (``sol_tree_attention``); ``window`` 0: none."""
     n, hq, d = q.shape
     pages, h, page_size, _ = cache.k.shape
     s, width = plan.page_table.shape
@@ -798,6 +801,12 @@ def launch_paged(q, cache, plan, scale, causal, window, sinks, out=None):
     fmt = CACHE_FORMATS[cache.k.dtype]
     size = _paged_size(n, s, width, page_size, hq, h, d, fmt, causal, window, sinks)
     ws = _workspace(size, dev)
+    if parents is not None:
+        _check(library().sol_tree_attention(
+            q.data_ptr(), _strides(q, True), n, cache.k.data_ptr(), cache.v.data_ptr(), _ptr(cache.k_scales),
+            _ptr(cache.v_scales), table, lengths, offsets, parents.data_ptr(), s, width, pages, page_size, hq, h, d, fmt,
+            scale, window, sinks, _ptr(ws), size, out.data_ptr(), _stream(dev)))
+        return out
     _check(library().sol_paged_attention(
         q.data_ptr(), _strides(q, True), n, cache.k.data_ptr(), cache.v.data_ptr(), _ptr(cache.k_scales),
         _ptr(cache.v_scales), table, lengths, offsets, s, width, pages, page_size, hq, h, d,

@@ -972,6 +972,52 @@ void window_params(sol::PagedParams* p, int64_t query_heads, int64_t heads, doub
   p->sinks = window == 0 ? 0 : int(std::min(sink_tokens, kMaxPositions));
 }
 
+// Attention of new tokens over the cache; `parents`: of a tree of them, or null.
+int attend_paged(const char* what, const void* q, const int64_t* q_strides, int64_t rows, const void* cache_k,
+                 const void* cache_v, const float* k_scales, const float* v_scales, const int32_t* page_table,
+                 const int32_t* context_lengths, const int32_t* query_offsets, const int32_t* parents,
+                 int64_t sequences, int64_t table_width, int64_t pages, int64_t page_size, int64_t query_heads,
+                 int64_t heads, int64_t head_dim, int format, double scale, int causal, int64_t window,
+                 int64_t sink_tokens, void* workspace, int64_t workspace_bytes, void* out, void* stream) {
+  auto refuse = [&](int code, const char* msg) {
+    g_last_error = std::string(what) + ": " + msg;
+    return code;
+  };
+  sol::PagedParams p;
+  std::memset(&p, 0, sizeof(p));
+  int rc = paged_batch_ok(what, page_table, context_lengths, query_offsets, rows, sequences, table_width, pages,
+                          page_size, heads, head_dim, format, &p.batch);
+  if (rc != SOL_OK) return rc;
+  if (!query_offsets) return refuse(SOL_ERR_INVALID, "query_offsets is required");
+  rc = store_ok(what, cache_k, cache_v, k_scales, v_scales, format);
+  if (rc != SOL_OK) return rc;
+  if (rows == 0) return SOL_OK;
+  rc = window_args_ok(what, query_heads, heads, scale, window, sink_tokens, out);
+  if (rc != SOL_OK) return rc;
+  if (!operand_ok(q, q_strides, true))
+    return refuse(SOL_ERR_INVALID, "Q needs 16-byte aligned rows and positive strides");
+  if (sequences > kMaxAttended)
+    return refuse(SOL_ERR_UNSUPPORTED, "at most 65,536 sequences in one call");
+  if (rows * query_heads >= (int64_t(1) << 31))
+    return refuse(SOL_ERR_UNSUPPORTED, "grid too large");
+  const sol::PagedSize size =
+      sol::paged_size(rows, sequences, window_keys(rows, table_width * page_size, causal, window, sink_tokens),
+                      window_keys(16, table_width * page_size, causal, window, sink_tokens), heads,
+                      query_heads / heads, head_dim, format, causal != 0, true);
+  rc = paged_workspace_ok(what, size, workspace, workspace_bytes);
+  if (rc != SOL_OK) return rc;
+  p.q = static_cast<const uint16_t*>(q);
+  p.q_st = q_strides[1], p.q_sh = q_strides[2];
+  for (int i = 0; i < 2; ++i) {
+    p.store[i] = static_cast<const uint8_t*>(i ? cache_v : cache_k);
+    p.scale[i] = i ? v_scales : k_scales;
+  }
+  window_params(&p, query_heads, heads, scale, causal, window, sink_tokens, out);
+  p.parents = parents;
+  p.workspace = workspace;
+  return hip_status(sol::launch_paged(p, size, int(head_dim), format, static_cast<hipStream_t>(stream)));
+}
+
 }  // namespace
 
 extern "C" {
@@ -1045,39 +1091,22 @@ int sol_paged_attention(const void* q, const int64_t* q_strides, int64_t rows, c
                         int64_t table_width, int64_t pages, int64_t page_size, int64_t query_heads, int64_t heads,
                         int64_t head_dim, int format, double scale, int causal, int64_t window, int64_t sink_tokens,
                         void* workspace, int64_t workspace_bytes, void* out, void* stream) {
-  const char* what = "sol_paged_attention";
-  sol::PagedParams p;
-  std::memset(&p, 0, sizeof(p));
-  int rc = paged_batch_ok(what, page_table, context_lengths, query_offsets, rows, sequences, table_width, pages,
-                          page_size, heads, head_dim, format, &p.batch);
-  if (rc != SOL_OK) return rc;
-  if (!query_offsets) return fail(SOL_ERR_INVALID, "sol_paged_attention: query_offsets is required");
-  rc = store_ok(what, cache_k, cache_v, k_scales, v_scales, format);
-  if (rc != SOL_OK) return rc;
-  if (rows == 0) return SOL_OK;
-  rc = window_args_ok(what, query_heads, heads, scale, window, sink_tokens, out);
-  if (rc != SOL_OK) return rc;
-  if (!operand_ok(q, q_strides, true))
-    return fail(SOL_ERR_INVALID, "sol_paged_attention: Q needs 16-byte aligned rows and positive strides");
-  if (sequences > kMaxAttended)
-    return fail(SOL_ERR_UNSUPPORTED, "sol_paged_attention: at most 65,536 sequences in one call");
-  if (rows * query_heads >= (int64_t(1) << 31))
-    return fail(SOL_ERR_UNSUPPORTED, "sol_paged_attention: grid too large");
-  const sol::PagedSize size =
-      sol::paged_size(rows, sequences, window_keys(rows, table_width * page_size, causal, window, sink_tokens),
-                      window_keys(16, table_width * page_size, causal, window, sink_tokens), heads,
-                      query_heads / heads, head_dim, format, causal != 0, true);
-  rc = paged_workspace_ok(what, size, workspace, workspace_bytes);
-  if (rc != SOL_OK) return rc;
-  p.q = static_cast<const uint16_t*>(q);
-  p.q_st = q_strides[1], p.q_sh = q_strides[2];
-  for (int i = 0; i < 2; ++i) {
-    p.store[i] = static_cast<const uint8_t*>(i ? cache_v : cache_k);
-    p.scale[i] = i ? v_scales : k_scales;
-  }
-  window_params(&p, query_heads, heads, scale, causal, window, sink_tokens, out);
-  p.workspace = workspace;
-  return hip_status(sol::launch_paged(p, size, int(head_dim), format, static_cast<hipStream_t>(stream)));
+  return attend_paged("sol_paged_attention", q, q_strides, rows, cache_k, cache_v, k_scales, v_scales, page_table,
+                      context_lengths, query_offsets, nullptr, sequences, table_width, pages, page_size, query_heads,
+                      heads, head_dim, format, scale, causal, window, sink_tokens, workspace, workspace_bytes, out,
+                      stream);
+}
+
+int sol_tree_attention(const void* q, const int64_t* q_strides, int64_t rows, const void* cache_k,
+                       const void* cache_v, const float* k_scales, const float* v_scales, const int32_t* page_table,
+                       const int32_t* context_lengths, const int32_t* query_offsets, const int32_t* parents,
+                       int64_t sequences, int64_t table_width, int64_t pages, int64_t page_size, int64_t query_heads,
+                       int64_t heads, int64_t head_dim, int format, double scale, int64_t window, int64_t sink_tokens,
+                       void* workspace, int64_t workspace_bytes, void* out, void* stream) {
+  if (!parents && rows) return fail(SOL_ERR_INVALID, "sol_tree_attention: parents is required");
+  return attend_paged("sol_tree_attention", q, q_strides, rows, cache_k, cache_v, k_scales, v_scales, page_table,
+                      context_lengths, query_offsets, parents, sequences, table_width, pages, page_size, query_heads,
+                      heads, head_dim, format, scale, 1, window, sink_tokens, workspace, workspace_bytes, out, stream);
 }
 
 int64_t sol_paged_attention_workspace_size(int64_t rows, int64_t sequences, int64_t table_width, int64_t page_size,

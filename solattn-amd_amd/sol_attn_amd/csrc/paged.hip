@@ -501,11 +501,188 @@ __device__ __forceinline__ void add_nonfinite(State<D>& st, const uint16_t* slot
   }
 }
 
-// This lane's query: its position, and whether it saw a key.
+// ---- trees of new tokens ----------------------------------------------------
+//
+// New token i of a sequence (a node; its key lies at place base + i) continues
+// its parent, a node before it, or the stored tokens (a root).  It sees the
+// stored tokens (places below base), its ancestors and itself; its position is
+// base plus its depth, and windows and first tokens go by positions.  What a node
+// sees of the tree is held by blocks of 32 places: a mask of the ancestors in its
+// own block, itself included, and the nearest ancestor in a block before (kNone:
+// none), where the walk to the blocks further on continues.  So a chain of n nodes
+// takes n / 32 steps, and each of them one read of LDS.
+
+constexpr int kTreeNodes = 1024;  // held in LDS; further ones are followed in memory
+constexpr uint32_t kNone = 0xFFFFu;
+
+template <bool TREE>
+struct TreeNodes {};
+
+template <>
+struct TreeNodes<true> {
+  uint32_t* mask;          // LDS [kTreeNodes]
+  uint16_t* next;
+  const int32_t* parents;  // of the sequence
+  int n, base, length;
+
+  __device__ __forceinline__ int block(int i) const { return (base + i) >> 5; }
+  __device__ __forceinline__ uint32_t bit(int i) const { return 1u << ((base + i) & 31); }
+  // A node's parent, -1: none.  Nodes follow their parents, whatever the caller's array holds.
+  __device__ __forceinline__ int parent(int i) const {
+    const int a = parents[i];
+    return a >= 0 && a < i ? a : -1;
+  }
+
+  // By all threads of the workgroup.
+  __device__ __forceinline__ void build(int tid) {
+    const int held = min(n, kTreeNodes);
+    constexpr int kEach = kTreeNodes / kNT;
+    for (int i = tid; i < held; i += kNT) next[i] = uint16_t(parent(i));
+    __syncthreads();
+    uint32_t m[kEach];
+    int a[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const int i = tid + k * kNT;
+      m[k] = 0;
+      a[k] = int(kNone);
+      if (i >= held) continue;
+      m[k] = bit(i);
+      a[k] = next[i];
+      while (a[k] != int(kNone) && block(a[k]) == block(i)) {
+        m[k] |= bit(a[k]);
+        a[k] = next[a[k]];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const int i = tid + k * kNT;
+      if (i < held) mask[i] = m[k], next[i] = uint16_t(a[k]);
+    }
+    __syncthreads();
+  }
+
+  // Node i's mask; i becomes the nearest ancestor in a block before, -1: none.
+  __device__ __forceinline__ uint32_t step(int& i) const {
+    if (i < kTreeNodes) {
+      const uint32_t m = mask[i], a = next[i];
+      i = a == kNone ? -1 : int(a);
+      return m;
+    }
+    const int here = block(i);
+    uint32_t m = 0;
+    do {
+      m |= bit(i);
+      i = parent(i);
+    } while (i >= 0 && block(i) == here);
+    return m;
+  }
+
+  __device__ __forceinline__ int depth(int i) const {
+    int d = -1;
+    while (i >= 0) d += __popc(step(i));
+    return d;
+  }
+
+  // A walk up from a node of depth d, from block to block in descending order.
+  struct Walk {
+    int at, above;  // the ancestor that the walk has come to; how many it has passed
+  };
+
+  // Which of the keys of block b a node of position pos sees.
+  __device__ __forceinline__ uint32_t seen(Walk& w, int b, int pos, const PagedParams& p) const {
+    while (w.at >= 0 && block(w.at) > b) w.above += __popc(step(w.at));
+    if (w.at < 0 || block(w.at) < b) return 0u;
+    uint32_t m = step(w.at);
+    const int count = __popc(m);
+    if (w.above + count > p.window) {
+      // The nearest window - above of them, and those at positions below the sinks:
+      // theirs are pos - above - count + 1 .. pos - above.
+      const int near = max(p.window - w.above, 0);
+      const int far = min(max(p.sinks - (pos - w.above - count + 1), 0), count);
+      uint32_t keep = m, first = m;
+      for (int k = near; k < count; ++k) keep &= keep - 1u;                          // the upper `near` bits
+      for (int k = far; k < count; ++k) first &= ~(0x80000000u >> __clz(int(first)));  // the lower `far`
+      m = keep | first;
+    }
+    w.above += count;
+    const int left = length - 32 * b;
+    return left >= 32 ? m : m & ((1u << max(left, 0)) - 1u);
+  }
+};
+
+// This lane's query: its position (of a tree, its depth's), and whether it saw a key.
 struct LaneRow {
   int pos;
   bool any;
+  int node;  // trees
 };
+
+// The keys of the stored tokens, and all others, that a lane's query may see.
+template <bool TREE>
+__device__ __forceinline__ Visible visible_to(const PagedParams& p, const LaneRow& row, const TreeNodes<TREE>& tree,
+                                              int length) {
+  Visible v = visible(p, fresh(row.pos), length);  // not held in registers over the stream
+  if constexpr (TREE) {
+    v.hi = min(tree.base, length) - 1;
+    v.sink = min(p.sinks, v.hi + 1);
+  }
+  return v;
+}
+
+// The bounds of a tile that rows see whole, and of those they see at all: as by
+// the first and the last of them.
+struct Bounds {
+  Visible a, b;
+};
+
+// Of rows whose tokens are first .. last of an item's sequence.
+template <bool TREE>
+__device__ __forceinline__ Bounds bounds_of(const PagedParams& p, const Item& it, const LaneRow& row, int first,
+                                            int last) {
+  Bounds x;
+  x.a = visible(p, it.pos0 + first, it.length);
+  x.b = visible(p, it.pos0 + last, it.length);
+  if constexpr (TREE) {
+    // Their positions, by depths; no tile with a node is seen whole.
+    int lo = row.pos, hi = row.pos;
+#pragma unroll
+    for (int off = 1; off < kWave; off <<= 1) {
+      lo = min(lo, __shfl_xor(lo, off));
+      hi = max(hi, __shfl_xor(hi, off));
+    }
+    x.a.lo = visible(p, __builtin_amdgcn_readfirstlane(lo), it.length).lo;
+    x.b.lo = visible(p, __builtin_amdgcn_readfirstlane(hi), it.length).lo;
+    x.a.hi = min(it.pos0, it.length) - 1;
+    x.a.sink = min(p.sinks, x.a.hi + 1);
+  }
+  return x;
+}
+
+// Makes a workgroup's nodes known to it, and a lane's query: its position.
+template <bool TREE>
+__device__ __forceinline__ TreeNodes<TREE> nodes_of(const PagedParams& p, const Item& it, bool drafts, LaneRow& row,
+                                                    int token) {
+  TreeNodes<TREE> tree;
+  row.pos = it.pos0 + token;
+  row.any = false;
+  if constexpr (TREE) {
+    __shared__ uint32_t s_mask[kTreeNodes];
+    __shared__ uint16_t s_next[kTreeNodes];
+    tree.mask = s_mask;
+    tree.next = s_next;
+    tree.parents = p.parents + it.off;
+    tree.n = it.n;
+    tree.base = it.pos0;
+    tree.length = it.length;
+    const bool windowed = p.window != 0x7FFFFFFF;
+    if (drafts || windowed) tree.build(threadIdx.x);
+    row.node = token;
+    if (windowed) row.pos = it.pos0 + tree.depth(token);
+  }
+  return tree;
+}
 
 // Sixteen per-key factors of this lane's score elements of a half (key 8 (e /
 // 4) + 4 hh + e % 4), from LDS.
@@ -525,13 +702,20 @@ __device__ __forceinline__ f32x16 key_factors(const float* half, int hh) {
 // and scale hold.
 // `valid`: bits of the half's two groups of 16 rows that have a page.  scales:
 // the half's K scales times c in LDS (V's scales TK floats on), or null.
-template <int D, int TK, int F>
-__device__ __forceinline__ void attend_masked(const PagedParams& p, int length, State<D>& st, LaneRow& row, f32x16 s,
-                                              const uint16_t* slot, int t, int j0, uint32_t valid, int lane_col,
-                                              int lane_hh, const float* scales) {
+template <int D, int TK, int F, bool TREE>
+__device__ __forceinline__ void attend_masked(const PagedParams& p, int length, State<D>& st, LaneRow& row,
+                                              const TreeNodes<TREE>& tree, f32x16 s, const uint16_t* slot, int t, int j0,
+                                              uint32_t valid, int lane_col, int lane_hh, const float* scales) {
   const int col = fresh(lane_col), hh = fresh(lane_hh);
   const float c = scales ? 1.f : p.scale_log2;
-  const Visible v = visible(p, fresh(row.pos), length);  // not held in registers over the stream
+  const Visible v = visible_to(p, row, tree, length);
+  uint32_t nodes = 0;  // of the tree that the query sees, this lane's from bit 0 on
+  if constexpr (TREE) {
+    if (j0 + 31 >= tree.base) {
+      typename TreeNodes<true>::Walk walk = {fresh(row.node), 0};
+      nodes = tree.seen(walk, j0 >> 5, fresh(row.pos), p) >> (4 * hh);
+    }
+  }
   if (scales) {
     const f32x16 sk = key_factors(scales, hh);
 #pragma unroll
@@ -542,7 +726,8 @@ __device__ __forceinline__ void attend_masked(const PagedParams& p, int length, 
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
     const int j = a + 8 * (e >> 2) + (e & 3);
-    const bool in = (((j <= v.hi) & (j >= v.lo)) | (j < v.sink)) & (((valid >> (e >> 3)) & 1u) != 0);
+    const bool node = TREE && ((nodes >> (8 * (e >> 2) + (e & 3))) & 1u) != 0;
+    const bool in = (((j <= v.hi) & (j >= v.lo)) | (j < v.sink) | node) & (((valid >> (e >> 3)) & 1u) != 0);
     s[e] = in ? s[e] : kNegInf;
     seen |= in ? 1u << e : 0u;
   }
@@ -971,9 +1156,9 @@ __device__ __forceinline__ void step_nonfinite(StepState<D>& st, const uint8_t* 
 // whatever their score, value and scale hold.
 // keys_read() runs once K has been read, values_due() before V is, which starts
 // the next tile's K and waits for this one's V.
-template <int D, int F, bool MASKED, typename KeysRead, typename ValuesDue>
+template <int D, int F, bool MASKED, bool TREE, typename KeysRead, typename ValuesDue>
 __device__ __forceinline__ void step_tile(const PagedParams& p, int length, StepState<D>& st, LaneRow& row,
-                                          const bf16x8 (&qf)[D / 32], const uint8_t* slot, const StepSlot<D, F>& at,
+                                          const TreeNodes<TREE>& tree, const bf16x8 (&qf)[D / 32], const uint8_t* slot, const StepSlot<D, F>& at,
                                           const float* scales, int tile, uint32_t valid, int lane, KeysRead keys_read,
                                           ValuesDue values_due) {
   using Slot = StepSlot<D, F>;
@@ -1008,13 +1193,24 @@ __device__ __forceinline__ void step_tile(const PagedParams& p, int length, Step
   keys_read();
   uint32_t seen = 0;
   if constexpr (MASKED) {
-    const Visible v = visible(p, fresh(row.pos), length);  // not held in registers over the stream
+    const Visible v = visible_to(p, row, tree, length);
+    uint32_t nodes[TK / 32];  // of the tree that the query sees
+    if constexpr (TREE) {
+#pragma unroll
+      for (int b = 0; b < TK / 32; ++b) nodes[b] = 0u;
+      if (tile * TK + TK > tree.base) {
+        typename TreeNodes<true>::Walk walk = {fresh(row.node), 0};
+#pragma unroll
+        for (int b = TK / 32 - 1; b >= 0; --b) nodes[b] = tree.seen(walk, tile * (TK / 32) + b, fresh(row.pos), p);
+      }
+    }
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int r = Slot::key(kb, g, e), j = tile * TK + r;
-        const bool in = (((j <= v.hi) & (j >= v.lo)) | (j < v.sink)) & (((valid >> (r >> 4)) & 1u) != 0);
+        const bool node = TREE && ((nodes[kb >> 1] >> (r & 31)) & 1u) != 0;
+        const bool in = (((j <= v.hi) & (j >= v.lo)) | (j < v.sink) | node) & (((valid >> (r >> 4)) & 1u) != 0);
         s[kb][e] = in ? s[kb][e] : kNegInf;
         seen |= in ? 1u << (4 * kb + e) : 0u;
       }
@@ -1112,7 +1308,7 @@ __device__ __forceinline__ void step_tile(const PagedParams& p, int length, Step
 // 19,003 keys 256 us, 183 now.)  One sequence of 84,672 INT8 keys: 179 MB in 38
 // us and the merge's 5.  Small calls are a chain of latencies: three single
 // tokens over up to 317 keys 7.5 us.
-template <int D, int F, bool PAGED>
+template <int D, int F, bool PAGED, bool TREE>
 __global__ __launch_bounds__(kNT, 2) void step_kernel(PagedParams p) {
   using Slot = StepSlot<D, F>;
   constexpr int R = 16, TK = Slot::TK;
@@ -1139,13 +1335,14 @@ __global__ __launch_bounds__(kNT, 2) void step_kernel(PagedParams p) {
   for (int ks = 0; ks < D / 32; ++ks)
     qf[ks] = as_bf16x8(load16(q + (SCALED ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1) : 32 * ks + 8 * g)));
   LaneRow row;
-  row.pos = pos0 + token;
-  row.any = false;
-  const int first = pos0 + it.r0 / p.G, last = pos0 + (it.r0 + it.rows - 1) / p.G;
-  const Span span = span_of<TK>(p, first, last, it.length);
+  const int first = it.r0 / p.G, last = (it.r0 + it.rows - 1) / p.G;
+  const Span span = span_of<TK>(p, pos0 + (TREE ? 0 : first), pos0 + last, it.length);
   const int t0 = int(int64_t(it.part) * span.n / it.parts), t1 = int(int64_t(it.part + 1) * span.n / it.parts);
+  const TreeNodes<TREE> tree =
+      nodes_of<TREE>(p, it, t0 < t1 && (span.tile(t1 - 1) + 1) * TK > pos0, row, token);
   // Tiles inside these bounds are seen whole by every row.
-  const Visible va = visible(p, first, it.length), vb = visible(p, last, it.length);
+  const Bounds bounds = bounds_of<TREE>(p, it, row, first, last);
+  const Visible va = bounds.a, vb = bounds.b;
 
   StepState<D> st;
 #pragma unroll
@@ -1179,7 +1376,7 @@ __global__ __launch_bounds__(kNT, 2) void step_kernel(PagedParams p) {
       const uint32_t valid = dma.valid;
       wait_vmcnt<Dma::kLoads>();
       step_tile<D, F, decltype(masked)::value>(
-          p, it.length, st, row, qf, slot, at, scales, tile_of(k), valid, lane,
+          p, it.length, st, row, tree, qf, slot, at, scales, tile_of(k), valid, lane,
           [&] {
             if (more) {
               prepare(k + 1);
@@ -1546,7 +1743,7 @@ __device__ __forceinline__ void wide_tile(State<D>& st, const uint16_t* buf, con
 // codes and 64 multiplications by scales per lane and tile: FP8 645 us, INT8
 // 688.  Two workgroups per CU hold 256 registers a wave and a ring of two tiles
 // each; with heads of 128 that leaves 6 (BF16) to 17 (codes) registers spilled.
-template <int D, int F, bool PAGED>
+template <int D, int F, bool PAGED, bool TREE>
 __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
   using S = Shape<D>;
   constexpr int R = 128, TK = 64;
@@ -1571,13 +1768,14 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
 #pragma unroll
   for (int ks = 0; ks < S::KT; ++ks) qf[ks] = as_bf16x8(load16(q + 16 * ks + 8 * hh));
   LaneRow row;
-  row.pos = pos0 + token;
-  row.any = false;
 
-  const Span span = span_of<TK>(p, pos0 + it.r0 / p.G, pos0 + (it.r0 + it.rows - 1) / p.G, it.length);
+  const Span span = span_of<TK>(p, pos0 + (TREE ? 0 : it.r0 / p.G), pos0 + (it.r0 + it.rows - 1) / p.G, it.length);
   const int t0 = int(int64_t(it.part) * span.n / it.parts), t1 = int(int64_t(it.part + 1) * span.n / it.parts);
-  const Visible va = visible(p, pos0 + (it.r0 + 32 * wave) / p.G, it.length);
-  const Visible vb = visible(p, pos0 + (it.r0 + 32 * wave + max(wrows, 1) - 1) / p.G, it.length);
+  const TreeNodes<TREE> tree =
+      nodes_of<TREE>(p, it, t0 < t1 && (span.tile(t1 - 1) + 1) * TK > pos0, row, token);
+  const Bounds bounds = bounds_of<TREE>(p, it, row, (it.r0 + 32 * wave) / p.G,
+                                        (it.r0 + 32 * wave + max(wrows, 1) - 1) / p.G);
+  const Visible va = bounds.a, vb = bounds.b;
 
   State<D> st;
   state_init(st);
@@ -1589,7 +1787,9 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
   enum Kind { kHidden, kPart, kWhole };
   auto kind_of = [&](int tile, uint32_t valid) {
     const int a = tile * TK, b = a + TK - 1;
-    if (wrows <= 0 || ((a > vb.hi || b < va.lo) && a >= vb.sink)) return kHidden;
+    // (A node at a position below the sinks may lie past them.)
+    const bool before = b < va.lo && (!TREE || b < pos0);
+    if (wrows <= 0 || ((a > vb.hi || before) && a >= vb.sink)) return kHidden;
     return valid == kAllGroups<TK> && b <= va.hi && (a >= vb.lo || b < va.sink) ? kWhole : kPart;
   };
   auto hidden = [&](int, uint32_t, const uint16_t*, const float*, const auto& refill) {
@@ -1609,7 +1809,7 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
       for (int ks = 0; ks < S::KT; ++ks)
         s = mfma32x32x16(as_bf16x8(TileImage<D, TK>::k(buf, fcol, fhh, t, ks)), qf[ks], s);
       chunk_end();
-      attend_masked<D, TK, F>(p, it.length, st, row, s, buf, t, tile * TK + 32 * t, valid >> (2 * t), col, hh,
+      attend_masked<D, TK, F>(p, it.length, st, row, tree, s, buf, t, tile * TK + 32 * t, valid >> (2 * t), col, hh,
                            SCALED ? scales + 32 * t : nullptr);
     }
     refill.late();
@@ -1711,22 +1911,28 @@ void launch_merge(const PagedParams& p, const PagedSize& size, hipStream_t strea
   hipLaunchKernelGGL((merge_kernel<D, R>), dim3(unsigned(p.headers * p.H), rows), dim3(kNT), 0, stream, p);
 }
 
-template <int D, int F, bool PAGED>
+template <int D, int F, bool PAGED, bool TREE = false>
 void launch_variant(const PagedParams& p, const PagedSize& size, hipStream_t stream) {
   const dim3 grid(unsigned(size.grid)), block(kNT);
   if (size.rows == 16) {
-    hipLaunchKernelGGL((step_kernel<D, F, PAGED>), grid, block, 0, stream, p);
+    hipLaunchKernelGGL((step_kernel<D, F, PAGED, TREE>), grid, block, 0, stream, p);
     if (p.records) launch_merge<D, 16>(p, size, stream);
   } else {
-    hipLaunchKernelGGL((wide_kernel<D, F, PAGED>), grid, block, 0, stream, p);
+    hipLaunchKernelGGL((wide_kernel<D, F, PAGED, TREE>), grid, block, 0, stream, p);
     if (p.records) launch_merge<D, 128>(p, size, stream);
   }
 }
 
 template <int D>
 void launch_format(const PagedParams& p, const PagedSize& size, int format, hipStream_t stream) {
-  if (!p.batch.table) launch_variant<D, kBf16, false>(p, size, stream);
-  else if (format == kBf16) launch_variant<D, kBf16, true>(p, size, stream);
+  if (!p.batch.table) return launch_variant<D, kBf16, false>(p, size, stream);
+  if (p.parents) {
+    if (format == kBf16) launch_variant<D, kBf16, true, true>(p, size, stream);
+    else if (format == kInt8) launch_variant<D, kInt8, true, true>(p, size, stream);
+    else launch_variant<D, kFp8, true, true>(p, size, stream);
+    return;
+  }
+  if (format == kBf16) launch_variant<D, kBf16, true>(p, size, stream);
   else if (format == kInt8) launch_variant<D, kInt8, true>(p, size, stream);
   else launch_variant<D, kFp8, true>(p, size, stream);
 }

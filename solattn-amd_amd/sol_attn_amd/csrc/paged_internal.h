@@ -60,6 +60,7 @@ struct PagedParams {
   float scale_log2;
   int causal;
   int window, sinks;          // window 2^31 - 1: none
+  const int32_t* parents;     // a tree of new tokens: each row's parent among its sequence's; or null
   // Keys split over workgroups (take_item in paged.hip); target 0: not split.
   int target, min_tiles;      // workgroups per head; key tiles of a part at least
   int64_t headers, records;   // PagedSize's

@@ -297,6 +297,32 @@ def paged_attention(q, cache, plan, *, causal=True, window=None, sink_tokens=0, 
     past the last offset are not computed: they are left as they were in
     ``out``, and are unspecified without it.
     """
+    return _attend(q, cache, plan, causal, window, sink_tokens, scale, out)
+
+
+def tree_attention(q, cache, plan, parents, *, window=None, sink_tokens=0, scale=None, out=None):
+    """BF16 attention of new tokens that are trees of drafts, over what ``cache`` stores.
+
+    As :func:`paged_attention`, but new token i of a sequence (row
+    ``plan.query_offsets[s] + i``, its K and V rows stored at position
+    ``context_lengths[s] - new + i`` first) need not follow the one before it:
+    ``parents`` (contiguous int32 ``[N]``, a number per row of ``q``) names the
+    new token of its sequence, one before it, that it continues; anything else,
+    -1 say, makes it a root, which continues the stored tokens.  It sees the
+    tokens before the new ones, its ancestors and itself.  With a ``window`` it
+    sees those whose position is less than ``window`` before its own, and the
+    first ``sink_tokens``; a draft's position is the number of stored tokens
+    plus its depth (0 for a root), which is also where :func:`rotate_heads` has
+    to turn it to.  :func:`cache_keep` keeps the accepted ones.
+    """
+    if not isinstance(parents, torch.Tensor) or parents.dtype != torch.int32 or not parents.is_contiguous():
+        raise ValueError("parents must be a contiguous int32 tensor")
+    if parents.shape != q.shape[:1]:
+        raise ValueError("parents must have an entry for each row of Q")
+    return _attend(q, cache, plan, True, window, sink_tokens, scale, out, parents)
+
+
+def _attend(q, cache, plan, causal, window, sink_tokens, scale, out, parents=None):
     _check_rows("Q", q)
     heads, dim = _validate(cache, plan, q.device)
     if q.shape[2] != dim or q.shape[1] == 0 or q.shape[1] % heads:
@@ -314,8 +340,10 @@ def paged_attention(q, cache, plan, *, causal=True, window=None, sink_tokens=0, 
         scales = () if cache.k.dtype == torch.bfloat16 else (cache.k_scales, cache.v_scales)
         if any(_overlap(out, x) for x in (q, cache.k, cache.v, *scales)):
             raise ValueError("out must not share memory with Q or the cache")
+    if parents is not None and parents.get_device() != q.get_device():
+        raise ValueError("parents must be on Q's device")
     with _on(q.device):
-        return _native.launch_paged(q, cache, plan, scale, causal, window, min(sink_tokens, MAX_POSITIONS), out)
+        return _native.launch_paged(q, cache, plan, scale, causal, window, min(sink_tokens, MAX_POSITIONS), out, parents)
 
 
 def _check_integers(name, x, shape, device):
