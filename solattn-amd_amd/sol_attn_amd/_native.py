@@ -833,34 +833,38 @@ def launch_window(q, k, v, scale, causal, window, sinks):
     return out
 
 
-def launch_rotate(q, k, positions, rotary, q_norm, k_norm, eps, outs):
-    """Norms and rotation of Q's and K's heads, BTHD or NHD (``sol_rotate_heads``); ``k`` may be None.  ``outs``: where
-    the results go, None for new tensors; returns them."""
-    args, results = [], []
-    for x, out in zip((q, k), outs):
-        if x is None:
-            args += [None, None, 0, None, None]
-            results.append(None)
-            continue
-        if out is None or out.data_ptr() != x.data_ptr():
-            x = _rows(x)
-        if out is None:
-            out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        results.append(out)
-        s, o = x.stride(), out.stride()
-        # (An NHD tensor is one entry, whose stride is not used.)
-        args += [x.data_ptr(), _stride_array(s[0], s[-3], s[-2]), x.shape[-2], out.data_ptr(),
-                 _stride_array(o[0], o[-3], o[-2])]
-    batched = q.dim() == 4
-    if q.shape[-3] == 0:
-        return results
-    at, norm = positions.stride(), q_norm if q_norm is not None else k_norm
+def _rotated_rows(x, out):
+    """(the result, the operand's five arguments) of ``sol_rotate_heads``: Q or K, BTHD or NHD, copied first when
+    misaligned, and where it goes, a new tensor if ``out`` is None.  (An NHD tensor is one entry, whose stride is not
+    used.)"""
+    if x is None:
+        return None, (None, None, 0, None, None)
+    ptr, s = x.data_ptr(), x.stride()
+    if (ptr & 15) or (s[0] | s[-3] | s[-2]) & 7:
+        x = x.clone(memory_format=torch.contiguous_format)
+        ptr, s = x.data_ptr(), x.stride()
+    if out is None:
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    o = out.stride()
+    return out, (ptr, _stride_array(s[0], s[-3], s[-2]), x.shape[-2], out.data_ptr(),
+                 _stride_array(o[0], o[-3], o[-2]))
+
+
+def launch_rotate(q, k, positions, rotary, q_norm, k_norm, eps, q_out, k_out):
+    """Norms and rotation of Q's and K's heads (``sol_rotate_heads``); ``k`` may be None.  Results go to ``q_out`` and
+    ``k_out``, new tensors if None."""
+    q_out, q_args = _rotated_rows(q, q_out)
+    k_out, k_args = _rotated_rows(k, k_out)
+    shape, at = q.shape, positions.stride()
+    batch, batch_stride = (shape[0], at[0]) if len(shape) == 4 else (1, 0)
+    if shape[-3] == 0:
+        return q_out, k_out
+    norm = k_norm if q_norm is None else q_norm
     _check(library().sol_rotate_heads(
-        *args, positions.data_ptr(), _stride_array(at[0] if batched else 0, at[-2], 0), positions.shape[-1],
+        *q_args, *k_args, positions.data_ptr(), _stride_array(batch_stride, at[-2], 0), positions.shape[-1],
         rotary.frequencies.data_ptr(), rotary.axes.data_ptr(), rotary.layout == "pairs", _ptr(q_norm), _ptr(k_norm),
-        norm is not None and norm.dtype == torch.bfloat16, eps, q.shape[0] if batched else 1, q.shape[-3], q.shape[-1],
-        _stream(q.device)))
-    return results
+        norm is not None and norm.dtype == torch.bfloat16, eps, batch, shape[-3], shape[-1], _stream(q.device)))
+    return q_out, k_out
 
 
 def _store_args(cache):
@@ -889,14 +893,18 @@ def launch_cache_fork(cache, refs, plan, parents, new_tokens, lengths, width):
     """``(table, lengths, offsets, refs, missing)`` of the next plan and pool (``sol_cache_fork``)."""
     pages, h, page_size, d = cache.k.shape
     s, old_width = plan.page_table.shape
-    n, dev = parents.shape[0], cache.k.device
-    table, *rest = torch.empty(n * width + 2 * n + 2 + pages, device=dev, dtype=torch.int32).split(
-        (n * width, n, n + 1, pages, 1))
-    table = table.view(n, width)
-    ws = _workspace(_fork_size(s, n, pages), dev)
+    n, dev = parents.shape[0], refs.device
+    size = _fork_size(s, n, pages)
+    if size < 0:
+        raise RuntimeError("the workspace size function rejected the sizes")
+    # One allocation for the workspace (a multiple of 16 bytes) and the results.
+    ws, table, new_lengths, offsets, new_refs, missing = torch.empty(
+        size // 4 + n * width + 2 * n + 2 + pages, device=dev, dtype=torch.int32).split(
+        (size // 4, n * width, n, n + 1, pages, 1))
     old_table, old_lengths, _ = _plan_args(plan)
     _check(library().sol_cache_fork(
         old_table, old_lengths, _ptr(lengths), s, old_width, parents.data_ptr(), new_tokens.data_ptr(), n, width,
         refs.data_ptr(), pages, page_size, h, d, CACHE_FORMATS[cache.k.dtype], *_store_args(cache), table.data_ptr(),
-        *(x.data_ptr() for x in rest), ws.data_ptr(), ws.shape[0], _stream(dev)))
-    return table, *rest
+        new_lengths.data_ptr(), offsets.data_ptr(), new_refs.data_ptr(), missing.data_ptr(), ws.data_ptr(), size,
+        _stream(dev)))
+    return table.view(n, width), new_lengths, offsets, new_refs, missing

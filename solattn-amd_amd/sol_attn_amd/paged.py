@@ -347,11 +347,13 @@ def _attend(q, cache, plan, causal, window, sink_tokens, scale, out, parents=Non
 
 
 def _check_integers(name, x, shape, device):
+    """Checks an int32 tensor on the GPU ``device`` (its index); None in ``shape``: any number."""
     if not isinstance(x, torch.Tensor) or x.dtype != torch.int32 or not x.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor")
-    if x.ndim != len(shape) or any(n is not None and n != m for n, m in zip(shape, x.shape)):
+    sizes = x.shape
+    if len(sizes) != len(shape) or (sizes[0] != shape[0] and shape[0] is not None):
         raise ValueError(f"{name} must have an entry for each sequence")
-    if x.get_device() != device.index:
+    if x.get_device() != device:
         raise ValueError(f"{name} must be on the cache's device")
 
 
@@ -374,7 +376,7 @@ def cache_keep(cache, plan, kept):
     device = cache.k.device if isinstance(cache, PagedCache) else None
     _validate(cache, plan, device)
     _separate(cache)
-    _check_integers("kept", kept, (plan.page_table.shape[0], None), device)
+    _check_integers("kept", kept, (plan.page_table.shape[0], None), device.index)
     with _on(device):
         return _native.launch_cache_keep(cache, plan, kept)
 
@@ -404,24 +406,26 @@ def cache_fork(cache, pool, plan, parents, new_tokens, *, lengths=None, width=No
     device = cache.k.device if isinstance(cache, PagedCache) else None
     _validate(cache, plan, device)
     _separate(cache)
-    sequences, page_size = plan.page_table.shape[0], cache.k.shape[2]
     if not isinstance(pool, PagePool):
         raise ValueError("An explicit PagePool is required")
-    _check_integers("parents", parents, (None,), device)
-    _check_integers("new_tokens", new_tokens, (parents.shape[0],), device)
+    at, table, store = device.index, plan.page_table.shape, cache.k.shape
+    _check_integers("parents", parents, (None,), at)
+    branches = parents.shape
+    _check_integers("new_tokens", new_tokens, branches, at)
     if lengths is not None:
-        _check_integers("lengths", lengths, (sequences,), device)
+        _check_integers("lengths", lengths, table[:1], at)
     refs = pool.refs
-    if refs.dtype != torch.int32 or refs.shape != cache.k.shape[:1] or not refs.is_contiguous():
+    if refs.dtype != torch.int32 or refs.ndim != 1 or refs.shape[0] != store[0] or not refs.is_contiguous():
         raise ValueError("Invalid pool; use PagePool.create with this cache")
-    if refs.get_device() != device.index:
+    if refs.get_device() != at:
         raise ValueError("The pool must be on the cache's device")
     if width is None:
-        width = plan.page_table.shape[1]
-    _nonnegative_integer("width", width)
-    if not 0 < width <= MAX_POSITIONS // page_size:
+        width = table[1]
+    else:
+        _nonnegative_integer("width", width)
+    if not 0 < width <= MAX_POSITIONS // store[2]:
         raise ValueError(f"width must name 1 to {MAX_POSITIONS} positions of each sequence")
-    if max(sequences, parents.shape[0]) > MAX_ATTENDED:
+    if max(table[0], branches[0]) > MAX_ATTENDED:
         raise ValueError(f"More than {MAX_ATTENDED} sequences in one call are not supported")
     with _on(device):
         table, lengths, offsets, refs, missing = _native.launch_cache_fork(cache, refs, plan, parents, new_tokens,

@@ -17,6 +17,7 @@ from . import _native
 from .attention import _nonnegative_integer, _on
 
 LAYOUTS = ("halves", "pairs")
+NORM_TYPES = (torch.float32, torch.bfloat16)
 
 
 @dataclass(frozen=True)
@@ -124,55 +125,61 @@ def rotate_heads(q, k, positions, rotary, *, q_norm=None, k_norm=None, eps=1e-6,
     (one where ``k`` is None) of any positive strides, which may be Q and K
     themselves.
     """
-    heads = [x for x in (q, k) if x is not None]
-    if q is None or q.ndim not in (3, 4) or any(x.ndim != q.ndim for x in heads):
+    alone = k is None
+    if q is None or q.ndim not in (3, 4) or (not alone and k.ndim != q.ndim):
         raise ValueError("Q and K must have BTHD rank-4 or NHD rank-3 layout")
-    if any(x.dtype != torch.bfloat16 for x in heads):
+    if q.dtype != torch.bfloat16 or (not alone and k.dtype != torch.bfloat16):
         raise ValueError("Only BF16 Q and K are implemented")
-    dim, device = q.shape[-1], q.device
-    if k is not None and (k.shape[:-2] != q.shape[:-2] or k.shape[-1] != dim):
+    shape, strides = q.shape, q.stride()
+    tokens, dim = shape[:-2], shape[-1]
+    if not alone and (k.shape[:-2] != tokens or k.shape[-1] != dim):
         raise ValueError("Q and K must be rows of the same tokens and head dimension")
-    if dim not in (64, 128):
+    if dim != 128 and dim != 64:
         raise ValueError("Only head dimensions 64 and 128 are implemented")
-    if any(x.shape[-2] == 0 or x.shape[0] == 0 and x.ndim == 4 for x in heads):
+    if shape[-2] == 0 or (not alone and k.shape[-2] == 0) or (len(shape) == 4 and shape[0] == 0):
         raise ValueError("Q and K need a batch entry and a head")
-    if any(x.requires_grad for x in heads):
+    if q.requires_grad or (not alone and k.requires_grad):
         raise ValueError("Inference only: Q and K must not require gradients")
-    if any(x.stride(-1) != 1 or min(x.stride()) <= 0 for x in heads):
+    if strides[-1] != 1 or min(strides) <= 0 or (not alone and (k.stride(-1) != 1 or min(k.stride()) <= 0)):
         raise ValueError("Q and K need positive strides and contiguous head dimension")
-    if positions.dtype != torch.int32 or positions.shape[:-1] != q.shape[:-2] or positions.shape[-1] == 0:
+    at = positions.shape
+    if positions.dtype != torch.int32 or at[:-1] != tokens or at[-1] == 0:
         raise ValueError("positions must be int32, an entry per axis for every token")
-    if positions.stride(-1) != 1 and positions.shape[-1] != 1:
+    if at[-1] != 1 and positions.stride(-1) != 1:
         raise ValueError("positions need contiguous axes")
     if not isinstance(rotary, RotaryAxes):
         raise ValueError("An explicit RotaryAxes is required")
     freq, axes = rotary.frequencies, rotary.axes
-    if (freq.dtype != torch.float64 or axes.dtype != torch.int32 or freq.shape != (dim // 2,) or axes.shape != (dim // 2,)
-            or not freq.is_contiguous() or not axes.is_contiguous() or rotary.layout not in LAYOUTS):
+    if (freq.dtype != torch.float64 or axes.dtype != torch.int32 or not freq.ndim == axes.ndim == 1
+            or not freq.numel() == axes.numel() == dim // 2 or not (freq.is_contiguous() and axes.is_contiguous())
+            or rotary.layout not in LAYOUTS):
         raise ValueError("Invalid rotary descriptor; use RotaryAxes.create for this head dimension")
-    norms = [w for w in (q_norm, k_norm) if w is not None]
-    if k is None and k_norm is not None:
+    if alone and k_norm is not None:
         raise ValueError("k_norm needs K")
-    for w in norms:
-        if w.dtype not in (torch.float32, torch.bfloat16) or w.shape != (dim,) or not w.is_contiguous():
+    device = q.get_device()
+    same = (positions.get_device() == device and freq.get_device() == device and axes.get_device() == device
+            and (alone or k.get_device() == device))
+    for w in (q_norm, k_norm):
+        if w is None:
+            continue
+        if w.dtype not in NORM_TYPES or w.ndim != 1 or w.numel() != dim or not w.is_contiguous():
             raise ValueError("Norm weights must be contiguous FP32 or BF16 of the head dimension")
         if w.requires_grad:
             raise ValueError("Inference only: norm weights must not require gradients")
-    if len(norms) == 2 and norms[0].dtype != norms[1].dtype:
+        same = same and w.get_device() == device
+    if q_norm is not None and k_norm is not None and q_norm.dtype != k_norm.dtype:
         raise ValueError("Norm weights must have one type")
-    eps = float(eps)
     if not 2.0 ** -126 <= eps < 2.0 ** 127:
         raise ValueError("eps must be a positive FP32 number")
-    if torch.version.hip is None or device.type != "cuda" or any(
-            x.device != device for x in (*heads, positions, freq, axes, *norms)):
+    if torch.version.hip is None or device < 0 or not same:
         raise ValueError("The HIP backend requires all tensors on the same AMD ROCm GPU")
-    outs = [None, None]
+    q_out = k_out = None
     if out is not None:
-        outs = [out] if k is None else list(out)
-        if len(outs) != len(heads):
+        outs = [out] if alone else list(out)
+        if len(outs) != 1 + (not alone):
             raise ValueError("out must be one tensor for Q and one for K")
-        _check_out(heads, outs)
-        outs += [None] * (2 - len(outs))
-    with _on(device):
-        q_out, k_out = _native.launch_rotate(q, k, positions, rotary, q_norm, k_norm, eps, outs)
-    return q_out if k is None else (q_out, k_out)
+        _check_out([q] if alone else [q, k], outs)
+        q_out, k_out = outs[0], None if alone else outs[1]
+    with _on(q.device):
+        q_out, k_out = _native.launch_rotate(q, k, positions, rotary, q_norm, k_norm, float(eps), q_out, k_out)
+    return q_out if alone else (q_out, k_out)
