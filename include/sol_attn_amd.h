@@ -514,14 +514,16 @@ int64_t sol_paged_attention_workspace_size(int64_t rows, int64_t sequences, int6
  * stored tokens.  Its K and V rows lie at position context_lengths[s] - n + i as
  * ever.  It sees the sequence's tokens before the n new ones, its ancestors and
  * itself; for window and sink_tokens its position is context_lengths[s] - n plus
- * its depth.  workspace: of sol_paged_attention_workspace_size() bytes for the
- * same sizes and causal = 1. */
+ * its depth.  workspace: of sol_tree_attention_workspace_size() bytes. */
 int sol_tree_attention(const void* q, const int64_t* q_strides, int64_t rows, const void* cache_k,
                        const void* cache_v, const float* k_scales, const float* v_scales, const int32_t* page_table,
                        const int32_t* context_lengths, const int32_t* query_offsets, const int32_t* parents,
                        int64_t sequences, int64_t table_width, int64_t pages, int64_t page_size, int64_t query_heads,
                        int64_t heads, int64_t head_dim, int format, double scale, int64_t window, int64_t sink_tokens,
                        void* workspace, int64_t workspace_bytes, void* out, void* stream);
+int64_t sol_tree_attention_workspace_size(int64_t rows, int64_t sequences, int64_t table_width, int64_t page_size,
+                                          int64_t query_heads, int64_t heads, int64_t head_dim, int format,
+                                          int64_t window, int64_t sink_tokens);
 
 /* The same over plain BF16 K and V [batch, key_tokens, heads, head_dim] and Q
  * [batch, query_tokens, query_heads, head_dim] by their {batch, token, head}

@@ -74,6 +74,7 @@ _SIGNATURES = {
     "sol_paged_attention_workspace_size": ([_i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _int, _i64, _i64], _i64),
     "sol_tree_attention": ([_p, _i64p, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64,
                             _int, _dbl, _i64, _i64, _p, _i64, _p, _p], ctypes.c_int),
+    "sol_tree_attention_workspace_size": ([_i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _i64, _i64], _i64),
     "sol_window_attention": ([_p, _i64p, _p, _i64p, _p, _i64p, _i64, _i64, _i64, _i64, _i64, _i64, _dbl, _int,
                               _i64, _i64, _p, _i64, _p, _p], ctypes.c_int),
     "sol_cache_keep": ([_p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _int, _p, _p, _p, _p, _p, _i64, _p, _p],
@@ -775,6 +776,11 @@ def _paged_size(n, s, width, page_size, hq, h, d, fmt, causal, window, sinks):
 
 
 @functools.lru_cache(maxsize=1024)
+def _tree_size(n, s, width, page_size, hq, h, d, fmt, window, sinks):
+    return library().sol_tree_attention_workspace_size(n, s, width, page_size, hq, h, d, fmt, window, sinks)
+
+
+@functools.lru_cache(maxsize=1024)
 def _window_size(b, tq, tk, hq, h, d, causal, window, sinks):
     return library().sol_window_attention_workspace_size(b, tq, tk, hq, h, d, causal, window, sinks)
 
@@ -799,14 +805,16 @@ def launch_paged(q, cache, plan, scale, causal, window, sinks, out=None, parents
     q = _rows(q)
     table, lengths, offsets = _plan_args(plan)
     fmt = CACHE_FORMATS[cache.k.dtype]
-    size = _paged_size(n, s, width, page_size, hq, h, d, fmt, causal, window, sinks)
-    ws = _workspace(size, dev)
     if parents is not None:
+        size = _tree_size(n, s, width, page_size, hq, h, d, fmt, window, sinks)
+        ws = _workspace(size, dev)
         _check(library().sol_tree_attention(
             q.data_ptr(), _strides(q, True), n, cache.k.data_ptr(), cache.v.data_ptr(), _ptr(cache.k_scales),
             _ptr(cache.v_scales), table, lengths, offsets, parents.data_ptr(), s, width, pages, page_size, hq, h, d, fmt,
             scale, window, sinks, _ptr(ws), size, out.data_ptr(), _stream(dev)))
         return out
+    size = _paged_size(n, s, width, page_size, hq, h, d, fmt, causal, window, sinks)
+    ws = _workspace(size, dev)
     _check(library().sol_paged_attention(
         q.data_ptr(), _strides(q, True), n, cache.k.data_ptr(), cache.v.data_ptr(), _ptr(cache.k_scales),
         _ptr(cache.v_scales), table, lengths, offsets, s, width, pages, page_size, hq, h, d,

@@ -1003,7 +1003,7 @@ int attend_paged(const char* what, const void* q, const int64_t* q_strides, int6
   const sol::PagedSize size =
       sol::paged_size(rows, sequences, window_keys(rows, table_width * page_size, causal, window, sink_tokens),
                       window_keys(16, table_width * page_size, causal, window, sink_tokens), heads,
-                      query_heads / heads, head_dim, format, causal != 0, true);
+                      query_heads / heads, head_dim, format, causal != 0, true, parents != nullptr);
   rc = paged_workspace_ok(what, size, workspace, workspace_bytes);
   if (rc != SOL_OK) return rc;
   p.q = static_cast<const uint16_t*>(q);
@@ -1016,6 +1016,20 @@ int attend_paged(const char* what, const void* q, const int64_t* q_strides, int6
   p.parents = parents;
   p.workspace = workspace;
   return hip_status(sol::launch_paged(p, size, int(head_dim), format, static_cast<hipStream_t>(stream)));
+}
+
+int64_t attend_workspace(int64_t rows, int64_t sequences, int64_t table_width, int64_t page_size, int64_t query_heads,
+                         int64_t heads, int64_t head_dim, int format, int causal, int64_t window, int64_t sink_tokens,
+                         bool tree) {
+  if (rows < 0 || rows >= kMaxPositions || sequences <= 0 || sequences > kMaxAttended || table_width <= 0 ||
+      page_size <= 0 || table_width > kMaxPositions / page_size || heads <= 0 || heads >= (1 << 16) || query_heads <= 0 ||
+      query_heads % heads || query_heads >= (1 << 16) || (head_dim != 64 && head_dim != 128) || format < SOL_CACHE_BF16 ||
+      format > SOL_CACHE_FP8 || window < 0 || sink_tokens < 0 || rows * query_heads >= (int64_t(1) << 31))
+    return -1;
+  if (rows == 0) return 0;
+  return sol::paged_size(rows, sequences, window_keys(rows, table_width * page_size, causal, window, sink_tokens),
+                         window_keys(16, table_width * page_size, causal, window, sink_tokens), heads,
+                         query_heads / heads, head_dim, format, causal != 0, true, tree).bytes;
 }
 
 }  // namespace
@@ -1112,15 +1126,15 @@ int sol_tree_attention(const void* q, const int64_t* q_strides, int64_t rows, co
 int64_t sol_paged_attention_workspace_size(int64_t rows, int64_t sequences, int64_t table_width, int64_t page_size,
                                            int64_t query_heads, int64_t heads, int64_t head_dim, int format,
                                            int causal, int64_t window, int64_t sink_tokens) {
-  if (rows < 0 || rows >= kMaxPositions || sequences <= 0 || sequences > kMaxAttended || table_width <= 0 ||
-      page_size <= 0 || table_width > kMaxPositions / page_size || heads <= 0 || heads >= (1 << 16) || query_heads <= 0 ||
-      query_heads % heads || query_heads >= (1 << 16) || (head_dim != 64 && head_dim != 128) || format < SOL_CACHE_BF16 ||
-      format > SOL_CACHE_FP8 || window < 0 || sink_tokens < 0 || rows * query_heads >= (int64_t(1) << 31))
-    return -1;
-  if (rows == 0) return 0;
-  return sol::paged_size(rows, sequences, window_keys(rows, table_width * page_size, causal, window, sink_tokens),
-                         window_keys(16, table_width * page_size, causal, window, sink_tokens), heads,
-                         query_heads / heads, head_dim, format, causal != 0, true).bytes;
+  return attend_workspace(rows, sequences, table_width, page_size, query_heads, heads, head_dim, format, causal, window,
+                          sink_tokens, false);
+}
+
+int64_t sol_tree_attention_workspace_size(int64_t rows, int64_t sequences, int64_t table_width, int64_t page_size,
+                                          int64_t query_heads, int64_t heads, int64_t head_dim, int format,
+                                          int64_t window, int64_t sink_tokens) {
+  return attend_workspace(rows, sequences, table_width, page_size, query_heads, heads, head_dim, format, 1, window,
+                          sink_tokens, true);
 }
 
 int sol_window_attention(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,

@@ -172,7 +172,7 @@ __device__ __forceinline__ bool take_plain_item(const PagedParams& p, int id, It
   return true;
 }
 
-template <int R, int TK, bool PAGED>
+template <int R, int TK, bool PAGED, bool TREE>
 __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item& it) {
   if constexpr (!PAGED) return take_plain_item<R, TK>(p, int(id), it);
   __shared__ int64_t s_total[kWaves];
@@ -216,6 +216,29 @@ __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item
     sum = int64_t(uniform64(uint64_t(sum)));
     z = part_tiles(p, sum);
     __syncthreads();
+    if constexpr (TREE && R == 128) {
+      // One round of workgroups: rounded up, the parts are more than p.target, and
+      // those that are too many would run for as long again as all the others (six
+      // trees of up to 701 nodes over up to 8,191 keys: 104 us with 568 parts of up
+      // to 17 tiles, XX with at most 512).
+      for (int tries = 0; tries < 8; ++tries) {
+        int64_t count = 0;
+        for (int s = tid; s < S; s += kNT) {
+          const Sizes x = s == tid ? mine0 : sizes(s);
+          if (x.row_tiles) count += int64_t(x.row_tiles) * ((x.key_tiles - 1) / max(z, cdiv_i(x.key_tiles, kMaxParts)) + 1);
+        }
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) count += __shfl_xor(count, off);
+        if (lane == 0) s_total[wave] = count;
+        __syncthreads();
+        count = 0;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) count += s_total[w];
+        __syncthreads();
+        if (int64_t(uniform64(uint64_t(count))) <= p.target) break;
+        z += max(1, z / 8);
+      }
+    }
   }
   int64_t base = 0;
   uint64_t split = 0;  // of the sequences before s0: parts of split tiles, times 2^32, and the tiles
@@ -702,20 +725,16 @@ __device__ __forceinline__ f32x16 key_factors(const float* half, int hh) {
 // and scale hold.
 // `valid`: bits of the half's two groups of 16 rows that have a page.  scales:
 // the half's K scales times c in LDS (V's scales TK floats on), or null.
+// nodes: the nodes of a tree that the query sees, by place.
 template <int D, int TK, int F, bool TREE>
 __device__ __forceinline__ void attend_masked(const PagedParams& p, int length, State<D>& st, LaneRow& row,
-                                              const TreeNodes<TREE>& tree, f32x16 s, const uint16_t* slot, int t, int j0,
-                                              uint32_t valid, int lane_col, int lane_hh, const float* scales) {
+                                              const TreeNodes<TREE>& tree, uint32_t nodes, f32x16 s,
+                                              const uint16_t* slot, int t, int j0, uint32_t valid, int lane_col,
+                                              int lane_hh, const float* scales) {
   const int col = fresh(lane_col), hh = fresh(lane_hh);
   const float c = scales ? 1.f : p.scale_log2;
   const Visible v = visible_to(p, row, tree, length);
-  uint32_t nodes = 0;  // of the tree that the query sees, this lane's from bit 0 on
-  if constexpr (TREE) {
-    if (j0 + 31 >= tree.base) {
-      typename TreeNodes<true>::Walk walk = {fresh(row.node), 0};
-      nodes = tree.seen(walk, j0 >> 5, fresh(row.pos), p) >> (4 * hh);
-    }
-  }
+  if constexpr (TREE) nodes >>= 4 * hh;  // this lane's
   if (scales) {
     const f32x16 sk = key_factors(scales, hh);
 #pragma unroll
@@ -1319,7 +1338,7 @@ __global__ __launch_bounds__(kNT, 2) void step_kernel(PagedParams p) {
 
   const int h = blockIdx.x % p.H;
   Item it;
-  if (!take_item<R, TK, PAGED>(p, blockIdx.x / p.H, it)) return;
+  if (!take_item<R, TK, PAGED, TREE>(p, blockIdx.x / p.H, it)) return;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, g = lane >> 4;
@@ -1753,7 +1772,7 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
 
   const int h = blockIdx.x % p.H;
   Item it;
-  if (!take_item<R, TK, PAGED>(p, blockIdx.x / p.H, it)) return;
+  if (!take_item<R, TK, PAGED, TREE>(p, blockIdx.x / p.H, it)) return;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, hh = lane >> 5;
@@ -1803,13 +1822,23 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
     refill.all();
 #pragma unroll 1
     for (int t = 0; t < 2; ++t) {
+      uint32_t nodes = 0;
+      if constexpr (TREE) {
+        const int j0 = tile * TK + 32 * t;
+        if (j0 + 31 >= pos0) {
+          typename TreeNodes<true>::Walk walk = {fresh(row.node), 0};
+          nodes = tree.seen(walk, j0 >> 5, fresh(row.pos), p);
+          // Most nodes of a large tree are no ancestors of these rows.
+          if (j0 >= pos0 && !__builtin_amdgcn_ballot_w64(nodes != 0)) continue;
+        }
+      }
       const int fcol = fresh(col), fhh = fresh(hh);
       f32x16 s = zero16();
 #pragma unroll
       for (int ks = 0; ks < S::KT; ++ks)
         s = mfma32x32x16(as_bf16x8(TileImage<D, TK>::k(buf, fcol, fhh, t, ks)), qf[ks], s);
       chunk_end();
-      attend_masked<D, TK, F>(p, it.length, st, row, tree, s, buf, t, tile * TK + 32 * t, valid >> (2 * t), col, hh,
+      attend_masked<D, TK, F>(p, it.length, st, row, tree, nodes, s, buf, t, tile * TK + 32 * t, valid >> (2 * t), col, hh,
                            SCALED ? scales + 32 * t : nullptr);
     }
     refill.late();
@@ -1965,7 +1994,7 @@ int64_t wide_target(int64_t tiles, int64_t heads, int64_t key_tiles, int64_t min
 }  // namespace
 
 PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t tile_keys, int64_t heads, int64_t group,
-                     int64_t head_dim, int format, bool causal, bool ragged) {
+                     int64_t head_dim, int format, bool causal, bool ragged, bool tree) {
   PagedSize s;
   auto likely_tiles = [&](int64_t R) { return (rows * group + R - 1) / R + (sequences - 1) / 2; };
   // The step kernel, whose tiles are 16 rows, for few rows per sequence; and for
@@ -1997,6 +2026,9 @@ PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t tile
     s.min_tiles = 8;
     const int64_t rounds = ragged && 2 * sequences * heads >= kResident ? 2 : 1;
     if (key_tiles > (format == kBf16 ? 48 : 20)) s.target = (rounds * kResident + heads - 1) / heads;
+  } else if (tree && likely * heads <= kResident) {
+    s.min_tiles = 8;
+    if (key_tiles > s.min_tiles) s.target = kResident / heads;
   } else if (uneven && 2 * likely * heads * key_tiles >= 3 * kResident * 24) {
     // Enough keys for one and a half rounds of parts of 24 tiles: those even the
     // lengths out (8 sequences of 600 .. 12,000 keys, 512 new tokens of 8 x 4
