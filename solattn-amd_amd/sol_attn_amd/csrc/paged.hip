@@ -199,6 +199,9 @@ __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item
   };
   const Sizes mine0 = sizes(tid);  // read once where there are no more sequences than threads
   int z = 1 << 30;
+  auto parts_of = [&](const Sizes& x) {
+    return p.target && x.row_tiles ? (x.key_tiles - 1) / max(z, cdiv_i(x.key_tiles, kMaxParts)) + 1 : 1;
+  };
   if (p.target) {
     int64_t sum = 0;
 #pragma unroll 4
@@ -217,15 +220,21 @@ __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item
     z = part_tiles(p, sum);
     __syncthreads();
     if constexpr (TREE && R == 128) {
-      // One round of workgroups: rounded up, the parts are more than p.target, and
-      // those that are too many would run for as long again as all the others (six
-      // trees of up to 701 nodes over up to 8,191 keys: 104 us with 568 parts of up
-      // to 17 tiles, XX with at most 512).
-      for (int tries = 0; tries < 8; ++tries) {
-        int64_t count = 0;
+      // Rounded up, the parts may be a few more than run at once (p.target is two
+      // rounds of them), and those few would run for as long as all the others:
+      // parts up to a quarter longer that make one round, or else two rounds.
+      // (Six trees of up to 701 nodes over up to 8,191 keys: 104 us with 568 parts of
+      // up to 17 tiles, 87 with at most 512; 40 sequences of 26 nodes over 4,000
+      // INT8 keys each, 8 heads: 229 us in one round of parts, XX in two.)
+      int rounds = 1;
+      z = part_tiles(p, 2 * sum);
+      const int limit = z + z / 4;
+#pragma unroll 1
+      for (int tries = 0; tries < 10; ++tries) {
+        int count = 0;
         for (int s = tid; s < S; s += kNT) {
           const Sizes x = s == tid ? mine0 : sizes(s);
-          if (x.row_tiles) count += int64_t(x.row_tiles) * ((x.key_tiles - 1) / max(z, cdiv_i(x.key_tiles, kMaxParts)) + 1);
+          count += x.row_tiles * parts_of(x);
         }
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) count += __shfl_xor(count, off);
@@ -233,18 +242,19 @@ __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item
         __syncthreads();
         count = 0;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) count += s_total[w];
+        for (int w = 0; w < kWaves; ++w) count += int(s_total[w]);
         __syncthreads();
-        if (int64_t(uniform64(uint64_t(count))) <= p.target) break;
+        if (__builtin_amdgcn_readfirstlane(count) <= (rounds * p.target + 1) / 2) break;
         z += max(1, z / 8);
+        if (rounds == 1 && z > limit) {
+          rounds = 2;
+          z = part_tiles(p, sum);
+        }
       }
     }
   }
   int64_t base = 0;
   uint64_t split = 0;  // of the sequences before s0: parts of split tiles, times 2^32, and the tiles
-  auto parts_of = [&](const Sizes& x) {
-    return p.target && x.row_tiles ? (x.key_tiles - 1) / max(z, cdiv_i(x.key_tiles, kMaxParts)) + 1 : 1;
-  };
   auto split_of = [&](const Sizes& x, int64_t items) {
     return items > x.row_tiles ? (uint64_t(items) << 32) + uint32_t(x.row_tiles) : 0ull;
   };
@@ -538,15 +548,38 @@ __device__ __forceinline__ void add_nonfinite(State<D>& st, const uint16_t* slot
 constexpr int kTreeNodes = 1024;  // held in LDS; further ones are followed in memory
 constexpr uint32_t kNone = 0xFFFFu;
 
-template <bool TREE>
-struct TreeNodes {};
+struct TreeLds {
+  uint32_t mask[kTreeNodes];
+  uint16_t next[kTreeNodes];
+  int base, off, length;
+  int lane[kNT][2];  // each lane's query: its node and its position
+};
 
-template <>
-struct TreeNodes<true> {
-  uint32_t* mask;          // LDS [kTreeNodes]
-  uint16_t* next;
+// (One per kernel.)
+__device__ __forceinline__ TreeLds& tree_lds() {
+  __shared__ TreeLds s;
+  return s;
+}
+
+// What is known of a sequence's tree: made at the beginning, and where it is needed
+// read again.  (Held over the stream of key tiles it made the compiler spill query
+// operands: 84,736 INT8 keys, 64 nodes of 8 x 3 heads XX us instead of 147.)
+struct TreeNodes {
+  TreeLds& lds;
   const int32_t* parents;  // of the sequence
-  int n, base, length;
+  int base, length;
+
+  __device__ __forceinline__ TreeNodes(const PagedParams& p)
+      : lds(tree_lds()),
+        parents(p.parents + __builtin_amdgcn_readfirstlane(lds.off)),
+        base(__builtin_amdgcn_readfirstlane(lds.base)),
+        length(__builtin_amdgcn_readfirstlane(lds.length)) {}
+  __device__ __forceinline__ TreeNodes(const PagedParams& p, const Item& it)
+      : lds(tree_lds()), parents(p.parents + it.off), base(it.pos0), length(it.length) {
+    lds.base = base;
+    lds.off = it.off;
+    lds.length = length;
+  }
 
   __device__ __forceinline__ int block(int i) const { return (base + i) >> 5; }
   __device__ __forceinline__ uint32_t bit(int i) const { return 1u << ((base + i) & 31); }
@@ -556,11 +589,11 @@ struct TreeNodes<true> {
     return a >= 0 && a < i ? a : -1;
   }
 
-  // By all threads of the workgroup.
-  __device__ __forceinline__ void build(int tid) {
+  // Of n nodes, by all threads of the workgroup.
+  __device__ __forceinline__ void build(int n, int tid) {
     const int held = min(n, kTreeNodes);
     constexpr int kEach = kTreeNodes / kNT;
-    for (int i = tid; i < held; i += kNT) next[i] = uint16_t(parent(i));
+    for (int i = tid; i < held; i += kNT) lds.next[i] = uint16_t(parent(i));
     __syncthreads();
     uint32_t m[kEach];
     int a[kEach];
@@ -571,17 +604,17 @@ struct TreeNodes<true> {
       a[k] = int(kNone);
       if (i >= held) continue;
       m[k] = bit(i);
-      a[k] = next[i];
+      a[k] = lds.next[i];
       while (a[k] != int(kNone) && block(a[k]) == block(i)) {
         m[k] |= bit(a[k]);
-        a[k] = next[a[k]];
+        a[k] = lds.next[a[k]];
       }
     }
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kEach; ++k) {
       const int i = tid + k * kNT;
-      if (i < held) mask[i] = m[k], next[i] = uint16_t(a[k]);
+      if (i < held) lds.mask[i] = m[k], lds.next[i] = uint16_t(a[k]);
     }
     __syncthreads();
   }
@@ -589,7 +622,7 @@ struct TreeNodes<true> {
   // Node i's mask; i becomes the nearest ancestor in a block before, -1: none.
   __device__ __forceinline__ uint32_t step(int& i) const {
     if (i < kTreeNodes) {
-      const uint32_t m = mask[i], a = next[i];
+      const uint32_t m = lds.mask[i], a = lds.next[i];
       i = a == kNone ? -1 : int(a);
       return m;
     }
@@ -608,13 +641,14 @@ struct TreeNodes<true> {
     return d;
   }
 
-  // A walk up from a node of depth d, from block to block in descending order.
+  // A walk up from a query's node, from block to block in descending order.
   struct Walk {
-    int at, above;  // the ancestor that the walk has come to; how many it has passed
+    int at, above, pos;  // the ancestor that it has come to; how many it has passed; the query's position
   };
+  __device__ __forceinline__ Walk walk(int tid) const { return Walk{lds.lane[tid][0], 0, lds.lane[tid][1]}; }
 
-  // Which of the keys of block b a node of position pos sees.
-  __device__ __forceinline__ uint32_t seen(Walk& w, int b, int pos, const PagedParams& p) const {
+  // Which of the keys of block b the query sees.
+  __device__ __forceinline__ uint32_t seen(Walk& w, int b, const PagedParams& p) const {
     while (w.at >= 0 && block(w.at) > b) w.above += __popc(step(w.at));
     if (w.at < 0 || block(w.at) < b) return 0u;
     uint32_t m = step(w.at);
@@ -623,7 +657,7 @@ struct TreeNodes<true> {
       // The nearest window - above of them, and those at positions below the sinks:
       // theirs are pos - above - count + 1 .. pos - above.
       const int near = max(p.window - w.above, 0);
-      const int far = min(max(p.sinks - (pos - w.above - count + 1), 0), count);
+      const int far = min(max(p.sinks - (w.pos - w.above - count + 1), 0), count);
       uint32_t keep = m, first = m;
       for (int k = near; k < count; ++k) keep &= keep - 1u;                          // the upper `near` bits
       for (int k = far; k < count; ++k) first &= ~(0x80000000u >> __clz(int(first)));  // the lower `far`
@@ -635,22 +669,20 @@ struct TreeNodes<true> {
   }
 };
 
-// This lane's query: its position (of a tree, its depth's), and whether it saw a key.
+// This lane's query: its position (trees: TreeLds has it), and whether it saw a key.
 struct LaneRow {
   int pos;
   bool any;
-  int node;  // trees
 };
 
-// The keys of the stored tokens, and all others, that a lane's query may see.
+// The keys that a lane's query sees; of a tree, the stored tokens alone.
 template <bool TREE>
-__device__ __forceinline__ Visible visible_to(const PagedParams& p, const LaneRow& row, const TreeNodes<TREE>& tree,
-                                              int length) {
-  Visible v = visible(p, fresh(row.pos), length);  // not held in registers over the stream
-  if constexpr (TREE) {
-    v.hi = min(tree.base, length) - 1;
-    v.sink = min(p.sinks, v.hi + 1);
-  }
+__device__ __forceinline__ Visible visible_to(const PagedParams& p, const LaneRow& row, int length) {
+  if constexpr (!TREE) return visible(p, fresh(row.pos), length);  // not held in registers over the stream
+  const TreeLds& lds = tree_lds();
+  Visible v = visible(p, lds.lane[threadIdx.x][1], length);
+  v.hi = min(__builtin_amdgcn_readfirstlane(lds.base), length) - 1;
+  v.sink = min(p.sinks, v.hi + 1);
   return v;
 }
 
@@ -660,51 +692,38 @@ struct Bounds {
   Visible a, b;
 };
 
-// Of rows whose tokens are first .. last of an item's sequence.
+// A lane's query (new token `token` of the item's sequence), and the bounds of its
+// wave's, first .. last.  drafts: the workgroup's keys reach the new tokens.
 template <bool TREE>
-__device__ __forceinline__ Bounds bounds_of(const PagedParams& p, const Item& it, const LaneRow& row, int first,
-                                            int last) {
+__device__ __forceinline__ Bounds begin_rows(const PagedParams& p, const Item& it, bool drafts, LaneRow& row, int token,
+                                             int first, int last) {
   Bounds x;
   x.a = visible(p, it.pos0 + first, it.length);
   x.b = visible(p, it.pos0 + last, it.length);
+  row.pos = it.pos0 + token;
+  row.any = false;
   if constexpr (TREE) {
-    // Their positions, by depths; no tile with a node is seen whole.
-    int lo = row.pos, hi = row.pos;
+    TreeNodes tree(p, it);
+    const bool windowed = p.window != 0x7FFFFFFF;
+    if (drafts || windowed) tree.build(it.n, threadIdx.x);
+    int lo = windowed ? it.pos0 + tree.depth(token) : row.pos, hi = lo;
+    tree.lds.lane[threadIdx.x][0] = token;
+    tree.lds.lane[threadIdx.x][1] = lo;
+    // No tile with a node is seen whole, or passed over for its distance (a node
+    // at a position below the sinks may lie past them).
+    if (windowed) {
 #pragma unroll
-    for (int off = 1; off < kWave; off <<= 1) {
-      lo = min(lo, __shfl_xor(lo, off));
-      hi = max(hi, __shfl_xor(hi, off));
+      for (int off = 1; off < kWave; off <<= 1) {
+        lo = min(lo, __shfl_xor(lo, off));
+        hi = max(hi, __shfl_xor(hi, off));
+      }
     }
-    x.a.lo = visible(p, __builtin_amdgcn_readfirstlane(lo), it.length).lo;
+    x.a.lo = min(visible(p, __builtin_amdgcn_readfirstlane(lo), it.length).lo, it.pos0);
     x.b.lo = visible(p, __builtin_amdgcn_readfirstlane(hi), it.length).lo;
     x.a.hi = min(it.pos0, it.length) - 1;
     x.a.sink = min(p.sinks, x.a.hi + 1);
   }
   return x;
-}
-
-// Makes a workgroup's nodes known to it, and a lane's query: its position.
-template <bool TREE>
-__device__ __forceinline__ TreeNodes<TREE> nodes_of(const PagedParams& p, const Item& it, bool drafts, LaneRow& row,
-                                                    int token) {
-  TreeNodes<TREE> tree;
-  row.pos = it.pos0 + token;
-  row.any = false;
-  if constexpr (TREE) {
-    __shared__ uint32_t s_mask[kTreeNodes];
-    __shared__ uint16_t s_next[kTreeNodes];
-    tree.mask = s_mask;
-    tree.next = s_next;
-    tree.parents = p.parents + it.off;
-    tree.n = it.n;
-    tree.base = it.pos0;
-    tree.length = it.length;
-    const bool windowed = p.window != 0x7FFFFFFF;
-    if (drafts || windowed) tree.build(threadIdx.x);
-    row.node = token;
-    if (windowed) row.pos = it.pos0 + tree.depth(token);
-  }
-  return tree;
 }
 
 // Sixteen per-key factors of this lane's score elements of a half (key 8 (e /
@@ -728,12 +747,11 @@ __device__ __forceinline__ f32x16 key_factors(const float* half, int hh) {
 // nodes: the nodes of a tree that the query sees, by place.
 template <int D, int TK, int F, bool TREE>
 __device__ __forceinline__ void attend_masked(const PagedParams& p, int length, State<D>& st, LaneRow& row,
-                                              const TreeNodes<TREE>& tree, uint32_t nodes, f32x16 s,
-                                              const uint16_t* slot, int t, int j0, uint32_t valid, int lane_col,
-                                              int lane_hh, const float* scales) {
+                                              uint32_t nodes, f32x16 s, const uint16_t* slot, int t, int j0,
+                                              uint32_t valid, int lane_col, int lane_hh, const float* scales) {
   const int col = fresh(lane_col), hh = fresh(lane_hh);
   const float c = scales ? 1.f : p.scale_log2;
-  const Visible v = visible_to(p, row, tree, length);
+  const Visible v = visible_to<TREE>(p, row, length);
   if constexpr (TREE) nodes >>= 4 * hh;  // this lane's
   if (scales) {
     const f32x16 sk = key_factors(scales, hh);
@@ -1177,7 +1195,7 @@ __device__ __forceinline__ void step_nonfinite(StepState<D>& st, const uint8_t* 
 // the next tile's K and waits for this one's V.
 template <int D, int F, bool MASKED, bool TREE, typename KeysRead, typename ValuesDue>
 __device__ __forceinline__ void step_tile(const PagedParams& p, int length, StepState<D>& st, LaneRow& row,
-                                          const TreeNodes<TREE>& tree, const bf16x8 (&qf)[D / 32], const uint8_t* slot, const StepSlot<D, F>& at,
+                                          const bf16x8 (&qf)[D / 32], const uint8_t* slot, const StepSlot<D, F>& at,
                                           const float* scales, int tile, uint32_t valid, int lane, KeysRead keys_read,
                                           ValuesDue values_due) {
   using Slot = StepSlot<D, F>;
@@ -1212,15 +1230,16 @@ __device__ __forceinline__ void step_tile(const PagedParams& p, int length, Step
   keys_read();
   uint32_t seen = 0;
   if constexpr (MASKED) {
-    const Visible v = visible_to(p, row, tree, length);
+    const Visible v = visible_to<TREE>(p, row, length);
     uint32_t nodes[TK / 32];  // of the tree that the query sees
     if constexpr (TREE) {
 #pragma unroll
       for (int b = 0; b < TK / 32; ++b) nodes[b] = 0u;
+      const TreeNodes tree(p);
       if (tile * TK + TK > tree.base) {
-        typename TreeNodes<true>::Walk walk = {fresh(row.node), 0};
+        TreeNodes::Walk walk = tree.walk(threadIdx.x);
 #pragma unroll
-        for (int b = TK / 32 - 1; b >= 0; --b) nodes[b] = tree.seen(walk, tile * (TK / 32) + b, fresh(row.pos), p);
+        for (int b = TK / 32 - 1; b >= 0; --b) nodes[b] = tree.seen(walk, tile * (TK / 32) + b, p);
       }
     }
 #pragma unroll
@@ -1357,10 +1376,9 @@ __global__ __launch_bounds__(kNT, 2) void step_kernel(PagedParams p) {
   const int first = it.r0 / p.G, last = (it.r0 + it.rows - 1) / p.G;
   const Span span = span_of<TK>(p, pos0 + (TREE ? 0 : first), pos0 + last, it.length);
   const int t0 = int(int64_t(it.part) * span.n / it.parts), t1 = int(int64_t(it.part + 1) * span.n / it.parts);
-  const TreeNodes<TREE> tree =
-      nodes_of<TREE>(p, it, t0 < t1 && (span.tile(t1 - 1) + 1) * TK > pos0, row, token);
   // Tiles inside these bounds are seen whole by every row.
-  const Bounds bounds = bounds_of<TREE>(p, it, row, first, last);
+  const Bounds bounds =
+      begin_rows<TREE>(p, it, t0 < t1 && (span.tile(t1 - 1) + 1) * TK > pos0, row, token, first, last);
   const Visible va = bounds.a, vb = bounds.b;
 
   StepState<D> st;
@@ -1394,8 +1412,8 @@ __global__ __launch_bounds__(kNT, 2) void step_kernel(PagedParams p) {
       const bool more = k + 1 < count;
       const uint32_t valid = dma.valid;
       wait_vmcnt<Dma::kLoads>();
-      step_tile<D, F, decltype(masked)::value>(
-          p, it.length, st, row, tree, qf, slot, at, scales, tile_of(k), valid, lane,
+      step_tile<D, F, decltype(masked)::value, TREE>(
+          p, it.length, st, row, qf, slot, at, scales, tile_of(k), valid, lane,
           [&] {
             if (more) {
               prepare(k + 1);
@@ -1754,6 +1772,54 @@ __device__ __forceinline__ void wide_tile(State<D>& st, const uint16_t* buf, con
   }
 }
 
+// The same of 32 keys, of a tile's half that begins at buf: for row tiles whose
+// halves are taken by waves of their own.
+template <int D, bool SCALED, typename Refill>
+__device__ __forceinline__ void wide_half(State<D>& st, const uint16_t* buf, const float* scales,
+                                          const bf16x8 (&qf)[Shape<D>::KT], int col, int hh, float c,
+                                          const Refill& refill) {
+  constexpr int KT = Shape<D>::KT, DT = Shape<D>::DT, kAhead = 4;
+  const FragLane<D> fl(fresh(col), fresh(hh));
+  const uint32_t vbase = fl.v_base(buf);
+  auto operand = [&](int n) { return n < KT ? fl.k(buf, 0, n) : fl.v(vbase, 0, (n - KT) / DT, (n - KT) % DT); };
+  u32x4 o[kAhead];
+#pragma unroll
+  for (int n = 0; n < kAhead; ++n) o[n] = operand(n);
+  WideHalf<D, SCALED> half;
+  half.s = zero16();
+  chunk_end();
+  auto next = [&](int n) { return as_bf16x8(o[n % kAhead]); };
+  auto ask = [&](int n) {
+    if (n + kAhead < KT + 2 * DT) o[n % kAhead] = operand(n + kAhead);
+  };
+#pragma unroll
+  for (int n = 0; n < KT; ++n) {
+    half.s = mfma32x32x16(next(n), qf[n], half.s);
+    ask(n);
+    refill.template after_step<KT>(n);
+    chunk_end();
+  }
+  half.ask(scales, 0, hh);
+  half.template step<1>(0, st, c, scales, hh);
+  half.finish(st, c, scales, hh, [&] {
+    const FragLane<D> fr(fresh(col), fresh(hh));
+    f32x16 s = zero16();
+#pragma unroll
+    for (int ks = 0; ks < KT; ++ks) {
+      s = mfma32x32x16(as_bf16x8(fr.k(buf, 0, ks)), qf[ks], s);
+      chunk_end();
+    }
+    return s;
+  });
+#pragma unroll
+  for (int f = 0; f < 2 * DT; ++f) {
+    st.acc[f % DT] = mfma32x32x16(next(KT + f), half.pb(f / DT), st.acc[f % DT]);
+    ask(KT + f);
+    refill.template late_step<2 * DT>(f);
+    chunk_end();
+  }
+}
+
 // Bound by the softmax's vector work beside the products: a half's 16 products
 // are 512 cycles of the matrix core, its exponentials, sums and packing about
 // 420 of the vector unit, of each of two waves.  4,096 queries of 16 heads of 128
@@ -1776,10 +1842,14 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, hh = lane >> 5;
-  const int wrows = min(32, it.rows - 32 * wave);  // this wave's rows (none: it only moves tiles)
+  // Trees, at most 64 rows: two waves share their rows, and take a half of every
+  // key tile each.  (Row tiles of trees are few and seldom full.)
+  const bool halved = TREE && it.rows <= 64;
+  const int block = halved ? wave & 1 : wave, half = wave >> 1;
+  const int wrows = min(32, it.rows - 32 * block);  // this wave's rows (none: it only moves tiles)
 
   const int pos0 = it.pos0;
-  const int r = it.r0 + min(32 * wave + col, it.rows - 1);
+  const int r = it.r0 + min(32 * block + col, it.rows - 1);
   const int token = r / p.G;
   const uint16_t* q = p.q + (PAGED ? (it.off + token) * p.q_st : it.s * p.q_sb + token * p.q_st) +
                       (h * p.G + r % p.G) * p.q_sh;
@@ -1790,10 +1860,9 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
 
   const Span span = span_of<TK>(p, pos0 + (TREE ? 0 : it.r0 / p.G), pos0 + (it.r0 + it.rows - 1) / p.G, it.length);
   const int t0 = int(int64_t(it.part) * span.n / it.parts), t1 = int(int64_t(it.part + 1) * span.n / it.parts);
-  const TreeNodes<TREE> tree =
-      nodes_of<TREE>(p, it, t0 < t1 && (span.tile(t1 - 1) + 1) * TK > pos0, row, token);
-  const Bounds bounds = bounds_of<TREE>(p, it, row, (it.r0 + 32 * wave) / p.G,
-                                        (it.r0 + 32 * wave + max(wrows, 1) - 1) / p.G);
+  const Bounds bounds =
+      begin_rows<TREE>(p, it, t0 < t1 && (span.tile(t1 - 1) + 1) * TK > pos0, row, token, (it.r0 + 32 * block) / p.G,
+                       (it.r0 + 32 * block + max(wrows, 1) - 1) / p.G);
   const Visible va = bounds.a, vb = bounds.b;
 
   State<D> st;
@@ -1806,115 +1875,154 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
   enum Kind { kHidden, kPart, kWhole };
   auto kind_of = [&](int tile, uint32_t valid) {
     const int a = tile * TK, b = a + TK - 1;
-    // (A node at a position below the sinks may lie past them.)
-    const bool before = b < va.lo && (!TREE || b < pos0);
-    if (wrows <= 0 || ((a > vb.hi || before) && a >= vb.sink)) return kHidden;
+    if (wrows <= 0 || ((a > vb.hi || b < va.lo) && a >= vb.sink)) return kHidden;
     return valid == kAllGroups<TK> && b <= va.hi && (a >= vb.lo || b < va.sink) ? kWhole : kPart;
   };
   auto hidden = [&](int, uint32_t, const uint16_t*, const float*, const auto& refill) {
     refill.all();
     refill.late();
   };
-  auto whole = [&](int, uint32_t, const uint16_t* buf, const float* scales, const auto& refill) {
-    wide_tile<D, SCALED>(st, buf, scales, qf, col, hh, p.scale_log2, refill);
-  };
-  auto part = [&](int tile, uint32_t valid, const uint16_t* buf, const float* scales, const auto& refill) {
-    refill.all();
+  auto attend_keys = [&](auto halves) {
+    constexpr bool HALVED = decltype(halves)::value;
+    auto whole = [&](int, uint32_t, const uint16_t* buf, const float* scales, const auto& refill) {
+      if constexpr (HALVED)
+        wide_half<D, SCALED>(st, buf + 32 * half * D, SCALED ? scales + 32 * half : scales, qf, col, hh, p.scale_log2,
+                             refill);
+      else
+        wide_tile<D, SCALED>(st, buf, scales, qf, col, hh, p.scale_log2, refill);
+    };
+    auto part = [&](int tile, uint32_t valid, const uint16_t* buf, const float* scales, const auto& refill) {
+      refill.all();
 #pragma unroll 1
-    for (int t = 0; t < 2; ++t) {
-      uint32_t nodes = 0;
-      if constexpr (TREE) {
-        const int j0 = tile * TK + 32 * t;
-        if (j0 + 31 >= pos0) {
-          typename TreeNodes<true>::Walk walk = {fresh(row.node), 0};
-          nodes = tree.seen(walk, j0 >> 5, fresh(row.pos), p);
-          // Most nodes of a large tree are no ancestors of these rows.
-          if (j0 >= pos0 && !__builtin_amdgcn_ballot_w64(nodes != 0)) continue;
+      for (int t = HALVED ? half : 0; t < (HALVED ? half + 1 : 2); ++t) {
+        uint32_t nodes = 0;
+        if constexpr (TREE) {
+          const int j0 = tile * TK + 32 * t;
+          const TreeNodes tree(p);
+          if (j0 + 31 >= tree.base) {
+            TreeNodes::Walk walk = tree.walk(fresh(tid));
+            nodes = tree.seen(walk, j0 >> 5, p);
+            // Most nodes of a large tree are no ancestors of these rows.
+            if (j0 >= tree.base && !__builtin_amdgcn_ballot_w64(nodes != 0)) continue;
+          }
+        }
+        const int fcol = fresh(col), fhh = fresh(hh);
+        f32x16 s = zero16();
+#pragma unroll
+        for (int ks = 0; ks < S::KT; ++ks)
+          s = mfma32x32x16(as_bf16x8(TileImage<D, TK>::k(buf, fcol, fhh, t, ks)), qf[ks], s);
+        chunk_end();
+        attend_masked<D, TK, F, TREE>(p, it.length, st, row, nodes, s, buf, t, tile * TK + 32 * t, valid >> (2 * t), col,
+                                      hh, SCALED ? scales + 32 * t : nullptr);
+      }
+      refill.late();
+    };
+    // One tile after another; consecutive tiles of a kind run in a loop of their
+    // own, so that the sums are not split across a branch per tile.  The waves of
+    // a workgroup may be in different loops: each meets one barrier per tile.
+    auto stream = [&](auto&& step, const uint32_t& valid) {
+      int i = t0;
+      while (i < t1) {
+        const Kind kind = kind_of(at(i), valid);
+        if (kind == kWhole) {
+          row.any = true;
+          do step(i, whole);
+          while (++i < t1 && kind_of(at(i), valid) == kWhole);
+        } else if (kind == kPart) {
+          do step(i, part);
+          while (++i < t1 && kind_of(at(i), valid) == kPart);
+        } else {
+          do step(i, hidden);
+          while (++i < t1 && kind_of(at(i), valid) == kHidden);
         }
       }
-      const int fcol = fresh(col), fhh = fresh(hh);
-      f32x16 s = zero16();
-#pragma unroll
-      for (int ks = 0; ks < S::KT; ++ks)
-        s = mfma32x32x16(as_bf16x8(TileImage<D, TK>::k(buf, fcol, fhh, t, ks)), qf[ks], s);
-      chunk_end();
-      attend_masked<D, TK, F>(p, it.length, st, row, tree, nodes, s, buf, t, tile * TK + 32 * t, valid >> (2 * t), col, hh,
-                           SCALED ? scales + 32 * t : nullptr);
-    }
-    refill.late();
-  };
-  // One tile after another; consecutive tiles of a kind run in a loop of their
-  // own, so that the sums are not split across a branch per tile.  The waves of
-  // a workgroup may be in different loops: each meets one barrier per tile.
-  auto stream = [&](auto&& step, const uint32_t& valid) {
-    int i = t0;
-    while (i < t1) {
-      const Kind kind = kind_of(at(i), valid);
-      if (kind == kWhole) {
-        row.any = true;
-        do step(i, whole);
-        while (++i < t1 && kind_of(at(i), valid) == kWhole);
-      } else if (kind == kPart) {
-        do step(i, part);
-        while (++i < t1 && kind_of(at(i), valid) == kPart);
+    };
+
+    if (t0 < t1) {
+      using Window = PageWindow<D, F, PAGED, TK>;
+      Window window;
+      auto fetch = [&](int i) { window.fetch(keys, [&](int k) { return at(i + k); }, lane); };
+      // Makes tile i's pages current, in order of i; returns its place in the
+      // window.  The next window is read half a window ahead.
+      auto turn_to = [&](int i) {
+        const int k = (i - t0) % Window::kTiles;
+        if (k == 0) window.turn(keys);
+        if (k == Window::kTiles / 2) fetch(i + Window::kTiles / 2);
+        return k;
+      };
+      fetch(t0);
+      int k = turn_to(t0);
+      uint32_t valid = window.valid(k);  // of the tile at hand
+      if constexpr (!SCALED) {
+        const typename DmaTile<D, PAGED>::Lane lanes(wave, lane);
+        DmaTile<D, PAGED>(keys, window, k, at(t0), ring_lds, wave, lanes).all();
+        stream([&](int i, auto&& attend) {
+          wait_vmcnt<0>();
+          lds_barrier();
+          const int slot = (i - t0) & 1;
+          const uint32_t now = valid;
+          k = turn_to(i + 1);
+          valid = window.valid(k);
+          // Past the last tile that tile again, into the slot nobody reads.
+          const DmaTile<D, PAGED> refill(keys, window, k, at(i + 1), ring_lds + uint32_t((slot ^ 1) * S::TILE * 2), wave,
+                                         lanes);
+          attend(at(i), now, ring[slot], static_cast<const float*>(nullptr), refill);
+        }, valid);
+        wait_vmcnt<0>();
       } else {
-        do step(i, hidden);
-        while (++i < t1 && kind_of(at(i), valid) == kHidden);
+        CodeTile<D, F> code;
+        code.load(keys, window, k, wave, lane);
+        CodeRefill<D, F>{code, ring[0], s_scale[0], tid, p.scale_log2}.late();
+        stream([&](int i, auto&& attend) {
+          lds_barrier();
+          const int slot = (i - t0) & 1;
+          const uint32_t now = valid;
+          k = turn_to(i + 1);
+          valid = window.valid(k);
+          code.load(keys, window, k, wave, lane);
+          attend(at(i), now, ring[slot], s_scale[slot],
+                 CodeRefill<D, F>{code, ring[slot ^ 1], s_scale[slot ^ 1], tid, p.scale_log2});
+        }, valid);
       }
     }
   };
-
-  if (t0 < t1) {
-    using Window = PageWindow<D, F, PAGED, TK>;
-    Window window;
-    auto fetch = [&](int i) { window.fetch(keys, [&](int k) { return at(i + k); }, lane); };
-    // Makes tile i's pages current, in order of i; returns its place in the
-    // window.  The next window is read half a window ahead.
-    auto turn_to = [&](int i) {
-      const int k = (i - t0) % Window::kTiles;
-      if (k == 0) window.turn(keys);
-      if (k == Window::kTiles / 2) fetch(i + Window::kTiles / 2);
-      return k;
-    };
-    fetch(t0);
-    int k = turn_to(t0);
-    uint32_t valid = window.valid(k);  // of the tile at hand
-    if constexpr (!SCALED) {
-      const typename DmaTile<D, PAGED>::Lane lanes(wave, lane);
-      DmaTile<D, PAGED>(keys, window, k, at(t0), ring_lds, wave, lanes).all();
-      stream([&](int i, auto&& attend) {
-        wait_vmcnt<0>();
-        lds_barrier();
-        const int slot = (i - t0) & 1;
-        const uint32_t now = valid;
-        k = turn_to(i + 1);
-        valid = window.valid(k);
-        // Past the last tile that tile again, into the slot nobody reads.
-        const DmaTile<D, PAGED> refill(keys, window, k, at(i + 1), ring_lds + uint32_t((slot ^ 1) * S::TILE * 2), wave,
-                                       lanes);
-        attend(at(i), now, ring[slot], static_cast<const float*>(nullptr), refill);
-      }, valid);
-      wait_vmcnt<0>();
-    } else {
-      CodeTile<D, F> code;
-      code.load(keys, window, k, wave, lane);
-      CodeRefill<D, F>{code, ring[0], s_scale[0], tid, p.scale_log2}.late();
-      stream([&](int i, auto&& attend) {
-        lds_barrier();
-        const int slot = (i - t0) & 1;
-        const uint32_t now = valid;
-        k = turn_to(i + 1);
-        valid = window.valid(k);
-        code.load(keys, window, k, wave, lane);
-        attend(at(i), now, ring[slot], s_scale[slot],
-               CodeRefill<D, F>{code, ring[slot ^ 1], s_scale[slot ^ 1], tid, p.scale_log2});
-      }, valid);
-    }
+  // (Each form in code of its own: in one loop nest they took registers from each other.)
+  if constexpr (TREE) {
+    if (halved)
+      attend_keys(std::true_type{});
+    else
+      attend_keys(std::false_type{});
+  } else {
+    attend_keys(std::false_type{});
   }
 
+  if constexpr (TREE) {
+    if (halved) {
+      // The waves of the tiles' second halves hand their states over.
+      __shared__ float s_state[2][3][kWave];
+      float* acc = reinterpret_cast<float*>(ring[0]) + block * S::DT * 16 * kWave;
+      lds_barrier();
+      if (half) {
+#pragma unroll
+        for (int i = 0; i < S::DT * 16; ++i) acc[i * kWave + lane] = st.acc[i / 16][i % 16];
+        s_state[block][0][lane] = st.m;
+        s_state[block][1][lane] = st.den;
+        s_state[block][2][lane] = row.any ? 1.f : 0.f;
+      }
+      lds_barrier();
+      if (half) return;
+      const float m = s_state[block][0][lane], mn = fmaxf(st.m, m);
+      const float a = st.m == kNegInf ? 1.f : fast_exp2(st.m - mn), b = m == kNegInf ? 1.f : fast_exp2(m - mn);
+      st.m = mn;
+      st.den = st.den * a + s_state[block][1][lane] * b;
+      row.any |= s_state[block][2][lane] != 0.f;
+#pragma unroll
+      for (int i = 0; i < S::DT * 16; ++i) st.acc[i / 16][i % 16] = st.acc[i / 16][i % 16] * a + acc[i * kWave + lane] * b;
+    }
+  }
   const float den = pair_sum(st.den), seen = pair_sum(row.any ? 1.f : 0.f);
   if (col >= wrows) return;
-  float* row_out = it.parts > 1 ? record<D, R>(p, it.record) + (32 * wave + col) * kRecordRow<D> : nullptr;
+  float* row_out = it.parts > 1 ? record<D, R>(p, it.record) + (32 * block + col) * kRecordRow<D> : nullptr;
   uint16_t* out = p.out + output_row<D>(p, it.off, r, h);
 #pragma unroll
   for (int c = 0; c < D / 8; ++c) {
@@ -2027,8 +2135,8 @@ PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t tile
     const int64_t rounds = ragged && 2 * sequences * heads >= kResident ? 2 : 1;
     if (key_tiles > (format == kBf16 ? 48 : 20)) s.target = (rounds * kResident + heads - 1) / heads;
   } else if (tree && likely * heads <= kResident) {
-    s.min_tiles = 8;
-    if (key_tiles > s.min_tiles) s.target = kResident / heads;
+    s.min_tiles = 6;  // take_item makes one or two rounds of parts
+    if (key_tiles > s.min_tiles) s.target = 2 * (kResident / heads);
   } else if (uneven && 2 * likely * heads * key_tiles >= 3 * kResident * 24) {
     // Enough keys for one and a half rounds of parts of 24 tiles: those even the
     // lengths out (8 sequences of 600 .. 12,000 keys, 512 new tokens of 8 x 4
