@@ -1582,18 +1582,30 @@ struct CodeTile {
   u32x4 x[2][kLoads];
   float scale;
 
+  // Lane l's row and chunk of a piece (64 chunks of 16 codes, 8 or 16 rows): so that
+  // the 16 lanes of a phase of put()'s stores meet different banks, V's rows of a
+  // quad, which lie side by side, are taken by neighbouring lanes.
+  __device__ static __forceinline__ int row_of(int kv, int l) {
+    return kv && D == 128 ? 4 * (l >> 5) + ((l >> 2) & 3) : l / kRowLanes;
+  }
+  __device__ static __forceinline__ int chunk_of(int kv, int l) {
+    return kv && D == 128 ? 4 * ((l >> 4) & 1) + (l & 3) : l % kRowLanes;
+  }
+
   // The window's tile i.
   template <typename Window>
   __device__ __forceinline__ void load(const Keys<D, F, true>& keys, const Window& window, int i, int wave, int lane) {
     const int l = fresh(lane);
     // A wave's 64 chunks are 8 (D = 128) or 16 rows of one group.
-    const uint32_t row = uint32_t(wave * kWave / kRowLanes % 16 + l / kRowLanes);
-    const uint32_t off = row * keys.kRowBytes + 16u * (l % kRowLanes);
+    const uint32_t row = uint32_t(wave * kWave / kRowLanes % 16);
+    uint32_t off[2];
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) off[kv] = (row + row_of(kv, l)) * keys.kRowBytes + 16u * chunk_of(kv, l);
 #pragma unroll
     for (int n = 0; n < kLoads; ++n) {
       const uint64_t at = window.offset(i, D == 128 ? 2 * n + (wave >> 1) : wave);
 #pragma unroll
-      for (int kv = 0; kv < 2; ++kv) x[kv][n] = load_chunk(keys.base[kv] + at + off);
+      for (int kv = 0; kv < 2; ++kv) x[kv][n] = load_chunk(keys.base[kv] + at + off[kv]);
     }
     // Wave 0 the keys' scales, wave 1 the values'.
     if (wave < 2) scale = (wave ? keys.scale[1] : keys.scale[0])[window.row(i, l)];
@@ -1602,8 +1614,8 @@ struct CodeTile {
   static constexpr int kPieces = 2 * kLoads;
   __device__ __forceinline__ void put(uint16_t* slot, int n, int thread) const {
     using Image = TileImage<D, 64>;
-    const int tid = fresh(thread), kv = n / kLoads, i = n % kLoads;
-    const int row = (i * kNT + tid) / kRowLanes, c = tid % kRowLanes;
+    const int tid = fresh(thread), l = tid & 63, kv = n / kLoads, i = n % kLoads;
+    const int row = (i * kNT + (tid & ~63)) / kRowLanes + row_of(kv, l), c = chunk_of(kv, l);
     Image::put(slot, kv, row, 2 * c, codes_to_bf16<F>(x[kv][i][0], x[kv][i][1]));
     Image::put(slot, kv, row, 2 * c + 1, codes_to_bf16<F>(x[kv][i][2], x[kv][i][3]));
   }
