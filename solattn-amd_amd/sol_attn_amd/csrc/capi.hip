@@ -1250,7 +1250,7 @@ int sol_cache_keep(const int32_t* page_table, const int32_t* context_lengths, co
   if (rc != SOL_OK) return rc;
   if (most < 0 || most >= kMaxPositions || (most && !kept) || !lengths_out)
     return fail(SOL_ERR_INVALID, "sol_cache_keep: kept and lengths_out are required");
-  if (sequences * heads > kMaxGrid / 8) return fail(SOL_ERR_UNSUPPORTED, "sol_cache_keep: grid too large");  // of 1,024 threads
+  if (sequences * heads > kMaxGrid / 16) return fail(SOL_ERR_UNSUPPORTED, "sol_cache_keep: grid too large");  // of 1,024 threads
   p.kept = kept;
   p.most = int(most);
   p.store[0] = static_cast<uint8_t*>(cache_k);

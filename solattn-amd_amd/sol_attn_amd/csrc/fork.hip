@@ -28,20 +28,30 @@ namespace {
 
 // Entry j of a sequence's list stands if the entries ascend up to it, inside
 // [0, n).
-__device__ __forceinline__ bool kept_stands(const int32_t* kept, int j, int64_t n) {
+__device__ __forceinline__ bool kept_ascends(const int32_t* kept, int j, int64_t n) {
   const int x = kept[j];
   return x > (j ? kept[j - 1] : -1) && x < n;
 }
 
-// How many entries of the list stand, for all threads.
+// How many entries of the list stand, for all threads: those before the first that
+// does not ascend.
 template <int NT>
 __device__ __forceinline__ int kept_count(const int32_t* kept, int most, int64_t n) {
+  constexpr int kEach = 4;  // entries that a thread reads at once
   __shared__ int s_least[NT / kWave];
-  for (int j0 = 0; j0 < most; j0 += NT) {
-    const int j = j0 + int(threadIdx.x);
-    const uint64_t bad = __builtin_amdgcn_ballot_w64(j >= most || !kept_stands(kept, j, n));
-    const int wave0 = j0 + int(threadIdx.x & ~63u);
-    int least = bad ? wave0 + __builtin_ctzll(bad) : 0x7FFFFFFF;
+  for (int j0 = 0; j0 < most; j0 += kEach * NT) {
+    bool bad[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      const int j = j0 + k * NT + int(threadIdx.x);
+      bad[k] = j >= most || !kept_ascends(kept, j, n);
+    }
+    int least = 0x7FFFFFFF;
+#pragma unroll
+    for (int k = kEach - 1; k >= 0; --k) {
+      const uint64_t lanes = __builtin_amdgcn_ballot_w64(bad[k]);
+      if (lanes) least = j0 + k * NT + int(threadIdx.x & ~63u) + __builtin_ctzll(lanes);
+    }
     if constexpr (NT > kWave) {
       s_least[threadIdx.x >> 6] = least;
       __syncthreads();
@@ -54,64 +64,77 @@ __device__ __forceinline__ int kept_count(const int32_t* kept, int most, int64_t
   return most;
 }
 
-// A workgroup moves the rows of one (sequence, head, K or V).  Rows only move
-// forward, k_j >= j, and in ascending order, so that a row is read before another
-// takes its place: a batch of rows is read whole before it is written, and the
-// batches follow one another.
+// A workgroup moves the rows of one (sequence, head, K or V), 128 bytes of them at
+// most (longer rows take two workgroups).  Rows only move forward, k_j >= j, and in
+// ascending order, so that a row is read before another takes its place: a batch
+// of rows is read whole before it is written, and the batches follow one another.
+// So the time is that of a batch's chain of reads (the list, the table, the rows),
+// and the workgroups are large: two frames of 4,032 tokens, thinned to some 1,500
+// and 600, 24 heads of 128, BF16, 18 MB: XX us (a workgroup per row and batches of
+// 512 rows: 15.6).
 template <int ROW, int WAVES, int U>
 __global__ __launch_bounds__(WAVES * kWave) void keep_kernel(KeepParams p) {
-  constexpr int NT = WAVES * kWave, kLanes = ROW / 16, kRows = NT / kLanes;
+  constexpr int NT = WAVES * kWave, kPiece = ROW < 128 ? ROW : 128, kPieces = ROW / kPiece;
+  constexpr int kLanes = kPiece / 16, kRows = NT / kLanes;
+  constexpr uint32_t kStays = 0xFFFFFFFFu;
   const PagedBatch& bt = p.batch;
-  const int kv = blockIdx.x & 1, h = int(blockIdx.x >> 1) % p.H, s = int(blockIdx.x >> 1) / p.H;
+  const int piece = int(blockIdx.x) % kPieces, unit = int(blockIdx.x) / kPieces;
+  const int kv = unit & 1, h = (unit >> 1) % p.H, s = (unit >> 1) / p.H;
   const int64_t n = int64_t(bt.offsets[s + 1]) - bt.offsets[s], base = int64_t(bt.lengths[s]) - max(n, int64_t(0));
   const int32_t* kept = p.kept + int64_t(s) * p.most;
-  const int count = kept_count<NT>(kept, p.most, n);
-  if (kv == 0 && h == 0 && threadIdx.x == 0) p.lengths_out[s] = int(max(base + count, int64_t(0)));
-  // Row of the cache at position `at`, -1: none.
-  auto row_of = [&](int64_t at) -> int64_t {
-    if (at < 0 || at >= bt.positions()) return -1;
+  // Row of the cache at position `at` (a cache of 2^32 rows does not fit the card), kStays: none.
+  auto row_of = [&](int64_t at) -> uint32_t {
+    if (at < 0 || at >= bt.positions()) return kStays;
     const int page = bt.table[int64_t(s) * bt.width + (at >> bt.page_shift)];
-    if (page < 0 || page >= bt.pages) return -1;
-    return ((int64_t(page) * p.H + h) << bt.page_shift) + (at & ((1 << bt.page_shift) - 1));
+    if (page < 0 || page >= bt.pages) return kStays;
+    return uint32_t((uint64_t(uint32_t(page)) * p.H + h) << bt.page_shift) + uint32_t(at & ((1 << bt.page_shift) - 1));
   };
   const int c = threadIdx.x % kLanes;
-  for (int j0 = 0; j0 < count; j0 += U * kRows) {
+  uint8_t* store = p.store[kv] + kPiece * piece + 16 * c;
+  const bool scales = p.scale[kv] && piece == 0 && c == 0;
+  int count = p.most;  // known once the first batch is on its way
+  for (int j0 = 0; j0 < count || j0 == 0; j0 += U * kRows) {
     u32x4 x[U];
     float scale[U];
-    int64_t to[U];
+    uint32_t to[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int j = j0 + u * kRows + int(threadIdx.x) / kLanes;
       const int k = j < count ? kept[j] : j;
-      to[u] = -1;
-      if (k != j) {
-        const int64_t from = row_of(base + k);
-        to[u] = from >= 0 ? row_of(base + j) : -1;
-        if (to[u] >= 0) {
-          x[u] = *reinterpret_cast<const u32x4*>(p.store[kv] + from * ROW + 16 * c);
-          if (p.scale[kv] && c == 0) scale[u] = p.scale[kv][from];
+      to[u] = kStays;
+      if (k != j && k >= 0 && k < n) {
+        const uint32_t from = row_of(base + k);
+        to[u] = from != kStays ? row_of(base + j) : kStays;
+        if (to[u] != kStays) {
+          x[u] = *reinterpret_cast<const u32x4*>(store + uint64_t(from) * ROW);
+          if (scales) scale[u] = p.scale[kv][from];
         }
       }
+    }
+    if (j0 == 0) {
+      count = kept_count<NT>(kept, p.most, n);
+      if (unit == 2 * p.H * s && piece == 0 && threadIdx.x == 0) p.lengths_out[s] = int(max(base + count, int64_t(0)));
     }
     // Every read of the batch has returned before anything is written.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     if constexpr (WAVES > 1) __syncthreads();
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (to[u] >= 0) {
-        *reinterpret_cast<u32x4*>(p.store[kv] + to[u] * ROW + 16 * c) = x[u];
-        if (p.scale[kv] && c == 0) p.scale[kv][to[u]] = scale[u];
+      if (to[u] != kStays && j0 + u * kRows + int(threadIdx.x) / kLanes < count) {
+        *reinterpret_cast<u32x4*>(store + uint64_t(to[u]) * ROW) = x[u];
+        if (scales) p.scale[kv][to[u]] = scale[u];
       }
   }
 }
 
 template <int ROW>
 void keep_variant(const KeepParams& p, hipStream_t stream) {
-  const dim3 grid(unsigned(int64_t(p.batch.S) * p.H * 2));
-  if (p.most <= 4 * 1024 / ROW)
+  constexpr int kPieces = ROW > 128 ? ROW / 128 : 1, kRows = kWave * 16 * kPieces / ROW;  // of a wave's load
+  const dim3 grid(unsigned(int64_t(p.batch.S) * p.H * 2 * kPieces));
+  if (p.most <= 4 * kRows)
     hipLaunchKernelGGL((keep_kernel<ROW, 1, 4>), grid, dim3(64), 0, stream, p);
   else
-    hipLaunchKernelGGL((keep_kernel<ROW, 16, 8>), grid, dim3(1024), 0, stream, p);
+    hipLaunchKernelGGL((keep_kernel<ROW, 16, 12>), grid, dim3(1024), 0, stream, p);
 }
 
 // ---- forks ------------------------------------------------------------------

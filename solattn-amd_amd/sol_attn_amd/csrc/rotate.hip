@@ -113,7 +113,7 @@ __global__ __launch_bounds__(kRotateThreads) void rotate_kernel(RotateParams p, 
   const int lane = threadIdx.x & 63, c = lane % kRotateLanes<D>;
   const int heads = p.x[0].heads + p.x[1].heads;
   const int groups = (heads + heads_each - 1) / heads_each;
-  const int64_t unit = int64_t(blockIdx.x) * (kRotateThreads / 64) + (threadIdx.x >> 6);
+  const int64_t unit = int64_t(blockIdx.x) * (kRotateThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t first = unit / groups * kRotateTokens<D>;
   if (first >= p.rows) return;
   const int h0 = int(unit % groups) * heads_each, h1 = min(h0 + heads_each, heads);
@@ -121,6 +121,22 @@ __global__ __launch_bounds__(kRotateThreads) void rotate_kernel(RotateParams p, 
   const bool mine = first + lane / kRotateLanes<D> < p.rows;
   const int64_t row = min(first + lane / kRotateLanes<D>, p.rows - 1);
   const int64_t b = row / p.tokens, t = row % p.tokens;
+
+  // The wave's heads h .. to - 1 of Q (n = 0), then of K.
+  int n = h0 < p.x[0].heads ? 0 : 1;
+  auto from = [&] { return max(h0 - (n ? p.x[0].heads : 0), 0); };
+  auto until = [&] { return min(h1 - (n ? p.x[0].heads : 0), p.x[n].heads); };
+  int h = from(), to = until();
+  u32x4 v[U][2];
+  auto load = [&] {
+    const RotateOperand& x = p.x[n];
+    const uint16_t* in = x.rows + b * x.sb + t * x.st + 8 * c;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) v[u][k] = load16(in + min(h + u, to - 1) * x.sh + k * (D / 2));
+  };
+  load();  // on their way while the angles are formed
 
   float cs[8], sn[8];
   const int32_t* at = p.positions + b * p.pb + t * p.pt;
@@ -133,33 +149,24 @@ __global__ __launch_bounds__(kRotateThreads) void rotate_kernel(RotateParams p, 
     sincospif(2.f * float(turns - rint(turns)), &sn[i], &cs[i]);
   }
 
-#pragma unroll
-  for (int n = 0; n < 2; ++n) {
+  for (;;) {
     const RotateOperand& x = p.x[n];
-    const int from = max(h0 - (n ? p.x[0].heads : 0), 0), to = min(h1 - (n ? p.x[0].heads : 0), x.heads);
-    if (from >= to) continue;
     LanePairs w;
     if (x.weight) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const int j = pair_of<D, PAIRS>(c, i), ja = PAIRS ? 2 * j : j, jb = PAIRS ? 2 * j + 1 : j + D / 2;
         if (p.weights_bf16) {
-          const uint16_t* v = static_cast<const uint16_t*>(x.weight);
-          w.a[i] = bf16_bits_to_f32(v[ja]), w.b[i] = bf16_bits_to_f32(v[jb]);
+          const uint16_t* from = static_cast<const uint16_t*>(x.weight);
+          w.a[i] = bf16_bits_to_f32(from[ja]), w.b[i] = bf16_bits_to_f32(from[jb]);
         } else {
-          const float* v = static_cast<const float*>(x.weight);
-          w.a[i] = v[ja], w.b[i] = v[jb];
+          const float* from = static_cast<const float*>(x.weight);
+          w.a[i] = from[ja], w.b[i] = from[jb];
         }
       }
     }
-    const uint16_t* in = x.rows + b * x.sb + t * x.st + 8 * c;
     uint16_t* out = x.out + b * x.ob + t * x.ot + 8 * c;
-    for (int h = from; h < to; h += U) {
-      u32x4 v[U][2];
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) v[u][k] = load16(in + min(h + u, to - 1) * x.sh + k * (D / 2));
+    for (;;) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         LanePairs y = unpack<PAIRS>(v[u]);
@@ -180,7 +187,15 @@ __global__ __launch_bounds__(kRotateThreads) void rotate_kernel(RotateParams p, 
           for (int k = 0; k < 2; ++k) *reinterpret_cast<u32x4*>(out + (h + u) * x.oh + k * (D / 2)) = v[u][k];
         }
       }
+      h += U;
+      if (h >= to) break;
+      load();
     }
+    if (n == 1) return;
+    n = 1;
+    h = from(), to = until();
+    if (h >= to) return;
+    load();
   }
 }
 
