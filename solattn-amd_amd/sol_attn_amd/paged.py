@@ -183,32 +183,36 @@ def _validate(cache, plan, device):
     k, v, table, lengths, offsets = cache.k, cache.v, plan.page_table, plan.context_lengths, plan.query_offsets
     shape, dtype = k.shape, k.dtype
     if (len(shape) != 4 or v.shape != shape or dtype not in _native.CACHE_FORMATS or v.dtype != dtype
-            or min(shape) <= 0 or not k.is_contiguous() or not v.is_contiguous()
-            or (k.data_ptr() | v.data_ptr()) & 15):
+            or k.numel() == 0 or not (k.is_contiguous() and v.is_contiguous()) or (k.data_ptr() | v.data_ptr()) & 15):
         raise ValueError("Invalid cache tensors; use PagedCache.create")
     if k.requires_grad or v.requires_grad:
         raise ValueError("Inference only: the cache must not require gradients")
-    if shape[3] not in (64, 128):
+    _, heads, page_size, dim = shape
+    if dim != 128 and dim != 64:
         raise ValueError("Only head dimensions 64 and 128 are implemented")
-    _page_size(shape[2])
+    if page_size < 16 or page_size > 4096 or page_size & (page_size - 1):
+        _page_size(page_size)
+    at = k.get_device()  # (integers compare in half the time of devices)
     if dtype != torch.bfloat16:
+        rows = shape[:3]
         for x in (cache.k_scales, cache.v_scales):
-            if (not isinstance(x, torch.Tensor) or x.dtype != torch.float32 or x.shape != shape[:3]
-                    or not x.is_contiguous() or x.get_device() != k.get_device()):
+            if (not isinstance(x, torch.Tensor) or x.dtype != torch.float32 or x.shape != rows
+                    or not x.is_contiguous() or x.get_device() != at):
                 raise ValueError("INT8 and FP8 caches need contiguous fp32 scales [pages, heads, page_size]")
-    if (table.ndim != 2 or lengths.ndim != 1 or offsets.ndim != 1 or lengths.shape[0] != table.shape[0]
-            or offsets.shape[0] != table.shape[0] + 1
+    if (table.ndim != 2 or lengths.ndim != 1 or offsets.ndim != 1
             or not table.dtype == lengths.dtype == offsets.dtype == torch.int32
             or not (table.is_contiguous() and lengths.is_contiguous() and offsets.is_contiguous())):
         raise ValueError("Invalid paged descriptor; use PagedPlan.create")
-    if table.shape[0] and not 0 < table.shape[1] <= MAX_POSITIONS // shape[2]:
+    sequences, width = table.shape
+    if lengths.numel() != sequences or offsets.numel() != sequences + 1:
+        raise ValueError("Invalid paged descriptor; use PagedPlan.create")
+    if sequences and not 0 < width <= MAX_POSITIONS // page_size:
         raise ValueError(f"page_table must name 1 to {MAX_POSITIONS} positions of each sequence")
-    at = k.get_device()  # (integers compare in half the time of devices)
     if torch.version.hip is None or device.type != "cuda" or at != device.index or at != v.get_device():
         raise ValueError("The HIP backend requires the tensors and the cache on the same AMD ROCm GPU")
     if at != table.get_device() or at != lengths.get_device() or at != offsets.get_device():
         raise ValueError("Transfer the plan to the cache's device first")
-    return shape[1], shape[3]
+    return heads, dim
 
 
 def _overlap(x, y):
