@@ -302,6 +302,14 @@ def test_more_sequences_than_threads():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("old", [4096, 4097])
+def test_more_sequences_than_a_workgroup_holds(old):
+    rng = random.Random(3)
+    b = Batch([rng.randint(1, 20) for _ in range(old)], spare=3000, width=2, heads=1)
+    b.fork([rng.choice((rng.randrange(old), old - 1 - i % 7)) for i in range(2500)], [rng.randint(0, 9) for _ in range(2500)])
+
+
+@pytest.mark.gpu
 def test_lengths_and_pages_that_make_no_sense_stay_inside_the_tensors():
     b = Batch([40, 35, 90], spare=10, width=6)
     b.table[0][1], b.table[1][2], b.table[2][5] = -3, 9999, 2147483647
