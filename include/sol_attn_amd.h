@@ -569,8 +569,8 @@ int sol_rotate_heads(const void* q, const int64_t* q_strides, int64_t query_head
  * first entry that does not ends the list.  Row base + kept[s][j] goes to row base
  * + j, K, V and scales of every head, as if all were read before any is written;
  * lengths_out[s] (int32 [sequences]) receives base + their count, at least 0.
- * Everything else is left as it was, as are rows whose source or target is in
- * no page. */
+ * A row that lies in no page moves as zeros, and none moves to where there is no
+ * page; everything else is left as it was. */
 int sol_cache_keep(const int32_t* page_table, const int32_t* context_lengths, const int32_t* query_offsets,
                    int64_t sequences, int64_t table_width, int64_t pages, int64_t page_size, int64_t heads,
                    int64_t head_dim, int format, void* cache_k, void* cache_v, float* k_scales, float* v_scales,
@@ -590,10 +590,12 @@ int sol_cache_keep(const int32_t* page_table, const int32_t* context_lengths, co
  * the others and behind them free ones, lowest first, in order of sequences and
  * places, whose first takes a copy of the parent's rows in it (its tokens
  * behind the last whole page).  Pages that become free are taken by later calls.
+ * A begun page that the parent does not have (entry outside [0, pages)) its
+ * children do not have either.
  * Outputs: new_table [new_sequences, new_width] (-1 past a sequence's pages, and
- * where no page was free), new_lengths, new_offsets [new_sequences + 1] (its
+ * where there is no page), new_lengths, new_offsets [new_sequences + 1] (its
  * new tokens are its last), new_refs [pages] (memory of its own), missing [1]: how
- * many pages were not to be had.  Sequences that are no one's parent end; refs of
+ * many pages, begun ones included, were not to be had.  Sequences that are no one's parent end; refs of
  * their pages fall.  workspace: 16-byte aligned, of
  * sol_cache_fork_workspace_size() bytes. */
 int64_t sol_cache_fork_workspace_size(int64_t sequences, int64_t new_sequences, int64_t pages);

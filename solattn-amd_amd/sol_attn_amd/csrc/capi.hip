@@ -1250,7 +1250,10 @@ int sol_cache_keep(const int32_t* page_table, const int32_t* context_lengths, co
   if (rc != SOL_OK) return rc;
   if (most < 0 || most >= kMaxPositions || (most && !kept) || !lengths_out)
     return fail(SOL_ERR_INVALID, "sol_cache_keep: kept and lengths_out are required");
-  if (sequences * heads > kMaxGrid / 16) return fail(SOL_ERR_UNSUPPORTED, "sol_cache_keep: grid too large");  // of 1,024 threads
+  const int row_bytes = int(head_dim) * (format == SOL_CACHE_BF16 ? 2 : 1);
+  const int64_t threads = most <= sol::keep_small_rows(row_bytes) ? 64 : 1024;
+  if (sequences * heads * 2 * cdiv(row_bytes, 128) * threads >= (int64_t(1) << 32))
+    return fail(SOL_ERR_UNSUPPORTED, "sol_cache_keep: grid too large");
   p.kept = kept;
   p.most = int(most);
   p.store[0] = static_cast<uint8_t*>(cache_k);
@@ -1328,6 +1331,7 @@ int sol_cache_fork(const int32_t* page_table, const int32_t* context_lengths, co
   p.first = reinterpret_cast<int32_t*>(ws + size.first);
   p.children = reinterpret_cast<int32_t*>(ws + size.children);
   p.start = reinterpret_cast<int64_t*>(ws + size.start);
+  p.lost = reinterpret_cast<int32_t*>(ws + size.lost);
   p.free_count = reinterpret_cast<int32_t*>(ws + size.free_count);
   p.free_list = reinterpret_cast<int32_t*>(ws + size.free_list);
   return hip_status(sol::launch_fork(p, static_cast<hipStream_t>(stream)));

@@ -13,7 +13,8 @@
 // lies in, where the parent has rows before it, is copied.  A page is free if
 // no table named it before the call: pages that a call frees are taken from the
 // next call on, so that no page is read and written by one call, and everything
-// follows from the state before it.
+// follows from the state before it.  A begun page that the parent does not have
+// (none was free, then) its children do not have either.
 // Reference counts change by whole numbers, in any order.
 #include <algorithm>
 
@@ -104,8 +105,10 @@ __global__ __launch_bounds__(WAVES * kWave) void keep_kernel(KeepParams p) {
       to[u] = kStays;
       if (k != j && k >= 0 && k < n) {
         const uint32_t from = row_of(base + k);
-        to[u] = from != kStays ? row_of(base + j) : kStays;
-        if (to[u] != kStays) {
+        to[u] = row_of(base + j);
+        x[u] = zero_u32x4();  // what has no page reads as zeros
+        scale[u] = 0.f;
+        if (from != kStays && to[u] != kStays) {
           x[u] = *reinterpret_cast<const u32x4*>(store + uint64_t(from) * ROW);
           if (scales) scale[u] = p.scale[kv][from];
         }
@@ -131,6 +134,7 @@ template <int ROW>
 void keep_variant(const KeepParams& p, hipStream_t stream) {
   constexpr int kPieces = ROW > 128 ? ROW / 128 : 1, kRows = kWave * 16 * kPieces / ROW;  // of a wave's load
   const dim3 grid(unsigned(int64_t(p.batch.S) * p.H * 2 * kPieces));
+  static_assert(4 * kRows == keep_small_rows(ROW), "the C entry's check of the grid");
   if (p.most <= 4 * kRows)
     hipLaunchKernelGGL((keep_kernel<ROW, 1, 4>), grid, dim3(64), 0, stream, p);
   else
@@ -148,6 +152,7 @@ struct Child {
   int kept, after;      // tokens before and with the new ones
   int full, held, used; // whole pages shared; pages of the parent; pages needed (of the new table's width)
   bool first;           // the parent's first child
+  bool lost;            // page `full` is begun, and the parent does not have it
 };
 
 __device__ __forceinline__ int pages_of(int64_t tokens, int shift) {
@@ -158,6 +163,10 @@ __device__ __forceinline__ int pages_of(int64_t tokens, int shift) {
 __device__ __forceinline__ int length_of(const ForkParams& p, int s) { return max(p.lengths[s], 0); }
 __device__ __forceinline__ int kept_of(const ForkParams& p, int s) {
   return min(max(p.continued[s], 0), length_of(p, s));
+}
+
+__device__ __forceinline__ int page_of(const ForkParams& p, int s, int e) {
+  return p.table[int64_t(s) * p.width + e];
 }
 
 __device__ __forceinline__ Child child_of(const ForkParams& p, int i, int first) {
@@ -171,11 +180,12 @@ __device__ __forceinline__ Child child_of(const ForkParams& p, int i, int first)
   x.held = min(pages_of(length, p.page_shift), p.width);
   x.used = min(pages_of(x.after, p.page_shift), p.new_width);
   x.first = first == i;
+  x.lost = false;
+  if ((x.kept & ((1 << p.page_shift) - 1)) && x.full < x.used) {
+    const int page = x.full < x.held ? page_of(p, x.parent, x.full) : -1;
+    x.lost = page < 0 || page >= p.pages;
+  }
   return x;
-}
-
-__device__ __forceinline__ int page_of(const ForkParams& p, int s, int e) {
-  return p.table[int64_t(s) * p.width + e];
 }
 
 // Whether the first child goes on in its parent's page e (>= full, < held): no other table names it.
@@ -186,7 +196,7 @@ __device__ __forceinline__ bool goes_on(const ForkParams& p, int s, int e) {
 
 // How many of the child's pages [full, e) it takes.
 __device__ __forceinline__ int taken_before(const ForkParams& p, const Child& x, int e) {
-  int n = max(e - x.full, 0);
+  int n = max(e - x.full - (x.lost ? 1 : 0), 0);
   if (x.first)
     for (int i = x.full; i < min(e, x.held); ++i) n -= goes_on(p, x.parent, i) ? 1 : 0;
   return n;
@@ -242,7 +252,8 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(ForkParams p) {
     return;
   }
   __shared__ int64_t s_taken[kPlanWaves], s_tokens[kPlanWaves];
-  __shared__ int s_first[kHeldSequences], s_children[kHeldSequences];
+  __shared__ int s_first[kHeldSequences], s_children[kHeldSequences], s_lost;
+  if (tid == 0) s_lost = 0;
   // First children and numbers of children: in LDS, or, of more sequences, in
   // memory, where each of the two barriers waits for the card's caches.  (48 beams:
   // 10.6 us that way, 3.8 in LDS.)
@@ -287,6 +298,7 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(ForkParams p) {
       x = child_of(p, i, first_of(i));
       n = taken_before(p, x, x.used);
       a = x.after - x.kept;
+      if (x.lost) atomicAdd(&s_lost, 1);
     }
     int64_t n_end = wave_scan(n, lane), a_end = wave_scan(a, lane);
     if (lane == 63) s_taken[wave] = n_end, s_tokens[wave] = a_end;
@@ -306,6 +318,7 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(ForkParams p) {
   }
   if (tid == 0) {
     p.start[p.N] = taken;
+    *p.lost = s_lost;
     p.new_offsets[p.N] = int(min(tokens, int64_t(0x7FFFFFFF)));
     if (p.N == 0) *p.missing = 0;  // (otherwise sequence 0's workgroup writes it)
   }
@@ -384,7 +397,8 @@ __global__ __launch_bounds__(kForkThreads) void fork_kernel(ForkParams p, int pi
     const Child x = child_of(p, i, s >= 0 && s < p.S ? p.first[s] : -1);
     const FreePages free(p, s_ends);
     const int64_t start = p.start[i];
-    if (i == 0 && tid == 0) *p.missing = int(min(max(p.start[p.N] - free.total, int64_t(0)), int64_t(0x7FFFFFFF)));
+    if (i == 0 && tid == 0)
+      *p.missing = int(min(max(p.start[p.N] - free.total, int64_t(0)) + *p.lost, int64_t(0x7FFFFFFF)));
     for (int e = tid; e < p.new_width; e += kForkThreads) {
       int page = -1;
       if (e < x.used) {
@@ -392,7 +406,7 @@ __global__ __launch_bounds__(kForkThreads) void fork_kernel(ForkParams p, int pi
           if (e < p.width) page = page_of(p, x.parent, e);
         } else if (x.first && e < x.held && goes_on(p, x.parent, e)) {
           page = page_of(p, x.parent, e);
-        } else {
+        } else if (!x.lost || e > x.full) {
           page = free.page(p, start + taken_before(p, x, e));
           if (page >= 0) atomicAdd(p.new_refs + page, 1);
         }
@@ -408,10 +422,9 @@ __global__ __launch_bounds__(kForkThreads) void fork_kernel(ForkParams p, int pi
   if (s < 0 || s >= p.S) return;
   const Child x = child_of(p, i, p.first[s]);
   const int rows = x.kept & ((1 << p.page_shift) - 1);
-  if (rows == 0 || x.full >= x.used || x.full >= x.held || piece * int64_t(kCopyBytes) >= int64_t(rows) * p.row_bytes)
-    return;
+  if (rows == 0 || x.full >= x.used || x.lost || piece * int64_t(kCopyBytes) >= int64_t(rows) * p.row_bytes) return;
   const int from = page_of(p, s, x.full);
-  if (from < 0 || from >= p.pages || (x.first && p.refs[from] == 1)) return;
+  if (x.first && p.refs[from] == 1) return;
   const FreePages free(p, s_ends);
   const int to = free.page(p, p.start[i]);
   if (to < 0) return;
@@ -442,6 +455,7 @@ ForkSize fork_size(int64_t sequences, int64_t new_sequences, int64_t pages) {
   s.first = part(4 * sequences);
   s.children = part(4 * sequences);
   s.start = part(8 * (new_sequences + 1));
+  s.lost = part(4);
   s.free_count = part(4 * s.slices);
   s.free_list = part(4 * s.slices * s.slice_pages);
   s.bytes = at;

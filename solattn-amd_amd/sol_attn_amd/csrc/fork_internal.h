@@ -42,6 +42,7 @@ struct ForkParams {
   int32_t* first;            // [S] first child, N: none
   int32_t* children;         // [S]
   int64_t* start;            // [N + 1] pages taken before sequence i's
+  int32_t* lost;             // [1] begun pages that are not to be had
   int32_t* free_count;       // [slices]
   int32_t* free_list;        // [slices, slice_pages]: a slice's free pages in ascending order
 };
@@ -52,9 +53,13 @@ constexpr int kForkStep = 4096;
 // Byte offsets of the workspace's parts, 16-byte aligned, and its size.
 struct ForkSize {
   int64_t slices, slice_pages;
-  int64_t first, children, start, free_count, free_list, bytes;
+  int64_t first, children, start, lost, free_count, free_list, bytes;
 };
 ForkSize fork_size(int64_t sequences, int64_t new_sequences, int64_t pages);
+
+// Lists of at most this many entries are moved by workgroups of 64 threads, longer
+// ones by workgroups of 1,024, one or two (rows of 256 bytes) per head of K and of V.
+constexpr int keep_small_rows(int row_bytes) { return 4 * 1024 / (row_bytes < 128 ? row_bytes : 128); }
 
 hipError_t launch_keep(const KeepParams& p, int D, int format, hipStream_t stream);
 hipError_t launch_fork(const ForkParams& p, hipStream_t stream);

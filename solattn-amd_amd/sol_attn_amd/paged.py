@@ -370,7 +370,7 @@ def cache_keep(cache, plan, kept):
     not ascend or is not one of them (-1, say) ends the list.  The K and V rows
     of new token ``kept[s, j]`` (of position ``context_lengths[s] - new +
     kept[s, j]``) move to that of new token j, in place; rows behind the kept
-    ones stay as they are.  Stored values move as they are: keys that were
+    ones stay as they are, and a row that has no page moves as zeros.  Stored values move as they are: keys that were
     turned by their positions keep those (:func:`rotate_heads` turns a draft by
     its depth, which is its place once it is kept).
 
@@ -401,7 +401,8 @@ def cache_fork(cache, pool, plan, parents, new_tokens, *, lengths=None, width=No
     own, and a copy of the rows that the first one begins with.  Pages are taken
     from those that ``pool`` has free, the lowest first, and freed pages are
     free for the next call.  Where none is left a table has -1, which is no page
-    (not written, not attended), and ``missing`` of the new pool counts them.
+    (not written, not attended), for the children that go on in it too, and
+    ``missing`` of the new pool counts them.
 
     ``width``: pages that a new table has room for, by default the old one's.
     ``plan`` and ``pool`` stay as they were, but the sequences they describe must

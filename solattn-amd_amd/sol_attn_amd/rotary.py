@@ -90,6 +90,16 @@ def _same(x, y):
     return x.data_ptr() == y.data_ptr() and x.stride() == y.stride()
 
 
+def _meets_itself(x):
+    """Whether a tensor's elements may share memory among themselves."""
+    reach = 1
+    for stride, size in sorted((s, n) for s, n in zip(x.stride(), x.shape) if n > 1):
+        if stride < reach:
+            return True
+        reach = stride * (size - 1) + reach
+    return False
+
+
 def _check_out(inputs, outs):
     """Outputs are new memory, or their own inputs."""
     for i, (x, out) in enumerate(zip(inputs, outs)):
@@ -99,6 +109,8 @@ def _check_out(inputs, outs):
             raise ValueError("Inference only: out must not require gradients")
         if out.numel() and (min(out.stride()) <= 0 or out.stride(-1) != 1 or not _native._aligned(out)):
             raise ValueError("out needs positive strides, contiguous head dimension and 16-byte aligned rows")
+        if _meets_itself(out):
+            raise ValueError("out must not share memory with itself")
         if not _same(x, out) and _meet(x, out):
             raise ValueError("out must be Q and K themselves or share no memory with them")
         for j, other in enumerate(inputs):
@@ -154,6 +166,8 @@ def rotate_heads(q, k, positions, rotary, *, q_norm=None, k_norm=None, eps=1e-6,
             or not freq.numel() == axes.numel() == dim // 2 or not (freq.is_contiguous() and axes.is_contiguous())
             or rotary.layout not in LAYOUTS):
         raise ValueError("Invalid rotary descriptor; use RotaryAxes.create for this head dimension")
+    if freq.requires_grad:
+        raise ValueError("Inference only: frequencies must not require gradients")
     if alone and k_norm is not None:
         raise ValueError("k_norm needs K")
     device = q.get_device()

@@ -55,12 +55,13 @@ def keep_in_python(store, table, lengths, new, kept, page_size, pages):
         out.append(max(0, base + count))
         for j, x in enumerate(picks[:count]):
             a, b = base + x, base + j
-            if min(a, b) < 0 or max(a, b) // page_size >= len(row):
+            if min(a, b) < 0 or b // page_size >= len(row):
                 continue
+            row = row + [-1] * (a // page_size + 1)
             p, q = row[a // page_size], row[b // page_size]
-            if 0 <= p < pages and 0 <= q < pages:
+            if 0 <= q < pages and a != b:
                 for x2, y2 in zip(store, before):
-                    x2[q, :, b % page_size] = y2[p, :, a % page_size]
+                    x2[q, :, b % page_size] = y2[p, :, a % page_size] if 0 <= p < pages else 0
     return store, out
 
 
@@ -126,8 +127,16 @@ def test_keep_leaves_what_has_no_page():
     want = plain(cache)
     plan = PagedPlan(ints([[0, 1], [2, 3]]), ints([3, 100]), ints([0, 9, 15]))
     # 9 new tokens of 3: positions -6 .. 2; and 6 of a sequence whose last pages are not in the table.
+    # Token 7 of the first is position 1, which stays empty of it: token 1's place is before the sequence.
     assert cache_keep(cache, plan, ints([[0, 7], [1, 3]])).tolist() == [0, 96]
     assert_same(cache, want)
+    # The second's tokens 0 and 1 have a page, the others none: they move as zeros.
+    plan = PagedPlan(ints([[0, 1], [2, 3]]), ints([3, 36]), ints([0, 0, 6]))
+    assert cache_keep(cache, plan, ints([[-1, -1], [1, 3]])).tolist() == [3, 32]
+    for x, y in zip(plain(cache), want):
+        assert torch.equal(x[3, :, 14], y[3, :, 15]) and not x[3, :, 15].any()
+        x[3, :, 14:], y[3, :, 14:] = 0, 0
+        assert torch.equal(x, y)
 
 
 @pytest.mark.gpu
@@ -171,12 +180,16 @@ def fork_in_python(store, refs, table, lengths, parents, new, page_size, continu
         for e in range(min(-(-after // page_size), width)):
             old = table[p][e] if p >= 0 and e < old_width else -1
             alone = 0 <= old < pages and refs[old] == 1
+            begun = e == kept // page_size and kept % page_size
             if e < kept // page_size or (first and e < held[p] and alone):
                 page = old
+            elif begun and not (e < held[p] and 0 <= old < pages):
+                page = -1
+                missing += 1
             else:
                 page = free.pop(0) if free else -1
                 missing += page < 0
-                if e == kept // page_size and kept % page_size and p >= 0 and e < held[p] and 0 <= old < pages and page >= 0:
+                if begun and page >= 0:
                     for x, y in zip(store, before):
                         x[page, :, :kept % page_size] = y[old, :, :kept % page_size]
             row.append(page)
@@ -282,7 +295,8 @@ def test_pages_that_run_out():
     assert b.fork([0, 0, 1, -1], [30, 30, 1, 40]) > 0
     assert b.fork([0, 1, 2, 3], [20, 20, 20, 20]) > 0
     b.fork([2], [1])
-    assert b.fork([0, -1], [1, 30]) == 0
+    assert b.fork([0, -1], [1, 30]) == 1  # the page that the first one had begun without
+    assert b.fork([1, -1], [1, 30]) == 0
 
 
 @pytest.mark.gpu

@@ -172,6 +172,10 @@ def test_gpu_refusals():
             rotate_heads(q, k, positions, rotary, out=out)
     with pytest.raises(ValueError, match="share no memory"):
         rotate_heads(wide[:6], None, positions, rotary, out=wide[1:])
+    rolling = torch.as_strided(wide, (6, 4, 128), (128, 128, 1))  # rows that tokens have in common
+    with pytest.raises(ValueError, match="with itself"):
+        rotate_heads(rolling, None, positions, rotary, out=rolling)
+    check(rotate_heads(rolling, None, positions, rotary), rolling, positions, rotary)
     with pytest.raises(ValueError, match="16-byte aligned"):
         rotate_heads(q, None, positions, rotary,
                      out=torch.empty(6 * 4 * 128 + 1, dtype=torch.bfloat16, device="cuda")[1:].view(6, 4, 128))
@@ -202,6 +206,8 @@ def call(**change):
     (dict(rotary=None), "RotaryAxes"), (dict(rotary=RotaryAxes.create(128, 64, device="cpu")), "Invalid rotary"),
     (dict(rotary=RotaryAxes(torch.zeros(32), torch.zeros(32, dtype=torch.int32))), "Invalid rotary"),
     (dict(rotary=RotaryAxes(torch.zeros(32, dtype=torch.float64), torch.zeros(32, dtype=torch.int32), "thirds")), "Invalid"),
+    (dict(rotary=RotaryAxes(torch.zeros(32, dtype=torch.float64, requires_grad=True), torch.zeros(32, dtype=torch.int32))),
+     "Inference only"),
     (dict(q_norm=torch.ones(32)), "Norm weights"), (dict(k_norm=torch.ones(64, dtype=torch.float16)), "Norm weights"),
     (dict(q_norm=torch.ones(64), k_norm=torch.ones(64, dtype=torch.bfloat16)), "one type"),
     (dict(q_norm=torch.ones(64, requires_grad=True)), "Inference only"), (dict(k=None, k_norm=torch.ones(64)), "needs K"),
