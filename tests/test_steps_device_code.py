@@ -1,5 +1,5 @@
 """Checks on the gfx950 device code of the rotation and of the cache's steps (CPU only): none of the packed FP32 forms
-that the build keeps out, and no memory of their own per lane."""
+that the build keeps out, and no memory of their own per lane (the compiler may hold a lane's arrays in LDS)."""
 
 import os
 import re
@@ -22,3 +22,5 @@ def test_no_packed_fp32_and_no_scratch(source, tmp_path):
     text = out.read_text()
     assert not re.search(r"\bv_pk_(add|mul|fma)_f32\b", text)
     assert not re.search(r"^\s+scratch_(load|store)", text, re.M)
+    if source == "rotate.hip":
+        assert set(re.findall(r"amdhsa_group_segment_fixed_size (\d+)", text)) == {"0"}
