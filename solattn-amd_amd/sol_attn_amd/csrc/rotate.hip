@@ -11,12 +11,12 @@
 // error of 2^-22, where FP32 would leave hundreds of turns.
 //
 // Bound by memory: every row is read and written once.  84,672 tokens of 24 + 24
-// heads of 128, norms and three axes, 2.08 GB: 427 us, 4.87 TB/s, as a copy of 4
-// GiB (4.83).  19,003 tokens of 12 + 3 heads of 64, 73 MB: 16.8 us, 4.3 TB/s.  A
-// decoding step of 48 tokens of 24 + 8 heads is a chain of latencies, 7 us, less
-// than the 12 that the host takes to make the call.  (The angles' arithmetic is
-// not what bounds it: sines of four multiply-adds each instead of the library's
-// took 0 to 3% off.)
+// heads of 128, norms and three axes, 2.08 GB: 389 us, 5.35 TB/s (a copy of 4 GiB
+// 4.83).  19,003 tokens of 12 + 3 heads of 64, 73 MB: 15.8 us, 4.6 TB/s.  A decoding
+// step of 48 tokens of 24 + 8 heads is a chain of latencies, 5.7 us, less than the
+// 12 that the host takes to make the call.  (The angles' arithmetic is not what
+// bounds it: sines of four multiply-adds each instead of the library's took 0 to 3%
+// off.)
 #include "rotate_internal.h"
 #include "sol_device.h"
 
@@ -226,13 +226,12 @@ template <int D, bool PAIRS>
 void rotate_variant(const RotateParams& p, hipStream_t stream) {
   const int64_t groups = (p.rows + kRotateTokens<D> - 1) / kRotateTokens<D>;
   const int heads = p.x[0].heads + p.x[1].heads;
-  // Four heads to a wave, eight where that still makes some 2,000 waves, more from
-  // 16,384 on: a wave has the angles to form first, and a card of 8,192 waves enough
-  // of them without.  Four and eight: 19,003 tokens of 12 + 3 heads of 64 19.8 and
-  // 16.8 us, of 128 37 and 33, 4,032 of 24 + 24 30 and 24; 19,003 of 24 + 24, 28,512
-  // waves of four, 107 with eight and 111 with sixteen.
-  int each = 4;
-  while (each < heads && groups * ((heads + each - 1) / each) > (each < 8 ? 4096 : 16384)) each *= 2;
+  // Four heads to a wave, eight where that makes 2,000 waves and more: a wave has the
+  // angles to form first, and neighbouring waves of few heads read neighbouring rows.
+  // Four and eight: 4,032 tokens of 24 + 24 heads of 128 22.1 and 20.1 us, 40,000 of 8
+  // + 1 40.1 and 37.9, 2,000 of 32 + 8 (2,500 waves of four) 12.5 and 13.3; eight
+  // and sixteen: 84,672 of 24 + 24 389 and 403.
+  const int each = groups * ((heads + 3) / 4) > 4096 ? 8 : 4;
   const int64_t units = groups * ((heads + each - 1) / each);
   hipLaunchKernelGGL((rotate_kernel<D, PAIRS>), dim3(unsigned((units + 3) / 4)), dim3(kRotateThreads), 0, stream, p,
                      each);
