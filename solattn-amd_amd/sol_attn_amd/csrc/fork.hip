@@ -70,9 +70,10 @@ __device__ __forceinline__ int kept_count(const int32_t* kept, int most, int64_t
 // ascending order, so that a row is read before another takes its place: a batch
 // of rows is read whole before it is written, and the batches follow one another.
 // So the time is that of a batch's chain of reads (the list, the table, the rows),
-// and the workgroups are large: two frames of 4,032 tokens, thinned to some 1,500
-// and 600, 24 heads of 128, BF16, 18 MB: 11 us (15.6 with batches of 512 whole rows);
-// 48 sequences' paths of up to 13 INT8 drafts, 8 heads: 4 us.
+// and the workgroups are large: two frames of 4,032 tokens, thinned to 927 and 23, 24
+// heads of 128, BF16, 18 MB: 9.3 us (15.6 with whole rows, 512 to a batch, and a wait
+// for each row's entry, page and bytes); 48 sequences' paths of up to 13 INT8 drafts,
+// 8 heads: 3.9 us.
 template <int ROW, int WAVES, int U>
 __global__ __launch_bounds__(WAVES * kWave) void keep_kernel(KeepParams p) {
   constexpr int NT = WAVES * kWave, kPiece = ROW < 128 ? ROW : 128, kPieces = ROW / kPiece;
@@ -83,49 +84,58 @@ __global__ __launch_bounds__(WAVES * kWave) void keep_kernel(KeepParams p) {
   const int kv = unit & 1, h = (unit >> 1) % p.H, s = (unit >> 1) / p.H;
   const int64_t n = int64_t(bt.offsets[s + 1]) - bt.offsets[s], base = int64_t(bt.lengths[s]) - max(n, int64_t(0));
   const int32_t* kept = p.kept + int64_t(s) * p.most;
-  // Row of the cache at position `at` (a cache of 2^32 rows does not fit the card), kStays: none.
-  auto row_of = [&](int64_t at) -> uint32_t {
-    if (at < 0 || at >= bt.positions()) return kStays;
-    const int page = bt.table[int64_t(s) * bt.width + (at >> bt.page_shift)];
-    if (page < 0 || page >= bt.pages) return kStays;
-    return uint32_t((uint64_t(uint32_t(page)) * p.H + h) << bt.page_shift) + uint32_t(at & ((1 << bt.page_shift) - 1));
-  };
   const int c = threadIdx.x % kLanes;
   uint8_t* store = p.store[kv] + kPiece * piece + 16 * c;
   const bool scales = p.scale[kv] && piece == 0 && c == 0;
+  const int32_t* table = bt.table + int64_t(s) * bt.width;
+  // Row of the cache at position `at`, whose page number is `page` (a cache of 2^32
+  // rows does not fit the card), kStays: none.
+  auto page_at = [&](int64_t at) { return table[min(max(at >> bt.page_shift, int64_t(0)), int64_t(bt.width - 1))]; };
+  auto row_of = [&](int64_t at, int page) -> uint32_t {
+    if (at < 0 || at >= bt.positions() || page < 0 || page >= bt.pages) return kStays;
+    return uint32_t((uint64_t(uint32_t(page)) * p.H + h) << bt.page_shift) + uint32_t(at & ((1 << bt.page_shift) - 1));
+  };
+  const bool speaks = unit == 2 * p.H * s && piece == 0 && threadIdx.x == 0;  // for the sequence
+  if (p.most == 0 && speaks) p.lengths_out[s] = int(max(base, int64_t(0)));
   int count = p.most;  // known once the first batch is on its way
-  for (int j0 = 0; j0 < count || j0 == 0; j0 += U * kRows) {
+  for (int j0 = 0; j0 < count; j0 += U * kRows) {
+    // Of all rows the list's entries, then their pages, then the rows, without a
+    // branch in between, so that each is one wait.
+    const int first = j0 + int(threadIdx.x) / kLanes;
     u32x4 x[U];
     float scale[U];
-    uint32_t to[U];
+    uint32_t to[U], from[U];
+    int k[U], pages[U][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u) k[u] = kept[min(first + u * kRows, p.most - 1)];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int j = j0 + u * kRows + int(threadIdx.x) / kLanes;
-      const int k = j < count ? kept[j] : j;
-      to[u] = kStays;
-      if (k != j && k >= 0 && k < n) {
-        const uint32_t from = row_of(base + k);
-        to[u] = row_of(base + j);
-        x[u] = zero_u32x4();  // what has no page reads as zeros
-        scale[u] = 0.f;
-        if (from != kStays && to[u] != kStays) {
-          x[u] = *reinterpret_cast<const u32x4*>(store + uint64_t(from) * ROW);
-          if (scales) scale[u] = p.scale[kv][from];
-        }
-      }
+      pages[u][0] = page_at(base + k[u]);
+      pages[u][1] = page_at(base + first + u * kRows);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = first + u * kRows;
+      const bool moves = j < count && k[u] != j && k[u] >= 0 && k[u] < n;
+      from[u] = moves ? row_of(base + k[u], pages[u][0]) : kStays;
+      to[u] = moves ? row_of(base + j, pages[u][1]) : kStays;
+      const uint64_t at = from[u] == kStays ? 0 : from[u];
+      x[u] = *reinterpret_cast<const u32x4*>(store + at * ROW);
+      scale[u] = scales ? p.scale[kv][at] : 0.f;
     }
     if (j0 == 0) {
       count = kept_count<NT>(kept, p.most, n);
-      if (unit == 2 * p.H * s && piece == 0 && threadIdx.x == 0) p.lengths_out[s] = int(max(base + count, int64_t(0)));
+      if (speaks) p.lengths_out[s] = int(max(base + count, int64_t(0)));
     }
     // Every read of the batch has returned before anything is written.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     if constexpr (WAVES > 1) __syncthreads();
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (to[u] != kStays && j0 + u * kRows + int(threadIdx.x) / kLanes < count) {
-        *reinterpret_cast<u32x4*>(store + uint64_t(to[u]) * ROW) = x[u];
-        if (scales) p.scale[kv][to[u]] = scale[u];
+      if (to[u] != kStays && first + u * kRows < count) {
+        const bool none = from[u] == kStays;  // what has no page reads as zeros
+        *reinterpret_cast<u32x4*>(store + uint64_t(to[u]) * ROW) = none ? zero_u32x4() : x[u];
+        if (scales) p.scale[kv][to[u]] = none ? 0.f : scale[u];
       }
   }
 }
@@ -138,7 +148,7 @@ void keep_variant(const KeepParams& p, hipStream_t stream) {
   if (p.most <= 4 * kRows)
     hipLaunchKernelGGL((keep_kernel<ROW, 1, 4>), grid, dim3(64), 0, stream, p);
   else
-    hipLaunchKernelGGL((keep_kernel<ROW, 16, 12>), grid, dim3(1024), 0, stream, p);
+    hipLaunchKernelGGL((keep_kernel<ROW, 16, 8>), grid, dim3(1024), 0, stream, p);
 }
 
 // ---- forks ------------------------------------------------------------------
@@ -432,9 +442,16 @@ __global__ __launch_bounds__(kForkThreads) void fork_kernel(ForkParams p, int pi
   const int64_t a = int64_t(piece) * kCopyBytes, b = min(a + kCopyBytes, int64_t(rows) * p.row_bytes);
   const uint8_t* in = p.store[kv] + source * p.row_bytes;
   uint8_t* out = p.store[kv] + target * p.row_bytes;
-#pragma unroll 4
-  for (int64_t at = a + 16 * tid; at < b; at += 16 * kForkThreads)
-    *reinterpret_cast<u32x4*>(out + at) = *reinterpret_cast<const u32x4*>(in + at);
+  constexpr int kAtOnce = 4;
+  for (int64_t at = a + 16 * tid; at < b; at += kAtOnce * 16 * kForkThreads) {
+    u32x4 x[kAtOnce];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k)
+      x[k] = *reinterpret_cast<const u32x4*>(in + min(at + k * 16 * kForkThreads, b - 16));
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k)
+      if (at + k * 16 * kForkThreads < b) *reinterpret_cast<u32x4*>(out + at + k * 16 * kForkThreads) = x[k];
+  }
   if (p.scale[kv] && piece == 0)
     for (int r = tid; r < rows; r += kForkThreads) p.scale[kv][target + r] = p.scale[kv][source + r];
 }
