@@ -358,6 +358,20 @@ __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item
   return true;
 }
 
+// The first of a span's tiles that part `part` takes.  Tiles with nodes of a tree are
+// masked one by one and not pipelined: they count twice.  (Six trees of up to 701 nodes
+// behind 8,191 fp8 tokens under a window of 4,096, and the same as chains: 88 and 108 us
+// in even parts, 82 and 102 with such tiles counted one and a half times, 80 and 98 at
+// twice and at three times.)
+template <int TK, bool TREE>
+__device__ __forceinline__ int part_begin(const Span& span, const Item& it, int part) {
+  if constexpr (!TREE) return int(int64_t(part) * span.n / it.parts);
+  const int q = max(it.pos0, 0) / TK;  // the first tile with a node
+  const int before = min(span.ns, q) + min(max(q - span.w0, 0), span.n - span.ns);
+  const int64_t x = int64_t(part) * (int64_t(span.n) + (span.n - before)) / it.parts;
+  return int(x < before ? x : before + (x - before) / 2);
+}
+
 // ---- where the keys lie -----------------------------------------------------
 
 // Key tiles are cut into groups of 16 rows, each of which lies in one page (a
@@ -1878,7 +1892,7 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
   LaneRow row;
 
   const Span span = span_of<TK>(p, pos0 + (TREE ? 0 : it.r0 / p.G), pos0 + (it.r0 + it.rows - 1) / p.G, it.length);
-  const int t0 = int(int64_t(it.part) * span.n / it.parts), t1 = int(int64_t(it.part + 1) * span.n / it.parts);
+  const int t0 = part_begin<TK, TREE>(span, it, it.part), t1 = part_begin<TK, TREE>(span, it, it.part + 1);
   const Bounds bounds =
       begin_rows<TREE>(p, it, t0 < t1 && (span.tile(t1 - 1) + 1) * TK > pos0, row, token, (it.r0 + 32 * block) / p.G,
                        (it.r0 + 32 * block + max(wrows, 1) - 1) / p.G);
