@@ -154,6 +154,7 @@ void keep_variant(const KeepParams& p, hipStream_t stream) {
 // ---- forks ------------------------------------------------------------------
 
 constexpr int kPlanThreads = 1024;
+constexpr int kFewPages = 32;         // that one thread looks up
 constexpr int kHeldSequences = 4096;  // old ones whose children a workgroup counts in LDS
 
 // What a new sequence takes over from its parent.
@@ -204,12 +205,12 @@ __device__ __forceinline__ bool goes_on(const ForkParams& p, int s, int e) {
   return page >= 0 && page < p.pages && p.refs[page] == 1;
 }
 
-// How many of the child's pages [full, e) it takes.
-__device__ __forceinline__ int taken_before(const ForkParams& p, const Child& x, int e) {
-  int n = max(e - x.full - (x.lost ? 1 : 0), 0);
-  if (x.first)
-    for (int i = x.full; i < min(e, x.held); ++i) n -= goes_on(p, x.parent, i) ? 1 : 0;
-  return n;
+// Up to which of its parent's pages the child may go on (from `full`).
+__device__ __forceinline__ int goes_until(const Child& x) { return x.first ? min(x.used, x.held) : x.full; }
+
+// How many of its pages [full, e) the child takes, of which it goes on in `going`.
+__device__ __forceinline__ int taken_before(const Child& x, int e, int going) {
+  return max(e - x.full - (x.lost ? 1 : 0), 0) - going;
 }
 
 template <typename T>
@@ -226,7 +227,7 @@ __device__ __forceinline__ T wave_scan(T x, int lane) {
 // of pages.  The others: a slice of the pool each, whose counts they copy and
 // whose free pages they list.
 __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(ForkParams p) {
-  constexpr int kPlanWaves = kPlanThreads / kWave;
+  constexpr int kPlanWaves = kPlanThreads / kWave, kAtOnce = 4;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if (blockIdx.x > 0) {
     __shared__ int s_count[kPlanWaves];
@@ -304,9 +305,31 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(ForkParams p) {
     const int i = i0 + tid;
     int64_t n = 0, a = 0;
     Child x = {};
+    int going = 0;
     if (i < p.N) {
       x = child_of(p, i, first_of(i));
-      n = taken_before(p, x, x.used);
+      if (goes_until(x) - x.full <= kFewPages)
+        for (int e = x.full; e < goes_until(x); e += kAtOnce) {
+          int page[kAtOnce], refs[kAtOnce];  // without a branch, so that each is one wait
+#pragma unroll
+          for (int k = 0; k < kAtOnce; ++k) page[k] = page_of(p, x.parent, min(e + k, goes_until(x) - 1));
+#pragma unroll
+          for (int k = 0; k < kAtOnce; ++k) refs[k] = p.refs[min(max(page[k], 0), p.pages - 1)];
+#pragma unroll
+          for (int k = 0; k < kAtOnce; ++k)
+            going += e + k < goes_until(x) && page[k] >= 0 && page[k] < p.pages && refs[k] == 1;
+        }
+    }
+    // Sequences that go back far: the wave counts their pages together.
+    for (uint64_t far = __builtin_amdgcn_ballot_w64(goes_until(x) - x.full > kFewPages); far; far &= far - 1) {
+      const int of = __builtin_ctzll(far), s = __shfl(x.parent, of), end = __shfl(goes_until(x), of);
+      int found = 0;
+      for (int e0 = __shfl(x.full, of); e0 < end; e0 += kWave)
+        found += __builtin_popcountll(__builtin_amdgcn_ballot_w64(e0 + lane < end && goes_on(p, s, e0 + lane)));
+      if (lane == of) going = found;
+    }
+    if (i < p.N) {
+      n = taken_before(x, x.used, going);
       a = x.after - x.kept;
       if (x.lost) atomicAdd(&s_lost, 1);
     }
@@ -409,15 +432,34 @@ __global__ __launch_bounds__(kForkThreads) void fork_kernel(ForkParams p, int pi
     const int64_t start = p.start[i];
     if (i == 0 && tid == 0)
       *p.missing = int(min(max(p.start[p.N] - free.total, int64_t(0)) + *p.lost, int64_t(0x7FFFFFFF)));
-    for (int e = tid; e < p.new_width; e += kForkThreads) {
+    const int end = goes_until(x);
+    __shared__ int s_going[kForkWaves];
+    int going = 0;  // pages below e0 that the child goes on in
+    for (int e0 = 0; e0 < p.new_width; e0 += kForkThreads) {
+      const int e = e0 + tid;
+      const bool goes = e >= x.full && e < end && goes_on(p, x.parent, e);
+      int before = going;  // pages below e
+      if (e0 < end && e0 + kForkThreads > x.full) {
+        const uint64_t lanes = __builtin_amdgcn_ballot_w64(goes);
+        if ((tid & 63) == 0) s_going[tid >> 6] = __builtin_popcountll(lanes);
+        __syncthreads();
+        before += __builtin_popcountll(lanes & ((uint64_t(1) << (tid & 63)) - 1));
+#pragma unroll
+        for (int w = 0; w < kForkWaves; ++w) {
+          before += w < tid >> 6 ? s_going[w] : 0;
+          going += s_going[w];
+        }
+        __syncthreads();
+      }
+      if (e >= p.new_width) continue;
       int page = -1;
       if (e < x.used) {
         if (e < x.full) {
           if (e < p.width) page = page_of(p, x.parent, e);
-        } else if (x.first && e < x.held && goes_on(p, x.parent, e)) {
+        } else if (goes) {
           page = page_of(p, x.parent, e);
         } else if (!x.lost || e > x.full) {
-          page = free.page(p, start + taken_before(p, x, e));
+          page = free.page(p, start + taken_before(x, e, before));
           if (page >= 0) atomicAdd(p.new_refs + page, 1);
         }
       }

@@ -290,6 +290,16 @@ def test_sequences_continued_from_a_part_of_their_tokens():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shared", [0, 33])
+def test_long_sequences_that_go_back_far(shared):
+    # Hundreds of the first children's pages lie behind what is kept, and some of them are other sequences' too.
+    b = Batch([16 * 1400 + 3, 16 * 700, 16 * 650 + 9, 16 * 620, 16 * 33 + 1], width=1500, spare=1500, shared=shared)
+    b.fork([0, 0, 1, 2, 2, 3, 4], [16 * 300, 5, 16 * 500, 1, 0, 7, 16 * 40], continued=[16 * 200 + 7, 16 * 600, 3, 0, 1])
+    b.fork([0, 2, 0, 2, 6], [16 * 900, 16 * 450, 16 * 20, 1, 300], continued=[16 * 400, 0, 16 * 400 + 1, 0, 0, 0, 2])
+    b.fork([1, 0, 3, 0], [16 * 1000, 16 * 1200, 0, 1], continued=[5, 16 * 20 + 2, 0, 0, 0])
+
+
+@pytest.mark.gpu
 def test_pages_that_run_out():
     b = Batch([40, 35], spare=3, width=9)
     assert b.fork([0, 0, 1, -1], [30, 30, 1, 40]) > 0
