@@ -79,6 +79,14 @@ def test_large_trees(window, sinks, fmt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fmt", ["bf16", "int8", "fp8"])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (150, 80), (900, 2000)])
+def test_parts_that_begin_and_end_among_the_nodes(window, sinks, fmt):
+    run([2300, 1500, 17 + 300], [700, 650, 300], ["chain", "odd", "any"], window=window, sinks=sinks, heads=2, group=2,
+        fmt=fmt, dim=128, page_size=32, seed=4)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kind", ["chain", "any", "star"])
 def test_trees_of_more_nodes_than_a_workgroup_holds(kind):
     run([1300, 1110], [1200, 1030], [kind, "level"], heads=1, seed=9)
