@@ -224,7 +224,7 @@ __device__ __forceinline__ bool take_item(const PagedParams& p, int64_t id, Item
     sum = int64_t(uniform64(uint64_t(sum)));
     z = part_tiles(p, sum);
     __syncthreads();
-    if constexpr (TREE && R == 128) {
+    if (TREE && R == 128 && p.rounds == 2) {
       // Rounded up, the parts may be a few more than run at once (p.target is two
       // rounds of them), and those few would run for as long as all the others:
       // parts up to a quarter longer that make one round, or else two rounds.
@@ -2178,6 +2178,7 @@ PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t tile
   // Row tiles that differ in their keys: other sequences, or the rows of a triangle.
   const bool uneven = (ragged && sequences > 1) || (causal && 2 * rows > keys * sequences);
   s.target = 0;
+  s.rounds = 1;
   if (step) {
     // A second launch costs 5 us, as much as 16 queries over 48 BF16 key tiles or
     // 20 of codes take alone (16 sequences, 4 heads: 1,024 BF16 keys 13.6 us whole,
@@ -2190,8 +2191,12 @@ PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t tile
     const int64_t rounds = ragged && 2 * sequences * heads >= kResident ? 2 : 1;
     if (key_tiles > (format == kBf16 ? 48 : 20)) s.target = (rounds * kResident + heads - 1) / heads;
   } else if (tree && likely * heads <= kResident) {
-    s.min_tiles = 6;  // take_item makes one or two rounds of parts
-    if (key_tiles > s.min_tiles) s.target = 2 * (kResident / heads);
+    // One or two rounds of parts, as take_item finds; none where few tiles would
+    // be cut.  (8 trees of 130 nodes of 8 x 4 heads behind 500 tokens: 41 us, 63
+    // in parts; 64 of up to 16 behind up to 9,000 INT8 tokens: 219, 154 in parts.)
+    s.min_tiles = 6;
+    if (wide_target(likely, heads, key_tiles, s.min_tiles) || (ragged && sequences > 1 && key_tiles > 48))
+      s.target = 2 * (kResident / heads), s.rounds = 2;
   } else if (uneven && 2 * likely * heads * key_tiles >= 3 * kResident * 24) {
     // Enough keys for one and a half rounds of parts of 24 tiles: those even the
     // lengths out (8 sequences of 600 .. 12,000 keys, 512 new tokens of 8 x 4
@@ -2219,6 +2224,7 @@ hipError_t launch_paged(const PagedParams& params, const PagedSize& size, int D,
   PagedParams p = params;
   p.target = int(size.target);
   p.min_tiles = int(size.min_tiles);
+  p.rounds = int(size.rounds);
   p.headers = size.headers;
   p.records = size.records;
   p.header_bytes = size.header_bytes;

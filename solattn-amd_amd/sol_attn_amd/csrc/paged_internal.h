@@ -63,6 +63,7 @@ struct PagedParams {
   const int32_t* parents;     // a tree of new tokens: each row's parent among its sequence's; or null
   // Keys split over workgroups (take_item in paged.hip); target 0: not split.
   int target, min_tiles;      // workgroups per head; key tiles of a part at least
+  int rounds;                 // 2: `target` is two rounds of them, of which take_item may make one
   int64_t headers, records;   // PagedSize's
   int64_t header_bytes, new_rows;
   void* workspace;            // PagedSize::bytes: headers, then records
@@ -72,7 +73,7 @@ struct PagedParams {
 struct PagedSize {
   int64_t rows;               // of a row tile: 16 (step_kernel) or 128 (wide_kernel)
   int64_t tiles;              // row tiles at most
-  int64_t target, min_tiles;
+  int64_t target, min_tiles, rounds;
   int64_t grid;               // workgroups
   int64_t headers;            // split row tiles per head at most, 0 without target
   int64_t records;            // their parts over all heads at most
