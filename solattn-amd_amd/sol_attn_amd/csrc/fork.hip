@@ -71,9 +71,9 @@ __device__ __forceinline__ int kept_count(const int32_t* kept, int most, int64_t
 // of rows is read whole before it is written, and the batches follow one another.
 // So the time is that of a batch's chain of reads (the list, the table, the rows),
 // and the workgroups are large: two frames of 4,032 tokens, thinned to 927 and 23, 24
-// heads of 128, BF16, 18 MB: 9.3 us (15.6 with whole rows, 512 to a batch, and a wait
+// heads of 128, BF16, 18 MB: 9.0 us (15.6 with whole rows, 512 to a batch, and a wait
 // for each row's entry, page and bytes); 48 sequences' paths of up to 13 INT8 drafts,
-// 8 heads: 3.9 us.
+// 8 heads: 3.7 us.
 template <int ROW, int WAVES, int U>
 __global__ __launch_bounds__(WAVES * kWave) void keep_kernel(KeepParams p) {
   constexpr int NT = WAVES * kWave, kPiece = ROW < 128 ? ROW : 128, kPieces = ROW / kPiece;

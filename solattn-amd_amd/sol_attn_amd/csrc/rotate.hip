@@ -12,8 +12,8 @@
 //
 // Bound by memory: every row is read and written once.  84,672 tokens of 24 + 24
 // heads of 128, norms and three axes, 2.08 GB: 389 us, 5.35 TB/s (a copy of 4 GiB
-// 4.83).  19,003 tokens of 12 + 3 heads of 64, 73 MB: 15.8 us, 4.6 TB/s.  A decoding
-// step of 48 tokens of 24 + 8 heads is a chain of latencies, 5.7 us, less than the
+// 4.83).  19,003 tokens of 12 + 3 heads of 64, 73 MB: 14.8 us, 4.9 TB/s.  A decoding
+// step of 48 tokens of 24 + 8 heads is a chain of latencies, 5.9 us, less than the
 // 12 that the host takes to make the call.  (The angles' arithmetic is not what
 // bounds it: sines of four multiply-adds each instead of the library's took 0 to 3%
 // off.)
