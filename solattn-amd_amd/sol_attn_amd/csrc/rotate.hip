@@ -165,7 +165,7 @@ __global__ __launch_bounds__(kRotateThreads) void rotate_kernel(RotateParams p, 
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const bool still = axis[i] < 0 || axis[i] >= p.axes;
-    const double turns = double(still ? 0 : position[i]) * frequency[i] * 0.15915494309189533577;
+    const double turns = still ? 0. : double(position[i]) * frequency[i] * 0.15915494309189533577;
     float s, c1;
     sincospif(2.f * float(turns - rint(turns)), &s, &c1);
     sn[i] = s, cs[i] = c1;

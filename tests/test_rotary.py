@@ -84,6 +84,9 @@ def test_misaligned_rows_and_pairs_without_an_axis():
     # An axis that the positions do not have turns nothing.
     odd = RotaryAxes(rotary.frequencies, torch.full_like(rotary.axes, 2), "halves")
     assert torch.equal(rotate_heads(q, None, positions, odd), q)
+    # Whatever its frequency.
+    odd = RotaryAxes(torch.full_like(rotary.frequencies, float("inf")), odd.axes, "pairs")
+    assert torch.equal(rotate_heads(q, None, positions, odd), q)
 
 
 @pytest.mark.gpu
