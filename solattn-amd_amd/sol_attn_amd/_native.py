@@ -905,9 +905,10 @@ def launch_cache_fork(cache, refs, plan, parents, new_tokens, lengths, width):
     size = _fork_size(s, n, pages)
     if size < 0:
         raise RuntimeError("the workspace size function rejected the sizes")
-    # One allocation for the workspace (a multiple of 16 bytes) and the results.
+    # One allocation for the workspace (a multiple of 16 bytes) and the results.  ("Unsafe" for gradients alone; split
+    # and its views took 2 of the call's 22 us on the host.)
     ws, table, new_lengths, offsets, new_refs, missing = torch.empty(
-        size // 4 + n * width + 2 * n + 2 + pages, device=dev, dtype=torch.int32).split(
+        size // 4 + n * width + 2 * n + 2 + pages, device=dev, dtype=torch.int32).unsafe_split_with_sizes(
         (size // 4, n * width, n, n + 1, pages, 1))
     old_table, old_lengths, _ = _plan_args(plan)
     _check(library().sol_cache_fork(
