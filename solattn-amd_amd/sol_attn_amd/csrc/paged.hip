@@ -879,7 +879,8 @@ __device__ __forceinline__ void store4(uint16_t* out, const f32x4& x, float den,
 // rows.  D / 4 lanes take 4 features each.  Tiles of 16 rows have many parts
 // and few rows: a row at a time, the 1,024 / D such groups of lanes take the
 // parts in turn, kMergeAhead each in flight, and their states join in a fixed
-// order.  Tiles of 128 rows have few parts: each group takes a row of its own.
+// order (!ROWS).  Tiles of 128 rows have few parts, or else PagedSize::many_parts:
+// each group takes a row of its own (ROWS).
 // Bound by its launch (5 us with its reads' latency) or by memory: two parts of
 // 4,032 rows of 24 heads of 128, 129 MB, 43 us after the attention, 3.0 TB/s (148
 // us a row at a time).
@@ -924,10 +925,10 @@ __device__ __forceinline__ Joined join_parts(const float* row, int64_t step, int
 }
 
 // Rows that a workgroup of the merge takes at once.
-template <int D, int R>
-constexpr int kMergeRows = R == 16 ? 1 : kNT / (D / 4);
+template <int D, bool ROWS>
+constexpr int kMergeRows = ROWS ? kNT / (D / 4) : 1;
 
-template <int D, int R>
+template <int D, int R, bool ROWS>
 __global__ __launch_bounds__(kNT) void merge_kernel(PagedParams p) {
   constexpr int kLanes = D / 4, kSlots = kNT / kLanes;
   __shared__ Joined s_state[kWaves][kLanes];
@@ -945,7 +946,7 @@ __global__ __launch_bounds__(kNT) void merge_kernel(PagedParams p) {
   auto store = [&](int r, const Joined& x) {
     store4(p.out + output_row<D>(p, hd.off, hd.r0 + r, h) + 4 * c, x.o, x.den, x.any != 0.f);
   };
-  if constexpr (kMergeRows<D, R> > 1) {
+  if constexpr (ROWS) {
     for (int r = blockIdx.y * kSlots + slot; r < hd.rows; r += gridDim.y * kSlots)
       store(r, join_parts<D>(base + r * kRecordRow<D>, step, hd.parts, 0, 1, c));
   } else {
@@ -2097,10 +2098,10 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
 
 // ---- launches ---------------------------------------------------------------
 
-template <int D, int R>
+template <int D, int R, bool ROWS>
 void launch_merge(const PagedParams& p, const PagedSize& size, hipStream_t stream) {
-  const unsigned rows = unsigned((size.merge_rows - 1) / kMergeRows<D, R> + 1);
-  hipLaunchKernelGGL((merge_kernel<D, R>), dim3(unsigned(p.headers * p.H), rows), dim3(kNT), 0, stream, p);
+  const unsigned rows = unsigned((size.merge_rows - 1) / kMergeRows<D, ROWS> + 1);
+  hipLaunchKernelGGL((merge_kernel<D, R, ROWS>), dim3(unsigned(p.headers * p.H), rows), dim3(kNT), 0, stream, p);
 }
 
 template <int D, int F, bool PAGED, bool TREE = false>
@@ -2108,10 +2109,13 @@ void launch_variant(const PagedParams& p, const PagedSize& size, hipStream_t str
   const dim3 grid(unsigned(size.grid)), block(kNT);
   if (size.rows == 16) {
     hipLaunchKernelGGL((step_kernel<D, F, PAGED, TREE>), grid, block, 0, stream, p);
-    if (p.records) launch_merge<D, 16>(p, size, stream);
+    if (p.records) launch_merge<D, 16, false>(p, size, stream);
   } else {
     hipLaunchKernelGGL((wide_kernel<D, F, PAGED, TREE>), grid, block, 0, stream, p);
-    if (p.records) launch_merge<D, 128>(p, size, stream);
+    if (p.records && size.many_parts)
+      launch_merge<D, 128, false>(p, size, stream);
+    else if (p.records)
+      launch_merge<D, 128, true>(p, size, stream);
   }
 }
 
@@ -2179,6 +2183,7 @@ PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t tile
   const bool uneven = (ragged && sequences > 1) || (causal && 2 * rows > keys * sequences);
   s.target = 0;
   s.rounds = 1;
+  s.many_parts = false;
   if (step) {
     // A second launch costs 5 us, as much as 16 queries over 48 BF16 key tiles or
     // 20 of codes take alone (16 sequences, 4 heads: 1,024 BF16 keys 13.6 us whole,
@@ -2197,6 +2202,12 @@ PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t tile
     s.min_tiles = 6;
     if (wide_target(likely, heads, key_tiles, s.min_tiles) || (ragged && sequences > 1 && key_tiles > 48))
       s.target = 2 * (kResident / heads), s.rounds = 2;
+    // Few row tiles over many keys: from 48 parts on the merge takes a row at a time
+    // of these tiles too.  (A tree of 20 nodes of 8 x 3 heads behind 84,672 INT8
+    // tokens, 64 parts, 82 and 72 us; one of 130 of 2 x 4 behind 40,000 fp8 ones, 51
+    // parts, 66 and 63; one of 64 of 8 x 3 behind 84,672, 32 parts, 155 and 156; one
+    // of 40 of 8 x 4 behind 9,000, 23 parts, 41 and 43.)
+    s.many_parts = std::min(key_tiles / s.min_tiles, s.target / 2 / s.tiles) >= 48;
   } else if (uneven && 2 * likely * heads * key_tiles >= 3 * kResident * 24) {
     // Enough keys for one and a half rounds of parts of 24 tiles: those even the
     // lengths out (8 sequences of 600 .. 12,000 keys, 512 new tokens of 8 x 4

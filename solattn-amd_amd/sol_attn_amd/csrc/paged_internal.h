@@ -74,6 +74,7 @@ struct PagedSize {
   int64_t rows;               // of a row tile: 16 (step_kernel) or 128 (wide_kernel)
   int64_t tiles;              // row tiles at most
   int64_t target, min_tiles, rounds;
+  bool many_parts;            // a row tile has many parts and few rows (merge_kernel)
   int64_t grid;               // workgroups
   int64_t headers;            // split row tiles per head at most, 0 without target
   int64_t records;            // their parts over all heads at most

@@ -102,6 +102,13 @@ def test_keys_split_over_workgroups(fmt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dim,fmt", [(64, "fp8"), (128, "bf16"), (128, "int8")])
+def test_few_rows_over_many_keys(dim, fmt):
+    run([20300, 19001], [40, 33], ["any", "chain"], fmt=fmt, heads=2, group=4, dim=dim, page_size=64)
+    run([20300], [35], ["level"], fmt=fmt, heads=2, group=4, dim=dim, page_size=64, window=19500, sinks=30)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("new", [5, 80])
 def test_a_chain_is_causal_attention(new):
     b = Sequences([200, 90 + new], [new, new], heads=2, dim=128)
