@@ -150,8 +150,9 @@ __global__ __launch_bounds__(kRotateThreads) void rotate_kernel(RotateParams p, 
   asm volatile("" ::: "memory");  // on their way while the angles are formed
 
   // The axes of all eight pairs, then all their positions: without a branch, so that
-  // each is one wait (a pair of no axis reads one and stays as it is).
+  // each is one wait (a pair of no axis reads one).
   float cs[8], sn[8];
+  bool still[8];  // the pair has no axis and stays as it is: a product with a sine of 0 is NaN next to an infinity
   const int32_t* at = p.positions + b * p.pb + t * p.pt;
   int axis[8], position[8];
   double frequency[8];
@@ -164,8 +165,8 @@ __global__ __launch_bounds__(kRotateThreads) void rotate_kernel(RotateParams p, 
   for (int i = 0; i < 8; ++i) position[i] = at[min(max(axis[i], 0), p.axes - 1)];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const bool still = axis[i] < 0 || axis[i] >= p.axes;
-    const double turns = still ? 0. : double(position[i]) * frequency[i] * 0.15915494309189533577;
+    still[i] = axis[i] < 0 || axis[i] >= p.axes;
+    const double turns = still[i] ? 0. : double(position[i]) * frequency[i] * 0.15915494309189533577;
     float s, c1;
     sincospif(2.f * float(turns - rint(turns)), &s, &c1);
     sn[i] = s, cs[i] = c1;
@@ -201,8 +202,8 @@ __global__ __launch_bounds__(kRotateThreads) void rotate_kernel(RotateParams p, 
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float a = y.a[i], bb = y.b[i];
-          y.a[i] = a * cs[i] - bb * sn[i];
-          y.b[i] = a * sn[i] + bb * cs[i];
+          y.a[i] = still[i] ? a : a * cs[i] - bb * sn[i];
+          y.b[i] = still[i] ? bb : a * sn[i] + bb * cs[i];
         }
         pack<PAIRS>(y, v[u]);
         if (mine && h + u < to) {

@@ -90,6 +90,32 @@ def test_misaligned_rows_and_pairs_without_an_axis():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["halves", "pairs"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_pairs_without_an_axis_stay_as_they_are_whatever_they_hold(dim, layout):
+    q = rows(21, 3, dim, seed=4, device="cuda")
+    half = dim // 2
+    # The last eight pairs have no axis: infinities, NaN and zeros of both signs beside ordinary partners and each other.
+    first, second = ((slice(half - 8, half), slice(dim - 8, dim)) if layout == "halves"
+                     else (slice(dim - 16, None, 2), slice(dim - 15, None, 2)))
+    inf, nan = float("inf"), float("nan")
+    q[..., first] = torch.tensor([inf, 1.5, -inf, inf, nan, -0.0, 2.0, -0.0], dtype=torch.bfloat16, device="cuda")
+    q[..., second] = torch.tensor([0.5, -inf, inf, -3.0, 1.0, -1.0, nan, 0.0], dtype=torch.bfloat16, device="cuda")
+    rotary = RotaryAxes.create(dim, half - 8, layout=layout)
+    positions = positions_of(21, axes=1, reach=5000, seed=5).cuda()
+    got = rotate_heads(q, None, positions, rotary)
+    for part in (first, second):
+        x, y = q[..., part], got[..., part]
+        assert torch.equal(x.isnan(), y.isnan())
+        assert torch.equal(x.view(torch.int16)[~x.isnan()], y.view(torch.int16)[~x.isnan()])
+    # The others turn as ever.
+    clean = q.clone()
+    clean[..., first] = clean[..., second] = 1.0
+    got[..., first] = got[..., second] = 1.0
+    check(got, clean, positions, rotary)
+
+
+@pytest.mark.gpu
 def test_turning_on_and_back():
     q = rows(40, 2, 128, seed=1, device="cuda")
     rotary = axes_of(128, 1, "halves")
