@@ -116,6 +116,24 @@ def test_pairs_without_an_axis_stay_as_they_are_whatever_they_hold(dim, layout):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["halves", "pairs"])
+@pytest.mark.parametrize("tokens,hq,hk,dim", [(32793, 5, 2, 64), (8203, 13, 3, 128), (8205, 3, 11, 128),
+                                              (33001, 6, 0, 64)])
+def test_calls_so_large_that_a_wave_takes_more_heads_than_it_loads_at_once(tokens, hq, hk, dim, layout):
+    # Heads that neither four nor eight divide, Q's end inside a wave's, tokens that end inside a wave's.
+    both = rows(tokens, hq + hk, dim, seed=6, device="cuda")
+    q, k = both[:, :hq], both[:, hq:] if hk else None
+    positions = positions_of(tokens, axes=3, reach=300, seed=7).cuda()
+    rotary = axes_of(dim, 3, layout, left=3)
+    norms = dict(q_norm=weights(dim, 8), k_norm=weights(dim, 9) if hk else None)
+    got = rotate_heads(q, k, positions, rotary, **norms)
+    for x, y, w in zip((q, k), got if hk else (got,), norms.values()):
+        check(y, x, positions, rotary, w)
+    rotate_heads(q, k, positions, rotary, out=(q, k) if hk else q, **norms)
+    assert torch.equal(both, torch.cat(got, 1) if hk else got)
+
+
+@pytest.mark.gpu
 def test_turning_on_and_back():
     q = rows(40, 2, 128, seed=1, device="cuda")
     rotary = axes_of(128, 1, "halves")
