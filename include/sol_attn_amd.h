@@ -570,7 +570,8 @@ int sol_rotate_heads(const void* q, const int64_t* q_strides, int64_t query_head
  * + j, K, V and scales of every head, as if all were read before any is written;
  * lengths_out[s] (int32 [sequences]) receives base + their count, at least 0.
  * A row that lies in no page moves as zeros, and none moves to where there is no
- * page; everything else is left as it was. */
+ * page; everything else is left as it was.  The cache's tensors and lengths_out
+ * share no memory with each other or with the other arguments (refused). */
 int sol_cache_keep(const int32_t* page_table, const int32_t* context_lengths, const int32_t* query_offsets,
                    int64_t sequences, int64_t table_width, int64_t pages, int64_t page_size, int64_t heads,
                    int64_t head_dim, int format, void* cache_k, void* cache_v, float* k_scales, float* v_scales,
@@ -594,10 +595,12 @@ int sol_cache_keep(const int32_t* page_table, const int32_t* context_lengths, co
  * children do not have either.
  * Outputs: new_table [new_sequences, new_width] (-1 past a sequence's pages, and
  * where there is no page), new_lengths, new_offsets [new_sequences + 1] (its
- * new tokens are its last), new_refs [pages] (memory of its own), missing [1]: how
+ * new tokens are its last), new_refs [pages], missing [1]: how
  * many pages, begun ones included, were not to be had.  Sequences that are no one's parent end; refs of
  * their pages fall.  workspace: 16-byte aligned, of
- * sol_cache_fork_workspace_size() bytes. */
+ * sol_cache_fork_workspace_size() bytes.  The cache's tensors, the outputs and the
+ * workspace share no memory with each other or with the other arguments
+ * (refused). */
 int64_t sol_cache_fork_workspace_size(int64_t sequences, int64_t new_sequences, int64_t pages);
 int sol_cache_fork(const int32_t* page_table, const int32_t* context_lengths, const int32_t* continued,
                    int64_t sequences, int64_t table_width, const int32_t* parents, const int32_t* new_tokens,

@@ -3,6 +3,7 @@
 #include <cmath>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 #include <string>
 
@@ -925,6 +926,34 @@ int store_ok(const char* what, const void* cache_k, const void* cache_v, const f
   return SOL_OK;
 }
 
+// Memory that a call reads or writes.
+struct Extent {
+  const void* at;
+  int64_t bytes;
+};
+
+bool meet(const Extent& a, const Extent& b) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+  return a.at && b.at && a.bytes > 0 && b.bytes > 0 && x < y + uintptr_t(b.bytes) && y < x + uintptr_t(a.bytes);
+}
+
+// Whether everything that a call writes is memory of its own: its workgroups read
+// the inputs again after others have written.
+bool apart(std::initializer_list<Extent> written, std::initializer_list<Extent> read) {
+  for (auto a = written.begin(); a != written.end(); ++a) {
+    for (auto b = written.begin(); b != a; ++b)
+      if (meet(*a, *b)) return false;
+    for (const Extent& b : read)
+      if (meet(*a, b)) return false;
+  }
+  return true;
+}
+
+// Rows of one of a cache's tensors, as far as there can be addresses for them.
+int64_t cache_rows(int64_t pages, int64_t heads, int64_t page_size) {
+  return std::min(pages * heads * page_size, int64_t(1) << 48);
+}
+
 // Arguments the two windowed attention entry points share.
 int window_args_ok(const char* what, int64_t query_heads, int64_t heads, double scale, int64_t window,
                    int64_t sink_tokens, const void* out) {
@@ -1254,6 +1283,12 @@ int sol_cache_keep(const int32_t* page_table, const int32_t* context_lengths, co
   const int64_t threads = most <= sol::keep_small_rows(row_bytes) ? 64 : 1024;
   if (sequences * heads * 2 * cdiv(row_bytes, 128) * threads >= (int64_t(1) << 32))
     return fail(SOL_ERR_UNSUPPORTED, "sol_cache_keep: grid too large");
+  const int64_t stored = cache_rows(pages, heads, page_size);
+  if (!apart({{cache_k, stored * row_bytes}, {cache_v, stored * row_bytes}, {k_scales, 4 * stored},
+              {v_scales, 4 * stored}, {lengths_out, 4 * sequences}},
+             {{page_table, 4 * sequences * table_width}, {context_lengths, 4 * sequences},
+              {query_offsets, 4 * (sequences + 1)}, {kept, 4 * sequences * most}}))
+    return fail(SOL_ERR_INVALID, "sol_cache_keep: the cache's tensors and lengths_out need memory of their own");
   p.kept = kept;
   p.most = int(most);
   p.store[0] = static_cast<uint8_t*>(cache_k);
@@ -1290,8 +1325,8 @@ int sol_cache_fork(const int32_t* page_table, const int32_t* context_lengths, co
   if (bytes < 0 || new_width <= 0 || new_width > kMaxPositions / page_size)
     return fail(SOL_ERR_INVALID, "sol_cache_fork: invalid shape");
   if ((new_sequences && (!parents || !new_tokens || !new_table || !new_lengths)) || !refs || !new_offsets ||
-      !new_refs || !missing || refs == new_refs)
-    return fail(SOL_ERR_INVALID, "sol_cache_fork: parents, new_tokens, refs and outputs of their own are required");
+      !new_refs || !missing)
+    return fail(SOL_ERR_INVALID, "sol_cache_fork: parents, new_tokens, refs and outputs are required");
   if (!workspace || !aligned16(workspace) || workspace_bytes < bytes)
     return fail(SOL_ERR_INVALID,
                 "sol_cache_fork: needs a 16-byte aligned workspace of the size its size function returns");
@@ -1299,6 +1334,13 @@ int sol_cache_fork(const int32_t* page_table, const int32_t* context_lengths, co
   // (A copied page takes a workgroup per 32 KB of each head's K and V.)
   if (new_sequences * heads * 2 * cdiv(page_size * row_bytes, 32768) + new_sequences + sequences > kMaxGrid)
     return fail(SOL_ERR_UNSUPPORTED, "sol_cache_fork: grid too large");
+  const int64_t stored = cache_rows(pages, heads, page_size);
+  if (!apart({{cache_k, stored * row_bytes}, {cache_v, stored * row_bytes}, {k_scales, 4 * stored},
+              {v_scales, 4 * stored}, {new_table, 4 * new_sequences * new_width}, {new_lengths, 4 * new_sequences},
+              {new_offsets, 4 * (new_sequences + 1)}, {new_refs, 4 * pages}, {missing, 4}, {workspace, bytes}},
+             {{page_table, 4 * sequences * table_width}, {context_lengths, 4 * sequences}, {continued, 4 * sequences},
+              {parents, 4 * new_sequences}, {new_tokens, 4 * new_sequences}, {refs, 4 * pages}}))
+    return fail(SOL_ERR_INVALID, "sol_cache_fork: the cache's tensors, outputs and workspace need memory of their own");
   const sol::ForkSize size = sol::fork_size(sequences, new_sequences, pages);
   sol::ForkParams p;
   std::memset(&p, 0, sizeof(p));

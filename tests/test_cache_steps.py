@@ -469,3 +469,68 @@ def test_the_c_entries_refuse():
         args = list(fork)
         args[at] = value
         assert lib.sol_cache_fork(*args) < 0, at
+
+
+def memory(n):
+    """Addresses apart from each other's by far (nothing is read there: the calls are refused)."""
+    return [ctypes.c_void_p((1 + i) << 32) for i in range(n)]
+
+
+def test_the_c_entries_refuse_outputs_that_meet_something():
+    lib = _native.library()
+    table, lengths, offsets, k, v, ks, vs, kept, out = memory(9)
+    # 70 sequences of 3 pages, 40 pages of 16 rows of 2 heads of 64 codes.
+    keep = [table, lengths, offsets, 70, 3, 40, 16, 2, 64, 1, k, v, ks, vs, kept, 5, out, None]
+    near = [(16, x.value + far) for x, far in ((table, 4 * 70 * 3 - 4), (lengths, 0), (lengths, 4 * 69), (lengths, -4 * 69),
+                                               (offsets, 4 * 70), (kept, 4 * 70 * 5 - 4), (k, 40 * 2 * 16 * 64 - 4),
+                                               (vs, 40 * 2 * 16 * 4 - 4))]
+    for at, value in near + [(11, k.value + 40 * 2 * 16 * 64 - 16), (13, ks.value), (14, k.value), (0, vs.value)]:
+        args = list(keep)
+        args[at] = ctypes.c_void_p(value)
+        assert lib.sol_cache_keep(*args) < 0 and b"memory of their own" in lib.sol_last_error(), (at, value)
+    (table, lengths, continued, parents, new, refs, k, v, ks, vs, new_table, new_lengths, new_offsets, new_refs, missing,
+     workspace) = memory(16)
+    size = lib.sol_cache_fork_workspace_size(70, 90, 40)
+    fork = [table, lengths, continued, 70, 3, parents, new, 90, 4, refs, 40, 16, 2, 64, 1, k, v, ks, vs, new_table,
+            new_lengths, new_offsets, new_refs, missing, workspace, size, None]
+    near = [(19, table.value), (19, table.value - 4 * 90 * 4 + 4), (20, lengths.value), (20, lengths.value + 4 * 69),
+            (20, continued.value), (20, new.value + 4 * 89), (21, parents.value - 4 * 90), (22, refs.value + 4 * 39),
+            (22, refs.value), (23, refs.value + 4 * 39), (23, new_table.value + 4 * 90 * 4 - 4), (23, missing.value + 0),
+            (24, table.value), (24, k.value - (size - 16)), (23, workspace.value + size - 4), (16, k.value), (18, ks.value)]
+    for at, value in near:
+        args = list(fork)
+        args[at] = ctypes.c_void_p(value)
+        if value == missing.value:
+            args[21] = ctypes.c_void_p(value - 4 * 90)
+        assert lib.sol_cache_fork(*args) < 0 and b"memory of their own" in lib.sol_last_error(), (at, value)
+
+
+@pytest.mark.gpu
+def test_neighbours_in_memory_are_not_refused():
+    # All of a batch's whole numbers one after another in one allocation, outputs between inputs.
+    b = Batch([33, 50, 70], spare=30, width=8)
+    want_plan, want_pool = cache_fork(b.cache, b.pool, b.plan, ints([0, 0, 2]), ints([1, 2, 3]))
+    pages, lib = b.pool.refs.numel(), _native.library()
+    size = lib.sol_cache_fork_workspace_size(3, 3, pages)
+    parts = dict(work=size // 4, table=24, lengths=3, new_lengths=3, parents=3, new_table=24, new=3, offsets=4, refs=pages,
+                 new_refs=pages, missing=1, keep_offsets=4, keep_lengths=3, kept=6)
+    at, flat = {}, torch.full((sum(parts.values()),), 99, dtype=torch.int32, device="cuda")
+    for name, n in parts.items():
+        at[name] = flat[sum(x.numel() for x in at.values()):][:n]
+    for name, x in (("table", b.plan.page_table.view(-1)), ("lengths", b.plan.context_lengths), ("parents", ints([0, 0, 2])),
+                    ("new", ints([1, 2, 3])), ("refs", b.pool.refs), ("keep_offsets", ints([0, 4, 8, 12])),
+                    ("kept", ints([0, 2, 1, 3, 0, 1]))):
+        at[name].copy_(x)
+    p = {name: x.data_ptr() for name, x in at.items()}
+    k, v = b.cache.k.data_ptr(), b.cache.v.data_ptr()
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.sol_cache_fork(p["table"], p["lengths"], None, 3, 8, p["parents"], p["new"], 3, 8, p["refs"], pages, 16, 2,
+                              64, 0, k, v, None, None, p["new_table"], p["new_lengths"], p["offsets"], p["new_refs"],
+                              p["missing"], p["work"], size, stream) == 0
+    for name, x in (("new_table", want_plan.page_table.view(-1)), ("new_lengths", want_plan.context_lengths),
+                    ("offsets", want_plan.query_offsets), ("new_refs", want_pool.refs), ("missing", want_pool.missing),
+                    ("table", b.plan.page_table.view(-1)), ("lengths", b.plan.context_lengths)):
+        assert torch.equal(at[name], x)
+    assert lib.sol_cache_keep(p["table"], p["lengths"], p["keep_offsets"], 3, 8, pages, 16, 2, 64, 0, k, v, None, None,
+                              p["kept"], 2, p["keep_lengths"], stream) == 0
+    assert at["keep_lengths"].tolist() == [31, 48, 68]
