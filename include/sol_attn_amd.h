@@ -591,13 +591,13 @@ int sol_cache_keep(const int32_t* page_table, const int32_t* context_lengths, co
  * the others and behind them free ones, lowest first, in order of sequences and
  * places, whose first takes a copy of the parent's rows in it (its tokens
  * behind the last whole page).  Pages that become free are taken by later calls.
- * A begun page that the parent does not have (entry outside [0, pages)) its
- * children do not have either.
+ * A page that the parent does not have (entry outside [0, pages)) its children do
+ * not have either, begun or whole; pages past new_width have no entry.
  * Outputs: new_table [new_sequences, new_width] (-1 past a sequence's pages, and
  * where there is no page), new_lengths, new_offsets [new_sequences + 1] (its
- * new tokens are its last), new_refs [pages], missing [1]: how
- * many pages, begun ones included, were not to be had.  Sequences that are no one's parent end; refs of
- * their pages fall.  workspace: 16-byte aligned, of
+ * new tokens are its last), new_refs [pages], missing [1]: how many pages this call
+ * was to take, or to go on in, and could not.  Sequences that are no one's parent
+ * end; refs of their pages fall.  workspace: 16-byte aligned, of
  * sol_cache_fork_workspace_size() bytes.  The cache's tensors, the outputs and the
  * workspace share no memory with each other or with the other arguments
  * (refused). */
@@ -608,6 +608,18 @@ int sol_cache_fork(const int32_t* page_table, const int32_t* context_lengths, co
                    int64_t heads, int64_t head_dim, int format, void* cache_k, void* cache_v, float* k_scales,
                    float* v_scales, int32_t* new_table, int32_t* new_lengths, int32_t* new_offsets, int32_t* new_refs,
                    int32_t* missing, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* The same, and absent [1] (8-byte aligned; NULL: not wanted): how many pages the
+ * new sequences' tokens need, ceil(new_lengths / page_size) each, that their tables
+ * do not name, for whatever reason: those missing now, whole pages that a parent
+ * did not have, and those past new_width.  0: every token has its place. */
+int sol_cache_fork_counted(const int32_t* page_table, const int32_t* context_lengths, const int32_t* continued,
+                           int64_t sequences, int64_t table_width, const int32_t* parents, const int32_t* new_tokens,
+                           int64_t new_sequences, int64_t new_width, const int32_t* refs, int64_t pages,
+                           int64_t page_size, int64_t heads, int64_t head_dim, int format, void* cache_k, void* cache_v,
+                           float* k_scales, float* v_scales, int32_t* new_table, int32_t* new_lengths,
+                           int32_t* new_offsets, int32_t* new_refs, int32_t* missing, int64_t* absent, void* workspace,
+                           int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -82,6 +82,8 @@ _SIGNATURES = {
     "sol_cache_fork_workspace_size": ([_i64, _i64, _i64], _i64),
     "sol_cache_fork": ([_p, _p, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _int, _p, _p, _p, _p,
                         _p, _p, _p, _p, _p, _p, _i64, _p], ctypes.c_int),
+    "sol_cache_fork_counted": ([_p, _p, _p, _i64, _i64, _p, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _int, _p, _p,
+                                _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _p], ctypes.c_int),
     "sol_rotate_heads": ([_p, _i64p, _i64, _p, _i64p, _p, _i64p, _i64, _p, _i64p, _p, _i64p, _i64, _p, _p, _int, _p, _p,
                           _int, _dbl, _i64, _i64, _i64, _p], ctypes.c_int),
     "sol_window_attention_workspace_size": ([_i64, _i64, _i64, _i64, _i64, _i64, _int, _i64, _i64], _i64),
@@ -898,7 +900,8 @@ def _fork_size(s, n, pages):
 
 
 def launch_cache_fork(cache, refs, plan, parents, new_tokens, lengths, width):
-    """``(table, lengths, offsets, refs, missing)`` of the next plan and pool (``sol_cache_fork``)."""
+    """``(table, lengths, offsets, refs, missing, absent)`` of the next plan and pool (``sol_cache_fork_counted``);
+    ``absent`` as two words."""
     pages, h, page_size, d = cache.k.shape
     s, old_width = plan.page_table.shape
     n, dev = parents.shape[0], refs.device
@@ -907,13 +910,13 @@ def launch_cache_fork(cache, refs, plan, parents, new_tokens, lengths, width):
         raise RuntimeError("the workspace size function rejected the sizes")
     # One allocation for the workspace (a multiple of 16 bytes) and the results.  ("Unsafe" for gradients alone; split
     # and its views took 2 of the call's 22 us on the host.)
-    ws, table, new_lengths, offsets, new_refs, missing = torch.empty(
-        size // 4 + n * width + 2 * n + 2 + pages, device=dev, dtype=torch.int32).unsafe_split_with_sizes(
-        (size // 4, n * width, n, n + 1, pages, 1))
+    ws, absent, table, new_lengths, offsets, new_refs, missing = torch.empty(
+        size // 4 + n * width + 2 * n + 4 + pages, device=dev, dtype=torch.int32).unsafe_split_with_sizes(
+        (size // 4, 2, n * width, n, n + 1, pages, 1))
     old_table, old_lengths, _ = _plan_args(plan)
-    _check(library().sol_cache_fork(
+    _check(library().sol_cache_fork_counted(
         old_table, old_lengths, _ptr(lengths), s, old_width, parents.data_ptr(), new_tokens.data_ptr(), n, width,
         refs.data_ptr(), pages, page_size, h, d, CACHE_FORMATS[cache.k.dtype], *_store_args(cache), table.data_ptr(),
-        new_lengths.data_ptr(), offsets.data_ptr(), new_refs.data_ptr(), missing.data_ptr(), ws.data_ptr(), size,
-        _stream(dev)))
-    return table.view(n, width), new_lengths, offsets, new_refs, missing
+        new_lengths.data_ptr(), offsets.data_ptr(), new_refs.data_ptr(), missing.data_ptr(),
+        absent.data_ptr(), ws.data_ptr(), size, _stream(dev)))
+    return table.view(n, width), new_lengths, offsets, new_refs, missing, absent

@@ -1307,12 +1307,13 @@ int64_t sol_cache_fork_workspace_size(int64_t sequences, int64_t new_sequences, 
   return sol::fork_size(sequences, new_sequences, pages).bytes;
 }
 
-int sol_cache_fork(const int32_t* page_table, const int32_t* context_lengths, const int32_t* continued,
-                   int64_t sequences, int64_t table_width, const int32_t* parents, const int32_t* new_tokens,
-                   int64_t new_sequences, int64_t new_width, const int32_t* refs, int64_t pages, int64_t page_size,
-                   int64_t heads, int64_t head_dim, int format, void* cache_k, void* cache_v, float* k_scales,
-                   float* v_scales, int32_t* new_table, int32_t* new_lengths, int32_t* new_offsets, int32_t* new_refs,
-                   int32_t* missing, void* workspace, int64_t workspace_bytes, void* stream) {
+int sol_cache_fork_counted(const int32_t* page_table, const int32_t* context_lengths, const int32_t* continued,
+                           int64_t sequences, int64_t table_width, const int32_t* parents, const int32_t* new_tokens,
+                           int64_t new_sequences, int64_t new_width, const int32_t* refs, int64_t pages,
+                           int64_t page_size, int64_t heads, int64_t head_dim, int format, void* cache_k, void* cache_v,
+                           float* k_scales, float* v_scales, int32_t* new_table, int32_t* new_lengths,
+                           int32_t* new_offsets, int32_t* new_refs, int32_t* missing, int64_t* absent, void* workspace,
+                           int64_t workspace_bytes, void* stream) {
   const char* what = "sol_cache_fork";
   sol::PagedBatch shape;
   int rc = paged_batch_ok(what, sequences ? page_table : refs, sequences ? context_lengths : refs, nullptr, 0,
@@ -1330,6 +1331,8 @@ int sol_cache_fork(const int32_t* page_table, const int32_t* context_lengths, co
   if (!workspace || !aligned16(workspace) || workspace_bytes < bytes)
     return fail(SOL_ERR_INVALID,
                 "sol_cache_fork: needs a 16-byte aligned workspace of the size its size function returns");
+  if (reinterpret_cast<uintptr_t>(absent) & 7u)
+    return fail(SOL_ERR_INVALID, "sol_cache_fork: absent must be 8-byte aligned");
   const int64_t row_bytes = head_dim * (format == SOL_CACHE_BF16 ? 2 : 1);
   // (A copied page takes a workgroup per 32 KB of each head's K and V.)
   if (new_sequences * heads * 2 * cdiv(page_size * row_bytes, 32768) + new_sequences + sequences > kMaxGrid)
@@ -1337,7 +1340,8 @@ int sol_cache_fork(const int32_t* page_table, const int32_t* context_lengths, co
   const int64_t stored = cache_rows(pages, heads, page_size);
   if (!apart({{cache_k, stored * row_bytes}, {cache_v, stored * row_bytes}, {k_scales, 4 * stored},
               {v_scales, 4 * stored}, {new_table, 4 * new_sequences * new_width}, {new_lengths, 4 * new_sequences},
-              {new_offsets, 4 * (new_sequences + 1)}, {new_refs, 4 * pages}, {missing, 4}, {workspace, bytes}},
+              {new_offsets, 4 * (new_sequences + 1)}, {new_refs, 4 * pages}, {missing, 4}, {absent, 8},
+              {workspace, bytes}},
              {{page_table, 4 * sequences * table_width}, {context_lengths, 4 * sequences}, {continued, 4 * sequences},
               {parents, 4 * new_sequences}, {new_tokens, 4 * new_sequences}, {refs, 4 * pages}}))
     return fail(SOL_ERR_INVALID, "sol_cache_fork: the cache's tensors, outputs and workspace need memory of their own");
@@ -1367,6 +1371,7 @@ int sol_cache_fork(const int32_t* page_table, const int32_t* context_lengths, co
   p.new_offsets = new_offsets;
   p.new_refs = new_refs;
   p.missing = missing;
+  p.absent = reinterpret_cast<uint64_t*>(absent);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.slices = int(size.slices);
   p.slice_pages = int(size.slice_pages);
@@ -1377,6 +1382,18 @@ int sol_cache_fork(const int32_t* page_table, const int32_t* context_lengths, co
   p.free_count = reinterpret_cast<int32_t*>(ws + size.free_count);
   p.free_list = reinterpret_cast<int32_t*>(ws + size.free_list);
   return hip_status(sol::launch_fork(p, static_cast<hipStream_t>(stream)));
+}
+
+int sol_cache_fork(const int32_t* page_table, const int32_t* context_lengths, const int32_t* continued,
+                   int64_t sequences, int64_t table_width, const int32_t* parents, const int32_t* new_tokens,
+                   int64_t new_sequences, int64_t new_width, const int32_t* refs, int64_t pages, int64_t page_size,
+                   int64_t heads, int64_t head_dim, int format, void* cache_k, void* cache_v, float* k_scales,
+                   float* v_scales, int32_t* new_table, int32_t* new_lengths, int32_t* new_offsets, int32_t* new_refs,
+                   int32_t* missing, void* workspace, int64_t workspace_bytes, void* stream) {
+  return sol_cache_fork_counted(page_table, context_lengths, continued, sequences, table_width, parents, new_tokens,
+                                new_sequences, new_width, refs, pages, page_size, heads, head_dim, format, cache_k,
+                                cache_v, k_scales, v_scales, new_table, new_lengths, new_offsets, new_refs, missing,
+                                nullptr, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

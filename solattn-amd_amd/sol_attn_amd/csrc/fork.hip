@@ -14,7 +14,10 @@
 // no table named it before the call: pages that a call frees are taken from the
 // next call on, so that no page is read and written by one call, and everything
 // follows from the state before it.  A begun page that the parent does not have
-// (none was free, then) its children do not have either.
+// (none was free, then) its children do not have either.  `missing` counts the
+// pages that this call was to take or go on in and could not; `absent` those that
+// the new sequences' tokens need and their tables do not name, for whatever reason:
+// those, whole pages that a parent lacks, and what new_width has no room for.
 // Reference counts change by whole numbers, in any order.
 #include <algorithm>
 
@@ -352,6 +355,7 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(ForkParams p) {
   if (tid == 0) {
     p.start[p.N] = taken;
     *p.lost = s_lost;
+    if (p.absent) *p.absent = 0;
     p.new_offsets[p.N] = int(min(tokens, int64_t(0x7FFFFFFF)));
     if (p.N == 0) *p.missing = 0;  // (otherwise sequence 0's workgroup writes it)
   }
@@ -435,6 +439,7 @@ __global__ __launch_bounds__(kForkThreads) void fork_kernel(ForkParams p, int pi
     const int end = goes_until(x);
     __shared__ int s_going[kForkWaves];
     int going = 0;  // pages below e0 that the child goes on in
+    uint64_t absent = tid == 0 ? uint64_t(pages_of(x.after, p.page_shift) - x.used) : 0;
     for (int e0 = 0; e0 < p.new_width; e0 += kForkThreads) {
       const int e = e0 + tid;
       const bool goes = e >= x.full && e < end && goes_on(p, x.parent, e);
@@ -462,9 +467,12 @@ __global__ __launch_bounds__(kForkThreads) void fork_kernel(ForkParams p, int pi
           page = free.page(p, start + taken_before(x, e, before));
           if (page >= 0) atomicAdd(p.new_refs + page, 1);
         }
+        absent += page < 0 || page >= p.pages;
       }
       p.new_table[int64_t(i) * p.new_width + e] = page;
     }
+    if (p.absent && absent)
+      atomicAdd(reinterpret_cast<unsigned long long*>(p.absent), static_cast<unsigned long long>(absent));
     return;
   }
   const int64_t unit = id - p.N - p.S;

@@ -37,6 +37,7 @@ struct ForkParams {
   int32_t* new_offsets;      // [N + 1]
   int32_t* new_refs;         // [pages]
   int32_t* missing;          // [1]
+  uint64_t* absent;          // [1] pages of the new sequences' tokens that their tables do not name; or null
   // Workspace.
   int slices, slice_pages;   // of the pool: up to kForkSlices, of whole kForkStep pages
   int32_t* first;            // [S] first child, N: none

@@ -345,6 +345,55 @@ def test_lengths_and_pages_that_make_no_sense_stay_inside_the_tensors():
     b.fork([0, 0, 1, 2, -2147483648, 2147483647], [2147483647, 1, 5, 2147483647, -9, 3])
 
 
+def absent(b):
+    """Pages that a batch's tokens need and its tables do not name."""
+    return sum(-(-max(n, 0) // b.page_size) - sum(0 <= x < len(b.refs) for x in row[:-(-max(n, 0) // b.page_size)])
+               for row, n in zip(b.table, b.lengths))
+
+
+@pytest.mark.gpu
+def test_pages_past_the_tables_width_are_counted():
+    b = Batch([100, 120, 96], shared=5, spare=64)
+    assert b.pool.absent.dtype == torch.int64 and b.pool.absent.tolist() == [0]
+    assert b.fork([0, 1, 2], [12, 8, 16]) == 0 and b.pool.absent.tolist() == [0]  # 7, 8 and 7 of 8 pages
+    assert b.fork([0, 1, 2], [16, 1, 0]) == 0 and b.pool.absent.tolist() == [1]  # the second one's 9th page
+    assert b.fork([0, 1, 2, 1, -1], [300, 0, 0, 0, 40]) == 0 and b.pool.absent.tolist() == [absent(b)] == [21]
+    assert b.fork([0, 2, 4], [0, 0, 0], width=1) == 0 and b.pool.absent.tolist() == [absent(b)] == [34]
+    assert b.fork([], []) == 0 and b.pool.absent.tolist() == [0]
+
+
+@pytest.mark.gpu
+def test_whole_pages_that_a_parent_lacks_are_counted():
+    b = Batch([40, 35], spare=3, width=9)
+    missing = b.fork([0, 0, 1, -1], [30, 30, 1, 40])
+    assert b.pool.absent.tolist() == [absent(b)] == [missing] and missing > 0
+    for parents, new in (([0, 1, 2, 3], [20] * 4), ([0, 1, 2, 3], [0] * 4), ([3, 1, 1], [9, 0, 50])):
+        b.fork(parents, new)
+        assert b.pool.absent.tolist() == [absent(b)] and absent(b) > 0
+    b.fork([2], [0], continued=[0, 0, 20])
+    assert b.pool.absent.tolist() == [absent(b)]
+
+
+@pytest.mark.gpu
+def test_absent_pages_of_many_and_of_lengths_that_make_no_sense():
+    rng = random.Random(6)
+    b = Batch([rng.randint(1, 400) for _ in range(900)], spare=50, width=25, heads=1)
+    b.fork([rng.randrange(-9, 900) for _ in range(700)], [rng.randint(0, 90) for _ in range(700)])
+    assert b.pool.absent.tolist() == [absent(b)]
+    # (Not in Python whole: the offsets of so many new tokens stop at what int32 holds.)
+    parents, most = [rng.randrange(700) for _ in range(800)], 2 ** 31 - 1
+    plan, pool = cache_fork(b.cache, b.pool, b.plan, ints(parents), ints([most] * 800), width=30)
+    assert plan.context_lengths.tolist() == [most] * 800 and plan.query_offsets.tolist()[-1] == most
+    b.table, b.lengths = plan.page_table.tolist(), [most] * 800
+    assert pool.absent.tolist() == [absent(b)] and absent(b) > 2 ** 31
+    b = Batch([40, 35, 90], spare=10, width=6)
+    b.table[0][1], b.table[1][2], b.table[2][0] = -3, 9999, 2147483647
+    b.lengths = [80, 35, 90]
+    b.plan = PagedPlan(ints(b.table), ints(b.lengths), ints([0] * 4))
+    b.fork([0, 1, 2, 2], [1, 5, 10, 0])
+    assert b.pool.absent.tolist() == [absent(b)] and absent(b) >= 3
+
+
 @pytest.mark.gpu
 def test_replays_follow_their_tensors():
     b = Batch([33, 50, 70], spare=30, width=8)
@@ -534,3 +583,25 @@ def test_neighbours_in_memory_are_not_refused():
     assert lib.sol_cache_keep(p["table"], p["lengths"], p["keep_offsets"], 3, 8, pages, 16, 2, 64, 0, k, v, None, None,
                               p["kept"], 2, p["keep_lengths"], stream) == 0
     assert at["keep_lengths"].tolist() == [31, 48, 68]
+
+
+def test_a_pool_counts_the_pages_that_its_tables_have_no_room_for():
+    cache, plan = parts()
+    assert PagePool.create(cache).absent.tolist() == [0] and PagePool.create(cache, plan).absent.tolist() == [0]
+    long = PagedPlan(plan.page_table[:, :1], torch.tensor([50, 5], dtype=torch.int32), plan.query_offsets)
+    assert PagePool.create(cache, long).absent.tolist() == [3]
+
+
+def test_the_counting_c_entry_refuses():
+    lib = _native.library()
+    (table, lengths, parents, new, refs, k, v, new_table, new_lengths, new_offsets, new_refs, missing, absent,
+     workspace) = memory(14)
+    size = lib.sol_cache_fork_workspace_size(7, 9, 40)
+    fork = [table, lengths, None, 7, 3, parents, new, 9, 4, refs, 40, 16, 2, 64, 0, k, v, None, None, new_table,
+            new_lengths, new_offsets, new_refs, missing, absent, workspace, size, None]
+    for at, value, match in ((24, absent.value + 4, b"aligned"), (24, missing.value - 4, b"aligned"),
+                             (24, refs.value + 8, b"own"), (24, lengths.value - 0, b"own"), (23, absent.value + 4, b"own"),
+                             (26, size - 1, b"workspace"), (5, None, b"parents")):
+        args = list(fork)
+        args[at] = value if at == 26 else ctypes.c_void_p(value)
+        assert lib.sol_cache_fork_counted(*args) < 0 and match in lib.sol_last_error(), (at, value)
