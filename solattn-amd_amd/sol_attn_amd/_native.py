@@ -894,6 +894,9 @@ def launch_cache_keep(cache, plan, kept):
     return lengths
 
 
+KEPT_WORKSPACE = 1 << 18  # bytes of scratch memory that may stay with a call's results
+
+
 @functools.lru_cache(maxsize=1024)
 def _fork_size(s, n, pages):
     return library().sol_cache_fork_workspace_size(s, n, pages)
@@ -908,11 +911,15 @@ def launch_cache_fork(cache, refs, plan, parents, new_tokens, lengths, width):
     size = _fork_size(s, n, pages)
     if size < 0:
         raise RuntimeError("the workspace size function rejected the sizes")
-    # One allocation for the workspace (a multiple of 16 bytes) and the results.  ("Unsafe" for gradients alone; split
-    # and its views took 2 of the call's 22 us on the host.)
+    # One allocation for the results, which a program keeps, and for a small workspace (a multiple of 16 bytes): one of its
+    # own takes 1.0 of the call's 21 us on the host.  A large one, of many pages, is not kept with them.  ("Unsafe" for
+    # gradients alone; split and its views took 2 us.)
+    room = size if size <= KEPT_WORKSPACE else 0
     ws, absent, table, new_lengths, offsets, new_refs, missing = torch.empty(
-        size // 4 + n * width + 2 * n + 4 + pages, device=dev, dtype=torch.int32).unsafe_split_with_sizes(
-        (size // 4, 2, n * width, n, n + 1, pages, 1))
+        room // 4 + n * width + 2 * n + 4 + pages, device=dev, dtype=torch.int32).unsafe_split_with_sizes(
+        (room // 4, 2, n * width, n, n + 1, pages, 1))
+    if not room:
+        ws = torch.empty(size, device=dev, dtype=torch.uint8)
     old_table, old_lengths, _ = _plan_args(plan)
     _check(library().sol_cache_fork_counted(
         old_table, old_lengths, _ptr(lengths), s, old_width, parents.data_ptr(), new_tokens.data_ptr(), n, width,

@@ -375,6 +375,21 @@ def test_whole_pages_that_a_parent_lacks_are_counted():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("pages", [40, 14000, 70001])
+def test_a_plan_and_a_pool_keep_no_large_workspace(pages):
+    cache = PagedCache.create(pages, 16, 1, 64, format="int8")
+    plan, pool = PagedPlan.create([], [], [], pages=pages, page_size=16).to("cuda"), PagePool.create(cache)
+    for parents, new in (([-1] * 3, [20, 300, 7]), ([0, 0, 1, 2], [1] * 4)):
+        plan, pool = cache_fork(cache, pool, plan, ints(parents), ints(new), width=21)
+        results = 4 * (len(new) * 21 + 2 * len(new) + 1 + pages + 1) + 8
+        kept = {x.untyped_storage().data_ptr(): x.untyped_storage().nbytes()
+                for x in (plan.page_table, plan.context_lengths, plan.query_offsets, pool.refs, pool.missing, pool.absent)}
+        assert sum(kept.values()) <= results + (1 << 18) + 512 * len(kept)
+        assert pool.refs.sum() == sum(-(-n // 16) for n in plan.context_lengths.tolist())
+        assert pool.missing.item() == pool.absent.item() == 0
+
+
+@pytest.mark.gpu
 def test_absent_pages_of_many_and_of_lengths_that_make_no_sense():
     rng = random.Random(6)
     b = Batch([rng.randint(1, 400) for _ in range(900)], spare=50, width=25, heads=1)
