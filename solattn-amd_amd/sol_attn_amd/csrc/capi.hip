@@ -1001,6 +1001,40 @@ void window_params(sol::PagedParams* p, int64_t query_heads, int64_t heads, doub
   p->sinks = window == 0 ? 0 : int(std::min(sink_tokens, kMaxPositions));
 }
 
+// paged_size() of new tokens over a cache of `keys` positions per sequence.  Under a
+// window a row tile of a tree streams all the nodes before its last one, wherever
+// their ancestors are: up to the sequence's, half of them in the mean (sequences
+// alike: they are not known here), beside the window and the first ones.  Tiles
+// that are mostly nodes, masked ones, cost wide_kernel more than others, so half of
+// the keys count for the choice; and twice of them for 8-bit heads of 64, of whose
+// step_kernel one workgroup fits a CU.  (422 shapes of 1 and 4 sequences of up to
+// 2,000 nodes under windows of 32 .. 1,500, in both kernels: 1.1% more than the
+// better one in the mean.  By 16 nodes and the window, as for causal calls, 2.7%:
+// 2,000 nodes of 8 heads of 128 under 64 65 us, 49 now, 4,000 of 4 heads 103 and 59.
+// By all nodes 2.7%, too: 700 of 16 heads under 16 44 us, 28 now.)
+sol::PagedSize attend_size(int64_t rows, int64_t sequences, int64_t keys, int64_t query_heads, int64_t heads,
+                           int64_t head_dim, int format, int causal, int64_t window, int64_t sink_tokens, bool tree) {
+  const bool windowed = tree && window > 0;
+  const int64_t nodes = windowed ? std::max(int64_t(16), cdiv(rows, sequences)) : 16;
+  const int64_t tile_keys = window_keys(nodes, keys, causal, window, sink_tokens);
+  int64_t step_keys = tile_keys;
+  if (windowed) {
+    step_keys = window_keys(std::max(int64_t(16), nodes / 2), keys, causal, window, sink_tokens);
+    step_keys = head_dim == 64 && format != SOL_CACHE_BF16 ? 2 * step_keys : step_keys / 2;
+  }
+  return sol::paged_size(rows, sequences, window_keys(rows, keys, causal, window, sink_tokens), tile_keys, step_keys,
+                         heads, query_heads / heads, head_dim, format, causal != 0, true, tree);
+}
+
+// paged_size() of the last tokens of plain K and V.
+sol::PagedSize window_size(int64_t batch, int64_t query_tokens, int64_t key_tokens, int64_t query_heads, int64_t heads,
+                           int64_t head_dim, int causal, int64_t window, int64_t sink_tokens) {
+  const int64_t tile_keys = window_keys(16, key_tokens, causal, window, sink_tokens);
+  return sol::paged_size(batch * query_tokens, batch,
+                         window_keys(query_tokens, key_tokens, causal, window, sink_tokens), tile_keys, tile_keys, heads,
+                         query_heads / heads, head_dim, SOL_CACHE_BF16, causal != 0, false);
+}
+
 // Attention of new tokens over the cache; `parents`: of a tree of them, or null.
 int attend_paged(const char* what, const void* q, const int64_t* q_strides, int64_t rows, const void* cache_k,
                  const void* cache_v, const float* k_scales, const float* v_scales, const int32_t* page_table,
@@ -1029,10 +1063,8 @@ int attend_paged(const char* what, const void* q, const int64_t* q_strides, int6
     return refuse(SOL_ERR_UNSUPPORTED, "at most 65,536 sequences in one call");
   if (rows * query_heads >= (int64_t(1) << 31))
     return refuse(SOL_ERR_UNSUPPORTED, "grid too large");
-  const sol::PagedSize size =
-      sol::paged_size(rows, sequences, window_keys(rows, table_width * page_size, causal, window, sink_tokens),
-                      window_keys(16, table_width * page_size, causal, window, sink_tokens), heads,
-                      query_heads / heads, head_dim, format, causal != 0, true, parents != nullptr);
+  const sol::PagedSize size = attend_size(rows, sequences, table_width * page_size, query_heads, heads, head_dim, format,
+                                          causal, window, sink_tokens, parents != nullptr);
   rc = paged_workspace_ok(what, size, workspace, workspace_bytes);
   if (rc != SOL_OK) return rc;
   p.q = static_cast<const uint16_t*>(q);
@@ -1056,9 +1088,8 @@ int64_t attend_workspace(int64_t rows, int64_t sequences, int64_t table_width, i
       format > SOL_CACHE_FP8 || window < 0 || sink_tokens < 0 || rows * query_heads >= (int64_t(1) << 31))
     return -1;
   if (rows == 0) return 0;
-  return sol::paged_size(rows, sequences, window_keys(rows, table_width * page_size, causal, window, sink_tokens),
-                         window_keys(16, table_width * page_size, causal, window, sink_tokens), heads,
-                         query_heads / heads, head_dim, format, causal != 0, true, tree).bytes;
+  return attend_size(rows, sequences, table_width * page_size, query_heads, heads, head_dim, format, causal, window,
+                     sink_tokens, tree).bytes;
 }
 
 }  // namespace
@@ -1184,8 +1215,7 @@ int sol_window_attention(const void* q, const int64_t* q_strides, const void* k,
   if (k_strides[1] >= kRowsStrideMax || v_strides[1] >= kRowsStrideMax)
     return fail(SOL_ERR_UNSUPPORTED, "sol_window_attention: K and V token strides must be below 2^24 elements");
   const sol::PagedSize size =
-      sol::paged_size(batch * query_tokens, batch, window_keys(query_tokens, key_tokens, causal, window, sink_tokens),
-                      window_keys(16, key_tokens, causal, window, sink_tokens), heads, query_heads / heads, head_dim, SOL_CACHE_BF16, causal != 0, false);
+      window_size(batch, query_tokens, key_tokens, query_heads, heads, head_dim, causal, window, sink_tokens);
   rc = paged_workspace_ok(what, size, workspace, workspace_bytes);
   if (rc != SOL_OK) return rc;
   sol::PagedParams p;
@@ -1212,9 +1242,7 @@ int64_t sol_window_attention_workspace_size(int64_t batch, int64_t query_tokens,
       heads <= 0 || heads >= (1 << 16) || query_heads % heads || window < 0 || sink_tokens < 0 ||
       batch * query_tokens * query_heads >= (int64_t(1) << 31))
     return -1;
-  return sol::paged_size(batch * query_tokens, batch,
-                         window_keys(query_tokens, key_tokens, causal, window, sink_tokens),
-                         window_keys(16, key_tokens, causal, window, sink_tokens), heads, query_heads / heads, head_dim, SOL_CACHE_BF16, causal != 0, false).bytes;
+  return window_size(batch, query_tokens, key_tokens, query_heads, heads, head_dim, causal, window, sink_tokens).bytes;
 }
 
 int sol_rotate_heads(const void* q, const int64_t* q_strides, int64_t query_heads, void* q_out,

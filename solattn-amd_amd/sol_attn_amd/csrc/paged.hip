@@ -2160,8 +2160,8 @@ int64_t wide_target(int64_t tiles, int64_t heads, int64_t key_tiles, int64_t min
 
 }  // namespace
 
-PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t tile_keys, int64_t heads, int64_t group,
-                     int64_t head_dim, int format, bool causal, bool ragged, bool tree) {
+PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t tile_keys, int64_t step_keys, int64_t heads,
+                     int64_t group, int64_t head_dim, int format, bool causal, bool ragged, bool tree) {
   PagedSize s;
   auto likely_tiles = [&](int64_t R) { return (rows * group + R - 1) / R + (sequences - 1) / 2; };
   // The step kernel, whose tiles are 16 rows, for few rows per sequence; and for
@@ -2173,7 +2173,7 @@ PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t tile
   // x 4 of 8 heads, 9,000 keys, 440 MB: 48 and 40.)
   const int64_t small = likely_tiles(16) * heads;
   const bool step = rows * group <= 32 * sequences ||
-                    (small <= 2 * kResident && small * tile_keys <= (int64_t(128) << 20) / (4 * head_dim));
+                    (small <= 2 * kResident && small * step_keys <= (int64_t(128) << 20) / (4 * head_dim));
   s.rows = step ? 16 : 128;
   const int64_t TK = step ? 8192 / (head_dim * (format == kBf16 ? 2 : 1)) : 64;  // StepSlot::TK
   s.tiles = rows * group / s.rows + sequences;  // row tiles: sum ceil(n_s G / R) at most

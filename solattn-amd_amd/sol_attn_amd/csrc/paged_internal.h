@@ -84,10 +84,11 @@ struct PagedSize {
 };
 
 // rows: new tokens in all; keys: what a sequence's see at most; tile_keys: what 16
-// neighbouring ones see; group: query heads per head; ragged: sequences may
-// differ in length; tree: the new tokens are trees.
-PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t tile_keys, int64_t heads, int64_t group,
-                     int64_t head_dim, int format, bool causal, bool ragged, bool tree = false);
+// neighbouring ones do (of trees, what their row tile streams); step_keys: the same
+// as it counts for the choice of kernel; group: query heads per head; ragged:
+// sequences may differ in length; tree: the new tokens are trees.
+PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t tile_keys, int64_t step_keys, int64_t heads,
+                     int64_t group, int64_t head_dim, int format, bool causal, bool ragged, bool tree = false);
 
 hipError_t launch_cache_write(const CacheParams& p, int D, int format, hipStream_t stream);
 hipError_t launch_cache_read(const CacheParams& p, int D, int format, hipStream_t stream);

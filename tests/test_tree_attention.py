@@ -109,6 +109,24 @@ def test_few_rows_over_many_keys(dim, fmt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fmt,dim", [("bf16", 128), ("fp8", 64)])
+@pytest.mark.parametrize("kind", ["chain", "level", "odd"])
+def test_trees_much_larger_than_their_window(kind, fmt, dim):
+    # Every row tile streams all the nodes before its last one, and sees few of them.
+    run([2050], [2000], [kind], fmt=fmt, heads=4, dim=dim, page_size=64, window=64, sinks=5, seed=3)
+    run([900, 1100, 40], [700, 1100, 40], [kind, "any", kind], fmt=fmt, heads=2, group=3, dim=dim, window=16, seed=4)
+
+
+def test_the_choice_of_kernel_goes_by_the_nodes_that_a_tile_streams():
+    # Row tiles of 128 rows whose keys are cut into parts, which take a workspace; by the window alone there are too few
+    # keys to cut, and tiles of 16 rows.
+    size = _native.library().sol_tree_attention_workspace_size
+    for n, heads in ((2000, 8), (4000, 4)):
+        assert size(n, 1, 64, 128, heads, heads, 128, 0, 64, 0) > 0
+    assert size(24, 4, 64, 128, 8, 8, 128, 0, 64, 0) == 0
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("new", [5, 80])
 def test_a_chain_is_causal_attention(new):
     b = Sequences([200, 90 + new], [new, new], heads=2, dim=128)
