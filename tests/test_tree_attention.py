@@ -242,6 +242,25 @@ def test_offsets_that_make_no_sense_stay_inside_the_tensors():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dim,fmt,past,group", [(64, "bf16", 60, 1), (128, "int8", 60, 4), (128, "bf16", 6000, 4),
+                                                (64, "fp8", 9000, 1)])
+@pytest.mark.parametrize("offsets", [[0, 70, 20, 60], [-9, 20, 40, 2 ** 31 - 1], [50, 10, 30, 60],
+                                     [-2 ** 31, 2 ** 31 - 1, 0, 61], [60, 60, 99, -1]])
+def test_offsets_that_make_no_sense_write_nothing_around_the_output(offsets, dim, fmt, past, group):
+    # One row tile and many, keys in one part and in several, whose states a second launch joins.
+    b = Sequences([past + 20, past // 2 + 20, 40], [20, 20, 20], heads=2, dim=dim, fmt=fmt, page_size=64)
+    q = rows(60, 2 * group, dim, seed=5, device="cuda")
+    around = torch.full((60 + 2 * 300, 2 * group, dim), 7.0, dtype=torch.bfloat16, device="cuda")
+    parents = ints(shape("odd", 60, 4))
+    plan = PagedPlan(b.plan.page_table, b.plan.context_lengths, ints(offsets))
+    stored = [x.clone() for x in (b.cache.k.view(torch.int8), b.cache.v.view(torch.int8))]
+    for how in (dict(), dict(window=30, sink_tokens=3)):
+        tree_attention(q, b.cache, plan, parents, out=around[300:360], **how)
+    assert bool((around[:300] == 7).all()) and bool((around[360:] == 7).all())
+    assert all(torch.equal(x.view(torch.int8), y) for x, y in zip((b.cache.k, b.cache.v), stored))
+
+
+@pytest.mark.gpu
 def test_empty_calls_and_refusals():
     b = Sequences([40], [3], heads=2, dim=64)
     q = rows(3, 4, 64, seed=1, device="cuda")
