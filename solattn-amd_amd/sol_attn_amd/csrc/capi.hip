@@ -1006,22 +1006,19 @@ void window_params(sol::PagedParams* p, int64_t query_heads, int64_t heads, doub
 // their ancestors are: up to the sequence's, half of them in the mean (sequences
 // alike: they are not known here), beside the window and the first ones.  Tiles
 // that are mostly nodes, masked ones, cost wide_kernel more than others, so half of
-// the keys count for the choice; and twice of them for 8-bit heads of 64, of whose
-// step_kernel one workgroup fits a CU.  (422 shapes of 1 and 4 sequences of up to
-// 2,000 nodes under windows of 32 .. 1,500, in both kernels: 1.1% more than the
-// better one in the mean.  By 16 nodes and the window, as for causal calls, 2.7%:
-// 2,000 nodes of 8 heads of 128 under 64 65 us, 49 now, 4,000 of 4 heads 103 and 59.
-// By all nodes 2.7%, too: 700 of 16 heads under 16 44 us, 28 now.)
+// the keys count for the choice.  (422 shapes of 1 and 4 sequences of up to 2,000
+// nodes under windows of 32 .. 1,500, in both kernels: 1.1% more than the better one
+// in the mean.  By 16 nodes and the window, as for causal calls, 1.7%: 2,000 nodes of
+// 8 heads of 128 under 64 65 us, 49 now, 4,000 of 4 heads 103 and 59.  By all nodes
+// 2.3%: 700 of 16 heads under 16 44 us, 28 now.)
 sol::PagedSize attend_size(int64_t rows, int64_t sequences, int64_t keys, int64_t query_heads, int64_t heads,
                            int64_t head_dim, int format, int causal, int64_t window, int64_t sink_tokens, bool tree) {
   const bool windowed = tree && window > 0;
   const int64_t nodes = windowed ? std::max(int64_t(16), cdiv(rows, sequences)) : 16;
   const int64_t tile_keys = window_keys(nodes, keys, causal, window, sink_tokens);
   int64_t step_keys = tile_keys;
-  if (windowed) {
-    step_keys = window_keys(std::max(int64_t(16), nodes / 2), keys, causal, window, sink_tokens);
-    step_keys = head_dim == 64 && format != SOL_CACHE_BF16 ? 2 * step_keys : step_keys / 2;
-  }
+  if (windowed)
+    step_keys = window_keys(std::max(int64_t(16), nodes / 2), keys, causal, window, sink_tokens) / 2;
   return sol::paged_size(rows, sequences, window_keys(rows, keys, causal, window, sink_tokens), tile_keys, step_keys,
                          heads, query_heads / heads, head_dim, format, causal != 0, true, tree);
 }

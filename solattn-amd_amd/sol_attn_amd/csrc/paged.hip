@@ -571,7 +571,10 @@ struct TreeLds {
   uint32_t mask[kTreeNodes];
   uint16_t next[kTreeNodes];
   int base, off, length;
-  int lane[kNT][3];  // each lane's query: where its walk is, and its position
+  // Each lane's query: where its walk is, and its position.  (After the stream of
+  // tiles step_kernel's waves hand over their states here, each in its own lanes'
+  // place: apart, 8-bit heads of 64 took 82,040 bytes, and one workgroup fit a CU.)
+  int lane[kNT][3];
 };
 
 // (One per kernel.)
@@ -1387,7 +1390,7 @@ __global__ __launch_bounds__(kNT, 2) void step_kernel(PagedParams p) {
   constexpr bool SCALED = F != kBf16;
   __shared__ __align__(256) uint8_t s_tile[kWaves][2 * Slot::kPlane];
   __shared__ __align__(16) float s_scale[kWaves][SCALED ? 2 * TK : 1];
-  __shared__ float s_md[kWaves][3][kWave];
+  __shared__ int s_md[TREE ? 1 : kWaves * 3 * kWave];  // (trees: TreeLds::lane)
 
   const int h = blockIdx.x % p.H;
   Item it;
@@ -1490,19 +1493,22 @@ __global__ __launch_bounds__(kNT, 2) void step_kernel(PagedParams p) {
   constexpr int FB = D / 16;
 #pragma unroll
   for (int fb = 0; fb < FB; ++fb) mine[fb * kWave + lane] = st.acc[fb];
-  s_md[wave][0][lane] = st.m;
-  s_md[wave][1][lane] = st.den;
-  s_md[wave][2][lane] = row.any ? 1.f : 0.f;
+  int* md = s_md;
+  if constexpr (TREE) md = &tree_lds().lane[0][0];
+  const auto handed = [&](int i, int k) { return __int_as_float(md[(3 * i + k) * kWave + lane]); };
+  const float state[3] = {st.m, st.den, row.any ? 1.f : 0.f};
+#pragma unroll
+  for (int k = 0; k < 3; ++k) md[(3 * wave + k) * kWave + lane] = __float_as_int(state[k]);
   __syncthreads();
   float m = kNegInf, den = 0.f, w[kWaves], seen = 0.f;
 #pragma unroll
-  for (int i = 0; i < kWaves; ++i) m = fmaxf(m, s_md[i][0][lane]);
+  for (int i = 0; i < kWaves; ++i) m = fmaxf(m, handed(i, 0));
 #pragma unroll
   for (int i = 0; i < kWaves; ++i) {
-    const float mi = s_md[i][0][lane];
+    const float mi = handed(i, 0);
     w[i] = mi == kNegInf ? 1.f : fast_exp2(mi - m);
-    den += w[i] * s_md[i][1][lane];
-    seen += s_md[i][2][lane];
+    den += w[i] * handed(i, 1);
+    seen += handed(i, 2);
   }
   // The four lanes of a query saw different keys of each tile.
   den = quad_sum(den);

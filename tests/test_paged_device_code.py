@@ -44,3 +44,19 @@ def test_inline_assembly_keeps_its_distance_from_vector_writes(asm):
 
 def test_no_packed_fp32(asm):
     assert not [line for line in asm[1] if re.search(r"\bv_pk_(add|mul|fma)_f32\b", line)]
+
+
+def test_two_workgroups_of_every_attention_kernel_fit_a_cu(asm):
+    source, text = asm
+    if source != "paged.hip":
+        pytest.skip("attention kernels alone")
+    sizes, kernel = {}, None
+    for line in text:
+        name = re.search(r"\.amdhsa_kernel (\S+)", line)
+        kernel = name.group(1) if name else kernel
+        size = re.search(r"\.amdhsa_group_segment_fixed_size (\d+)", line)
+        if size:
+            sizes[kernel] = int(size.group(1))
+    held = {k: n for k, n in sizes.items() if "step_kernel" in k or "wide_kernel" in k}
+    assert len(held) == 28
+    assert all(n <= 163840 // 2 for n in held.values()), {k: n for k, n in held.items() if n > 163840 // 2}
