@@ -11,7 +11,9 @@
 // most, which averages out over the keys; the denominator sums the unrounded
 // ones), where few rows leave them time as two BF16 terms.  (Two terms in
 // wide_kernel would be half as many products again in a kernel whose matrix
-// cores are busy for half of its time and more.)
+// cores are busy for half of its time and more over chunks.  With few rows over
+// many 8-bit keys, as of a tree, they are busy for a fifth of it, but a second
+// term of a half takes eight registers, and with heads of 128 all 256 are taken.)
 //
 // The rows of a (sequence, K/V head) are its new tokens times the G query
 // heads that share the head, token by token: row r is token r / G, query head
@@ -1382,7 +1384,9 @@ __device__ __forceinline__ void step_tile(const PagedParams& p, int length, Step
 // 210 us.  (BF16 tiles through registers, 32 x 32 products: 48 sequences of up to
 // 19,003 keys 256 us, 183 now.)  One sequence of 84,672 INT8 keys: 179 MB in 38
 // us and the merge's 5.  Small calls are a chain of latencies: three single
-// tokens over up to 317 keys 7.5 us.
+// tokens over up to 317 keys 7.5 us.  Trees: 48 sequences of up to 7 nodes behind up
+// to 9,000 tokens, 32 heads of 8, heads of 128 BF16 129 us, INT8 94, FP8 87; heads
+// of 64 69, 68 and 63.
 template <int D, int F, bool PAGED, bool TREE>
 __global__ __launch_bounds__(kNT, 2) void step_kernel(PagedParams p) {
   using Slot = StepSlot<D, F>;
@@ -1882,7 +1886,9 @@ __device__ __forceinline__ void wide_half(State<D>& st, const uint16_t* buf, con
 // 485); heads of 64 317 us, 0.87 PFLOP/s.  8-bit codes add a conversion of 64
 // codes and 64 multiplications by scales per lane and tile: FP8 645 us, INT8
 // 688.  Two workgroups per CU hold 256 registers a wave and a ring of two tiles
-// each; with heads of 128 that leaves 6 (BF16) to 17 (codes) registers spilled.
+// each; with heads of 128 that leaves 6 (BF16) to 17 (codes) registers spilled, of
+// trees 5 (BF16), 25 (INT8) and 28 (FP8): whole row tiles alone would spill 6, 20
+// and 22.
 template <int D, int F, bool PAGED, bool TREE>
 __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
   using S = Shape<D>;
@@ -2048,7 +2054,8 @@ __global__ __launch_bounds__(kNT, 2) void wide_kernel(PagedParams p) {
       }
     }
   };
-  // (Each form in code of its own: in one loop nest they took registers from each other.)
+  // (Each form in code of its own: in one loop nest they took registers from each
+  // other.  Both in one kernel still spill more than either: wide_kernel's comment.)
   if constexpr (TREE) {
     if (halved)
       attend_keys(std::true_type{});
@@ -2204,7 +2211,11 @@ PagedSize paged_size(int64_t rows, int64_t sequences, int64_t keys, int64_t tile
   } else if (tree && likely * heads <= kResident) {
     // One or two rounds of parts, as take_item finds; none where few tiles would
     // be cut.  (8 trees of 130 nodes of 8 x 4 heads behind 500 tokens: 41 us, 63
-    // in parts; 64 of up to 16 behind up to 9,000 INT8 tokens: 219, 154 in parts.)
+    // in parts.)  Sequences may differ in length, which wide_target does not know:
+    // from 48 key tiles on they are cut whatever it says.  (64 of up to 16 nodes of 8
+    // x 4 heads behind up to 9,000 tokens: INT8 156 us, 220 by wide_target alone, BF16
+    // 172 and 205; 40 of 26 of 8 x 3 heads behind 4,000 INT8 tokens each 169 and 183; 30
+    // of up to 64 of 8 heads behind up to 12,000 113 and 113.)
     s.min_tiles = 6;
     if (wide_target(likely, heads, key_tiles, s.min_tiles) || (ragged && sequences > 1 && key_tiles > 48))
       s.target = 2 * (kResident / heads), s.rounds = 2;

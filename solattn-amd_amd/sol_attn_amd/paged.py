@@ -330,7 +330,10 @@ def tree_attention(q, cache, plan, parents, *, window=None, sink_tokens=0, scale
     sees those whose position is less than ``window`` before its own, and the
     first ``sink_tokens``; a draft's position is the number of stored tokens
     plus its depth (0 for a root), which is also where :func:`rotate_heads` has
-    to turn it to.  :func:`cache_keep` keeps the accepted ones.
+    to turn it to.  Probabilities are rounded as there: to BF16 in calls of many
+    new tokens per sequence, times the query heads that share a head, and not
+    before 16 bits in those of few and in small calls.  :func:`cache_keep` keeps
+    the accepted ones.
     """
     if not isinstance(parents, torch.Tensor) or parents.dtype != torch.int32 or not parents.is_contiguous():
         raise ValueError("parents must be a contiguous int32 tensor")
@@ -383,9 +386,10 @@ def cache_keep(cache, plan, kept):
     not ascend or is not one of them (-1, say) ends the list.  The K and V rows
     of new token ``kept[s, j]`` (of position ``context_lengths[s] - new +
     kept[s, j]``) move to that of new token j, in place; rows behind the kept
-    ones stay as they are, and a row that has no page moves as zeros.  Stored values move as they are: keys that were
-    turned by their positions keep those (:func:`rotate_heads` turns a draft by
-    its depth, which is its place once it is kept).
+    ones stay as they are, and a row that has no page moves as zeros.  Stored
+    values move as they are: keys that were turned by their positions keep those
+    (:func:`rotate_heads` turns a draft by its depth, which is its place once it is
+    kept).
 
     Returns the sequences' lengths then, int32 ``[sequences]``: what
     :func:`cache_fork` continues from, or the lengths of a plan of your own.
