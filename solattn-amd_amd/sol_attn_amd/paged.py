@@ -427,7 +427,8 @@ def cache_fork(cache, pool, plan, parents, new_tokens, *, lengths=None, width=No
     ``width``: pages that a new table has room for, by default the old one's; the
     lengths go on past it, the tokens there are not stored or attended.
     ``plan`` and ``pool`` stay as they were, but the sequences they describe must
-    not be written any more: their pages have new owners.
+    not be written any more: their pages have new owners.  (Two calls on one pool
+    take the same pages: only one of the results can be gone on with.)
     """
     device = cache.k.device if isinstance(cache, PagedCache) else None
     _validate(cache, plan, device)

@@ -48,8 +48,6 @@ def test_no_packed_fp32(asm):
 
 def test_two_workgroups_of_every_attention_kernel_fit_a_cu(asm):
     source, text = asm
-    if source != "paged.hip":
-        pytest.skip("attention kernels alone")
     sizes, kernel = {}, None
     for line in text:
         name = re.search(r"\.amdhsa_kernel (\S+)", line)
@@ -58,5 +56,5 @@ def test_two_workgroups_of_every_attention_kernel_fit_a_cu(asm):
         if size:
             sizes[kernel] = int(size.group(1))
     held = {k: n for k, n in sizes.items() if "step_kernel" in k or "wide_kernel" in k}
-    assert len(held) == 28
+    assert len(held) == (28 if source == "paged.hip" else 0)
     assert all(n <= 163840 // 2 for n in held.values()), {k: n for k, n in held.items() if n > 163840 // 2}
